@@ -339,6 +339,171 @@ ATTN_API int attn_kv_cache_append(attn_kv_cache *c, int layer, int pos,
                          const float *krow, const float *vrow, attn_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Serving over a paged cache (no counterpart in the reference, whose caches
+ * are one slab per sequence): a step is attn_page_plan_ex (which cache row
+ * each new token takes), attn_rope_append_ex (positions turned into Q and K,
+ * K and V written to those rows) and attn_prefix_decode_ex (one query token
+ * per request over the rows its group shares and its own).
+ * None of these allocates, except attn_prefix_decode_ex without a workspace;
+ * all run on the caller's stream and may be captured in a graph.
+ * ---------------------------------------------------------------------- */
+/* A cache of `rows` token rows.  Page p of a P-token page size is rows
+ * [p*P, (p+1)*P); row r of head h starts at element r*row_stride + h*d, as in
+ * the other caches.  ATTN_I8 rows hold codes, with one fp32 scale per
+ * (row, head) at [r*kv_heads + h]. */
+typedef struct {
+    int kv_dtype;               /* ATTN_F32, ATTN_BF16 or ATTN_I8              */
+    long long rows;             /* token rows of k and v                       */
+    long long row_stride;       /* elements between rows (0: kv_heads*head_dim) */
+    void *k, *v;                /* 16-byte aligned                             */
+    float *kscale, *vscale;     /* ATTN_I8 only                                */
+} attn_paged_kv;
+
+typedef struct {
+    int n_seq;                  /* requests of the step, <= 16384              */
+    int page_size;              /* tokens per page: a power of two, <= 1024    */
+    int max_pages;              /* block_table columns                         */
+    int max_tokens;             /* rows of slot_map, positions and token_seq   */
+    int n_pages;                /* entries of free_pages                       */
+    int table_stride;           /* ints between block_table rows (0: max_pages) */
+} attn_page_shape;
+
+/* Plans one step from the requests' lengths, on the GPU.  Request s holds
+ * lens[s] tokens in pages block_table[s][0 .. ceil(lens[s]/page_size)) and
+ * receives new_lens[s] more, or ends when new_lens[s] < 0: its pages go back
+ * and its length becomes 0.
+ *   Pages are taken from the end of one list: free_pages[0 .. *free_count),
+ * then the pages of the ended requests in request and page order.  Request
+ * after request takes what its tokens need beyond its last page.  A request is
+ * refused, and nothing of it changes, when the list runs out at it or was run
+ * out by one before it, when its length would pass max_pages*page_size, or
+ * when its tokens would pass row max_tokens; one that needs no page is served
+ * whatever the list holds.
+ *   Written: block_table (the new entries only), free_pages (entries at and
+ * past *free_count only), and
+ *   lens_out[n_seq]: the lengths after the step;
+ *   cu_new[n_seq+1]: request s's new tokens are rows [cu_new[s], cu_new[s+1]),
+ *     refused ones included (2^31-1 where the sum passes that);
+ *   slot_map[max_tokens]: the cache row of each token row, -1 for tokens of
+ *     refused requests and for rows past the last token;
+ *   positions[max_tokens]: pos_base[s] (0 where NULL; the length of a shared
+ *     prefix, say) + the token's index in the request, 0 past the last token;
+ *   token_seq[max_tokens] (may be NULL): its request, -1 past the last token;
+ *   counts[4]: the free pages after the step, the tokens, the requests
+ *     refused, the pages taken.
+ * lens_out and counts must not overlap lens and free_count: a step's outputs
+ * are the next step's inputs.  One launch, no workspace, the same result on
+ * every run. */
+ATTN_API int attn_page_plan_ex(const attn_page_shape *s, const int *lens, const int *new_lens,
+                const int *pos_base, int *free_pages, const int *free_count, int *block_table,
+                int *lens_out, int *cu_new, long long *slot_map, int *positions,
+                int *token_seq, int *counts, attn_stream_t stream);
+
+/* Frequencies of a rotary table for contexts past the trained one.  Pair i of
+ * rot_dim/2 has frequency f_i = base^(-2i/rot_dim), and position p turns it by
+ * p * f_i.
+ *   ATTN_ROPE_PLAIN   f_i as they are
+ *   ATTN_ROPE_LINEAR  f_i / factor (positions interpolated)
+ *   ATTN_ROPE_BASE    base stretched to base * factor^(rot_dim/(rot_dim-2)),
+ *                     so the slowest pair slows by factor and the fastest
+ *                     stays (rot_dim > 2)
+ *   ATTN_ROPE_RAMP    by wavelength: a pair that turns more than `fast` times
+ *                     within trained_len tokens keeps f_i, one that turns less
+ *                     than `slow` times takes f_i / factor, and between them
+ *                     the two are mixed linearly in the pair's index
+ * Every table entry is multiplied by `magnitude` (0: 1). */
+enum { ATTN_ROPE_PLAIN = 0, ATTN_ROPE_LINEAR = 1, ATTN_ROPE_BASE = 2, ATTN_ROPE_RAMP = 3 };
+typedef struct {
+    int rot_dim;                /* even, 2 .. 128                              */
+    int max_pos;                /* rows of the table                           */
+    int scaling;                /* ATTN_ROPE_PLAIN ...                         */
+    int trained_len;            /* ATTN_ROPE_RAMP: tokens of the trained context */
+    double base;                /* 10000, say                                  */
+    double factor;              /* >= 1 (unused for ATTN_ROPE_PLAIN)           */
+    double fast, slow;          /* ATTN_ROPE_RAMP: turns, fast > slow > 0      */
+    double magnitude;
+} attn_rope_config;
+/* table[max_pos][rot_dim/2][2] = cos, sin (fp32, angles in fp64). */
+ATTN_API int attn_rope_table_ex(const attn_rope_config *c, float *table, attn_stream_t stream);
+
+typedef struct {
+    int tokens;
+    int seq_len;                /* position of row t when positions is NULL:
+                                   t % seq_len                                 */
+    int heads, kv_heads, head_dim;   /* head_dim 32, 64, 96 or 128             */
+    int rot_dim;                /* leading elements of each head that turn:
+                                   even, 0 .. head_dim; the others are copied  */
+    int interleaved;            /* pairs (2i, 2i+1); 0: (i, i + rot_dim/2)     */
+    int max_pos;                /* rows of the table                           */
+    long long q_row_stride, k_row_stride, v_row_stride;  /* elements (0: dense) */
+    long long q_out_row_stride, k_out_row_stride;
+} attn_rope_shape;
+
+/* q_out, k_out = q, k with each pair (a, b) of a head turned by its token's
+ * table row: (a cos - b sin, b cos + a sin), in fp32 from `dtype` (ATTN_F32 or
+ * ATTN_BF16), rounded once.  transpose = 1 turns back ((a cos + b sin,
+ * b cos - a sin)): the gradient of q and k from that of q_out and k_out.
+ * positions: DEVICE ints, one per token, or NULL.  q may be q_out and k may be
+ * k_out; otherwise they must not overlap.  k and k_out may both be NULL.
+ * A position outside the table records 0x701 in the device error word and the
+ * nearest row of the table is used. */
+ATTN_API int attn_rope_ex(const attn_rope_shape *s, int dtype, const float *table,
+                const int *positions, const void *q, const void *k, void *q_out, void *k_out,
+                int transpose, attn_stream_t stream);
+
+/* The serving form: q turned into q_out; k turned and v as it is written to
+ * cache row slot_map[t] (a DEVICE array; a token whose slot is outside the
+ * cache, -1 say, writes nothing there).  dtype ATTN_F32 into an ATTN_F32 or
+ * ATTN_I8 cache (quantised per (token, head) as attn_kv_quantize_int8 does),
+ * ATTN_BF16 into an ATTN_BF16 cache.  Slots of a call must differ from one
+ * another. */
+ATTN_API int attn_rope_append_ex(const attn_rope_shape *s, const attn_paged_kv *cache, int dtype,
+                const float *table, const int *positions, const long long *slot_map,
+                const void *q, const void *k, const void *v, void *q_out, attn_stream_t stream);
+
+typedef struct {
+    int n_seq;                  /* requests, one query token each, <= 65535    */
+    int n_groups;               /* groups that share a prefix (0: none)        */
+    int heads, kv_heads;        /* heads a multiple of kv_heads; query head h
+                                   reads key head h / (heads / kv_heads)       */
+    int head_dim;               /* 32, 64, 96 or 128                           */
+    int dtype;                  /* of q and out: ATTN_BF16 with an ATTN_BF16
+                                   cache, else ATTN_F32                        */
+    int page_size;              /* a power of two, <= 1024                     */
+    int max_prefix_pages;       /* prefix_table columns                        */
+    int max_pages;              /* block_table columns                         */
+    int max_prefix_len;         /* upper bounds of prefix_lens and lens        */
+    int max_len;
+    long long q_row_stride, out_row_stride;   /* elements (0: heads*head_dim)  */
+    float scale;                /* of the scores (0: 1/sqrt(head_dim))         */
+} attn_prefix_shape;
+
+/* Bytes of device workspace attn_prefix_decode_ex needs. */
+ATTN_API size_t attn_prefix_decode_workspace_bytes(const attn_prefix_shape *s, const attn_paged_kv *cache);
+
+/* Decodes one query token per request over the rows of its group's prefix and
+ * its own rows, as one softmax: out = sum_j softmax_j(scale q.k_j) v_j.  The
+ * prefix is read once for all requests of a group.
+ *   group_begin[n_groups+1] (DEVICE, ascending): group g is requests
+ *     [group_begin[g], group_begin[g+1]); a request of no group has no prefix.
+ *   prefix_table[n_groups][max_prefix_pages], prefix_lens[n_groups],
+ *   block_table[n_seq][max_pages], lens[n_seq]: DEVICE ints; entries past a
+ *     length's pages are not read, nor are cache rows past a length.
+ *   lse (may be NULL): n_seq x heads floats, the natural log of the sum of
+ *     exponentials.
+ * A request with no row at all gets out = 0 and lse = -inf.  A length outside
+ * [0, max] is clamped and records 0x703 in the device error word; a page
+ * outside the cache records 0x702 and its rows count as absent.  fp32 and INT8
+ * caches: fp32 arithmetic or products of exact parts with fp32 sums; bf16:
+ * bf16 products, probabilities rounded to bf16, fp32 sums and statistics.
+ * workspace (256-byte aligned) may be NULL: the library's own per-device
+ * buffer, grown on demand; calls that use it must not overlap on the GPU. */
+ATTN_API int attn_prefix_decode_ex(const attn_prefix_shape *s, const attn_paged_kv *cache,
+                const void *q, const int *group_begin, const int *prefix_table,
+                const int *prefix_lens, const int *block_table, const int *lens, void *out,
+                float *lse, void *workspace, size_t workspace_bytes, attn_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Multi-GPU partitioning by (batch x head) units
  * ---------------------------------------------------------------------- */
 /* Contiguous split of n_units over `world` ranks: rank gets [*begin, *end). */

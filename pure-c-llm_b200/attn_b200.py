@@ -17,6 +17,7 @@ OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA, ERR_NOMEM, ERR_WORKSPACE, ERR_DEVICE
 PROBS_LSE_OUT, PROBS_LSE = 0, 1      # attn_set_probs_mode
 F32, BF16, I8 = 0, 1, 2
 MAX_LAYERS = 64
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_RAMP = range(4)   # attn_rope_config.scaling
 STATIC_SCRATCH_BYTES = 4 << 20      # ATTN_DECODE_STATIC_SCRATCH_BYTES
 
 
@@ -55,6 +56,41 @@ class QKVShape(ctypes.Structure):
                 ("x_row_stride", ctypes.c_longlong), ("out_row_stride", ctypes.c_longlong)]
 
 
+class PagedKV(ctypes.Structure):
+    _fields_ = [("kv_dtype", ctypes.c_int), ("rows", ctypes.c_longlong), ("row_stride", ctypes.c_longlong),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("kscale", ctypes.c_void_p), ("vscale", ctypes.c_void_p)]
+
+
+class PageShape(ctypes.Structure):
+    _fields_ = [("n_seq", ctypes.c_int), ("page_size", ctypes.c_int), ("max_pages", ctypes.c_int),
+                ("max_tokens", ctypes.c_int), ("n_pages", ctypes.c_int), ("table_stride", ctypes.c_int)]
+
+
+class RopeConfig(ctypes.Structure):
+    _fields_ = [("rot_dim", ctypes.c_int), ("max_pos", ctypes.c_int), ("scaling", ctypes.c_int),
+                ("trained_len", ctypes.c_int), ("base", ctypes.c_double), ("factor", ctypes.c_double),
+                ("fast", ctypes.c_double), ("slow", ctypes.c_double), ("magnitude", ctypes.c_double)]
+
+
+class RopeShape(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int), ("seq_len", ctypes.c_int), ("heads", ctypes.c_int),
+                ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("rot_dim", ctypes.c_int),
+                ("interleaved", ctypes.c_int), ("max_pos", ctypes.c_int),
+                ("q_row_stride", ctypes.c_longlong), ("k_row_stride", ctypes.c_longlong),
+                ("v_row_stride", ctypes.c_longlong), ("q_out_row_stride", ctypes.c_longlong),
+                ("k_out_row_stride", ctypes.c_longlong)]
+
+
+class PrefixShape(ctypes.Structure):
+    _fields_ = [("n_seq", ctypes.c_int), ("n_groups", ctypes.c_int), ("heads", ctypes.c_int),
+                ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("dtype", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("max_prefix_pages", ctypes.c_int), ("max_pages", ctypes.c_int),
+                ("max_prefix_len", ctypes.c_int), ("max_len", ctypes.c_int),
+                ("q_row_stride", ctypes.c_longlong), ("out_row_stride", ctypes.c_longlong),
+                ("scale", ctypes.c_float)]
+
+
 class Split(ctypes.Structure):
     _fields_ = [("batch0", ctypes.c_int), ("batch", ctypes.c_int), ("head0", ctypes.c_int),
                 ("heads", ctypes.c_int), ("nb", ctypes.c_int), ("nh", ctypes.c_int)]
@@ -90,6 +126,12 @@ SIGNATURES = {
     "attn_kv_cache_alloc": (I, [ctypes.POINTER(KVCache), I, I, I, I, I]),
     "attn_kv_cache_free": (I, [ctypes.POINTER(KVCache)]),
     "attn_kv_cache_append": (I, [ctypes.POINTER(KVCache), I, I, P, P, P]),
+    "attn_page_plan_ex": (I, [ctypes.POINTER(PageShape), P, P, P, P, P, P, P, P, P, P, P, P, P]),
+    "attn_rope_table_ex": (I, [ctypes.POINTER(RopeConfig), P, P]),
+    "attn_rope_ex": (I, [ctypes.POINTER(RopeShape), I, P, P, P, P, P, P, I, P]),
+    "attn_rope_append_ex": (I, [ctypes.POINTER(RopeShape), ctypes.POINTER(PagedKV), I, P, P, P, P, P, P, P, P]),
+    "attn_prefix_decode_workspace_bytes": (SZ, [ctypes.POINTER(PrefixShape), ctypes.POINTER(PagedKV)]),
+    "attn_prefix_decode_ex": (I, [ctypes.POINTER(PrefixShape), ctypes.POINTER(PagedKV), P, P, P, P, P, P, P, P, P, SZ, P]),
     "attn_shard_range": (I, [LL, I, I, ctypes.POINTER(LL), ctypes.POINTER(LL)]),
     "attn_shard_lpt": (I, [P, I, I, I, P, P]),
     "attn_gather_permute": (I, [P, P, I, I, I, I, I, I, P]),
@@ -286,4 +328,88 @@ def gather_permute_t(staging, world, batch, seq_len, heads, head_dim):
     out = torch.empty((batch * seq_len, heads * head_dim), dtype=staging.dtype, device=staging.device)
     check(lib.attn_gather_permute(staging.data_ptr(), out.data_ptr(), world, batch, seq_len, heads, head_dim,
                                   _dtype_code(staging), _stream()))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# serving over a paged cache
+# ---------------------------------------------------------------------------
+class PageCache(PagedKV):
+    """A paged cache over k and v tensors of (rows, kv_heads * d), which it keeps alive.  An int8 cache brings its
+    (rows, kv_heads) fp32 scales."""
+
+    @classmethod
+    def of(cls, k, v, kscale=None, vscale=None):
+        import torch
+        kv = I8 if k.dtype == torch.int8 else _dtype_code(k)
+        if v.dtype != k.dtype or v.shape != k.shape or v.stride() != k.stride() or k.stride(1) != 1:
+            raise ValueError("k and v must have one type, shape and layout, with dense rows")
+        if kv == I8 and not (kscale is not None and vscale is not None and kscale.is_contiguous() and
+                             vscale.is_contiguous()):
+            raise ValueError("an int8 cache needs dense kscale and vscale")
+        c = cls(kv, k.shape[0], k.stride(0), k.data_ptr(), v.data_ptr(), _ptr(kscale), _ptr(vscale))
+        c.tensors = (k, v, kscale, vscale)
+        return c
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def page_outputs(shape: PageShape, device="cuda"):
+    """Tensors that page_plan_t writes for this shape, by name."""
+    import torch
+    out = {k: torch.empty(n, dtype=torch.int32, device=device)
+           for k, n in (("lens", shape.n_seq), ("cu_new", shape.n_seq + 1), ("positions", shape.max_tokens),
+                        ("token_seq", shape.max_tokens), ("counts", 4))}
+    out["slot_map"] = torch.empty(shape.max_tokens, dtype=torch.int64, device=device)
+    return out
+
+
+def page_plan_t(shape: PageShape, lens, new_lens, free_pages, free_count, block_table, out, pos_base=None):
+    """attn_page_plan_ex: int32 CUDA tensors; `out` as page_outputs makes it (slot_map int64).  Writes `out`, the new
+    entries of block_table and the returned pages in free_pages; out["lens"] and out["counts"][:1] are the next step's
+    lens and free_count."""
+    check(lib.attn_page_plan_ex(shape, lens.data_ptr(), new_lens.data_ptr(), _ptr(pos_base), free_pages.data_ptr(),
+                                free_count.data_ptr(), block_table.data_ptr(), out["lens"].data_ptr(),
+                                out["cu_new"].data_ptr(), out["slot_map"].data_ptr(), out["positions"].data_ptr(),
+                                _ptr(out.get("token_seq")), out["counts"].data_ptr(), _stream()))
+    return out
+
+
+def rope_table_t(config: RopeConfig, device="cuda"):
+    """The (max_pos, rot_dim / 2, 2) fp32 table of cosines and sines of a configuration."""
+    import torch
+    table = torch.empty((config.max_pos, config.rot_dim // 2, 2), dtype=torch.float32, device=device)
+    check(lib.attn_rope_table_ex(config, table.data_ptr(), _stream()))
+    return table
+
+
+def rope_t(shape: RopeShape, table, positions, q, k, q_out, k_out, transpose=False):
+    """attn_rope_ex on (tokens, heads * d) fp32 or bf16 tensors; positions int32 or None; k and k_out may be None."""
+    check(lib.attn_rope_ex(shape, _dtype_code(q), _ptr(table), _ptr(positions), q.data_ptr(), _ptr(k),
+                           q_out.data_ptr(), _ptr(k_out), int(transpose), _stream()))
+    return q_out, k_out
+
+
+def rope_append_t(shape: RopeShape, cache: PagedKV, table, positions, slot_map, q, k, v, q_out):
+    """attn_rope_append_ex: positions int32 or None, slot_map int64."""
+    check(lib.attn_rope_append_ex(shape, cache, _dtype_code(q), _ptr(table), _ptr(positions), slot_map.data_ptr(),
+                                  q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), _stream()))
+    return q_out
+
+
+def prefix_decode_workspace_bytes(shape: PrefixShape, cache: PagedKV) -> int:
+    return lib.attn_prefix_decode_workspace_bytes(shape, cache)
+
+
+def prefix_decode_t(shape: PrefixShape, cache: PagedKV, q, group_begin, prefix_table, prefix_lens, block_table, lens,
+                    out, lse=None, workspace=None):
+    """attn_prefix_decode_ex: q and out (n_seq, heads * d); tables and lengths int32; group_begin, prefix_table and
+    prefix_lens may be None when shape.n_groups is 0."""
+    check(lib.attn_prefix_decode_ex(shape, cache, q.data_ptr(), _ptr(group_begin), _ptr(prefix_table),
+                                    _ptr(prefix_lens), block_table.data_ptr(), lens.data_ptr(), out.data_ptr(),
+                                    _ptr(lse), _ptr(workspace),
+                                    workspace.numel() * workspace.element_size() if workspace is not None else 0,
+                                    _stream()))
     return out
