@@ -192,6 +192,10 @@ static int check_prefix(const attn_prefix_shape *s, const attn_paged_kv *c, long
                          s->max_len, s->max_pages, s->max_prefix_len, s->max_prefix_pages, s->page_size);
     const int st = check_cache(c, s->kv_heads, s->head_dim, rs, "prefix decode");
     if (st) return st;
+    if (c->rows > 0x7fffffffLL)
+        return set_error(ATTN_ERR_UNSUPPORTED, "prefix decode: a cache of %lld rows, at most 2^31 - 1", c->rows);
+    if (c->rows < s->page_size && (s->max_len || (s->n_groups && s->max_prefix_len)))
+        return set_error(ATTN_ERR_INVALID, "prefix decode: a cache of %lld rows holds no page of %d", c->rows, s->page_size);
     if (s->dtype != (c->kv_dtype == ATTN_BF16 ? ATTN_BF16 : ATTN_F32))
         return set_error(ATTN_ERR_UNSUPPORTED, "prefix decode: dtype %d with a cache of dtype %d", s->dtype, c->kv_dtype);
     const long long hd = (long long)s->heads * s->head_dim;
@@ -248,7 +252,7 @@ int attn_prefix_decode_ex(const attn_prefix_shape *s, const attn_paged_kv *cache
     p.n_seq = s->n_seq; p.n_groups = s->n_groups; p.heads = s->heads; p.kv_heads = s->kv_heads;
     p.ratio = s->heads / s->kv_heads;
     p.log_page = __builtin_ctz((unsigned)s->page_size);
-    p.n_pages = (int)std::min<long long>(cache->rows / s->page_size, 0x7fffffffLL);
+    p.n_pages = (int)(cache->rows / s->page_size);
     p.max_prefix_pages = s->max_prefix_pages; p.max_pages = s->max_pages;
     p.max_prefix_len = s->max_prefix_len; p.max_len = s->max_len;
     p.scale_log2 = attn::kLog2e * (s->scale > 0.f ? s->scale : 1.f / sqrtf((float)s->head_dim));

@@ -6,8 +6,9 @@ Tolerances, from the arithmetic:
             result, 2^-8 of it at most (2^-9 and the fp32 error before it).
   prefix    a score is off by at most delta = 2^-21 (1 + scale sum|q k|) (products off by 2^-22 where an operand is
             split in parts, fp32 sums, the exponential's argument), so a probability by the factor 1 +- 2 delta and
-            the output by 4 delta sum p|v| (numerator and denominator); for bf16 2^-8 sum p|v| more, half of it for
-            probabilities rounded to bf16 and half for the output.  A probability under 2^-126, the smallest normal
+            the output by 4 delta sum p|v| (numerator and denominator); for bf16 2^-8 sum p|v| more, the most that rounding
+            the output can take (probabilities rounded to bf16 err at random, so over many keys they stay far below it;
+            over few keys the kernel keeps what the rounding drops).  A probability under 2^-126, the smallest normal
             fp32 number, may count as 0: 2^-126 max|v| more for each key.  lse: delta + 2^-22 |lse|."""
 import ctypes
 

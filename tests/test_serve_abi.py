@@ -107,6 +107,7 @@ def test_prefix_decode_refusals():
     assert A.prefix_decode_workspace_bytes(shape, kv()) > 0
     assert decode(shape, None) == A.ERR_INVALID and decode(shape, kv(kv_dtype=A.I8)) == A.ERR_INVALID
     assert decode(shape, kv(kv_dtype=A.BF16)) == A.ERR_UNSUPPORTED
+    assert decode(shape, kv(rows=15)) == A.ERR_INVALID and decode(shape, kv(rows=2 ** 31)) == A.ERR_UNSUPPORTED
     for bad in (dict(q=None), dict(out=None), dict(lens=None), dict(table=None), dict(begin=None), dict(ptable=None), dict(plens=None),
                 dict(q=P + 8), dict(out=Q + 4), dict(lens=P + 2), dict(lse=P + 1)):
         assert decode(shape, kv(), **bad) == A.ERR_INVALID, bad
