@@ -16,10 +16,10 @@
 // (its piece) goes to the workspace, at slot segment + team, and
 // prefix_merge_kernel joins the pieces of each query row.
 //
-// Bound: HBM (the cache rows, once).  Little else may cost: the rows go from
-// global memory to the lanes in the layout in which the arithmetic takes
-// them (prefix_paths.cuh), the next steps' copies in flight during a step's
-// arithmetic.
+// Bound: HBM (the cache rows, once).  Little else may cost: each warp
+// copies its rows through a ring of its own in shared memory, from which the
+// lanes read them in the layout that the arithmetic takes (prefix_paths.cuh),
+// and meets no other warp until the merge.
 #include <algorithm>
 
 #include "prefix.cuh"
@@ -84,7 +84,8 @@ __device__ __forceinline__ void run_piece(const Params &p, uint32_t ring, const 
     const int lane = threadIdx.x & 31;
     Path path;
     // Cache row of this lane's key of a step: bad pages and keys past the line
-    // have no valid row and stand on row 0.
+    // have no valid row.  In pages of 16 rows or more, a run of 16 keys is
+    // copied from its first key's row, which keys past the line do not decide.
     auto row_of = [&](int step, bool &valid) {
         const int t = step * Path::KEYS + lane;
         valid = lane < Path::KEYS && t < keys && step < b;
@@ -102,7 +103,10 @@ __device__ __forceinline__ void run_piece(const Params &p, uint32_t ring, const 
     path.begin(p, first_req, row0, rows, hk);
     auto issue = [&](int step, int stage) {
         masks[stage] = __ballot_sync(0xffffffffu, next_valid);
-        if (step < b) path.issue(p, ring + stage * Path::STAGE, next_row);
+        if (step < b) {
+            if (p.log_page >= 4) path.template issue<true>(p, ring + stage * Path::STAGE, next_row);
+            else path.template issue<false>(p, ring + stage * Path::STAGE, next_row);
+        }
         asm volatile("cp.async.commit_group;" ::: "memory");
         next_row = row_of(step + 1, next_valid);
     };
@@ -115,9 +119,11 @@ __device__ __forceinline__ void run_piece(const Params &p, uint32_t ring, const 
             if (step + u < b) {
                 issue(step + u + STAGES - 1, (u + STAGES - 1) % STAGES);
                 asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+                __syncwarp();             // every lane's copies of the stage are there
                 const uint32_t st = ring + u * Path::STAGE;
                 if (masks[u] == all) path.template compute<false>(p, st, all);
                 else path.template compute<true>(p, st, masks[u]);
+                __syncwarp();             // the stage may be copied over
             }
         }
     }
@@ -130,7 +136,7 @@ template <class Own, class Pre> struct Ring {
     static constexpr int FIT = (208 * 1024 / kWarps) / STAGE;
     static constexpr int STAGES = FIT > 4 ? 4 : FIT;
     static constexpr int BYTES = STAGES * STAGE;
-    static_assert(STAGES >= 2, "ring");
+    static_assert(STAGES >= 2 && Own::STAGE % 128 == 0 && Pre::STAGE % 128 == 0, "ring");
 };
 
 template <class Own, class Pre, int D>
@@ -138,7 +144,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
 prefix_rows_kernel(const __grid_constant__ Params p, const __grid_constant__ Work w)
 {
     using R = Ring<Own, Pre>;
-    extern __shared__ __align__(16) uint8_t ring_bytes[];
+    extern __shared__ __align__(128) uint8_t ring_bytes[];
     __shared__ long long sums[kEntries + 1];
     __shared__ long long warp_sums[kWarps];
     pdl_begin();                          // launched by launch_pdl
@@ -404,10 +410,19 @@ int run(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s) {
 template <int D>
 int run_d(const attn::prefix::Params &p, int kv_dtype, void *ws, size_t *need, cudaStream_t s) {
     using namespace attn::prefix;
-    if (kv_dtype == ATTN_BF16)
-        return p.ratio <= 8 ? run<Bf16Path<D, false>, Bf16Path<D, true>, __nv_bfloat16, D>(p, ws, need, s)
-                            : run<Bf16Path<D, true>, Bf16Path<D, true>, __nv_bfloat16, D>(p, ws, need, s);
-    if (kv_dtype == ATTN_I8) return run<I8Path<D>, I8Path<D>, float, D>(p, ws, need, s);
+    // Tiles of query rows per warp: own rows as the request needs (more rows
+    // than two tiles hold make more blocks); for a prefix, K and V are read
+    // again for every block, so as many as the registers hold (o takes D NT / 4).
+    if (kv_dtype == ATTN_BF16) {
+        constexpr int N = D == 32 ? 8 : D == 64 ? 4 : 2;
+        return p.ratio <= 8 ? run<Bf16Path<D, 1>, Bf16Path<D, N>, __nv_bfloat16, D>(p, ws, need, s)
+                            : run<Bf16Path<D, 2>, Bf16Path<D, N>, __nv_bfloat16, D>(p, ws, need, s);
+    }
+    if (kv_dtype == ATTN_I8) {
+        constexpr int N = D <= 64 ? 4 : 2;
+        return p.ratio <= 4 ? run<I8Path<D, 1>, I8Path<D, N>, float, D>(p, ws, need, s)
+                            : run<I8Path<D, 2>, I8Path<D, N>, float, D>(p, ws, need, s);
+    }
     // own rows with the request's query rows, up to 8 at a time; prefixes with 8
     if (p.ratio == 1) return run<F32Path<D, 1>, F32Path<D, 8>, float, D>(p, ws, need, s);
     if (p.ratio == 2) return run<F32Path<D, 2>, F32Path<D, 8>, float, D>(p, ws, need, s);

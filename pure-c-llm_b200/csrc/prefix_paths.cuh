@@ -7,10 +7,18 @@
 // Row i of a block is query head hk * ratio + (row0 + i) % ratio of request
 // first_req + (row0 + i) / ratio.
 //
-// A lane copies exactly the bytes that it will use, into words that only it
-// reads (chunk i of lane n at 32 i + n, so neither side has bank conflicts):
-// a stage is an extension of the lane's registers, and waiting for the lane's
-// own copies is all the synchronisation there is.
+// bf16 and INT8 form the scores as S^T = K Q^T and the outputs as O^T = V^T P^T
+// with mma.sync m16n8k16: the cache side is the 16-row operand, so a tile of 8
+// columns of queries costs one instruction where a 16-row tile of queries
+// would be mostly empty, and K and V fragments serve NT such tiles.  A lane
+// (g, c) = (lane / 4, lane % 4) gets S of keys g, g + 8 and columns 2c, 2c + 1;
+// the columns' probabilities, packed, become the second product's operand by
+// one 8 x 8 transposition (movmatrix), and the columns of O^T are the lane's
+// own again, so a rescaling needs no exchange.
+//
+// The warp copies the rows as they lie in memory, 16 bytes a lane, to rows of
+// shared memory in which the 16- or 32-byte pieces change places by row number,
+// so that what eight lanes read together lies in different banks.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -42,24 +50,88 @@ __device__ __forceinline__ float quad_max(float v) {
     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
     return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
-__device__ __forceinline__ float quad_sum(float v) {
-    v += __shfl_xor_sync(0xffffffffu, v, 1);
-    return v + __shfl_xor_sync(0xffffffffu, v, 2);
-}
 // a and b as bf16, and what that leaves of them
 __device__ __forceinline__ void bf16_parts(float a, float b, uint32_t &hi, uint32_t &lo) {
     hi = pack_bf16(a, b);
     lo = pack_bf16(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
 }
 
-// Copies to a stage and reads from it.  The data are read once (16 bytes past
-// L1) or by lanes that share sectors (smaller pieces, through L1).
+// Copies to a stage and reads from it.
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-template <int N>
-__device__ __forceinline__ void copy_small(uint32_t dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+__device__ __forceinline__ void copy4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// Order of the 16-byte pieces of a row in shared memory: as they are; the
+// 64-byte halves of each 128 bytes swapped in odd rows; whole 32-byte sectors
+// XORed with (row / 2) % 4; or pieces XORed for 8 x 8 tiles (TILES): with row % 8
+// where rows lie a multiple of 128 bytes apart, else with (row / 2) % 4.
+enum Order { AS_IS, HALVES, SECTORS, TILES };
+template <int PITCH, Order ORDER>
+__device__ __forceinline__ constexpr uint32_t order_bits(int row) {
+    return ORDER == HALVES ? (row & 1) << 6
+         : ORDER == SECTORS ? (row >> 1 & 3) << 5
+         : ORDER == TILES ? (PITCH % 128 == 0 ? row & 7 : row >> 1 & 3) << 4 : 0;
+}
+// KEYS rows of BYTES, the first at `base`, to `st` at PITCH.  RUNS: lane n's
+// `row` is the cache row of key n, and every 16 keys' rows follow one another
+// (pages of 16 rows or more); otherwise each key has a row of its own.
+template <int KEYS, int BYTES, int PITCH, Order ORDER, bool RUNS>
+__device__ __forceinline__ void copy_rows(uint32_t st, const char *base, long long stride, int row) {
+    constexpr int CPR = BYTES / 16;                             // copies per row
+    constexpr int P = CPR % 3 ? 1 : 3, RP = 32 * P / CPR;       // after P copies, RP rows on, lanes repeat
+    const int lane = threadIdx.x & 31;
+    static_assert(KEYS * CPR % 32 == 0 && (P == 1 || RP % 8 == 0 || CPR == 24), "whole warps of copies");
+    constexpr int SPAN = KEYS < 16 ? KEYS : 16, PER = SPAN * CPR / 32;   // rows of a run, its copies
+#pragma unroll
+    for (int s = 0; s < KEYS / SPAN; s++) {
+        const char *run = RUNS ? base + __shfl_sync(0xffffffffu, row, s * SPAN) * stride : nullptr;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int n = i % P * 32 + lane, lk = n / CPR, ch = n % CPR;          // within the period
+            const int first = s * SPAN + i / P * RP;
+            const char *src = RUNS ? run + (i / P * RP) * stride + lk * stride + ch * 16
+                                   : base + __shfl_sync(0xffffffffu, row, first + lk) * stride + ch * 16;
+            copy16(st + first * PITCH + ((lk * PITCH + ch * 16) ^ order_bits<PITCH, ORDER>(first + lk)), src);
+        }
+    }
+}
+// Pitch of INT8 V rows in SECTORS order: a multiple of 64, and of 128 past it.
+constexpr int v_pitch(int bytes) { return bytes <= 64 ? 64 : (bytes + 127) / 128 * 128; }
+// Byte `off` of V row 2c + odd + 8 n, from the row's start; `lane_off` is off's
+// part that depends on the lane (under 128), XORed with c << 5 already.
+template <int PITCH>
+__device__ __forceinline__ uint32_t v_at(int odd, uint32_t lane_off, int off) {
+    return PITCH == 64 ? (lane_off ^ (odd ? 64u : 0u)) + off : odd * PITCH + lane_off + off;
+}
+// Four 8 x 8 tiles of 16-bit elements: lane n gives the address of row n % 8 of
+// tile n / 8 and gets elements (g, 2c), (g, 2c + 1) of each, or (2c, g),
+// (2c + 1, g) with T.
+template <bool T>
+__device__ __forceinline__ void tiles(uint32_t (&r)[4], uint32_t a) {
+    if constexpr (T)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+// over the 8 lanes of the same c
+__device__ __forceinline__ float keys_max(float v) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float keys_sum(float v) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
 }
 __device__ __forceinline__ uint4 lds16(uint32_t a) {
     uint4 v;
@@ -85,207 +157,166 @@ __device__ __forceinline__ const T *query(const Params &p, int first_req, int ro
 }
 
 // ---------------------------------------------------------------------------
-// bf16: both products on mma.sync m16n8k16, 8 or 16 query rows.
+// bf16, 8 NT query rows: column n of tile t is row 8 t + n.
 //
-// A dot product may take its k positions in any order, and an output its n
-// positions, so each lane's share of a cache row is 16 contiguous bytes and
-// serves as it was loaded:
-//   scores: lane (g, c) = (lane / 4, lane % 4) holds dims (4 j + c) 8 .. + 7 of
-//     key g, whose four words are the B fragments of k-steps 2j and 2j + 1;
-//   values: lane (g, c) holds dims 8 g .. 8 g + 7 (of each 64) of keys 2c,
-//     2c + 1, 2c + 8, 2c + 9; one byte permutation pairs two keys' values of a
-//     dim into a B fragment, and dim 8 g + i is column g of n-tile i.
-// Probabilities are rounded to bf16 for the second product (their sum is not);
-// with 8 rows, the rounding's rest goes through the 8 MMA rows that are free.
+// Probabilities are rounded to bf16 for the second product (their sum is not).
+// With one tile, which is what a request's own, perhaps few, rows take, the
+// rounding's rest goes through a second instruction.
 // ---------------------------------------------------------------------------
-template <int D, bool HI>                 // HI: rows 8 .. 15 are used
+template <int D, int NT>
 struct Bf16Path {
-    static constexpr int ROWS = HI ? 16 : 8, KEYS = D <= 64 ? 32 : 16;
-    static constexpr int KT = KEYS / 8, KH = KEYS / 16, KC = D / 32, B64 = D / 64, REM = D % 64 != 0;
-    static constexpr int NT = D / 8, NR = HI ? 2 : 1;         // n-tiles of the output; rows of a lane
-    static constexpr int OFF_V = KT * KC * 512, OFF_W = OFF_V + KH * 4 * B64 * 512, STAGE = OFF_W + REM * KH * 4 * 256;
-    uint32_t q[2 * KC][2 * NR];
-    float o[NT][4], m[NR], l[NR];
+    static constexpr int ROWS = 8 * NT, KEYS = D <= 64 ? 32 : 16;
+    static constexpr int KM = KEYS / 16, KS = D / 16;         // 16-key tiles; 16-dim tiles
+    static constexpr int PITCH = 2 * D, OFF_V = KEYS * PITCH, STAGE = 2 * OFF_V;
+    uint32_t q[NT][KS][2];
+    float o[NT][KS][4], m[NT][2], l[NT][2];
     const char *kb, *vb;
 
     __device__ __forceinline__ void begin(const Params &p, int first_req, int row0, int rows, int hk) {
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
-        for (int r = 0; r < NR; r++) {
-            const __nv_bfloat16 *a = query<__nv_bfloat16>(p, first_req, row0 + min(g + 8 * r, rows - 1), hk, D);
+        for (int t = 0; t < NT; t++) {
+            const __nv_bfloat16 *a = query<__nv_bfloat16>(p, first_req, row0 + min(8 * t + g, rows - 1), hk, D) + 2 * c;
 #pragma unroll
-            for (int j = 0; j < KC; j++) {
-                const uint4 x = __ldg(reinterpret_cast<const uint4 *>(a) + 4 * j + c);
-                q[2 * j][r] = x.x; q[2 * j][NR + r] = x.y;
-                q[2 * j + 1][r] = x.z; q[2 * j + 1][NR + r] = x.w;
+            for (int j = 0; j < KS; j++) {
+                q[t][j][0] = __ldg(reinterpret_cast<const uint32_t *>(a + 16 * j));
+                q[t][j][1] = __ldg(reinterpret_cast<const uint32_t *>(a + 16 * j + 8));
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[t][j][e] = 0.f;
             }
-            m[r] = -INFINITY;
-            l[r] = 0.f;
+            m[t][0] = m[t][1] = -INFINITY;
+            l[t][0] = l[t][1] = 0.f;
         }
-#pragma unroll
-        for (int i = 0; i < NT; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[i][e] = 0.f;
-        kb = static_cast<const char *>(p.k) + (long long)hk * D * 2 + c * 16;
+        kb = static_cast<const char *>(p.k) + (long long)hk * D * 2;
         vb = static_cast<const char *>(p.v) + (long long)hk * D * 2;
     }
+    template <bool RUNS>
     __device__ __forceinline__ void issue(const Params &p, uint32_t st, int row) const {
-        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-        const long long stride = p.row_stride * 2;
-#pragma unroll
-        for (int t = 0; t < KT; t++) {
-            const char *at = kb + __shfl_sync(0xffffffffu, row, t * 8 + g) * stride;
-#pragma unroll
-            for (int j = 0; j < KC; j++) copy16(st + (t * KC + j) * 512 + lane * 16, at + 64 * j);
-        }
-#pragma unroll
-        for (int n = 0; n < 4 * KH; n++) {
-            const char *at = vb + __shfl_sync(0xffffffffu, row, (n >> 1) * 8 + 2 * c + (n & 1)) * stride;
-#pragma unroll
-            for (int x = 0; x < B64; x++) copy16(st + OFF_V + (n * B64 + x) * 512 + lane * 16, at + 128 * x + 16 * g);
-            if constexpr (REM) copy_small<8>(st + OFF_W + n * 256 + lane * 8, at + 128 * B64 + 8 * g);
-        }
+        copy_rows<KEYS, 2 * D, PITCH, TILES, RUNS>(st, kb, p.row_stride * 2, row);
+        copy_rows<KEYS, 2 * D, PITCH, TILES, RUNS>(st + OFF_V, vb, p.row_stride * 2, row);
     }
     template <bool EDGE>                  // EDGE: some keys of the step have no row
     __device__ __forceinline__ void compute(const Params &p, uint32_t st, unsigned mask) {
-        const int lane = threadIdx.x & 31, c = lane & 3;
-        st += lane * 16;
-        float s[KT][4];
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        // rows and pieces that this lane addresses: K tiles (keys, +8 keys, +8 dims), V (keys, +8 dims, +8 keys)
+        const uint32_t turn = order_bits<PITCH, TILES>(lane & 7);
+        const uint32_t kst = st + ((lane >> 3 & 1) * 8 + (lane & 7)) * PITCH, kbits = turn ^ (lane >> 4) << 4;
+        const uint32_t vst = st + OFF_V + ((lane >> 4) * 8 + (lane & 7)) * PITCH, vbits = turn ^ (lane >> 3 & 1) << 4;
+        float s[NT][KM][4];
 #pragma unroll
-        for (int t = 0; t < KT; t++) {
-            s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int j = 0; j < KC; j++) {
-                const uint4 k = lds16(st + (t * KC + j) * 512);
-                mma(s[t], q[2 * j], k.x, k.y);
-                mma(s[t], q[2 * j + 1], k.z, k.w);
+            for (int i = 0; i < KM; i++) s[t][i][0] = s[t][i][1] = s[t][i][2] = s[t][i][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < KM; i++)
+#pragma unroll
+            for (int j = 0; j < KS; j++) {
+                uint32_t a[4];
+                tiles<false>(a, kst + i * 16 * PITCH + (kbits ^ 32 * j));
+#pragma unroll
+                for (int t = 0; t < NT; t++) mma_bf16(s[t][i], a, q[t][j][0], q[t][j][1]);
             }
-        }
-        if (EDGE) {
+        uint32_t hi[NT][KM][2], lo[KM][2];
 #pragma unroll
-            for (int t = 0; t < KT; t++)
+        for (int t = 0; t < NT; t++) {
+            float neg[2], alpha[2];
+            bool grows = false;
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (!(mask >> (t * 8 + 2 * c + (e & 1)) & 1)) s[t][e] = -INFINITY;
-        }
-        float neg[NR];
+            for (int e = 0; e < 2; e++) {
+                float mx = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < NR; r++) {
-            float mx = s[0][2 * r];
-#pragma unroll
-            for (int t = 0; t < KT; t++) mx = fmaxf(mx, fmaxf(s[t][2 * r], s[t][2 * r + 1]));
-            mx = fmaxf(m[r], quad_max(mx) * p.scale_log2);
-            neg[r] = mx == -INFINITY ? 0.f : -mx;
-            if (__any_sync(0xffffffffu, mx != m[r])) {
-                const float a = ex2(m[r] + neg[r]);
-                l[r] *= a;
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (!HI || e >> 1 == r) o[i][e] *= a;
-            }
-            m[r] = mx;
-        }
-#pragma unroll
-        for (int t = 0; t < KT; t++)
-#pragma unroll
-            for (int e = 0; e < 2 * NR; e++) {
-                s[t][e] = ex2(fmaf(s[t][e], p.scale_log2, neg[e >> 1]));
-                l[e >> 1] += s[t][e];
-            }
-#pragma unroll
-        for (int h = 0; h < KH; h++) {
-            uint32_t a[4];
-            if constexpr (HI) {
-                a[0] = pack_bf16(s[2 * h][0], s[2 * h][1]);
-                a[1] = pack_bf16(s[2 * h][2], s[2 * h][3]);
-                a[2] = pack_bf16(s[2 * h + 1][0], s[2 * h + 1][1]);
-                a[3] = pack_bf16(s[2 * h + 1][2], s[2 * h + 1][3]);
-            } else {
-                bf16_parts(s[2 * h][0], s[2 * h][1], a[0], a[1]);
-                bf16_parts(s[2 * h + 1][0], s[2 * h + 1][1], a[2], a[3]);
-            }
-            // a key with no row has probability 0, and values that may be NaN
-            auto there = [&](int i) { return !EDGE || (mask >> (h * 16 + (i >> 1) * 8 + 2 * c + (i & 1)) & 1); };
-#pragma unroll
-            for (int x = 0; x < B64; x++) {
-                uint32_t v[4][4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint4 y = lds16(st + OFF_V + ((h * 4 + i) * B64 + x) * 512);
-                    if (!there(i)) y = make_uint4(0, 0, 0, 0);
-                    v[i][0] = y.x; v[i][1] = y.y; v[i][2] = y.z; v[i][3] = y.w;
+                for (int i = 0; i < KM; i++) {
+                    if (EDGE) {
+                        if (!(mask >> (16 * i + g) & 1)) s[t][i][e] = -INFINITY;
+                        if (!(mask >> (16 * i + g + 8) & 1)) s[t][i][e + 2] = -INFINITY;
+                    }
+                    mx = fmaxf(mx, fmaxf(s[t][i][e], s[t][i][e + 2]));
                 }
+                mx = fmaxf(m[t][e], keys_max(mx) * p.scale_log2);
+                neg[e] = mx == -INFINITY ? 0.f : -mx;
+                grows |= mx != m[t][e];
+                alpha[e] = ex2(m[t][e] + neg[e]);
+                m[t][e] = mx;
+                l[t][e] *= alpha[e];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const uint32_t sel = i & 1 ? 0x7632 : 0x5410;
-                    mma_bf16(o[8 * x + i], a, prmt(v[0][i / 2], v[1][i / 2], sel), prmt(v[2][i / 2], v[3][i / 2], sel));
+                for (int i = 0; i < KM; i++) {
+                    s[t][i][e] = ex2(fmaf(s[t][i][e], p.scale_log2, neg[e]));
+                    s[t][i][e + 2] = ex2(fmaf(s[t][i][e + 2], p.scale_log2, neg[e]));
+                    l[t][e] += s[t][i][e] + s[t][i][e + 2];
                 }
             }
-            if constexpr (REM) {
-                uint32_t v[4][2];
+            if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint2 y = lds8(st - lane * 8 + OFF_W + (h * 4 + i) * 256);
-                    if (!there(i)) y = make_uint2(0, 0);
-                    v[i][0] = y.x; v[i][1] = y.y;
-                }
+                for (int j = 0; j < KS; j++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t sel = i & 1 ? 0x7632 : 0x5410;
-                    mma_bf16(o[8 * B64 + i], a, prmt(v[0][i / 2], v[1][i / 2], sel), prmt(v[2][i / 2], v[3][i / 2], sel));
-                }
+                    for (int e = 0; e < 4; e++) o[t][j][e] *= alpha[e & 1];
             }
+#pragma unroll
+            for (int i = 0; i < KM; i++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    if constexpr (NT == 1) {
+                        bf16_parts(s[t][i][2 * n], s[t][i][2 * n + 1], hi[t][i][n], lo[i][n]);
+                        lo[i][n] = transposed(lo[i][n]);
+                    } else {
+                        hi[t][i][n] = pack_bf16(s[t][i][2 * n], s[t][i][2 * n + 1]);
+                    }
+                    hi[t][i][n] = transposed(hi[t][i][n]);
+                }
         }
-    }
-    __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[2 * NR], uint32_t b0, uint32_t b1) {
-        const uint32_t x[4] = {a[0], HI ? a[NR - 1] : 0u, a[NR], HI ? a[2 * NR - 1] : 0u};
-        mma_bf16(d, x, b0, b1);
+#pragma unroll
+        for (int i = 0; i < KM; i++)
+#pragma unroll
+            for (int j = 0; j < KS; j++) {
+                uint32_t a[4];
+                tiles<true>(a, vst + i * 16 * PITCH + (vbits ^ 32 * j));
+                if (EDGE) {               // keys with no row have probability 0, and values that may be NaN
+#pragma unroll
+                    for (int n = 0; n < 4; n++) {
+                        const unsigned two = mask >> (16 * i + (n >> 1) * 8 + 2 * c) & 3;
+                        a[n] &= (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < NT; t++) mma_bf16(o[t][j], a, hi[t][i][0], hi[t][i][1]);
+                if constexpr (NT == 1) mma_bf16(o[0][j], a, lo[i][0], lo[i][1]);
+            }
     }
     __device__ __forceinline__ void finish(float *out, float2 *ml, int rows) {
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-        if constexpr (!HI) {
 #pragma unroll
-            for (int i = 0; i < NT; i++) { o[i][0] += o[i][2]; o[i][1] += o[i][3]; }
-        }
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int r = 0; r < NR; r++) {
-            const float sum = quad_sum(l[r]);
-            const int row = g + 8 * r;
-            if (row >= rows) continue;
-            if (c == 0) ml[row] = make_float2(m[r], sum);
+            for (int e = 0; e < 2; e++) {
+                const float sum = keys_sum(l[t][e]);
+                const int row = 8 * t + 2 * c + e;
+                if (row >= rows) continue;
+                if (g == 0) ml[row] = make_float2(m[t][e], sum);
 #pragma unroll
-            for (int n = 0; n < 2; n++) {        // columns 2c, 2c + 1 of every n-tile
-                float *at = out + row * D;
-#pragma unroll
-                for (int x = 0; x < B64; x++) {
-#pragma unroll
-                    for (int i = 0; i < 8; i += 4)
-                        *reinterpret_cast<float4 *>(at + 64 * x + 8 * (2 * c + n) + i) =
-                            make_float4(o[8 * x + i][2 * r + n], o[8 * x + i + 1][2 * r + n], o[8 * x + i + 2][2 * r + n],
-                                        o[8 * x + i + 3][2 * r + n]);
+                for (int j = 0; j < KS; j++) {
+                    out[row * D + 16 * j + g] = o[t][j][e];
+                    out[row * D + 16 * j + g + 8] = o[t][j][e + 2];
                 }
-                if constexpr (REM)
-                    *reinterpret_cast<float4 *>(at + 64 * B64 + 4 * (2 * c + n)) =
-                        make_float4(o[8 * B64][2 * r + n], o[8 * B64 + 1][2 * r + n], o[8 * B64 + 2][2 * r + n],
-                                    o[8 * B64 + 3][2 * r + n]);
             }
-        }
     }
 };
 
 // ---------------------------------------------------------------------------
-// INT8 codes: the same products in f16, in which a code is exact; 8 query rows.
+// INT8 codes, 4 NT query rows: the same products in f16, in which a code is
+// exact.
 //
-// A query and a weight go in as two f16 parts, high in MMA row g and the rest
-// in row g + 8, whose sums are added: 22 bits of each.  The query row is
-// first scaled by a power of two that puts its largest element in [2^7, 2^8),
-// the weights p * vscale by one, kept for the piece, that keeps them under 2,
+// A query and a weight p * vscale go in as two f16 parts, columns 2 r and
+// 2 r + 1 of the row's tile, whose results are added: 22 bits of each.  The
+// query row is first scaled by a power of two that puts its largest element in
+// [2^7, 2^8), the weights by one, kept for the piece, that keeps them under 2,
 // so the second parts stay above f16's smallest numbers.  A code c becomes f16
 // as the low byte of 1024 + (c + 128) minus 1152, all exact.  The tensor core
 // rounds its sums towards zero, which drifts over a long piece, so every
 // FOLD steps the output sums move to fp32 registers.
+//
+// A dot product may take its k positions in any order, and O^T its rows: lane
+// (g, c) reads 16 contiguous codes of a K row (four k-steps' fragments) and 8
+// dims of a V row, whose pairs of keys one byte permutation brings together.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t codes_f16(uint32_t biased, uint32_t sel) {   // two bytes of code + 128
     const uint32_t x = prmt(biased, 0x64646464u, sel);
@@ -305,174 +336,203 @@ __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) 
 // exponent of x > 0, within [-100, 100]
 __device__ __forceinline__ int exponent(float x) { return min(100, max(-100, (__float_as_int(x) >> 23 & 255) - 127)); }
 
-template <int D>
+template <int D, int NT>
 struct I8Path {
-    static constexpr int ROWS = 8, KEYS = 32, FOLD = 8;
-    static constexpr int KT = KEYS / 8, KH = KEYS / 16, B64 = D / 64, REM = D % 64 != 0;
-    static constexpr int KW = D / 16;                         // words of a K row per lane = k-steps
-    static constexpr int NT = D / 8;
-    static constexpr int OFF_KR = KT * B64 * 512, OFF_V = OFF_KR + REM * KT * 256, OFF_VR = OFF_V + KH * 4 * B64 * 256;
-    static constexpr int OFF_S = OFF_VR + REM * KH * 4 * 128, STAGE = OFF_S + 256;
-    uint32_t q[KW][4];
-    float o[NT][4], f[NT][2], m, l;
-    float qscale;                                             // scale log2(e) / the query's power of two
+    static constexpr int ROWS = 4 * NT, KEYS = 32, FOLD = 8;
+    static constexpr int KM = KEYS / 16, B64 = D / 64, REM = D % 64 != 0;
+    static constexpr int KW = D / 16;                         // words of a K row per lane = k-steps = 16-dim tiles
+    static constexpr int VP = v_pitch(D), OFF_V = KEYS * D, OFF_S = OFF_V + KEYS * VP, STAGE = OFF_S + 2 * 4 * KEYS;
+    static constexpr bool SWAP = D == 128;
+    uint32_t q[NT][KW][2];
+    float o[NT][KW][4], f[NT][KW][2], m[NT], l[NT];
+    float qscale[NT];                                         // scale log2(e) / the query row's power of two
     float wscale;                                             // the weights' power of two
-    int folded, hk_;
+    int folded, head;
     const char *kb, *vb;
 
     __device__ __forceinline__ void begin(const Params &p, int first_req, int row0, int rows, int hk) {
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-        const float *a = query<float>(p, first_req, row0 + min(g, rows - 1), hk, D);
-        float4 x[KW];
-        float amax = 0.f;
 #pragma unroll
-        for (int j = 0; j < KW; j++) {
-            // word j of this lane: 16 codes of each 64 dims, then 8 of the last 32
-            const int dim = j < 4 * B64 ? 64 * (j / 4) + 16 * c + 4 * (j % 4) : 64 * B64 + 8 * c + 4 * (j - 4 * B64);
-            x[j] = __ldg(reinterpret_cast<const float4 *>(a + dim));
-            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w))));
+        for (int t = 0; t < NT; t++) {
+            const float *a = query<float>(p, first_req, row0 + min(4 * t + (g >> 1), rows - 1), hk, D);
+            float4 x[KW];
+            float amax = 0.f;
+#pragma unroll
+            for (int j = 0; j < KW; j++) {
+                // word j of this lane: 16 codes of each 64 dims, then 8 of the last 32
+                const int dim = j < 4 * B64 ? 64 * (j / 4) + 16 * c + 4 * (j % 4) : 64 * B64 + 8 * c + 4 * (j - 4 * B64);
+                x[j] = __ldg(reinterpret_cast<const float4 *>(a + dim));
+                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w))));
+            }
+            amax = quad_max(amax);
+            const int e = amax > 0.f ? 7 - exponent(amax) : 0;
+            const float up = pow2i(e);
+            qscale[t] = __shfl_sync(0xffffffffu, p.scale_log2 * pow2i(-e), 8 * c);   // of row c
+#pragma unroll
+            for (int j = 0; j < KW; j++) {
+                uint32_t hi, lo;
+                f16_parts(x[j].x * up, x[j].y * up, hi, lo);
+                q[t][j][0] = g & 1 ? lo : hi;
+                f16_parts(x[j].z * up, x[j].w * up, hi, lo);
+                q[t][j][1] = g & 1 ? lo : hi;
+#pragma unroll
+                for (int n = 0; n < 4; n++) o[t][j][n] = 0.f;
+                f[t][j][0] = f[t][j][1] = 0.f;
+            }
+            m[t] = -INFINITY;
+            l[t] = 0.f;
         }
-        amax = quad_max(amax);
-        const int e = amax > 0.f ? 7 - exponent(amax) : 0;
-        const float up = pow2i(e);
-        qscale = p.scale_log2 * pow2i(-e);
-#pragma unroll
-        for (int j = 0; j < KW; j++) {
-            f16_parts(x[j].x * up, x[j].y * up, q[j][0], q[j][1]);
-            f16_parts(x[j].z * up, x[j].w * up, q[j][2], q[j][3]);
-        }
-#pragma unroll
-        for (int i = 0; i < NT; i++) {
-#pragma unroll
-            for (int n = 0; n < 4; n++) o[i][n] = 0.f;
-            f[i][0] = f[i][1] = 0.f;
-        }
-        m = -INFINITY;
-        l = 0.f;
         wscale = 0.f;
         folded = 0;
-        hk_ = hk;
+        head = hk;
         kb = static_cast<const char *>(p.k) + (long long)hk * D;
         vb = static_cast<const char *>(p.v) + (long long)hk * D;
     }
+    template <bool RUNS>
     __device__ __forceinline__ void issue(const Params &p, uint32_t st, int row) const {
-        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-        const long long at_scale = (long long)row * p.kv_heads + hk_;
-        copy_small<4>(st + OFF_S + lane * 4, p.kscale + at_scale);
-        copy_small<4>(st + OFF_S + 128 + lane * 4, p.vscale + at_scale);
-#pragma unroll
-        for (int t = 0; t < KT; t++) {
-            const char *at = kb + __shfl_sync(0xffffffffu, row, t * 8 + g) * p.row_stride;
-#pragma unroll
-            for (int x = 0; x < B64; x++) copy16(st + (t * B64 + x) * 512 + lane * 16, at + 64 * x + 16 * c);
-            if constexpr (REM) copy_small<8>(st + OFF_KR + t * 256 + lane * 8, at + 64 * B64 + 8 * c);
-        }
-#pragma unroll
-        for (int n = 0; n < 4 * KH; n++) {
-            const char *at = vb + __shfl_sync(0xffffffffu, row, (n >> 1) * 8 + 2 * c + (n & 1)) * p.row_stride;
-#pragma unroll
-            for (int x = 0; x < B64; x++) copy_small<8>(st + OFF_V + (n * B64 + x) * 256 + lane * 8, at + 64 * x + 8 * g);
-            if constexpr (REM) copy_small<4>(st + OFF_VR + n * 128 + lane * 4, at + 64 * B64 + 4 * g);
-        }
+        const int lane = threadIdx.x & 31;
+        const long long at_scale = (long long)row * p.kv_heads + head;
+        copy4(st + OFF_S + lane * 4, p.kscale + at_scale);
+        copy4(st + OFF_S + 128 + lane * 4, p.vscale + at_scale);
+        copy_rows<KEYS, D, D, SWAP ? HALVES : AS_IS, RUNS>(st, kb, p.row_stride, row);
+        copy_rows<KEYS, D, VP, SECTORS, RUNS>(st + OFF_V, vb, p.row_stride, row);
     }
     __device__ __forceinline__ void fold() {
 #pragma unroll
-        for (int i = 0; i < NT; i++)
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                f[i][n] += o[i][n] + o[i][n + 2];
-                o[i][n] = o[i][n + 2] = 0.f;
-            }
+            for (int j = 0; j < KW; j++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    f[t][j][n] += o[t][j][2 * n] + o[t][j][2 * n + 1];
+                    o[t][j][2 * n] = o[t][j][2 * n + 1] = 0.f;
+                }
         folded = 0;
     }
-    __device__ __forceinline__ void scale_output(float a) {
+    __device__ __forceinline__ void scale_output(int t, float a) {
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
+        for (int j = 0; j < KW; j++) {
 #pragma unroll
-            for (int n = 0; n < 4; n++) o[i][n] *= a;
-            f[i][0] *= a;
-            f[i][1] *= a;
+            for (int n = 0; n < 4; n++) o[t][j][n] *= a;
+            f[t][j][0] *= a;
+            f[t][j][1] *= a;
+        }
+    }
+    // Two 16-dim tiles from one word (4 dims) of each of the lane's keys 2c, 2c + 1, 2c + 8, 2c + 9.
+    __device__ __forceinline__ void values(int j, const uint32_t (&w)[NT][2], uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
+        const uint32_t a01 = prmt(v0, v1, 0x5140) ^ 0x80808080u, a23 = prmt(v0, v1, 0x7362) ^ 0x80808080u;
+        const uint32_t b01 = prmt(v2, v3, 0x5140) ^ 0x80808080u, b23 = prmt(v2, v3, 0x7362) ^ 0x80808080u;
+        const uint32_t x[4] = {codes_f16(a01, 0x4140), codes_f16(a01, 0x4342), codes_f16(b01, 0x4140), codes_f16(b01, 0x4342)};
+        const uint32_t y[4] = {codes_f16(a23, 0x4140), codes_f16(a23, 0x4342), codes_f16(b23, 0x4140), codes_f16(b23, 0x4342)};
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            mma_f16(o[t][j], x, w[t][0], w[t][1]);
+            mma_f16(o[t][j + 1], y, w[t][0], w[t][1]);
         }
     }
     template <bool EDGE>
     __device__ __forceinline__ void compute(const Params &, uint32_t st, unsigned mask) {
-        const int lane = threadIdx.x & 31, c = lane & 3;
-        const float my_ks = __uint_as_float(lds4(st + OFF_S + lane * 4)), my_vs = __uint_as_float(lds4(st + OFF_S + 128 + lane * 4));
-        float s[KT][4];
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        const uint32_t kst = st + g * D, swap = SWAP ? (g & 1) * 64 : 0, vst = st + OFF_V + 2 * c * VP;
+        const uint32_t v8 = 8 * g ^ c << 5, v4 = 4 * g ^ c << 5;
+        float s[NT][KM][4];
 #pragma unroll
-        for (int t = 0; t < KT; t++) {
-            s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-            uint32_t w[KW];
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int x = 0; x < B64; x++) {
-                const uint4 k = lds16(st + (t * B64 + x) * 512 + lane * 16);
-                w[4 * x] = k.x; w[4 * x + 1] = k.y; w[4 * x + 2] = k.z; w[4 * x + 3] = k.w;
-            }
-            if constexpr (REM) {
-                const uint2 k = lds8(st + OFF_KR + t * 256 + lane * 8);
-                w[4 * B64] = k.x; w[4 * B64 + 1] = k.y;
+            for (int i = 0; i < KM; i++) s[t][i][0] = s[t][i][1] = s[t][i][2] = s[t][i][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < KM; i++) {
+            uint32_t w[2][KW];                                // codes + 128 of keys g and g + 8
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const uint32_t at = kst + (16 * i + 8 * n) * D;
+#pragma unroll
+                for (int x = 0; x < B64; x++) {
+                    const uint4 k = lds16(at + 64 * x + 16 * c + (x & 1 ? -swap : swap));
+                    w[n][4 * x] = k.x; w[n][4 * x + 1] = k.y; w[n][4 * x + 2] = k.z; w[n][4 * x + 3] = k.w;
+                }
+                if constexpr (REM) {
+                    const uint2 k = lds8(at + 64 * B64 + 8 * c);
+                    w[n][4 * B64] = k.x; w[n][4 * B64 + 1] = k.y;
+                }
             }
 #pragma unroll
             for (int j = 0; j < KW; j++) {
-                w[j] ^= 0x80808080u;
-                mma_f16(s[t], q[j], codes_f16(w[j], 0x4140), codes_f16(w[j], 0x4342));
+                const uint32_t u = w[0][j] ^ 0x80808080u, v = w[1][j] ^ 0x80808080u;
+                const uint32_t a[4] = {codes_f16(u, 0x4140), codes_f16(v, 0x4140), codes_f16(u, 0x4342), codes_f16(v, 0x4342)};
+#pragma unroll
+                for (int t = 0; t < NT; t++) mma_f16(s[t][i], a, q[t][j][0], q[t][j][1]);
             }
         }
+        // scales of the lane's keys: g, g + 8 of each 16; absent keys' scales are not numbers to go by
+        float ks[KM][2], vs[KM][2], big = 0.f;
+#pragma unroll
+        for (int i = 0; i < KM; i++)
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const int key = 16 * i + 8 * n + g;
+                ks[i][n] = __uint_as_float(lds4(st + OFF_S + key * 4));
+                vs[i][n] = __uint_as_float(lds4(st + OFF_S + 128 + key * 4));
+                if (EDGE && !(mask >> key & 1)) vs[i][n] = 0.f;
+                big = fmaxf(big, fabsf(vs[i][n]));
+            }
         // weights' scale: the power of two over the largest vscale so far
-        const bool valid = !EDGE || (mask >> lane & 1);
-        const unsigned big = __reduce_max_sync(0xffffffffu, valid ? __float_as_uint(my_vs) & 0x7fffffffu : 0u);
-        if (big && (wscale == 0.f || __uint_as_float(big) * wscale >= 2.f)) {
-            const float now = pow2i(-exponent(__uint_as_float(big)));
-            if (wscale != 0.f) scale_output(now / wscale);
+        if (__any_sync(0xffffffffu, big > 0.f && (wscale == 0.f || big * wscale >= 2.f))) {
+            const float now = pow2i(-exponent(keys_max(big)));
+            if (wscale != 0.f) {
+#pragma unroll
+                for (int t = 0; t < NT; t++) scale_output(t, now / wscale);
+            }
             wscale = now;
         }
-        float mx = -INFINITY;
+        uint32_t pw[KM][NT][2];
 #pragma unroll
-        for (int t = 0; t < KT; t++)
+        for (int t = 0; t < NT; t++) {
+            float x[KM][2], mx = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const int key = t * 8 + 2 * c + n;
-                const float ks = __shfl_sync(0xffffffffu, my_ks, key);
-                s[t][n] = !EDGE || (mask >> key & 1) ? (s[t][n] + s[t][n + 2]) * qscale * ks : -INFINITY;
-                mx = fmaxf(mx, s[t][n]);
+            for (int i = 0; i < KM; i++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    x[i][n] = (s[t][i][2 * n] + s[t][i][2 * n + 1]) * qscale[t] * ks[i][n];
+                    if (EDGE && !(mask >> (16 * i + 8 * n + g) & 1)) x[i][n] = -INFINITY;
+                    mx = fmaxf(mx, x[i][n]);
+                }
+            mx = fmaxf(m[t], keys_max(mx));
+            const float neg = mx == -INFINITY ? 0.f : -mx;
+            if (__any_sync(0xffffffffu, mx != m[t])) {
+                const float a = ex2(m[t] + neg);
+                l[t] *= a;
+                scale_output(t, a);
             }
-        mx = fmaxf(m, quad_max(mx));
-        const float neg = mx == -INFINITY ? 0.f : -mx;
-        if (__any_sync(0xffffffffu, mx != m)) {
-            const float a = ex2(m + neg);
-            l *= a;
-            scale_output(a);
+            m[t] = mx;
+#pragma unroll
+            for (int i = 0; i < KM; i++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const float e = ex2(x[i][n] + neg), w = e * (vs[i][n] * wscale);
+                    l[t] += e;
+                    const __half hi = __float2half_rn(w);
+                    const __half2 both = __halves2half2(hi, __float2half_rn(w - __half2float(hi)));
+                    pw[i][t][n] = transposed(*reinterpret_cast<const uint32_t *>(&both));
+                }
         }
-        m = mx;
-        uint32_t hi[KT], lo[KT];
 #pragma unroll
-        for (int t = 0; t < KT; t++) {
-            float w[2];
+        for (int i = 0; i < KM; i++) {
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const int key = t * 8 + 2 * c + n;
-                const float e = ex2(s[t][n] + neg);
-                const float vs = __shfl_sync(0xffffffffu, my_vs, key);
-                l += e;
-                w[n] = !EDGE || (mask >> key & 1) ? e * vs * wscale : 0.f;
+            for (int x = 0; x < B64; x++) {
+                uint2 v[4];
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+                    v[n] = lds8(vst + (i * 16 + (n >> 1) * 8) * VP + v_at<VP>(n & 1, x & 1 ? v8 ^ 64 : v8, x / 2 * 128));
+                values(4 * x, pw[i], v[0].x, v[1].x, v[2].x, v[3].x);
+                values(4 * x + 2, pw[i], v[0].y, v[1].y, v[2].y, v[3].y);
             }
-            f16_parts(w[0], w[1], hi[t], lo[t]);
-        }
-#pragma unroll
-        for (int h = 0; h < KH; h++) {
-            const uint32_t a[4] = {hi[2 * h], lo[2 * h], hi[2 * h + 1], lo[2 * h + 1]};
-#pragma unroll
-            for (int x = 0; x < 2 * B64 + REM; x++) {         // 4 dims of each of the lane's keys
+            if constexpr (REM) {
                 uint32_t v[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[i] = lds4(x < 2 * B64 ? st + OFF_V + ((h * 4 + i) * B64 + x / 2) * 256 + lane * 8 + x % 2 * 4
-                                                                    : st + OFF_VR + (h * 4 + i) * 128 + lane * 4);
-                const uint32_t a01 = prmt(v[0], v[1], 0x5140) ^ 0x80808080u, a23 = prmt(v[0], v[1], 0x7362) ^ 0x80808080u;
-                const uint32_t b01 = prmt(v[2], v[3], 0x5140) ^ 0x80808080u, b23 = prmt(v[2], v[3], 0x7362) ^ 0x80808080u;
-                mma_f16(o[4 * x], a, codes_f16(a01, 0x4140), codes_f16(b01, 0x4140));
-                mma_f16(o[4 * x + 1], a, codes_f16(a01, 0x4342), codes_f16(b01, 0x4342));
-                mma_f16(o[4 * x + 2], a, codes_f16(a23, 0x4140), codes_f16(b23, 0x4140));
-                mma_f16(o[4 * x + 3], a, codes_f16(a23, 0x4342), codes_f16(b23, 0x4342));
+                for (int n = 0; n < 4; n++)
+                    v[n] = lds4(vst + (i * 16 + (n >> 1) * 8) * VP + v_at<VP>(n & 1, B64 ? v4 ^ 64 : v4, 0));
+                values(4 * B64, pw[i], v[0], v[1], v[2], v[3]);
             }
         }
         if (++folded == FOLD) fold();
@@ -480,24 +540,20 @@ struct I8Path {
     __device__ __forceinline__ void finish(float *out, float2 *ml, int rows) {
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
         fold();
-        const float sum = quad_sum(l);
-        if (g >= rows) return;
-        if (c == 0) ml[g] = make_float2(m, sum);
         const float down = wscale == 0.f ? 0.f : 1.f / wscale;
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-            float *at = out + g * D;
+        for (int t = 0; t < NT; t++) {
+            const float sum = keys_sum(l[t]);
+            const int row = 4 * t + c;
+            if (row >= rows) continue;
+            if (g == 0) ml[row] = make_float2(m[t], sum);
+            // tile j's rows g and g + 8 are dims 2j and 2j + 1 (of 8, or 4) of the lane's
 #pragma unroll
-            for (int x = 0; x < B64; x++)
-#pragma unroll
-                for (int i = 0; i < 8; i += 4)
-                    *reinterpret_cast<float4 *>(at + 64 * x + 8 * (2 * c + n) + i) =
-                        make_float4(f[8 * x + i][n] * down, f[8 * x + i + 1][n] * down, f[8 * x + i + 2][n] * down,
-                                    f[8 * x + i + 3][n] * down);
-            if constexpr (REM)
-                *reinterpret_cast<float4 *>(at + 64 * B64 + 4 * (2 * c + n)) =
-                    make_float4(f[8 * B64][n] * down, f[8 * B64 + 1][n] * down, f[8 * B64 + 2][n] * down,
-                                f[8 * B64 + 3][n] * down);
+            for (int j = 0; j < KW; j += 2) {
+                const int dim = j < 4 * B64 ? 64 * (j / 4) + 8 * g + 2 * (j % 4) : 64 * B64 + 4 * g;
+                *reinterpret_cast<float4 *>(out + row * D + dim) =
+                    make_float4(f[t][j][0] * down, f[t][j][1] * down, f[t][j + 1][0] * down, f[t][j + 1][1] * down);
+            }
         }
     }
 };
@@ -514,25 +570,24 @@ struct I8Path {
 template <int D, int R>
 struct F32Path {
     static constexpr int ROWS = R;
-    // q and o take 2 E R registers: 64 at most, 96 for 12 dims of 4 rows
-    static constexpr int LPK = R == 8 ? (D == 32 ? 8 : 16) : D <= 64 && R < 4 || D == 32 ? 4 : 8;
-    static constexpr int E = D / LPK, W = E % 4 ? 2 : 4, N = E / W;   // floats per lane, per copy, copies
+    // 8 or 16 lanes read 128 bytes of a row together; q and o take 2 E R registers, 64 to 96
+    static constexpr int LPK = R == 8 && D > 32 ? 16 : 8;
+    static constexpr int E = D / LPK, W = E % 4 ? 2 : 4, N = E / W;   // floats per lane, per read, reads
     static constexpr int G = 32 / LPK;                        // keys at a time
-    static constexpr int U = D == 32 ? 4 : 2;                    // keys of a group per step
-    static constexpr int KEYS = G * U, CHUNK = 32 * W * 4;
-    static constexpr int OFF_V = U * N * CHUNK, STAGE = 2 * OFF_V;
+    static constexpr int U = D == 128 ? 8 / G : D == 96 ? 8 / G : D == 64 ? 16 / G : 32 / G;   // keys of a group per step
+    static constexpr int KEYS = G * U, OFF_V = KEYS * D * 4, STAGE = 2 * OFF_V;
     static_assert(KEYS <= 32 && LPK * E == D && N * W == E, "lane geometry");
     uint64_t q[R][E / 2], o[R][E / 2];
     float m[R], l[R];
-    const float *kb, *vb;
+    const char *kb, *vb;
 
     __device__ __forceinline__ static void read(uint64_t (&x)[E / 2], uint32_t at) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
             if constexpr (W == 4)
-                asm volatile("ld.shared.v2.u64 {%0,%1}, [%2];" : "=l"(x[2 * i]), "=l"(x[2 * i + 1]) : "r"(at + i * CHUNK) : "memory");
+                asm volatile("ld.shared.v2.u64 {%0,%1}, [%2];" : "=l"(x[2 * i]), "=l"(x[2 * i + 1]) : "r"(at + i * LPK * 16) : "memory");
             else
-                asm volatile("ld.shared.u64 %0, [%1];" : "=l"(x[i]) : "r"(at + i * CHUNK) : "memory");
+                asm volatile("ld.shared.u64 %0, [%1];" : "=l"(x[i]) : "r"(at + i * LPK * 8) : "memory");
         }
     }
     __device__ __forceinline__ void begin(const Params &p, int first_req, int row0, int rows, int hk) {
@@ -550,37 +605,23 @@ struct F32Path {
             m[r] = -INFINITY;
             l[r] = 0.f;
         }
-        kb = static_cast<const float *>(p.k) + (long long)hk * D + sub * W;
-        vb = static_cast<const float *>(p.v) + (long long)hk * D + sub * W;
+        kb = static_cast<const char *>(p.k) + (long long)hk * D * 4;
+        vb = static_cast<const char *>(p.v) + (long long)hk * D * 4;
     }
+    template <bool RUNS>
     __device__ __forceinline__ void issue(const Params &p, uint32_t st, int row) const {
-        const int lane = threadIdx.x & 31, g = lane / LPK;
-        st += lane * W * 4;
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const long long at = __shfl_sync(0xffffffffu, row, u * G + g) * p.row_stride;
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const uint32_t to = st + (u * N + i) * CHUNK;
-                if constexpr (W == 4) {
-                    copy16(to, kb + at + i * LPK * W);
-                    copy16(to + OFF_V, vb + at + i * LPK * W);
-                } else {
-                    copy_small<8>(to, kb + at + i * LPK * W);
-                    copy_small<8>(to + OFF_V, vb + at + i * LPK * W);
-                }
-            }
-        }
+        copy_rows<KEYS, D * 4, D * 4, AS_IS, RUNS>(st, kb, p.row_stride * 4, row);
+        copy_rows<KEYS, D * 4, D * 4, AS_IS, RUNS>(st + OFF_V, vb, p.row_stride * 4, row);
     }
     template <bool EDGE>
     __device__ __forceinline__ void compute(const Params &, uint32_t st, unsigned mask) {
         const int lane = threadIdx.x & 31, g = lane / LPK;
-        st += lane * W * 4;
+        st += g * D * 4 + lane % LPK * W * 4;
         float x[R][U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             uint64_t k[E / 2];
-            read(k, st + u * N * CHUNK);
+            read(k, st + u * G * D * 4);
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 uint64_t a = 0ull;
@@ -622,7 +663,7 @@ struct F32Path {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             uint64_t v[E / 2];
-            read(v, st + OFF_V + u * N * CHUNK);
+            read(v, st + OFF_V + u * G * D * 4);
             if (EDGE && !(mask >> (u * G + g) & 1)) {       // probability 0, and values that may be NaN
 #pragma unroll
                 for (int i = 0; i < E / 2; i++) v[i] = 0ull;
