@@ -6,15 +6,16 @@
 // the keys gives triples (m, l, o) that join exactly: with M = max m_i,
 // l = sum l_i 2^(m_i - M) and o likewise.
 //
-// Work.  A "line" is one page-table line: a group's prefix, with the query
-// rows of all its requests, or a request's own rows, with its heads/kv_heads
-// query rows per key head.  A segment is a line x a block of query rows x a
-// block of key heads; its keys are counted in steps of KEYS.  All steps of all
-// segments, in order, are cut into equal ranges, one per team of warps, so no
-// length decides how busy an SM is; a team's warps take one key head each and
-// read adjacent parts of the same cache rows.  What a warp leaves of a segment
-// (its piece) goes to the workspace, at slot segment + team, and
-// prefix_merge_kernel joins the pieces of each query row.
+// Work.  There are two parts with a launch each: the groups' prefixes, with the
+// query rows of all their requests, and the requests' own rows, with
+// heads/kv_heads query rows per key head.  A "line" is one page-table line of
+// a part; a segment is a line x a block of query rows x a block of key heads,
+// its keys counted in steps of KEYS.  All steps of a part, in order, are cut
+// into equal ranges, one per team of warps, so no length decides how busy an
+// SM is; a team's warps take one key head each and read adjacent parts of the
+// same cache rows.  What a warp leaves of a segment (its piece) goes to the
+// workspace, at slot segment + team, and prefix_merge_kernel joins the pieces
+// of each query row.
 //
 // Bound: HBM (the cache rows, once).  Little else may cost: each warp
 // copies its rows through a ring of its own in shared memory, from which the
@@ -28,60 +29,70 @@
 namespace attn {
 namespace prefix {
 
-constexpr int kEntries = 2048;            // running sums of steps kept per CTA
+constexpr int kEntries = 512;             // running sums of steps kept per CTA
 constexpr int kWarps = 8;
+constexpr int kBegin = 1;                 // steps that the beginning and end of a segment count for
 
-struct Work {
-    float *own_o, *pre_o;                 // pieces: [slot][heads of the block][rows][D]
-    float2 *own_ml, *pre_ml;              //         [slot][heads of the block][rows] (m in base 2, l)
+// One part of the work.
+struct Part {
+    float *o;                             // pieces: [slot][heads of the block][rows][D]
+    float2 *ml;                           //         [slot][heads of the block][rows] (m in base 2, l)
     long long *line_first;                // first step of each line, and the total
     int lines, per_entry;                 // lines, lines per entry of the running sums
-    int pre_lines;                        // prefix lines this kernel takes (0 or n_groups)
-    int head_block, n_blocks;             // key heads per team, teams' blocks
-    int splits;                           // teams per CTA
-    int own_blocks;                       // blocks of query rows of an own line
-    int own_rows, pre_rows;               // rows of a slot
-    int own_seg_rows, pre_seg_rows;       // rows of a block
+    int head_block, n_blocks;             // key heads per team, their blocks
+    int splits, teams;                    // teams per CTA, in all
+    int blocks;                           // blocks of query rows of an own line
+    int seg_rows, rows;                   // query rows of a block, of a slot
+    int keys;                             // KEYS
 };
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Blocks of query rows of a group, and the index of its first one: an
+// Query rows of a group and their blocks, and the index of the first block: an
 // ascending numbering without a sum over the groups before.
-__device__ __forceinline__ void group_blocks(const Params &p, const Work &w, int g, int &first_req, int &rows,
+__device__ __forceinline__ void group_blocks(const Params &p, const Part &w, int g, int &first_req, int &rows,
                                              int &blocks, int &base) {
     first_req = group_first(p, g);
     rows = max(group_first(p, g + 1) - first_req, 0) * p.ratio;
-    blocks = ceil_div(rows, w.pre_seg_rows);
-    base = first_req * p.ratio / w.pre_seg_rows + g;
+    blocks = ceil_div(rows, w.seg_rows);
+    base = first_req * p.ratio / w.seg_rows + g;
 }
 
 struct Line {
     int keys, steps, blocks;              // blocks of query rows
-    __device__ long long total(const Work &w) const { return (long long)steps * blocks * w.n_blocks; }
+    int first_req, rows, base;            // of the line's query rows; index of its first block
+    // cost of a segment, and of the line, in steps
+    __device__ int cost() const { return steps + kBegin; }
+    __device__ long long total(const Part &w) const { return steps ? (long long)cost() * blocks * w.n_blocks : 0; }
 };
-template <int OWN_KEYS, int PRE_KEYS>
-__device__ __forceinline__ Line line_of(const Params &p, const Work &w, int i) {
+template <bool PRE>
+__device__ __forceinline__ Line line_of(const Params &p, const Part &w, int i) {
     Line l;
-    if (i < w.pre_lines) {
-        int first, rows, base;
-        group_blocks(p, w, i, first, rows, l.blocks, base);
-        l.keys = rows ? prefix_len(p, i) : 0;
-        l.steps = ceil_div(l.keys, PRE_KEYS);
+    if (PRE) {
+        group_blocks(p, w, i, l.first_req, l.rows, l.blocks, l.base);
+        l.keys = l.rows ? prefix_len(p, i) : 0;
     } else {
-        l.keys = own_len(p, i - w.pre_lines);
-        l.blocks = w.own_blocks;
-        l.steps = ceil_div(l.keys, OWN_KEYS);
+        l.first_req = i;
+        l.rows = p.ratio;
+        l.blocks = w.blocks;
+        l.base = i * w.blocks;
+        l.keys = own_len(p, i);
     }
+    l.steps = ceil_div(l.keys, w.keys);
     return l;
 }
 
 // One warp's piece: steps [a, b) of a line for the query rows of one block and
-// one key head.
-template <class Path, int STAGES>
+// one key head.  The ring holds SLOTS halves of steps (K, V, K, ...): AHEAD
+// whole steps are in flight beside the half at work.
+template <class Path, int SLOTS>
 __device__ __forceinline__ void run_piece(const Params &p, uint32_t ring, const int *table, int keys, int a, int b,
                                           int first_req, int row0, int rows, int hk, float *o, float2 *ml) {
+    static_assert(SLOTS % 2 == 1 && SLOTS >= 3, "ring");
+    constexpr int AHEAD = SLOTS / 2;
+    constexpr unsigned all = Path::KEYS == 32 ? 0xffffffffu : (1u << (Path::KEYS & 31)) - 1;
     const int lane = threadIdx.x & 31;
+    const bool runs = p.log_page >= 4;
     Path path;
     // Cache row of this lane's key of a step: bad pages and keys past the line
     // have no valid row.  In pages of 16 rows or more, a run of 16 keys is
@@ -97,57 +108,80 @@ __device__ __forceinline__ void run_piece(const Params &p, uint32_t ring, const 
         }
         return row;
     };
-    unsigned masks[STAGES];               // keys with a row, of the steps in flight
     bool next_valid;
-    int next_row = row_of(a, next_valid);
+    int next_row = row_of(a, next_valid), row = 0;
     path.begin(p, first_req, row0, rows, hk);
-    auto issue = [&](int step, int stage) {
-        masks[stage] = __ballot_sync(0xffffffffu, next_valid);
+    unsigned masks[AHEAD + 1];            // keys with a row, of this step and the ones in flight
+    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+    auto copy_k = [&](int step, int slot) {
+        row = next_row;
         if (step < b) {
-            if (p.log_page >= 4) path.template issue<true>(p, ring + stage * Path::STAGE, next_row);
-            else path.template issue<false>(p, ring + stage * Path::STAGE, next_row);
+            if (runs) path.template copy_k<true>(p, ring + slot * Path::SLOT, row);
+            else path.template copy_k<false>(p, ring + slot * Path::SLOT, row);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        commit();
+        const unsigned mask = __ballot_sync(0xffffffffu, next_valid);
         next_row = row_of(step + 1, next_valid);
+        return mask;
+    };
+    auto copy_v = [&](int step, int slot) {
+        if (step < b) {
+            if (runs) path.template copy_v<true>(p, ring + slot * Path::SLOT, row);
+            else path.template copy_v<false>(p, ring + slot * Path::SLOT, row);
+        }
+        commit();
+    };
+    auto wait = [] {
+        asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 1) : "memory");
+        __syncwarp();                     // every lane's copies of the half are there
     };
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; i++) issue(a + i, i);
-    constexpr unsigned all = Path::KEYS == 32 ? 0xffffffffu : (1u << (Path::KEYS & 31)) - 1;
-    for (int step = a; step < b; step += STAGES) {
+    for (int i = 0; i < AHEAD; i++) {
+        masks[i] = copy_k(a + i, 2 * i);
+        copy_v(a + i, 2 * i + 1);
+    }
+    int at = 0;                           // slot of this step's K
+    for (int step = a; step < b; step++) {
+        const int after = at + 1 == SLOTS ? 0 : at + 1, before = at ? at - 1 : SLOTS - 1;
+        masks[AHEAD] = copy_k(step + AHEAD, before);
+        wait();
+        if (masks[0] == all) path.template scores<false>(p, ring + at * Path::SLOT, all);
+        else path.template scores<true>(p, ring + at * Path::SLOT, masks[0]);
+        __syncwarp();                     // K's slot may be copied over
+        copy_v(step + AHEAD, at);
+        wait();
+        if (masks[0] == all) path.template values<false>(p, ring + after * Path::SLOT, all);
+        else path.template values<true>(p, ring + after * Path::SLOT, masks[0]);
+        __syncwarp();
 #pragma unroll
-        for (int u = 0; u < STAGES; u++) {
-            if (step + u < b) {
-                issue(step + u + STAGES - 1, (u + STAGES - 1) % STAGES);
-                asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-                __syncwarp();             // every lane's copies of the stage are there
-                const uint32_t st = ring + u * Path::STAGE;
-                if (masks[u] == all) path.template compute<false>(p, st, all);
-                else path.template compute<true>(p, st, masks[u]);
-                __syncwarp();             // the stage may be copied over
-            }
-        }
+        for (int i = 0; i < AHEAD; i++) masks[i] = masks[i + 1];
+        at = after + 1 == SLOTS ? 0 : after + 1;
     }
     path.finish(o, ml, rows);
 }
 
-// Stages of a warp's ring: as many as fit a CTA's shared memory, up to 6.
-template <class Own, class Pre> struct Ring {
-    static constexpr int STAGE = Own::STAGE > Pre::STAGE ? Own::STAGE : Pre::STAGE;
-    static constexpr int FIT = (208 * 1024 / kWarps) / STAGE;
-    static constexpr int STAGES = FIT > 4 ? 4 : FIT;
-    static constexpr int BYTES = STAGES * STAGE;
-    static_assert(STAGES >= 2 && Own::STAGE % 128 == 0 && Pre::STAGE % 128 == 0, "ring");
+// Slots of a warp's ring: as many (an odd number) as CTAS rings of kWarps fit an SM, up to 7.
+template <class Path, int CTAS> struct Ring {
+    static constexpr int FIT = (CTAS == 1 ? 216 : 108) * 1024 / kWarps / Path::SLOT;
+    static constexpr int SLOTS = FIT > 7 ? 7 : (FIT - 1) / 2 * 2 + 1;
+    static constexpr int BYTES = SLOTS * Path::SLOT;
+    static_assert(Path::SLOT % 128 == 0, "swizzled rows begin on 128 bytes");
 };
 
-template <class Own, class Pre, int D>
-__global__ void __launch_bounds__(kWarps * 32, 1)
-prefix_rows_kernel(const __grid_constant__ Params p, const __grid_constant__ Work w)
+// PRE: the groups' prefixes; otherwise the requests' own rows.  `second`: the
+// launch before this one is the prefix part's, which has waited for the work
+// before it when this one may start; the two run side by side, and this one
+// ends after both.
+template <class Path, bool PRE, int D, int CTAS>
+__global__ void __launch_bounds__(kWarps * 32, CTAS)
+prefix_rows_kernel(const __grid_constant__ Params p, const __grid_constant__ Part w, int second)
 {
-    using R = Ring<Own, Pre>;
+    using R = Ring<Path, CTAS>;
     extern __shared__ __align__(128) uint8_t ring_bytes[];
     __shared__ long long sums[kEntries + 1];
     __shared__ long long warp_sums[kWarps];
-    pdl_begin();                          // launched by launch_pdl
+    if (!second) asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // running sums of the steps, per entry of w.per_entry lines
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -158,7 +192,7 @@ prefix_rows_kernel(const __grid_constant__ Params p, const __grid_constant__ Wor
         long long v = 0;
         if (e < entries)
             for (int i = e * w.per_entry; i < min((e + 1) * w.per_entry, w.lines); i++)
-                v += line_of<Own::KEYS, Pre::KEYS>(p, w, i).total(w);
+                v += line_of<PRE>(p, w, i).total(w);
         long long s = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -183,62 +217,54 @@ prefix_rows_kernel(const __grid_constant__ Params p, const __grid_constant__ Wor
             long long at = sums[e];
             for (int i = e * w.per_entry; i < min((e + 1) * w.per_entry, w.lines); i++) {
                 w.line_first[i] = at;
-                at += line_of<Own::KEYS, Pre::KEYS>(p, w, i).total(w);
+                at += line_of<PRE>(p, w, i).total(w);
             }
         }
         if (threadIdx.x == 0) w.line_first[w.lines] = total;
     }
 
-    // this team's range
+    // This team's range.  No more teams than steps, so that none between a
+    // segment's first and last is without a piece.
     const uint32_t ring = sm100::smem_u32(ring_bytes) + warp * R::BYTES;
     const int team_warp = warp % w.head_block, split = warp / w.head_block;
-    // no more teams than steps, so that none between a segment's first and last is without a piece
-    const int teams = (int)min((long long)gridDim.x * w.splits, total), team = split * (int)gridDim.x + (int)blockIdx.x;
-    if (split >= w.splits || team >= teams) return;
-    const long long first = total * team / teams, last = total * (team + 1) / teams;
-    int e;
-    {
-        int lo = 0, hi = entries;         // the last entry that begins at or before `first`
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (sums[mid] <= first) lo = mid;
-            else hi = mid;
+    const int teams = (int)min((long long)w.teams, total), team = split * (int)gridDim.x + (int)blockIdx.x;
+    if (team < teams) {
+        const long long first = total * team / teams, last = total * (team + 1) / teams;
+        int e;
+        {
+            int lo = 0, hi = entries;     // the last entry that begins at or before `first`
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (sums[mid] <= first) lo = mid;
+                else hi = mid;
+            }
+            e = lo;
         }
-        e = lo;
-    }
-    long long at = sums[e];
-    for (int i = e * w.per_entry; i < w.lines && at < last; i++) {
-        const Line l = line_of<Own::KEYS, Pre::KEYS>(p, w, i);
-        const long long n = l.total(w);
-        if (at + n > first && n > 0) {
-            // segments of the line that the range meets
-            const int s0 = (int)((max(first, at) - at) / l.steps), s1 = (int)((min(last, at + n) - 1 - at) / l.steps);
-            for (int s = s0; s <= s1; s++) {
-                const long long begin = at + (long long)s * l.steps;
-                const int a = (int)(max(first, begin) - begin), b = (int)(min(last, begin + l.steps) - begin);
-                const int rb = s / w.n_blocks, hb = s - rb * w.n_blocks;
-                const int hk = hb * w.head_block + team_warp;
-                if (hk >= p.kv_heads) continue;
-                if (i < w.pre_lines) {
-                    int req, rows, blocks, base;
-                    group_blocks(p, w, i, req, rows, blocks, base);
-                    const long long slot =
-                        ((long long)(base + rb) * w.n_blocks + hb + team) * w.head_block + team_warp;
-                    run_piece<Pre, R::STAGES>(p, ring, p.prefix_table + (long long)i * p.max_prefix_pages, l.keys, a, b, req,
-                                   rb * w.pre_seg_rows, min(rows - rb * w.pre_seg_rows, w.pre_seg_rows), hk,
-                                   w.pre_o + slot * w.pre_rows * D, w.pre_ml + slot * w.pre_rows);
-                } else {
-                    const int req = i - w.pre_lines;
-                    const long long slot =
-                        (((long long)req * w.own_blocks + rb) * w.n_blocks + hb + team) * w.head_block + team_warp;
-                    run_piece<Own, R::STAGES>(p, ring, p.block_table + (long long)req * p.max_pages, l.keys, a, b, req,
-                                   rb * w.own_seg_rows, min(p.ratio - rb * w.own_seg_rows, w.own_seg_rows), hk,
-                                   w.own_o + slot * w.own_rows * D, w.own_ml + slot * w.own_rows);
+        long long at = sums[e];
+        for (int i = e * w.per_entry; i < w.lines && at < last; i++) {
+            const Line l = line_of<PRE>(p, w, i);
+            const long long n = l.total(w);
+            if (at + n > first && n > 0) {
+                // segments of the line that the range meets
+                const int s0 = (int)((max(first, at) - at) / l.cost()), s1 = (int)((min(last, at + n) - 1 - at) / l.cost());
+                for (int s = s0; s <= s1; s++) {
+                    const long long begin = at + (long long)s * l.cost() + kBegin;
+                    const int a = (int)(max(first, begin) - begin), b = (int)(min(last, begin + l.steps) - begin);
+                    const int rb = s / w.n_blocks, hb = s - rb * w.n_blocks;
+                    const int hk = hb * w.head_block + team_warp;
+                    if (a >= b || hk >= p.kv_heads) continue;
+                    const long long slot = ((long long)(l.base + rb) * w.n_blocks + hb + team) * w.head_block + team_warp;
+                    const int *table = PRE ? p.prefix_table + (long long)i * p.max_prefix_pages
+                                           : p.block_table + (long long)i * p.max_pages;
+                    run_piece<Path, R::SLOTS>(p, ring, table, l.keys, a, b, l.first_req, rb * w.seg_rows,
+                                              min(l.rows - rb * w.seg_rows, w.seg_rows), hk,
+                                              w.o + slot * w.rows * D, w.ml + slot * w.rows);
                 }
             }
+            at += n;
         }
-        at += n;
     }
+    if (second) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Joins the pieces of one query row: a CTA per (request, query head), its
@@ -251,46 +277,40 @@ struct Pieces {
 };
 constexpr int kMergeWarps = 4;
 
+template <int D>
+__device__ __forceinline__ Pieces pieces_of(const Part &w, const Line &l, int line, int row, int hk) {
+    Pieces r = {};
+    if (l.steps == 0) return r;
+    const int rb = row / w.seg_rows, hb = hk / w.head_block, hw = hk - hb * w.head_block;
+    const long long total = w.line_first[w.lines], teams = min((long long)w.teams, total);
+    const long long begin = w.line_first[line] + (long long)(rb * w.n_blocks + hb) * l.cost() + kBegin;
+    // the team whose range [total t / teams, total (t + 1) / teams) holds a step
+    const int t0 = (int)(((begin + 1) * teams - 1) / total), t1 = (int)(((begin + l.steps) * teams - 1) / total);
+    const long long seg = (long long)(l.base + rb) * w.n_blocks + hb;
+    const long long slot = ((seg + t0) * w.head_block + hw) * w.rows + row - rb * w.seg_rows;
+    r.o = w.o + slot * D;
+    r.ml = w.ml + slot;
+    r.step = (long long)w.head_block * w.rows;
+    r.n = t1 - t0 + 1;
+    return r;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kMergeWarps * 32)
-prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Work w, int all_teams, int own_keys, int pre_keys)
+prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Part own, const __grid_constant__ Part pre)
 {
     pdl_begin();                          // launched by launch_pdl
     constexpr int E = D / 32;
     __shared__ float s_m[kMergeWarps], s_l[kMergeWarps], s_o[kMergeWarps][D];
     const int s = blockIdx.y, h = blockIdx.x, hk = h / p.ratio, hr = h - hk * p.ratio;
-    const int hb = hk / w.head_block, hw = hk - hb * w.head_block;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long total = w.line_first[w.lines];
-    const long long teams = min((long long)all_teams, total);
-    // the team whose range [total t / teams, total (t + 1) / teams) holds a step
-    auto team_of = [&](long long step) { return (int)(((step + 1) * teams - 1) / total); };
-    auto find = [&](int line, int seg_in_line, long long seg, int keys, int keys_per_step, int rows, int row,
-                    const float *o, const float2 *ml) {
-        Pieces r = {};
-        const int steps = ceil_div(keys, keys_per_step);
-        if (steps == 0) return r;
-        const long long begin = w.line_first[line] + (long long)seg_in_line * steps;
-        const int t0 = team_of(begin), t1 = team_of(begin + steps - 1);
-        const long long slot = ((seg + t0) * w.head_block + hw) * rows + row;
-        r.o = o + slot * D;
-        r.ml = ml + slot;
-        r.step = (long long)w.head_block * rows;
-        r.n = t1 - t0 + 1;
-        return r;
-    };
-    const int rb = hr / w.own_seg_rows;
     Pieces part[2];
-    part[0] = find(w.pre_lines + s, rb * w.n_blocks + hb, ((long long)s * w.own_blocks + rb) * w.n_blocks + hb,
-                   own_len(p, s), own_keys, w.own_rows, hr - rb * w.own_seg_rows, w.own_o, w.own_ml);
+    part[0] = own.lines ? pieces_of<D>(own, line_of<false>(p, own, s), s, hr, hk) : Pieces{};
     part[1] = Pieces{};
-    for (int g = 0; g < w.pre_lines; g++) {
-        int req, rows, blocks, base;
-        group_blocks(p, w, g, req, rows, blocks, base);
-        if (s < req || (s - req) * p.ratio >= rows) continue;
-        const int row = (s - req) * p.ratio + hr, b = row / w.pre_seg_rows;
-        part[1] = find(g, b * w.n_blocks + hb, (long long)(base + b) * w.n_blocks + hb, prefix_len(p, g), pre_keys,
-                       w.pre_rows, row - b * w.pre_seg_rows, w.pre_o, w.pre_ml);
+    for (int g = 0; g < pre.lines; g++) {
+        const Line l = line_of<true>(p, pre, g);
+        if (s < l.first_req || (s - l.first_req) * p.ratio >= l.rows) continue;
+        part[1] = pieces_of<D>(pre, l, g, (s - l.first_req) * p.ratio + hr, hk);
         break;
     }
     float m = -INFINITY, l = 0.f, o[E];
@@ -346,64 +366,69 @@ bool ensure_smem_attr(const void *func, size_t bytes);
 
 namespace {
 
+// The parts of a call on the workspace `base` (NULL to learn its size).
 struct Layout {
-    attn::prefix::Work w;
-    int grid_ctas;
+    attn::prefix::Part own, pre;
     size_t bytes;
 };
 
-// The workspace of a call, on `base` (NULL to learn its size).
-Layout lay_out(int n_seq, int n_groups, int ratio, int kv_heads, int d, int own_seg_rows, int pre_seg_rows, int ctas,
-               char *base) {
+Layout lay_out(const attn::prefix::Params &p, int d, int own_rows, int own_keys, int own_ctas, int pre_rows, int pre_keys,
+               int pre_ctas, char *base) {
     using namespace attn::prefix;
     Layout r = {};
-    Work &w = r.w;
-    w.pre_lines = n_groups;
-    w.lines = n_groups + n_seq;
-    w.per_entry = std::max(1, (w.lines + kEntries - 1) / kEntries);
-    w.n_blocks = (kv_heads + kWarps - 1) / kWarps;
-    w.head_block = (kv_heads + w.n_blocks - 1) / w.n_blocks;
-    w.splits = kWarps / w.head_block;
-    w.own_seg_rows = own_seg_rows;
-    w.pre_seg_rows = pre_seg_rows;
-    w.own_blocks = (ratio + own_seg_rows - 1) / own_seg_rows;
-    w.own_rows = std::min(ratio, own_seg_rows);
-    w.pre_rows = (int)std::min<long long>((long long)n_seq * ratio, pre_seg_rows);
-    r.grid_ctas = ctas;
-    const long long teams = (long long)ctas * w.splits;
-    const long long own_slots = ((long long)n_seq * w.own_blocks * w.n_blocks + teams) * w.head_block * w.own_rows;
-    const long long pre_segs = n_groups ? (long long)n_seq * ratio / pre_seg_rows + n_groups : 0;
-    const long long pre_slots = n_groups ? (pre_segs * w.n_blocks + teams) * w.head_block * w.pre_rows : 0;
     size_t off = 0;
     auto take = [&](size_t bytes) {
         char *at = base ? base + off : nullptr;
         off += (bytes + 255) / 256 * 256;
         return at;
     };
-    w.line_first = reinterpret_cast<long long *>(take(((size_t)w.lines + 1) * 8));
-    w.own_ml = reinterpret_cast<float2 *>(take((size_t)own_slots * 8));
-    w.pre_ml = reinterpret_cast<float2 *>(take((size_t)pre_slots * 8));
-    w.own_o = reinterpret_cast<float *>(take((size_t)own_slots * d * 4));
-    w.pre_o = reinterpret_cast<float *>(take((size_t)pre_slots * d * 4));
-    r.bytes = off;
+    auto part = [&](Part &w, int lines, int seg_rows, int keys, int ctas, bool pre) {
+        if (!lines) return;
+        w.lines = lines;
+        w.per_entry = (lines + kEntries - 1) / kEntries;
+        w.n_blocks = (p.kv_heads + kWarps - 1) / kWarps;
+        w.head_block = (p.kv_heads + w.n_blocks - 1) / w.n_blocks;
+        w.splits = kWarps / w.head_block;
+        w.teams = sm_count_here() * ctas * w.splits;
+        w.seg_rows = seg_rows;
+        w.keys = keys;
+        w.blocks = (p.ratio + seg_rows - 1) / seg_rows;
+        const long long all_rows = (long long)p.n_seq * p.ratio;
+        w.rows = (int)std::min<long long>(pre ? all_rows : p.ratio, seg_rows);
+        const long long blocks = pre ? all_rows / seg_rows + lines : (long long)lines * w.blocks;
+        const size_t slots = (size_t)(blocks * w.n_blocks + w.teams) * w.head_block * w.rows;
+        w.line_first = reinterpret_cast<long long *>(take(((size_t)lines + 1) * 8));
+        w.ml = reinterpret_cast<float2 *>(take(slots * 8));
+        w.o = reinterpret_cast<float *>(take(slots * d * 4));
+    };
+    part(r.own, p.max_len ? p.n_seq : 0, own_rows, own_keys, own_ctas, false);
+    part(r.pre, p.max_prefix_len ? p.n_groups : 0, pre_rows, pre_keys, pre_ctas, true);
+    r.bytes = std::max<size_t>(off, 256);
     return r;
+}
+
+template <class Path, bool PRE, int D, int CTAS>
+int run_part(const attn::prefix::Params &p, const attn::prefix::Part &w, int second, cudaStream_t s) {
+    using namespace attn::prefix;
+    using R = Ring<Path, CTAS>;
+    const auto kernel = prefix_rows_kernel<Path, PRE, D, CTAS>;
+    const int warps = w.splits * w.head_block;
+    if (!ensure_smem_attr((const void *)kernel, (size_t)R::BYTES * kWarps))
+        return set_error(ATTN_ERR_CUDA, "prefix decode: cannot set shared-memory size");
+    return check_pdl(launch_pdl(kernel, dim3(w.teams / w.splits), dim3(warps * 32), (size_t)R::BYTES * warps, s, p, w, second),
+                     "prefix_rows_kernel");
 }
 
 template <class Own, class Pre, typename T, int D>
 int run(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s) {
     using namespace attn::prefix;
-    const Layout L = lay_out(p.n_seq, p.n_groups, p.ratio, p.kv_heads, D, Own::ROWS, Pre::ROWS,
-                             sm_count_here(), static_cast<char *>(ws));
+    constexpr int OWN_CTAS = Own::LEAN ? 2 : 1, PRE_CTAS = 1;
+    const Layout L = lay_out(p, D, Own::ROWS, Own::KEYS, OWN_CTAS, Pre::ROWS, Pre::KEYS, PRE_CTAS, static_cast<char *>(ws));
     if (need) { *need = L.bytes; return ATTN_OK; }
-    const int warps = L.w.splits * L.w.head_block;
-    const size_t smem = (size_t)Ring<Own, Pre>::BYTES * warps;
-    if (!ensure_smem_attr((const void *)prefix_rows_kernel<Own, Pre, D>, (size_t)Ring<Own, Pre>::BYTES * kWarps))
-        return set_error(ATTN_ERR_CUDA, "prefix decode: cannot set shared-memory size");
-    int st = check_pdl(launch_pdl(prefix_rows_kernel<Own, Pre, D>, dim3(L.grid_ctas), dim3(warps * 32), smem, s, p, L.w),
-                       "prefix_rows_kernel");
-    if (st) return st;
-    return check_pdl(launch_pdl(prefix_merge_kernel<T, D>, dim3(p.heads, p.n_seq), dim3(kMergeWarps * 32), 0, s, p, L.w,
-                                L.grid_ctas * L.w.splits, (int)Own::KEYS, (int)Pre::KEYS),
+    int st;
+    if (L.pre.lines && (st = run_part<Pre, true, D, PRE_CTAS>(p, L.pre, 0, s))) return st;
+    if (L.own.lines && (st = run_part<Own, false, D, OWN_CTAS>(p, L.own, L.pre.lines != 0, s))) return st;
+    return check_pdl(launch_pdl(prefix_merge_kernel<T, D>, dim3(p.heads, p.n_seq), dim3(kMergeWarps * 32), 0, s, p, L.own, L.pre),
                      "prefix_merge_kernel");
 }
 
@@ -423,7 +448,7 @@ int run_d(const attn::prefix::Params &p, int kv_dtype, void *ws, size_t *need, c
         return p.ratio <= 4 ? run<I8Path<D, 1>, I8Path<D, N>, float, D>(p, ws, need, s)
                             : run<I8Path<D, 2>, I8Path<D, N>, float, D>(p, ws, need, s);
     }
-    // own rows with the request's query rows, up to 8 at a time; prefixes with 8
+    // fp32: FMAs grow with the rows, so own rows take the request's, up to 8
     if (p.ratio == 1) return run<F32Path<D, 1>, F32Path<D, 8>, float, D>(p, ws, need, s);
     if (p.ratio == 2) return run<F32Path<D, 2>, F32Path<D, 8>, float, D>(p, ws, need, s);
     if (p.ratio <= 4) return run<F32Path<D, 4>, F32Path<D, 8>, float, D>(p, ws, need, s);
@@ -445,6 +470,7 @@ size_t prefix_decode_workspace(const attn_prefix_shape *s, int kv_dtype) {
     attn::prefix::Params p = {};
     p.n_seq = s->n_seq; p.n_groups = s->n_groups; p.heads = s->heads; p.kv_heads = s->kv_heads;
     p.ratio = s->heads / s->kv_heads;
+    p.max_len = s->max_len; p.max_prefix_len = s->max_prefix_len;
     size_t need = 0;
     run_any(p, s->head_dim, kv_dtype, nullptr, &need, nullptr);
     return need;

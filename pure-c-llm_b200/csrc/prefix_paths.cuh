@@ -2,8 +2,9 @@
 // head, for bf16, INT8 and fp32 caches (prefix_decode.cu runs them).
 //
 // A path holds up to ROWS query rows and their running (m, l, o), and takes
-// KEYS cache rows a step: issue() starts a step's copies of K and V into a
-// stage of shared memory, compute() folds them in, finish() writes the state.
+// KEYS cache rows a step, K and V each in a slot of shared memory: copy_k() and
+// copy_v() start the copies, scores() and values() fold them in, finish()
+// writes the state.  LEAN paths hold few enough registers for two CTAs per SM.
 // Row i of a block is query head hk * ratio + (row0 + i) % ratio of request
 // first_req + (row0 + i) / ratio.
 //
@@ -165,10 +166,10 @@ __device__ __forceinline__ const T *query(const Params &p, int first_req, int ro
 // ---------------------------------------------------------------------------
 template <int D, int NT>
 struct Bf16Path {
-    static constexpr int ROWS = 8 * NT, KEYS = D <= 64 ? 32 : 16;
+    static constexpr int ROWS = 8 * NT, KEYS = D <= 64 ? 32 : 16, LEAN = NT == 1;
     static constexpr int KM = KEYS / 16, KS = D / 16;         // 16-key tiles; 16-dim tiles
-    static constexpr int PITCH = 2 * D, OFF_V = KEYS * PITCH, STAGE = 2 * OFF_V;
-    uint32_t q[NT][KS][2];
+    static constexpr int PITCH = 2 * D, SLOT = KEYS * PITCH;
+    uint32_t q[NT][KS][2], hi[NT][KM][2], lo[KM][2];          // queries; the step's probabilities
     float o[NT][KS][4], m[NT][2], l[NT][2];
     const char *kb, *vb;
 
@@ -191,17 +192,19 @@ struct Bf16Path {
         vb = static_cast<const char *>(p.v) + (long long)hk * D * 2;
     }
     template <bool RUNS>
-    __device__ __forceinline__ void issue(const Params &p, uint32_t st, int row) const {
+    __device__ __forceinline__ void copy_k(const Params &p, uint32_t st, int row) const {
         copy_rows<KEYS, 2 * D, PITCH, TILES, RUNS>(st, kb, p.row_stride * 2, row);
-        copy_rows<KEYS, 2 * D, PITCH, TILES, RUNS>(st + OFF_V, vb, p.row_stride * 2, row);
+    }
+    template <bool RUNS>
+    __device__ __forceinline__ void copy_v(const Params &p, uint32_t st, int row) const {
+        copy_rows<KEYS, 2 * D, PITCH, TILES, RUNS>(st, vb, p.row_stride * 2, row);
     }
     template <bool EDGE>                  // EDGE: some keys of the step have no row
-    __device__ __forceinline__ void compute(const Params &p, uint32_t st, unsigned mask) {
-        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-        // rows and pieces that this lane addresses: K tiles (keys, +8 keys, +8 dims), V (keys, +8 dims, +8 keys)
-        const uint32_t turn = order_bits<PITCH, TILES>(lane & 7);
-        const uint32_t kst = st + ((lane >> 3 & 1) * 8 + (lane & 7)) * PITCH, kbits = turn ^ (lane >> 4) << 4;
-        const uint32_t vst = st + OFF_V + ((lane >> 4) * 8 + (lane & 7)) * PITCH, vbits = turn ^ (lane >> 3 & 1) << 4;
+    __device__ __forceinline__ void scores(const Params &p, uint32_t st, unsigned mask) {
+        const int lane = threadIdx.x & 31, g = lane >> 2;
+        // the row and piece that this lane addresses: tiles (keys, dims), (+8, dims), (keys, +8), (+8, +8)
+        const uint32_t kst = st + ((lane >> 3 & 1) * 8 + (lane & 7)) * PITCH;
+        const uint32_t kbits = order_bits<PITCH, TILES>(lane & 7) ^ (lane >> 4) << 4;
         float s[NT][KM][4];
 #pragma unroll
         for (int t = 0; t < NT; t++)
@@ -216,7 +219,6 @@ struct Bf16Path {
 #pragma unroll
                 for (int t = 0; t < NT; t++) mma_bf16(s[t][i], a, q[t][j][0], q[t][j][1]);
             }
-        uint32_t hi[NT][KM][2], lo[KM][2];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             float neg[2], alpha[2];
@@ -264,6 +266,13 @@ struct Bf16Path {
                     hi[t][i][n] = transposed(hi[t][i][n]);
                 }
         }
+    }
+    template <bool EDGE>
+    __device__ __forceinline__ void values(const Params &, uint32_t st, unsigned mask) {
+        const int lane = threadIdx.x & 31, c = lane & 3;
+        // tiles (keys, dims), (keys, +8), (+8, dims), (+8, +8), read transposed
+        const uint32_t vst = st + ((lane >> 4) * 8 + (lane & 7)) * PITCH;
+        const uint32_t vbits = order_bits<PITCH, TILES>(lane & 7) ^ (lane >> 3 & 1) << 4;
 #pragma unroll
         for (int i = 0; i < KM; i++)
 #pragma unroll
@@ -338,12 +347,14 @@ __device__ __forceinline__ int exponent(float x) { return min(100, max(-100, (__
 
 template <int D, int NT>
 struct I8Path {
-    static constexpr int ROWS = 4 * NT, KEYS = 32, FOLD = 8;
+    static constexpr int ROWS = 4 * NT, KEYS = 32, FOLD = 8, LEAN = NT == 1;
     static constexpr int KM = KEYS / 16, B64 = D / 64, REM = D % 64 != 0;
     static constexpr int KW = D / 16;                         // words of a K row per lane = k-steps = 16-dim tiles
-    static constexpr int VP = v_pitch(D), OFF_V = KEYS * D, OFF_S = OFF_V + KEYS * VP, STAGE = OFF_S + 2 * 4 * KEYS;
+    // a V slot holds its rows and both scales (K's are used with V's, once the code sums are there)
+    static constexpr int VP = v_pitch(D), OFF_S = KEYS * VP, SLOT = OFF_S + 2 * 4 * KEYS;
     static constexpr bool SWAP = D == 128;
     uint32_t q[NT][KW][2];
+    float s[NT][KM][4];                                       // the step's code sums
     float o[NT][KW][4], f[NT][KW][2], m[NT], l[NT];
     float qscale[NT];                                         // scale log2(e) / the query row's power of two
     float wscale;                                             // the weights' power of two
@@ -389,13 +400,16 @@ struct I8Path {
         vb = static_cast<const char *>(p.v) + (long long)hk * D;
     }
     template <bool RUNS>
-    __device__ __forceinline__ void issue(const Params &p, uint32_t st, int row) const {
+    __device__ __forceinline__ void copy_k(const Params &p, uint32_t st, int row) const {
+        copy_rows<KEYS, D, D, SWAP ? HALVES : AS_IS, RUNS>(st, kb, p.row_stride, row);
+    }
+    template <bool RUNS>
+    __device__ __forceinline__ void copy_v(const Params &p, uint32_t st, int row) const {
         const int lane = threadIdx.x & 31;
         const long long at_scale = (long long)row * p.kv_heads + head;
         copy4(st + OFF_S + lane * 4, p.kscale + at_scale);
         copy4(st + OFF_S + 128 + lane * 4, p.vscale + at_scale);
-        copy_rows<KEYS, D, D, SWAP ? HALVES : AS_IS, RUNS>(st, kb, p.row_stride, row);
-        copy_rows<KEYS, D, VP, SECTORS, RUNS>(st + OFF_V, vb, p.row_stride, row);
+        copy_rows<KEYS, D, VP, SECTORS, RUNS>(st, vb, p.row_stride, row);
     }
     __device__ __forceinline__ void fold() {
 #pragma unroll
@@ -419,7 +433,7 @@ struct I8Path {
         }
     }
     // Two 16-dim tiles from one word (4 dims) of each of the lane's keys 2c, 2c + 1, 2c + 8, 2c + 9.
-    __device__ __forceinline__ void values(int j, const uint32_t (&w)[NT][2], uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
+    __device__ __forceinline__ void pair(int j, const uint32_t (&w)[NT][2], uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
         const uint32_t a01 = prmt(v0, v1, 0x5140) ^ 0x80808080u, a23 = prmt(v0, v1, 0x7362) ^ 0x80808080u;
         const uint32_t b01 = prmt(v2, v3, 0x5140) ^ 0x80808080u, b23 = prmt(v2, v3, 0x7362) ^ 0x80808080u;
         const uint32_t x[4] = {codes_f16(a01, 0x4140), codes_f16(a01, 0x4342), codes_f16(b01, 0x4140), codes_f16(b01, 0x4342)};
@@ -431,11 +445,9 @@ struct I8Path {
         }
     }
     template <bool EDGE>
-    __device__ __forceinline__ void compute(const Params &, uint32_t st, unsigned mask) {
+    __device__ __forceinline__ void scores(const Params &, uint32_t st, unsigned) {
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-        const uint32_t kst = st + g * D, swap = SWAP ? (g & 1) * 64 : 0, vst = st + OFF_V + 2 * c * VP;
-        const uint32_t v8 = 8 * g ^ c << 5, v4 = 4 * g ^ c << 5;
-        float s[NT][KM][4];
+        const uint32_t kst = st + g * D, swap = SWAP ? (g & 1) * 64 : 0;
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -464,6 +476,11 @@ struct I8Path {
                 for (int t = 0; t < NT; t++) mma_f16(s[t][i], a, q[t][j][0], q[t][j][1]);
             }
         }
+    }
+    template <bool EDGE>
+    __device__ __forceinline__ void values(const Params &, uint32_t st, unsigned mask) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        const uint32_t vst = st + 2 * c * VP, v8 = 8 * g ^ c << 5, v4 = 4 * g ^ c << 5;
         // scales of the lane's keys: g, g + 8 of each 16; absent keys' scales are not numbers to go by
         float ks[KM][2], vs[KM][2], big = 0.f;
 #pragma unroll
@@ -524,15 +541,15 @@ struct I8Path {
 #pragma unroll
                 for (int n = 0; n < 4; n++)
                     v[n] = lds8(vst + (i * 16 + (n >> 1) * 8) * VP + v_at<VP>(n & 1, x & 1 ? v8 ^ 64 : v8, x / 2 * 128));
-                values(4 * x, pw[i], v[0].x, v[1].x, v[2].x, v[3].x);
-                values(4 * x + 2, pw[i], v[0].y, v[1].y, v[2].y, v[3].y);
+                pair(4 * x, pw[i], v[0].x, v[1].x, v[2].x, v[3].x);
+                pair(4 * x + 2, pw[i], v[0].y, v[1].y, v[2].y, v[3].y);
             }
             if constexpr (REM) {
                 uint32_t v[4];
 #pragma unroll
                 for (int n = 0; n < 4; n++)
                     v[n] = lds4(vst + (i * 16 + (n >> 1) * 8) * VP + v_at<VP>(n & 1, B64 ? v4 ^ 64 : v4, 0));
-                values(4 * B64, pw[i], v[0], v[1], v[2], v[3]);
+                pair(4 * B64, pw[i], v[0], v[1], v[2], v[3]);
             }
         }
         if (++folded == FOLD) fold();
@@ -571,14 +588,14 @@ template <int D, int R>
 struct F32Path {
     static constexpr int ROWS = R;
     // 8 or 16 lanes read 128 bytes of a row together; q and o take 2 E R registers, 64 to 96
-    static constexpr int LPK = R == 8 && D > 32 ? 16 : 8;
+    static constexpr int LPK = R >= 4 && D > 32 ? 16 : 8, LEAN = R <= 4;
     static constexpr int E = D / LPK, W = E % 4 ? 2 : 4, N = E / W;   // floats per lane, per read, reads
     static constexpr int G = 32 / LPK;                        // keys at a time
-    static constexpr int U = D == 128 ? 8 / G : D == 96 ? 8 / G : D == 64 ? 16 / G : 32 / G;   // keys of a group per step
-    static constexpr int KEYS = G * U, OFF_V = KEYS * D * 4, STAGE = 2 * OFF_V;
+    static constexpr int U = (D >= 96 ? 8 : D == 64 ? 16 : 32) / G;   // keys of a group per step
+    static constexpr int KEYS = G * U, SLOT = KEYS * D * 4;
     static_assert(KEYS <= 32 && LPK * E == D && N * W == E, "lane geometry");
     uint64_t q[R][E / 2], o[R][E / 2];
-    float m[R], l[R];
+    float m[R], l[R], x[R][U];                                // x: the step's scores, then probabilities
     const char *kb, *vb;
 
     __device__ __forceinline__ static void read(uint64_t (&x)[E / 2], uint32_t at) {
@@ -609,15 +626,17 @@ struct F32Path {
         vb = static_cast<const char *>(p.v) + (long long)hk * D * 4;
     }
     template <bool RUNS>
-    __device__ __forceinline__ void issue(const Params &p, uint32_t st, int row) const {
+    __device__ __forceinline__ void copy_k(const Params &p, uint32_t st, int row) const {
         copy_rows<KEYS, D * 4, D * 4, AS_IS, RUNS>(st, kb, p.row_stride * 4, row);
-        copy_rows<KEYS, D * 4, D * 4, AS_IS, RUNS>(st + OFF_V, vb, p.row_stride * 4, row);
+    }
+    template <bool RUNS>
+    __device__ __forceinline__ void copy_v(const Params &p, uint32_t st, int row) const {
+        copy_rows<KEYS, D * 4, D * 4, AS_IS, RUNS>(st, vb, p.row_stride * 4, row);
     }
     template <bool EDGE>
-    __device__ __forceinline__ void compute(const Params &, uint32_t st, unsigned mask) {
+    __device__ __forceinline__ void scores(const Params &, uint32_t st, unsigned mask) {
         const int lane = threadIdx.x & 31, g = lane / LPK;
         st += g * D * 4 + lane % LPK * W * 4;
-        float x[R][U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             uint64_t k[E / 2];
@@ -660,10 +679,15 @@ struct F32Path {
                 l[r] += x[r][u];
             }
         }
+    }
+    template <bool EDGE>
+    __device__ __forceinline__ void values(const Params &, uint32_t st, unsigned mask) {
+        const int lane = threadIdx.x & 31, g = lane / LPK;
+        st += g * D * 4 + lane % LPK * W * 4;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             uint64_t v[E / 2];
-            read(v, st + OFF_V + u * G * D * 4);
+            read(v, st + u * G * D * 4);
             if (EDGE && !(mask >> (u * G + g) & 1)) {       // probability 0, and values that may be NaN
 #pragma unroll
                 for (int i = 0; i < E / 2; i++) v[i] = 0ull;
