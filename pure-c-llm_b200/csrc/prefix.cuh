@@ -47,5 +47,174 @@ __device__ __forceinline__ long long cache_row(const Params &p, const int *line,
     return ((long long)page << p.log_page) + (t & ((1 << p.log_page) - 1));
 }
 
+// ---------------------------------------------------------------------------
+// The division of the work (prefix_decode.cu describes it)
+// ---------------------------------------------------------------------------
+constexpr int kEntries = 512;             // running sums of steps kept per CTA
+constexpr int kBegin = 1;                 // steps that the beginning and end of a segment count for
+
+// One part of the work.
+struct Part {
+    float *o;                             // pieces: [slot][heads of the block][rows][D]
+    float2 *ml;                           //         [slot][heads of the block][rows] (m in base 2, l)
+    long long *line_first;                // first step of each line, and the total
+    int lines, per_entry;                 // lines, lines per entry of the running sums
+    int head_block, n_blocks;             // key heads per team, their blocks
+    int splits, teams;                    // teams per CTA, in all
+    int blocks;                           // blocks of query rows of an own line
+    int seg_rows, rows;                   // query rows of a block, of a slot
+    int keys;                             // keys of a step
+    int half;                             // see Pieces (0: one piece per slot)
+};
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Query rows of a group and their blocks, and the index of the first block: an
+// ascending numbering without a sum over the groups before.
+__device__ __forceinline__ void group_blocks(const Params &p, const Part &w, int g, int &first_req, int &rows,
+                                             int &blocks, int &base) {
+    first_req = group_first(p, g);
+    rows = max(group_first(p, g + 1) - first_req, 0) * p.ratio;
+    blocks = ceil_div(rows, w.seg_rows);
+    base = first_req * p.ratio / w.seg_rows + g;
+}
+
+struct Line {
+    int keys, steps, blocks;              // blocks of query rows
+    int first_req, rows, base;            // of the line's query rows; index of its first block
+    // cost of a segment, and of the line, in steps
+    __device__ int cost() const { return steps + kBegin; }
+    __device__ long long total(const Part &w) const { return steps ? (long long)cost() * blocks * w.n_blocks : 0; }
+};
+template <bool PRE>
+__device__ __forceinline__ Line line_of(const Params &p, const Part &w, int i) {
+    Line l;
+    if (PRE) {
+        group_blocks(p, w, i, l.first_req, l.rows, l.blocks, l.base);
+        l.keys = l.rows ? prefix_len(p, i) : 0;
+    } else {
+        l.first_req = i;
+        l.rows = p.ratio;
+        l.blocks = w.blocks;
+        l.base = i * w.blocks;
+        l.keys = own_len(p, i);
+    }
+    l.steps = ceil_div(l.keys, w.keys);
+    return l;
+}
+
+// Running sums of the lines' costs, one per entry of w.per_entry lines, in
+// sums[0 .. entries], by all threads of the CTA; CTA 0 also writes each line's
+// own for the merge.  Returns the total.
+template <bool PRE>
+__device__ __forceinline__ long long sum_lines(const Params &p, const Part &w, long long *sums, long long *warp_sums) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int entries = ceil_div(w.lines, w.per_entry);
+    long long carry = 0;
+    for (int e0 = 0; e0 < entries; e0 += (int)blockDim.x) {
+        const int e = e0 + threadIdx.x;
+        long long v = 0;
+        if (e < entries)
+            for (int i = e * w.per_entry; i < min((e + 1) * w.per_entry, w.lines); i++)
+                v += line_of<PRE>(p, w, i).total(w);
+        long long s = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += u;
+        }
+        if (lane == 31) warp_sums[warp] = s;
+        __syncthreads();
+        long long before = carry;
+        for (int i = 0; i < (int)blockDim.x / 32; i++) {
+            if (i < warp) before += warp_sums[i];
+            carry += warp_sums[i];
+        }
+        if (e < entries) sums[e + 1] = before + s;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) sums[0] = 0;
+    __syncthreads();
+    const long long total = entries ? sums[entries] : 0;
+    if (blockIdx.x == 0) {
+        for (int e = threadIdx.x; e < entries; e += blockDim.x) {
+            long long at = sums[e];
+            for (int i = e * w.per_entry; i < min((e + 1) * w.per_entry, w.lines); i++) {
+                w.line_first[i] = at;
+                at += line_of<PRE>(p, w, i).total(w);
+            }
+        }
+        if (threadIdx.x == 0) w.line_first[w.lines] = total;
+    }
+    return total;
+}
+
+// Steps [a, b) of a segment: keys of a page-table line against query rows
+// [row0, row0 + rows) of the line, for block hb of key heads.
+struct Piece {
+    const int *table;
+    long long slot;
+    int keys, a, b, first_req, row0, rows, hb;
+};
+
+// The pieces of team `team`'s range [total t / teams, total (t + 1) / teams).
+// No more teams than steps, so that none between a segment's first and last is
+// without a piece.
+template <bool PRE>
+struct Walk {
+    const Params &p;
+    const Part &w;
+    long long first = 0, last = 0, at = 0;
+    int i = 0, s = 0, s1 = -1, team;
+    Line l;
+
+    __device__ __forceinline__ Walk(const Params &p_, const Part &w_, const long long *sums, long long total, int team_)
+        : p(p_), w(w_), team(team_) {
+        const int teams = (int)min((long long)w.teams, total);
+        l.steps = l.blocks = 0;
+        if (team >= teams) return;
+        first = total * team / teams;
+        last = total * (team + 1) / teams;
+        int lo = 0, hi = ceil_div(w.lines, w.per_entry);   // the last entry that begins at or before `first`
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (sums[mid] <= first) lo = mid;
+            else hi = mid;
+        }
+        i = lo * w.per_entry - 1;
+        at = sums[lo];
+    }
+    __device__ __forceinline__ bool next(Piece &x) {
+        while (true) {
+            while (s > s1) {              // the next line that the range meets, and its segments in the range
+                at += l.total(w);
+                if (++i >= w.lines || at >= last) { i = w.lines; at = last; l.steps = 0; return false; }
+                l = line_of<PRE>(p, w, i);
+                const long long n = l.total(w);
+                s = 0;
+                s1 = -1;
+                if (n > 0 && at + n > first) {
+                    s = (int)((max(first, at) - at) / l.cost());
+                    s1 = (int)((min(last, at + n) - 1 - at) / l.cost());
+                }
+            }
+            const long long begin = at + (long long)s * l.cost() + kBegin;
+            x.a = (int)(max(first, begin) - begin);
+            x.b = (int)(min(last, begin + l.steps) - begin);
+            const int rb = s / w.n_blocks;
+            x.hb = s - rb * w.n_blocks;
+            s++;
+            if (x.a >= x.b) continue;     // the range holds the segment's beginning alone
+            x.slot = (long long)(l.base + rb) * w.n_blocks + x.hb + team;
+            x.table = PRE ? p.prefix_table + (long long)i * p.max_prefix_pages : p.block_table + (long long)i * p.max_pages;
+            x.keys = l.keys;
+            x.first_req = l.first_req;
+            x.row0 = rb * w.seg_rows;
+            x.rows = min(l.rows - x.row0, w.seg_rows);
+            return true;
+        }
+    }
+};
+
 }  // namespace prefix
 }  // namespace attn

@@ -29,58 +29,7 @@
 namespace attn {
 namespace prefix {
 
-constexpr int kEntries = 512;             // running sums of steps kept per CTA
 constexpr int kWarps = 8;
-constexpr int kBegin = 1;                 // steps that the beginning and end of a segment count for
-
-// One part of the work.
-struct Part {
-    float *o;                             // pieces: [slot][heads of the block][rows][D]
-    float2 *ml;                           //         [slot][heads of the block][rows] (m in base 2, l)
-    long long *line_first;                // first step of each line, and the total
-    int lines, per_entry;                 // lines, lines per entry of the running sums
-    int head_block, n_blocks;             // key heads per team, their blocks
-    int splits, teams;                    // teams per CTA, in all
-    int blocks;                           // blocks of query rows of an own line
-    int seg_rows, rows;                   // query rows of a block, of a slot
-    int keys;                             // KEYS
-};
-
-__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
-
-// Query rows of a group and their blocks, and the index of the first block: an
-// ascending numbering without a sum over the groups before.
-__device__ __forceinline__ void group_blocks(const Params &p, const Part &w, int g, int &first_req, int &rows,
-                                             int &blocks, int &base) {
-    first_req = group_first(p, g);
-    rows = max(group_first(p, g + 1) - first_req, 0) * p.ratio;
-    blocks = ceil_div(rows, w.seg_rows);
-    base = first_req * p.ratio / w.seg_rows + g;
-}
-
-struct Line {
-    int keys, steps, blocks;              // blocks of query rows
-    int first_req, rows, base;            // of the line's query rows; index of its first block
-    // cost of a segment, and of the line, in steps
-    __device__ int cost() const { return steps + kBegin; }
-    __device__ long long total(const Part &w) const { return steps ? (long long)cost() * blocks * w.n_blocks : 0; }
-};
-template <bool PRE>
-__device__ __forceinline__ Line line_of(const Params &p, const Part &w, int i) {
-    Line l;
-    if (PRE) {
-        group_blocks(p, w, i, l.first_req, l.rows, l.blocks, l.base);
-        l.keys = l.rows ? prefix_len(p, i) : 0;
-    } else {
-        l.first_req = i;
-        l.rows = p.ratio;
-        l.blocks = w.blocks;
-        l.base = i * w.blocks;
-        l.keys = own_len(p, i);
-    }
-    l.steps = ceil_div(l.keys, w.keys);
-    return l;
-}
 
 // One warp's piece: steps [a, b) of a line for the query rows of one block and
 // one key head.  The ring holds SLOTS halves of steps (K, V, K, ...): AHEAD
@@ -179,96 +128,29 @@ prefix_rows_kernel(const __grid_constant__ Params p, const __grid_constant__ Par
     using R = Ring<Path, CTAS>;
     extern __shared__ __align__(128) uint8_t ring_bytes[];
     __shared__ long long sums[kEntries + 1];
-    __shared__ long long warp_sums[kWarps];
+    __shared__ long long warp_sums[32];
     if (!second) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    // running sums of the steps, per entry of w.per_entry lines
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int entries = ceil_div(w.lines, w.per_entry);
-    long long carry = 0;
-    for (int e0 = 0; e0 < entries; e0 += (int)blockDim.x) {
-        const int e = e0 + threadIdx.x;
-        long long v = 0;
-        if (e < entries)
-            for (int i = e * w.per_entry; i < min((e + 1) * w.per_entry, w.lines); i++)
-                v += line_of<PRE>(p, w, i).total(w);
-        long long s = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xffffffffu, s, o);
-            if (lane >= o) s += u;
-        }
-        if (lane == 31) warp_sums[warp] = s;
-        __syncthreads();
-        long long before = carry;
-        for (int i = 0; i < (int)blockDim.x / 32; i++) {
-            if (i < warp) before += warp_sums[i];
-            carry += warp_sums[i];
-        }
-        if (e < entries) sums[e + 1] = before + s;
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) sums[0] = 0;
-    __syncthreads();
-    const long long total = entries ? sums[entries] : 0;
-    if (blockIdx.x == 0) {                // for the merge
-        for (int e = threadIdx.x; e < entries; e += blockDim.x) {
-            long long at = sums[e];
-            for (int i = e * w.per_entry; i < min((e + 1) * w.per_entry, w.lines); i++) {
-                w.line_first[i] = at;
-                at += line_of<PRE>(p, w, i).total(w);
-            }
-        }
-        if (threadIdx.x == 0) w.line_first[w.lines] = total;
-    }
-
-    // This team's range.  No more teams than steps, so that none between a
-    // segment's first and last is without a piece.
+    const long long total = sum_lines<PRE>(p, w, sums, warp_sums);
+    const int warp = threadIdx.x >> 5;
     const uint32_t ring = sm100::smem_u32(ring_bytes) + warp * R::BYTES;
-    const int team_warp = warp % w.head_block, split = warp / w.head_block;
-    const int teams = (int)min((long long)w.teams, total), team = split * (int)gridDim.x + (int)blockIdx.x;
-    if (team < teams) {
-        const long long first = total * team / teams, last = total * (team + 1) / teams;
-        int e;
-        {
-            int lo = 0, hi = entries;     // the last entry that begins at or before `first`
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (sums[mid] <= first) lo = mid;
-                else hi = mid;
-            }
-            e = lo;
-        }
-        long long at = sums[e];
-        for (int i = e * w.per_entry; i < w.lines && at < last; i++) {
-            const Line l = line_of<PRE>(p, w, i);
-            const long long n = l.total(w);
-            if (at + n > first && n > 0) {
-                // segments of the line that the range meets
-                const int s0 = (int)((max(first, at) - at) / l.cost()), s1 = (int)((min(last, at + n) - 1 - at) / l.cost());
-                for (int s = s0; s <= s1; s++) {
-                    const long long begin = at + (long long)s * l.cost() + kBegin;
-                    const int a = (int)(max(first, begin) - begin), b = (int)(min(last, begin + l.steps) - begin);
-                    const int rb = s / w.n_blocks, hb = s - rb * w.n_blocks;
-                    const int hk = hb * w.head_block + team_warp;
-                    if (a >= b || hk >= p.kv_heads) continue;
-                    const long long slot = ((long long)(l.base + rb) * w.n_blocks + hb + team) * w.head_block + team_warp;
-                    const int *table = PRE ? p.prefix_table + (long long)i * p.max_prefix_pages
-                                           : p.block_table + (long long)i * p.max_pages;
-                    run_piece<Path, R::SLOTS>(p, ring, table, l.keys, a, b, l.first_req, rb * w.seg_rows,
-                                              min(l.rows - rb * w.seg_rows, w.seg_rows), hk,
-                                              w.o + slot * w.rows * D, w.ml + slot * w.rows);
-                }
-            }
-            at += n;
-        }
+    const int team_warp = warp % w.head_block, team = warp / w.head_block * (int)gridDim.x + (int)blockIdx.x;
+    Walk<PRE> walk(p, w, sums, total, team);
+    for (Piece x; walk.next(x);) {
+        const int hk = x.hb * w.head_block + team_warp;
+        if (hk >= p.kv_heads) continue;
+        const long long slot = x.slot * w.head_block + team_warp;
+        run_piece<Path, R::SLOTS>(p, ring, x.table, x.keys, x.a, x.b, x.first_req, x.row0, x.rows, hk,
+                                  w.o + slot * w.rows * D, w.ml + slot * w.rows);
     }
     if (second) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Joins the pieces of one query row: a CTA per (request, query head), its
 // warps taking the pieces in turn, a lane D/32 elements.
+// A slot of the tile kernel (w.half rows twice) holds, for a block of up to
+// w.half query rows, the pieces of its two warpgroups, which share the keys.
 struct Pieces {
     const float *o;
     const float2 *ml;
@@ -292,6 +174,10 @@ __device__ __forceinline__ Pieces pieces_of(const Part &w, const Line &l, int li
     r.ml = w.ml + slot;
     r.step = (long long)w.head_block * w.rows;
     r.n = t1 - t0 + 1;
+    if (w.half && l.rows - rb * w.seg_rows <= w.half) {      // two pieces in each slot, one behind the other
+        r.step = w.half;
+        r.n *= 2;
+    }
     return r;
 }
 
@@ -363,6 +249,7 @@ namespace attn_host {
 
 int sm_count_here();
 bool ensure_smem_attr(const void *func, size_t bytes);
+int launch_prefix_tile(const attn::prefix::Params &p, const attn::prefix::Part &w, int d, cudaStream_t s);
 
 namespace {
 
@@ -373,7 +260,7 @@ struct Layout {
 };
 
 Layout lay_out(const attn::prefix::Params &p, int d, int own_rows, int own_keys, int own_ctas, int pre_rows, int pre_keys,
-               int pre_ctas, char *base) {
+               int pre_ctas, bool tile, char *base) {
     using namespace attn::prefix;
     Layout r = {};
     size_t off = 0;
@@ -386,15 +273,16 @@ Layout lay_out(const attn::prefix::Params &p, int d, int own_rows, int own_keys,
         if (!lines) return;
         w.lines = lines;
         w.per_entry = (lines + kEntries - 1) / kEntries;
-        w.n_blocks = (p.kv_heads + kWarps - 1) / kWarps;
+        w.n_blocks = pre && tile ? p.kv_heads : (p.kv_heads + kWarps - 1) / kWarps;
         w.head_block = (p.kv_heads + w.n_blocks - 1) / w.n_blocks;
-        w.splits = kWarps / w.head_block;
+        w.splits = pre && tile ? 1 : kWarps / w.head_block;
         w.teams = sm_count_here() * ctas * w.splits;
         w.seg_rows = seg_rows;
         w.keys = keys;
         w.blocks = (p.ratio + seg_rows - 1) / seg_rows;
         const long long all_rows = (long long)p.n_seq * p.ratio;
-        w.rows = (int)std::min<long long>(pre ? all_rows : p.ratio, seg_rows);
+        w.rows = pre && tile ? seg_rows : (int)std::min<long long>(pre ? all_rows : p.ratio, seg_rows);
+        w.half = pre && tile ? 128 : 0;
         const long long blocks = pre ? all_rows / seg_rows + lines : (long long)lines * w.blocks;
         const size_t slots = (size_t)(blocks * w.n_blocks + w.teams) * w.head_block * w.rows;
         w.line_first = reinterpret_cast<long long *>(take(((size_t)lines + 1) * 8));
@@ -402,7 +290,7 @@ Layout lay_out(const attn::prefix::Params &p, int d, int own_rows, int own_keys,
         w.o = reinterpret_cast<float *>(take(slots * d * 4));
     };
     part(r.own, p.max_len ? p.n_seq : 0, own_rows, own_keys, own_ctas, false);
-    part(r.pre, p.max_prefix_len ? p.n_groups : 0, pre_rows, pre_keys, pre_ctas, true);
+    part(r.pre, p.max_prefix_len ? p.n_groups : 0, tile ? 256 : pre_rows, tile ? 128 : pre_keys, pre_ctas, true);
     r.bytes = std::max<size_t>(off, 256);
     return r;
 }
@@ -423,10 +311,15 @@ template <class Own, class Pre, typename T, int D>
 int run(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s) {
     using namespace attn::prefix;
     constexpr int OWN_CTAS = Own::LEAN ? 2 : 1, PRE_CTAS = 1;
-    const Layout L = lay_out(p, D, Own::ROWS, Own::KEYS, OWN_CTAS, Pre::ROWS, Pre::KEYS, PRE_CTAS, static_cast<char *>(ws));
+    // The tensor-core tiles take prefixes of bf16 caches from 32 query rows a
+    // group on (counted on average: the groups' sizes are on the device).
+    const bool tile = sizeof(T) == 2 && (D == 64 || D == 128) && p.n_groups &&
+                      (long long)p.n_seq * p.ratio >= 32LL * p.n_groups;
+    const Layout L = lay_out(p, D, Own::ROWS, Own::KEYS, OWN_CTAS, Pre::ROWS, Pre::KEYS, PRE_CTAS, tile, static_cast<char *>(ws));
     if (need) { *need = L.bytes; return ATTN_OK; }
     int st;
-    if (L.pre.lines && (st = run_part<Pre, true, D, PRE_CTAS>(p, L.pre, 0, s))) return st;
+    if (L.pre.lines && (st = tile ? launch_prefix_tile(p, L.pre, D, s) : run_part<Pre, true, D, PRE_CTAS>(p, L.pre, 0, s)))
+        return st;
     if (L.own.lines && (st = run_part<Own, false, D, OWN_CTAS>(p, L.own, L.pre.lines != 0, s))) return st;
     return check_pdl(launch_pdl(prefix_merge_kernel<T, D>, dim3(p.heads, p.n_seq), dim3(kMergeWarps * 32), 0, s, p, L.own, L.pre),
                      "prefix_merge_kernel");
