@@ -259,8 +259,8 @@ struct Layout {
     size_t bytes;
 };
 
-Layout lay_out(const attn::prefix::Params &p, int d, int own_rows, int own_keys, int own_ctas, int pre_rows, int pre_keys,
-               int pre_ctas, bool tile, char *base) {
+Layout lay_out(const attn::prefix::Params &p, int d, int own_rows, int own_keys, int own_grid, int pre_rows, int pre_keys,
+               int pre_grid, bool tile, char *base) {
     using namespace attn::prefix;
     Layout r = {};
     size_t off = 0;
@@ -269,14 +269,14 @@ Layout lay_out(const attn::prefix::Params &p, int d, int own_rows, int own_keys,
         off += (bytes + 255) / 256 * 256;
         return at;
     };
-    auto part = [&](Part &w, int lines, int seg_rows, int keys, int ctas, bool pre) {
+    auto part = [&](Part &w, int lines, int seg_rows, int keys, int grid, bool pre) {
         if (!lines) return;
         w.lines = lines;
         w.per_entry = (lines + kEntries - 1) / kEntries;
         w.n_blocks = pre && tile ? p.kv_heads : (p.kv_heads + kWarps - 1) / kWarps;
         w.head_block = (p.kv_heads + w.n_blocks - 1) / w.n_blocks;
         w.splits = pre && tile ? 1 : kWarps / w.head_block;
-        w.teams = sm_count_here() * ctas * w.splits;
+        w.teams = grid * w.splits;
         w.seg_rows = seg_rows;
         w.keys = keys;
         w.blocks = (p.ratio + seg_rows - 1) / seg_rows;
@@ -289,8 +289,8 @@ Layout lay_out(const attn::prefix::Params &p, int d, int own_rows, int own_keys,
         w.ml = reinterpret_cast<float2 *>(take(slots * 8));
         w.o = reinterpret_cast<float *>(take(slots * d * 4));
     };
-    part(r.own, p.max_len ? p.n_seq : 0, own_rows, own_keys, own_ctas, false);
-    part(r.pre, p.max_prefix_len ? p.n_groups : 0, tile ? 256 : pre_rows, tile ? 128 : pre_keys, pre_ctas, true);
+    part(r.own, p.max_len ? p.n_seq : 0, own_rows, own_keys, own_grid, false);
+    part(r.pre, p.max_prefix_len ? p.n_groups : 0, tile ? 256 : pre_rows, tile ? 128 : pre_keys, pre_grid, true);
     r.bytes = std::max<size_t>(off, 256);
     return r;
 }
@@ -315,7 +315,8 @@ int run(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s) {
     // group on (counted on average: the groups' sizes are on the device).
     const bool tile = sizeof(T) == 2 && (D == 64 || D == 128) && p.n_groups &&
                       (long long)p.n_seq * p.ratio >= 32LL * p.n_groups;
-    const Layout L = lay_out(p, D, Own::ROWS, Own::KEYS, OWN_CTAS, Pre::ROWS, Pre::KEYS, PRE_CTAS, tile, static_cast<char *>(ws));
+    const Layout L = lay_out(p, D, Own::ROWS, Own::KEYS, sm_count_here() * OWN_CTAS, Pre::ROWS, Pre::KEYS,
+                             sm_count_here() * PRE_CTAS, tile, static_cast<char *>(ws));
     if (need) { *need = L.bytes; return ATTN_OK; }
     int st;
     if (L.pre.lines && (st = tile ? launch_prefix_tile(p, L.pre, D, s) : run_part<Pre, true, D, PRE_CTAS>(p, L.pre, 0, s)))

@@ -11,27 +11,34 @@
 // 256 query rows: with more than 128, warpgroup w takes rows [128 w, 128 w + 128)
 // of every step; with fewer, both take the same rows and every other step, and
 // the merge finds two pieces in the slot.  12 warps:
-//   warps 0-1   copy Q rows and the keys' K and V rows, found through the page
-//               table, into the tensor cores' 128-byte swizzled layout, 16 bytes
-//               a lane; rows of no key are filled with zeros, so that a
-//               probability of 0 never meets a NaN.  They report a copied half
-//               (K or V of a step) when kLag more are on their way.
-//   warp 2      S_w = Q_w K^T, M = N = 128, both operands in shared memory
-//   warp 3      O_w += P_w V (P from TMEM, V as it lies, MN-major)
+//   warps 0-1   bring in Q rows and the keys' K and V rows.  A step whose 128
+//               keys all have rows is a few TMA boxes of a page's rows x 64 dims;
+//               at a line's end, with pages of fewer than 8 rows or outside the
+//               cache, and for Q, the lanes copy 16 bytes each into the same
+//               128-byte swizzled layout, with zeros for keys without a row, so
+//               that a probability of 0 never meets a NaN.  They report such a
+//               half (K or V of a step) when kLag more are on their way.  (All
+//               steps by lanes: 299 us for the prefixes above, the copying
+//               warps' instructions setting the pace.)
+//   warp 2      S_wu = Q_w K_u^T for the two halves u of a step's keys, M = 128,
+//               N = 64, both operands in shared memory
+//   warp 3      O_w += P_wu V_u (P from TMEM, V as it lies, MN-major)
 //   warps 4-7   softmax of warpgroup 0, warps 8-11 of warpgroup 1: a thread owns
 //               a row (a TMEM lane), keeps its maximum and sum, writes its bf16
 //               probabilities to TMEM, and rescales O when the maximum grew by
 //               more than 2^8 (a stale one leaves P <= 256, and the piece's
 //               (m, l, o) stay consistent).  All exponentials on MUFU: lse is an
 //               output.
-// At d 64 TMEM holds two S, two P and two O (512 columns), and S of a step may
-// follow as soon as its predecessor is in registers.  At d 128 P lies over its
-// own S, so S waits for the product that reads P; the two warpgroups then fill
-// each other's gaps.
+// TMEM: four S of 64 columns, each overwritten by its P, and two O (512 columns
+// at d 128).  S_w1 is formed while S_w0 is in the softmax, so a warpgroup does
+// not wait for its own products.  (With 128 keys in one S per warpgroup the
+// chain softmax, PV, next S took 5,300 cycles a step, of which the exponentials
+// of both warpgroups are 2,048.)
 //
 // Every wait is bounded; a timeout records a code in the device error word and
 // raises a CTA-wide flag, on which all roles fall through to the teardown.
 #include <algorithm>
+#include <cudaTypedefs.h>
 
 #include "prefix.cuh"
 #include "sm100.cuh"
@@ -42,29 +49,30 @@ namespace ptile {
 using namespace sm100;
 using namespace prefix;
 
-constexpr int BM = 128, BN = 128;
+constexpr int BM = 128, BN = 128, BH = 64;   // query rows; keys of a step, of an S
 constexpr int kThreads = 384;
 constexpr int kLag = 2;                   // halves on their way when one is reported
+constexpr int kMasks = 8;                 // steps whose key masks are kept: more than the ring holds, and the one at work
 
 template <int D>
 struct Cfg {
-    static constexpr int STAGES = D == 64 ? 4 : 2;
-    static constexpr bool OVER = D == 128;                    // P over S
+    static constexpr int SLOTS = D == 64 ? 8 : 5;             // ring of halves: K, V, K, ...
     static constexpr int TILE = BM * D * 2;                   // Q tile, K or V tile: D / 64 blocks of 128 rows x 128 bytes
-    static constexpr int OFF_K = 2 * TILE, STAGE = 2 * TILE;
-    static constexpr int OFF_BAR = OFF_K + STAGES * STAGE;
-    static constexpr int OFF_MASK = OFF_BAR + 256;
-    static constexpr int SMEM = OFF_MASK + STAGES * 16 + 1024;
-    static constexpr int S0 = 0, S1 = 128, O0 = 256, O1 = 256 + D;
-    static constexpr int P0 = OVER ? S0 : 256 + 2 * D, P1 = OVER ? S1 : P0 + 64;
+    static constexpr int OFF_KV = 2 * TILE;
+    static constexpr int OFF_BAR = OFF_KV + SLOTS * TILE;
+    static constexpr int OFF_MASK = OFF_BAR + 320;
+    static constexpr int SMEM = OFF_MASK + kMasks * 16 + 1024;
 };
+// TMEM columns
+__device__ __forceinline__ uint32_t col_s(int wg, int u) { return (uint32_t)(wg * 2 + u) * BH; }
+template <int D> __device__ __forceinline__ uint32_t col_o(int wg) { return 4 * BH + (uint32_t)wg * D; }
 
 enum {
     B_QF = 0, B_QE = 1,                   // Q copied; its last S finished
-    B_SF = 2, B_SE = 4,                   // per warpgroup: S ready; S in registers
-    B_PF = 6, B_OD = 8, B_OF = 10,        // P written; PV finished; O read out
-    B_KF = 12, B_VF = 16, B_KVE = 20,     // per stage: K, V copied; both used
-    B_COUNT = 24
+    B_OF = 2,                             // per warpgroup: O read out
+    B_SF = 4, B_PF = 8, B_OD = 12,        // per warpgroup and half (2 w + u): S ready; P written; PV finished
+    B_FULL = 16, B_FREE = 24,             // per slot: copied; used
+    B_COUNT = 32
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
@@ -73,36 +81,33 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
-prefix_tile_kernel(const __grid_constant__ Params p, const __grid_constant__ Part w)
+prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                   const __grid_constant__ Params p, const __grid_constant__ Part w, int boxes)
 {
     using C = Cfg<D>;
     constexpr int CPR = D / 8;            // 16-byte pieces of a row
     extern __shared__ uint8_t smem_raw[];
-    __shared__ long long sums[kEntries + 1];
-    __shared__ long long warp_sums[32];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t *sb = smem_raw + (base - raw);
-    const uint32_t sQ = base, sKV = base + C::OFF_K, bar0 = base + C::OFF_BAR;
+    const uint32_t sQ = base, sKV = base + C::OFF_KV, bar0 = base + C::OFF_BAR;
 #define BAR(i) (bar0 + 8u * (uint32_t)(i))
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sb + C::OFF_BAR + 224);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(sb + C::OFF_BAR + 228);
-    volatile uint32_t *masks = reinterpret_cast<volatile uint32_t *>(sb + C::OFF_MASK);   // [stage][4]: keys with a row
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sb + C::OFF_BAR + 256);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(sb + C::OFF_BAR + 260);
+    volatile uint32_t *masks = reinterpret_cast<volatile uint32_t *>(sb + C::OFF_MASK);   // [step % kMasks][4]: keys with a row
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(BAR(B_QF), 64);
         mbar_init(BAR(B_QE), 1);
-        for (int i = 0; i < 2; i++) {
-            mbar_init(BAR(B_SF + i), 1);
-            mbar_init(BAR(B_SE + i), 128);
+        for (int i = 0; i < 2; i++) mbar_init(BAR(B_OF + i), 128);
+        for (int i = 0; i < 4; i++) {
+            mbar_init(BAR(B_SF + i), 2);
             mbar_init(BAR(B_PF + i), 128);
             mbar_init(BAR(B_OD + i), 1);
-            mbar_init(BAR(B_OF + i), 128);
         }
-        for (int s = 0; s < C::STAGES; s++) {
-            mbar_init(BAR(B_KF + s), 64);
-            mbar_init(BAR(B_VF + s), 64);
-            mbar_init(BAR(B_KVE + s), 2);
+        for (int s = 0; s < C::SLOTS; s++) {
+            mbar_init(BAR(B_FULL + s), 64);
+            mbar_init(BAR(B_FREE + s), 1);
         }
         *abort_flag = 0;
         fence_mbar_init();
@@ -114,16 +119,19 @@ prefix_tile_kernel(const __grid_constant__ Params p, const __grid_constant__ Par
     // The own rows' launch may start once this one's CTAs have all seen the work before them finished.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const long long total = sum_lines<true>(p, w, sums, warp_sums);
+    // (the sums lie where the query rows come after the next barrier)
+    long long *sums = reinterpret_cast<long long *>(sb);
+    static_assert((kEntries + 1 + 32) * 8 <= 2 * C::TILE, "sums in the query tiles");
+    const long long total = sum_lines<true>(p, w, sums, sums + kEntries + 1);
+    Walk<true> walk(p, w, sums, total, (int)blockIdx.x);
+    Piece x;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    Walk<true> walk(p, w, sums, total, (int)blockIdx.x);
-    Piece x;
 
-    // 384 x 168 registers at launch: 128 x 72 + 256 x 216
-    if (warp < 4) regs_dec<72>();
+    // 384 x 168 registers at launch: 128 x 88 + 256 x 208
+    if (warp < 4) regs_dec<88>();
     if (warp < 2) {
         // ------------------------------------------------------------ copies
         auto wait = [&](int b, int parity, int code) -> bool {
@@ -156,6 +164,7 @@ prefix_tile_kernel(const __grid_constant__ Params p, const __grid_constant__ Par
                 if (i < n_due) report(due[i]);
             n_due = 0;
         };
+        const bool leader = elect_one();
         constexpr int RPI = 32 / CPR;     // rows per copy instruction of a warp
         const int lr = lane / CPR, ch = lane % CPR;
         // a 16-byte piece's place in a tile: 64-column block, row, piece XOR row % 8
@@ -177,39 +186,73 @@ prefix_tile_kernel(const __grid_constant__ Params p, const __grid_constant__ Par
                     copy16(sQ + t * C::TILE + place(r), src, there);
                 }
             copied(B_QF);
+            // cache rows of a step's 128 keys (-1: none), four per lane in both warps, read a step ahead
+            int next[4];
+            auto look_up = [&](int j) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int t = j * BN + 32 * i + lane;
+                    next[i] = j < x.b && t < x.keys ? (int)cache_row(p, x.table, t) : -1;
+                }
+            };
+            look_up(x.a);
             for (int j = x.a; j < x.b; j++, g++) {
-                const int st = g % C::STAGES;
-                // cache rows of this warp's 64 keys, two per lane
-                int row[2];
-                bool valid[2];
+                int row[4];
+                unsigned valid[4];
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int t = j * BN + warp * 64 + 32 * i + lane;
-                    long long at = -1;
-                    if (t < x.keys) at = cache_row(p, x.table, t);
-                    valid[i] = at >= 0;
-                    row[i] = max((int)at, 0);
+                for (int i = 0; i < 4; i++) {
+                    valid[i] = __ballot_sync(0xffffffffu, next[i] >= 0);
+                    row[i] = max(next[i], 0);
                 }
-                if (g >= C::STAGES && !(ok = wait(B_KVE + st, g / C::STAGES + 1, 0x802))) break;
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const unsigned m = __ballot_sync(0xffffffffu, valid[i]);
-                    if (lane == 0) masks[st * 4 + 2 * warp + i] = m;
-                }
+                look_up(j + 1);
+                const bool whole = boxes && (valid[0] & valid[1] & valid[2] & valid[3]) == 0xffffffffu;
 #pragma unroll
                 for (int kv = 0; kv < 2; kv++) {
+                    const int half = 2 * g + kv, slot = half % C::SLOTS;
+                    const uint32_t to = sKV + slot * C::TILE;
+                    if (half >= C::SLOTS) {
+                        if (whole) flush();       // nothing may stay due behind the wait
+                        if (!(ok = wait(B_FREE + slot, half / C::SLOTS + 1, 0x802))) break;
+                    }
+                    if (kv == 0 && warp == 0 && lane == 0) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) masks[g % kMasks * 4 + i] = valid[i];
+                    }
+                    __syncwarp();
+                    if (whole) {
+                        if (warp == 0) {
+                            if (leader) mbar_arrive_expect_tx(BAR(B_FULL + slot), C::TILE);
+                            __syncwarp();
+                            const int rows = BN / boxes;      // of a box
+                            for (int n = 0; n < boxes; n++) {
+                                const int key = n * rows;
+                                const int r = __shfl_sync(0xffffffffu, key < 64 ? (key < 32 ? row[0] : row[1]) : (key < 96 ? row[2] : row[3]), key & 31);
+                                if (leader) {
+#pragma unroll
+                                    for (int d = 0; d < D / 64; d++)
+                                        tma_load_3d(to + d * BN * 128 + key * 128, kv ? &tv : &tk, BAR(B_FULL + slot),
+                                                    x.hb * D + 64 * d, r, 0);
+                                }
+                                __syncwarp();
+                            }
+                        }
+                        if (warp != 0 || !leader) mbar_arrive(BAR(B_FULL + slot));
+                        __syncwarp();
+                        if (kv) flush();          // the query rows, behind the first step's boxes
+                        continue;
+                    }
                     const __nv_bfloat16 *from = static_cast<const __nv_bfloat16 *>(kv ? p.v : p.k) + (long long)x.hb * D + ch * 8;
-                    const uint32_t to = sKV + st * C::STAGE + kv * C::TILE;
 #pragma unroll
                     for (int i = 0; i < 2; i++)
 #pragma unroll 4
                         for (int r0 = 0; r0 < 32; r0 += RPI) {
-                            const int r = __shfl_sync(0xffffffffu, row[i], r0 + lr);
-                            const bool there = __shfl_sync(0xffffffffu, (int)valid[i], r0 + lr);
+                            const int r = __shfl_sync(0xffffffffu, warp ? row[2 + i] : row[i], r0 + lr);
+                            const bool there = (warp ? valid[2 + i] : valid[i]) >> (r0 + lr) & 1;
                             copy16(to + place(warp * 64 + 32 * i + r0 + lr), from + (long long)r * p.row_stride, there);
                         }
-                    copied((kv ? B_VF : B_KF) + st);
+                    copied(B_FULL + slot);
                 }
+                if (!ok) break;
             }
         }
         if (ok) flush();
@@ -220,36 +263,40 @@ prefix_tile_kernel(const __grid_constant__ Params p, const __grid_constant__ Par
         auto wait = [&](int b, int parity, int code) -> bool {
             return __all_sync(0xffffffffu, mbar_wait(BAR(b), parity & 1, abort_flag, p.err, code));
         };
-        constexpr uint32_t id = idesc_bf16(BM, BN, 0, 0);
-        int g = 0, t[2] = {0, 0};         // steps; S products per warpgroup
+        constexpr uint32_t id = idesc_bf16(BM, BH, 0, 0);
+        int g = 0, t[2] = {0, 0};         // steps; steps per warpgroup
         bool ok = true;
         for (int k = 0; ok && walk.next(x); k++) {
             const bool two = x.rows > BM;
             if (!(ok = wait(B_QF, k, 0x811))) break;
             for (int j = x.a; ok && j < x.b; j++, g++) {
-                const int st = g % C::STAGES;
-                if (!(ok = wait(B_KF + st, g / C::STAGES, 0x812))) break;
+                const int slot = 2 * g % C::SLOTS;
+                if (!(ok = wait(B_FULL + slot, 2 * g / C::SLOTS, 0x812))) break;
 #pragma unroll
-                for (int wg = 0; wg < 2; wg++) {
+                for (int n = 0; n < 4; n++) {
+                    const int u = n >> 1, wg = n & 1, b = 2 * wg + u;
                     if (!two && ((j - x.a) & 1) != wg) continue;
-                    if (t[wg] > 0 && !(ok = wait((C::OVER ? B_OD : B_SE) + wg, t[wg] - 1, 0x813 + wg))) break;
+                    // the product that reads this half's last P is done
+                    if (ok && t[wg] > 0) ok = wait(B_OD + b, t[wg] - 1, 0x813 + n);
+                    if (!ok) break;
                     tc_fence_after();
                     if (leader) {
                         const uint64_t qd = sw128_desc(sQ + (two ? wg : 0) * C::TILE, 16, 1024);
-                        const uint64_t kd = sw128_desc(sKV + st * C::STAGE, 16, 1024);
+                        const uint64_t kd = sw128_desc(sKV + slot * C::TILE + u * BH * 128, 16, 1024);
 #pragma unroll
                         for (int kk = 0; kk < D / 16; kk++) {   // 32 bytes on per step, a block of 16 KB on per 64 dims
                             const uint32_t off = (kk / 4) * (BM * 128 >> 4) + (kk % 4) * 2;
-                            mma_bf16_ss(tmem + (wg ? C::S1 : C::S0), qd + off, kd + off, id, kk > 0);
+                            mma_bf16_ss(tmem + col_s(wg, u), qd + off, kd + off, id, kk > 0);
                         }
-                        mma_commit(BAR(B_SF + wg));
+                        mma_commit(BAR(B_SF + b));
+                        mbar_arrive(BAR(B_SF + b));               // (hands on the copying warps' masks)
                     }
                     __syncwarp();
-                    t[wg]++;
+                    if (u == 1) t[wg]++;
                 }
                 if (!ok) break;
                 if (leader) {
-                    mma_commit(BAR(B_KVE + st));
+                    mma_commit(BAR(B_FREE + slot));
                     if (j == x.b - 1) mma_commit(BAR(B_QE));
                 }
                 __syncwarp();
@@ -262,33 +309,34 @@ prefix_tile_kernel(const __grid_constant__ Params p, const __grid_constant__ Par
             return __all_sync(0xffffffffu, mbar_wait(BAR(b), parity & 1, abort_flag, p.err, code));
         };
         constexpr uint32_t id = idesc_bf16(BM, D, 0, 1);
-        int g = 0, t[2] = {0, 0}, done[2] = {0, 0};   // steps; products and pieces per warpgroup
+        int g = 0, t[2] = {0, 0}, done[2] = {0, 0};   // steps; steps and pieces per warpgroup
         bool ok = true;
         while (ok && walk.next(x)) {
             const bool two = x.rows > BM;
             for (int j = x.a; ok && j < x.b; j++, g++) {
-                const int st = g % C::STAGES;
-                if (!(ok = wait(B_VF + st, g / C::STAGES, 0x821))) break;
+                const int slot = (2 * g + 1) % C::SLOTS;
+                if (!(ok = wait(B_FULL + slot, (2 * g + 1) / C::SLOTS, 0x821))) break;
 #pragma unroll
-                for (int wg = 0; wg < 2; wg++) {
+                for (int n = 0; n < 4; n++) {
+                    const int u = n >> 1, wg = n & 1, b = 2 * wg + u;
                     if (!two && ((j - x.a) & 1) != wg) continue;
-                    const bool first = j - x.a < (two ? 1 : 2);   // of this warpgroup in this piece
-                    if (first && done[wg] > 0 && !(ok = wait(B_OF + wg, done[wg] - 1, 0x822 + wg))) break;
-                    if (!(ok = wait(B_PF + wg, t[wg], 0x824 + wg))) break;
+                    const bool first = u == 0 && j - x.a < (two ? 1 : 2);   // of this warpgroup in this piece
+                    if (ok && first && done[wg] > 0) ok = wait(B_OF + wg, done[wg] - 1, 0x822 + wg);
+                    if (ok) ok = wait(B_PF + b, t[wg], 0x824 + n);
+                    if (!ok) break;
                     tc_fence_after();
                     if (leader) {
-                        const uint64_t vd = sw128_desc(sKV + st * C::STAGE + C::TILE, BM * 128, 1024);
+                        const uint64_t vd = sw128_desc(sKV + slot * C::TILE + u * BH * 128, BM * 128, 1024);
 #pragma unroll
-                        for (int kk = 0; kk < BN / 16; kk++)      // 16 keys: 8 columns of P, 2 KB of V
-                            mma_bf16_ts(tmem + (wg ? C::O1 : C::O0), tmem + (wg ? C::P1 : C::P0) + kk * 8, vd + 128 * kk, id,
-                                        !first || kk > 0);
-                        mma_commit(BAR(B_OD + wg));
+                        for (int kk = 0; kk < BH / 16; kk++)      // 16 keys: 8 columns of P, 2 KB of V
+                            mma_bf16_ts(tmem + col_o<D>(wg), tmem + col_s(wg, u) + kk * 8, vd + 128 * kk, id, !first || kk > 0);
+                        mma_commit(BAR(B_OD + b));
                     }
                     __syncwarp();
-                    t[wg]++;
+                    if (u == 1) t[wg]++;
                 }
                 if (!ok) break;
-                if (leader) mma_commit(BAR(B_KVE + st));
+                if (leader) mma_commit(BAR(B_FREE + slot));
                 __syncwarp();
             }
             done[0]++;
@@ -296,11 +344,9 @@ prefix_tile_kernel(const __grid_constant__ Params p, const __grid_constant__ Par
         }
     } else {
         // ------------------------------------------------------------ softmax
-        regs_inc<216>();
+        regs_inc<208>();
         const int wg = (warp - 4) >> 2, quad = warp & 3, row = quad * 32 + lane;
-        const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-        const uint32_t tS = tmem + lane_base + (wg ? C::S1 : C::S0), tP = tmem + lane_base + (wg ? C::P1 : C::P0);
-        const uint32_t tO = tmem + lane_base + (wg ? C::O1 : C::O0);
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16), tO = lanes + col_o<D>(wg);
         int g = 0, t = 0;                 // steps of the CTA; of this warpgroup
         bool ok = true;
         while (ok && walk.next(x)) {
@@ -309,111 +355,96 @@ prefix_tile_kernel(const __grid_constant__ Params p, const __grid_constant__ Par
             const bool idle = quad * 32 >= mine;                  // none of them in this warp: it only keeps step
             float m = -INFINITY, l = 0.f;
             bool any = false;
-            for (int j = x.a; j < x.b; j++) {
+            for (int j = x.a; ok && j < x.b; j++) {
                 if (!two && ((j - x.a) & 1) != wg) continue;
-                const int at = g + j - x.a, st = at % C::STAGES;
-                // S is ready; then K's barrier, for the copying warps' masks, is past its phase too
-                ok = mbar_wait(BAR(B_SF + wg), t & 1, abort_flag, p.err, 0x831) &&
-                     mbar_wait(BAR(B_KF + st), at / C::STAGES & 1, abort_flag, p.err, 0x832);
-                if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                tc_fence_after();
-                if (idle) {
-                    if (!C::OVER) mbar_arrive(BAR(B_SE + wg));
-                    if (t > 0) ok = mbar_wait(BAR(B_OD + wg), (t - 1) & 1, abort_flag, p.err, 0x833);
+#pragma unroll 1
+                for (int u = 0; u < 2; u++) {
+                    const int b = 2 * wg + u;
+                    const uint32_t tS = lanes + col_s(wg, u);
+                    ok = mbar_wait(BAR(B_SF + b), t & 1, abort_flag, p.err, 0x831 + u);
                     if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                    mbar_arrive(BAR(B_PF + wg));
-                    t++;
-                    any = true;
-                    continue;
-                }
-                uint32_t s[128];
+                    tc_fence_after();
+                    if (!idle) {
+                        uint32_t s[BH];
 #pragma unroll
-                for (int q4 = 0; q4 < 4; q4++) {
-                    uint32_t tt[32];
-                    tmem_ld32(tS + 32 * q4, tt);
+                        for (int q = 0; q < BH / 32; q++) {
+                            uint32_t tt[32];
+                            tmem_ld32(tS + 32 * q, tt);
 #pragma unroll
-                    for (int c = 0; c < 32; c++) s[32 * q4 + c] = tt[c];
-                }
-                uint32_t valid[4];
+                            for (int c = 0; c < 32; c++) s[32 * q + c] = tt[c];
+                        }
+                        uint32_t valid[2];
 #pragma unroll
-                for (int i = 0; i < 4; i++) valid[i] = masks[st * 4 + i];
-                tmem_wait_ld();
-                if (!C::OVER) {
-                    tc_fence_before();
-                    mbar_arrive(BAR(B_SE + wg));                  // S may be overwritten
-                }
-                if ((valid[0] & valid[1] & valid[2] & valid[3]) != 0xffffffffu) {
-#pragma unroll
-                    for (int c = 0; c < 128; c++)
-                        if (!(valid[c >> 5] >> (c & 31) & 1)) s[c] = __float_as_uint(-INFINITY);
-                }
-                float mp[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) mp[i] = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < 128; c += 2)
-                    mp[(c >> 1) & 7] = max3(mp[(c >> 1) & 7], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-                float mx = max3(max3(mp[0], mp[1], mp[2]), max3(mp[3], mp[4], mp[5]), fmaxf(mp[6], mp[7]));
-                mx *= p.scale_log2;
-                float alpha = 1.f;
-                const bool grow = mx > m + 8.f;                   // also at the first step with a key
-                if (grow) {
-                    alpha = ex2(m - mx);
-                    m = mx;
-                    l *= alpha;
-                }
-                const float neg = m == -INFINITY ? 0.f : -m;
-                const uint64_t scale2 = f2(p.scale_log2, p.scale_log2), neg2 = f2(neg, neg);
-                uint64_t l2[4] = {0ull, 0ull, 0ull, 0ull};
-                uint32_t pk[64];
-#pragma unroll
-                for (int c = 0; c < 64; c++) {
-                    float a, b;
-                    f2_split(fma2(f2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), scale2, neg2), a, b);
-                    a = ex2(a);
-                    b = ex2(b);
-                    l2[c & 3] = add2(l2[c & 3], f2(a, b));
-                    pk[c] = pack_bf16(a, b);
-                }
-                {
-                    float a, b;
-                    f2_split(add2(add2(l2[0], l2[1]), add2(l2[2], l2[3])), a, b);
-                    l += a + b;
-                }
-                // P and O belong to the previous product until it is done
-                if (t > 0) ok = mbar_wait(BAR(B_OD + wg), (t - 1) & 1, abort_flag, p.err, 0x834);
-                if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                tc_fence_after();
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    uint32_t tt[32];
-#pragma unroll
-                    for (int c = 0; c < 32; c++) tt[c] = pk[32 * half + c];
-                    tmem_st32(tP + 32 * half, tt);
-                }
-                if (__any_sync(0xffffffffu, any && grow)) {
-                    uint32_t o[32];
-#pragma unroll
-                    for (int c0 = 0; c0 < D; c0 += 32) {
-                        tmem_ld32(tO + c0, o);
+                        for (int i = 0; i < 2; i++) valid[i] = masks[(g + j - x.a) % kMasks * 4 + 2 * u + i];
                         tmem_wait_ld();
+                        if ((valid[0] & valid[1]) != 0xffffffffu) {
 #pragma unroll
-                        for (int c = 0; c < 32; c++) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
-                        tmem_st32(tO + c0, o);
+                            for (int c = 0; c < BH; c++)
+                                if (!(valid[c >> 5] >> (c & 31) & 1)) s[c] = __float_as_uint(-INFINITY);
+                        }
+                        float mp[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) mp[i] = -INFINITY;
+#pragma unroll
+                        for (int c = 0; c < BH; c += 2)
+                            mp[(c >> 1) & 3] = max3(mp[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+                        const float mx = fmaxf(max3(mp[0], mp[1], mp[2]), mp[3]) * p.scale_log2;
+                        float alpha = 1.f;
+                        const bool grow = mx > m + 8.f;           // also at the first half with a key
+                        if (grow) {
+                            alpha = ex2(m - mx);
+                            m = mx;
+                            l *= alpha;
+                        }
+                        const float neg = m == -INFINITY ? 0.f : -m;
+                        const uint64_t scale2 = f2(p.scale_log2, p.scale_log2), neg2 = f2(neg, neg);
+                        uint64_t l2[4] = {0ull, 0ull, 0ull, 0ull};
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int c = 0; c < 32; c++) {
+                            float e, f;
+                            f2_split(fma2(f2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), scale2, neg2), e, f);
+                            e = ex2(e);
+                            f = ex2(f);
+                            l2[c & 3] = add2(l2[c & 3], f2(e, f));
+                            pk[c] = pack_bf16(e, f);
+                        }
+                        {
+                            float e, f;
+                            f2_split(add2(add2(l2[0], l2[1]), add2(l2[2], l2[3])), e, f);
+                            l += e + f;
+                        }
+                        tmem_st32(tS, pk);                        // over S, which is in registers
+                        if (__any_sync(0xffffffffu, any && grow)) {
+                            // O is the previous half's product's until that is done
+                            ok = mbar_wait(BAR(B_OD + 2 * wg + 1 - u), (t - 1 + u) & 1, abort_flag, p.err, 0x833 + u);
+                            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                            tc_fence_after();
+                            uint32_t o[32];
+#pragma unroll
+                            for (int c0 = 0; c0 < D; c0 += 32) {
+                                tmem_ld32(tO + c0, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int c = 0; c < 32; c++) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+                                tmem_st32(tO + c0, o);
+                            }
+                        }
+                        tmem_wait_st();
+                        tc_fence_before();
                     }
+                    mbar_arrive(BAR(B_PF + b));
+                    any = true;
                 }
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(BAR(B_PF + wg));
                 t++;
-                any = true;
             }
             if (!ok) break;
             g += x.b - x.a;
             // the piece: this warpgroup's half of the slot
             const long long at = x.slot * w.rows + wg * BM + row;
             if (any) {
-                ok = mbar_wait(BAR(B_OD + wg), (t - 1) & 1, abort_flag, p.err, 0x835);
+                ok = mbar_wait(BAR(B_OD + 2 * wg), (t - 1) & 1, abort_flag, p.err, 0x835) &&
+                     mbar_wait(BAR(B_OD + 2 * wg + 1), (t - 1) & 1, abort_flag, p.err, 0x836);
                 if (!(ok = __all_sync(0xffffffffu, ok))) break;
                 tc_fence_after();
                 if (!idle) {
@@ -459,12 +490,41 @@ namespace attn_host {
 
 bool ensure_smem_attr(const void *func, size_t bytes);
 
+static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+    void *ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+        return nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+}
+
+// {key heads x D, rows} of a bf16 cache in boxes of 64 dims x `box` rows, 128-byte swizzle.
+static bool cache_map(CUtensorMap *m, const void *ptr, int cols, long long rows, long long stride, int box) {
+    static const PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
+    if (!encode) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 1};
+    const cuuint64_t strides[2] = {(cuuint64_t)stride * 2, (cuuint64_t)stride * 2 * (cuuint64_t)rows};
+    const cuuint32_t extent[3] = {64, (cuuint32_t)box, 1}, steps[3] = {1, 1, 1};
+    return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(ptr), dims, strides, extent, steps,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D>
 static int launch_d(const attn::prefix::Params &p, const attn::prefix::Part &w, cudaStream_t s) {
     using namespace attn::ptile;
     if (!ensure_smem_attr((const void *)prefix_tile_kernel<D>, Cfg<D>::SMEM))
         return set_error(ATTN_ERR_CUDA, "prefix decode: cannot set shared-memory size");
-    return check_pdl(launch_pdl(prefix_tile_kernel<D>, dim3(w.teams), dim3(kThreads), Cfg<D>::SMEM, s, p, w), "prefix_tile_kernel");
+    // A step is BN / box boxes; a box of the swizzled layout begins on 8 rows.
+    CUtensorMap tk = {}, tv = {};
+    const int box = std::min(1 << p.log_page, BN);
+    const long long rows = (long long)p.n_pages << p.log_page;
+    const bool maps = box >= 8 && cache_map(&tk, p.k, p.kv_heads * D, rows, p.row_stride, box) &&
+                      cache_map(&tv, p.v, p.kv_heads * D, rows, p.row_stride, box);
+    return check_pdl(launch_pdl(prefix_tile_kernel<D>, dim3(w.teams), dim3(kThreads), Cfg<D>::SMEM, s, tk, tv, p, w,
+                                maps ? BN / box : 0),
+                     "prefix_tile_kernel");
 }
 
 int launch_prefix_tile(const attn::prefix::Params &p, const attn::prefix::Part &w, int d, cudaStream_t s) {
