@@ -229,8 +229,9 @@ def _dtype_code(t):
 
 
 def _stream():
+    """Handle of torch's current stream on the current device."""
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def forward_t(q, k, v, heads: int, batch: int, out=None, lse=None, want_lse=True):

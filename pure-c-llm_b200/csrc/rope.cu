@@ -9,10 +9,13 @@
 // read by the few threads that hold its pairs.
 //
 // A thread owns one vector position within a head (E elements and, in the
-// halves layout, the E elements rot/2 behind them) for kHeads heads of one
-// token: it reads its cosines and sines once for all of them, and its loads
-// are issued together.  Consecutive threads take consecutive vectors, so a
-// head's row goes out in full sectors.
+// halves layout, the E elements rot/2 behind them) for kHeads heads: it reads
+// a token's cosines and sines once for all of them, and its loads are issued
+// together and kept as they come until their turn, so that the 768 threads
+// of an SM hold 128 bytes each in flight.  It keeps its place in the token's row
+// and strides over the tokens, the next token's position and slot read ahead.
+// Consecutive threads take consecutive vectors, so a head's row goes out in
+// full sectors.
 #include <algorithm>
 
 #include "common.cuh"
@@ -21,7 +24,12 @@ namespace attn {
 namespace rope {
 
 constexpr int kThreads = 256;
-constexpr int kHeads = 4;                 // heads per thread
+// Heads per thread, and CTAs per SM that its registers leave.  32749 tokens of
+// 32/8 heads of 128 in bf16 (822 MB): 136 us, 6.06 TB/s; with 2 heads and 4
+// CTAs 150 us, with 4 and 2 157 us, 1 and 8 (spilling) 343 us.  64 tokens of
+// 16 heads of 64 in fp32 go the other way: 3.3 us, and 2.9 with 2 heads.
+constexpr int kHeads = 4;
+constexpr int ctas_of(bool pairs) { return pairs ? 4 : 3; }
 
 struct Params {
     const void *q, *k, *v;
@@ -34,7 +42,7 @@ struct Params {
     long long rows;                       // cache rows (slots != NULL)
     int tokens, seq_len, d, rot, max_pos;
     int q_heads, all_heads, kv_heads;     // heads [0, q_heads) q, then kv_heads of k, then of v
-    int items, chunks, tokens_per_block;
+    int items, per_token, tokens_per_block;   // vectors of a head; threads of a token
     float sign;                           // -1: transpose
 };
 
@@ -54,71 +62,89 @@ __device__ __forceinline__ void turn(float &a, float &b, float c, float s) {
     a = x;
 }
 
-template <typename T, int E> struct Vec;
-template <> struct Vec<float, 4> {
-    static __device__ __forceinline__ void load(const float *p, float (&x)[4]) {
-        const float4 v = *reinterpret_cast<const float4 *>(p);
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+// E elements as they lie in memory, and as floats.
+template <typename T, int E> struct Vec {           // one or two elements, of any alignment
+    T raw[E];
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < E; i++) raw[i] = p[i];
     }
-    static __device__ __forceinline__ void store(float *p, const float (&x)[4]) {
-        *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    __device__ __forceinline__ void store(T *p) const {
+#pragma unroll
+        for (int i = 0; i < E; i++) p[i] = raw[i];
+    }
+    __device__ __forceinline__ void get(float (&x)[E]) const {
+#pragma unroll
+        for (int i = 0; i < E; i++) x[i] = to_f32(raw[i]);
+    }
+    __device__ __forceinline__ void set(const float (&x)[E]) {
+#pragma unroll
+        for (int i = 0; i < E; i++) raw[i] = from_f32<T>(x[i]);
     }
 };
+template <> struct Vec<float, 4> {
+    float4 raw;
+    __device__ __forceinline__ void load(const float *p) { raw = *reinterpret_cast<const float4 *>(p); }
+    __device__ __forceinline__ void store(float *p) const { *reinterpret_cast<float4 *>(p) = raw; }
+    __device__ __forceinline__ void get(float (&x)[4]) const { x[0] = raw.x; x[1] = raw.y; x[2] = raw.z; x[3] = raw.w; }
+    __device__ __forceinline__ void set(const float (&x)[4]) { raw = make_float4(x[0], x[1], x[2], x[3]); }
+};
 template <> struct Vec<__nv_bfloat16, 8> {
-    static __device__ __forceinline__ void load(const __nv_bfloat16 *p, float (&x)[8]) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint4 raw;
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { raw = *reinterpret_cast<const uint4 *>(p); }
+    __device__ __forceinline__ void store(__nv_bfloat16 *p) const { *reinterpret_cast<uint4 *>(p) = raw; }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             x[2 * i] = __uint_as_float(w[i] << 16);
             x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
     }
-    static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float (&x)[8]) {
+    __device__ __forceinline__ void set(const float (&x)[8]) {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
             w[i] = *reinterpret_cast<const uint32_t *>(&h);
         }
-        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-};
-template <typename T> struct Vec<T, 1> {
-    static __device__ __forceinline__ void load(const T *p, float (&x)[1]) { x[0] = to_f32(p[0]); }
-    static __device__ __forceinline__ void store(T *p, const float (&x)[1]) { p[0] = from_f32<T>(x[0]); }
-};
-template <typename T> struct Vec<T, 2> {
-    static __device__ __forceinline__ void load(const T *p, float (&x)[2]) { x[0] = to_f32(p[0]); x[1] = to_f32(p[1]); }
-    static __device__ __forceinline__ void store(T *p, const float (&x)[2]) {
-        p[0] = from_f32<T>(x[0]);
-        p[1] = from_f32<T>(x[1]);
+        raw = make_uint4(w[0], w[1], w[2], w[3]);
     }
 };
 
 // E elements per vector: 16 bytes, or 1 (halves) and 2 (interleaved pairs)
 // where an address, a stride or rot is not a multiple of that.
 template <typename T, int E, bool PAIRS>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, ctas_of(PAIRS))
 rope_kernel(const __grid_constant__ Params p)
 {
     pdl_begin();                          // launched by launch_pdl
     using V = Vec<T, E>;
     const int half = p.rot / 2;
     const int turned = PAIRS ? p.rot / E : half / E;        // items of a head that turn
-    const int per_token = p.items * p.chunks;
-    const int t0 = (int)blockIdx.x * p.tokens_per_block;
-    const int n = min(p.tokens_per_block, p.tokens - t0) * per_token;
-    for (int u = threadIdx.x; u < n; u += kThreads) {
-        const int tl = u / per_token, r = u - tl * per_token;
-        const int chunk = r / p.items, item = r - chunk * p.items;
-        const int t = t0 + tl;
-        const bool turns = item < turned;
-        const int off_a = PAIRS || turns ? item * E : p.rot + (item - turned) * E;
-        constexpr int C = PAIRS ? (E + 1) / 2 : E;          // pairs of this item
+    // this thread's place: a token of the block's, a group of heads, a vector of a head
+    const int u = blockIdx.y * kThreads + threadIdx.x;
+    const int tl = u / p.per_token, r = u - tl * p.per_token;
+    if (tl >= p.tokens_per_block) return;
+    const int chunk = r / p.items, item = r - chunk * p.items;
+    const bool turns = item < turned;
+    const int off = PAIRS || turns ? item * E : p.rot + (item - turned) * E;
+    constexpr int C = PAIRS ? (E + 1) / 2 : E;              // pairs of this item
+
+    const int stride = (int)gridDim.x * p.tokens_per_block;
+    int t = (int)blockIdx.x * p.tokens_per_block + tl;
+    auto position = [&](int t) { return turns && t < p.tokens ? position_of(p, t) : 0; };
+    auto slot = [&](int t) { return p.slots && t < p.tokens ? __ldg(p.slots + t) : (long long)t; };
+    int next_pos = position(t);
+    long long next_row = slot(t);
+    for (; t < p.tokens; t += stride) {
+        const int pos = next_pos;
+        const long long row = !p.slots || (next_row >= 0 && next_row < p.rows) ? next_row : -1;
+        next_pos = position(t + stride);
+        next_row = slot(t + stride);
         float c[C], s[C];
         if (turns) {
-            const float *cs = p.table + ((long long)position_of(p, t) * half + item * C) * 2;
+            const float *cs = p.table + ((long long)pos * half + item * C) * 2;
             if constexpr (C % 2 == 0) {
 #pragma unroll
                 for (int i = 0; i < C; i += 2) {
@@ -133,12 +159,7 @@ rope_kernel(const __grid_constant__ Params p)
                 }
             }
         }
-        long long row = t;
-        if (p.slots) {
-            row = __ldg(p.slots + t);
-            if (row < 0 || row >= p.rows) row = -1;
-        }
-        float a[kHeads][E], b[kHeads][E];
+        V a[kHeads], b[kHeads];
         T *dst[kHeads];
 #pragma unroll
         for (int i = 0; i < kHeads; i++) {
@@ -147,37 +168,41 @@ rope_kernel(const __grid_constant__ Params p)
             if (h >= p.all_heads) continue;
             const T *src;
             if (h < p.q_heads) {
-                src = static_cast<const T *>(p.q) + t * p.q_stride + (long long)h * p.d;
-                dst[i] = static_cast<T *>(p.q_out) + t * p.qo_stride + (long long)h * p.d;
+                src = static_cast<const T *>(p.q) + t * p.q_stride + h * p.d + off;
+                dst[i] = static_cast<T *>(p.q_out) + t * p.qo_stride + h * p.d + off;
             } else {
                 if (row < 0) continue;
                 const int hk = h - p.q_heads;
                 if (hk < p.kv_heads) {
-                    src = static_cast<const T *>(p.k) + t * p.k_stride + (long long)hk * p.d;
-                    dst[i] = static_cast<T *>(p.k_out) + row * p.ko_stride + (long long)hk * p.d;
+                    src = static_cast<const T *>(p.k) + t * p.k_stride + hk * p.d + off;
+                    dst[i] = static_cast<T *>(p.k_out) + row * p.ko_stride + hk * p.d + off;
                 } else {
-                    src = static_cast<const T *>(p.v) + t * p.v_stride + (long long)(hk - p.kv_heads) * p.d;
-                    dst[i] = static_cast<T *>(p.v_out) + row * p.ko_stride + (long long)(hk - p.kv_heads) * p.d;
+                    src = static_cast<const T *>(p.v) + t * p.v_stride + (hk - p.kv_heads) * p.d + off;
+                    dst[i] = static_cast<T *>(p.v_out) + row * p.ko_stride + (hk - p.kv_heads) * p.d + off;
                 }
             }
-            V::load(src + off_a, a[i]);
-            if (!PAIRS && turns) V::load(src + off_a + half, b[i]);
+            a[i].load(src);
+            if (!PAIRS && turns) b[i].load(src + half);
         }
 #pragma unroll
         for (int i = 0; i < kHeads; i++) {
             if (!dst[i]) continue;
-            const bool is_v = chunk * kHeads + i >= p.q_heads + p.kv_heads;
-            if (turns && !is_v) {
+            if (turns && chunk * kHeads + i < p.q_heads + p.kv_heads) {
+                float x[E], y[E];
+                a[i].get(x);
                 if constexpr (PAIRS) {
 #pragma unroll
-                    for (int e = 0; e + 1 < E; e += 2) turn(a[i][e], a[i][e + 1], c[e / 2], s[e / 2]);
+                    for (int e = 0; e + 1 < E; e += 2) turn(x[e], x[e + 1], c[e / 2], s[e / 2]);
                 } else {
+                    b[i].get(y);
 #pragma unroll
-                    for (int e = 0; e < E; e++) turn(a[i][e], b[i][e], c[e], s[e]);
+                    for (int e = 0; e < E; e++) turn(x[e], y[e], c[e], s[e]);
+                    b[i].set(y);
                 }
+                a[i].set(x);
             }
-            V::store(dst[i] + off_a, a[i]);
-            if (!PAIRS && turns) V::store(dst[i] + off_a + half, b[i]);
+            a[i].store(dst[i]);
+            if (!PAIRS && turns) b[i].store(dst[i] + half);
         }
     }
 }
@@ -259,6 +284,8 @@ __global__ void rope_table_kernel(const attn_rope_config c, double low, double h
 
 namespace attn_host {
 
+int sm_count_here();
+
 int launch_rope_table(const attn_rope_config *c, float *table, cudaStream_t s) {
     attn_rope_config k = *c;
     double low = 0, high = 1;
@@ -289,10 +316,12 @@ static int launch_rope_typed(attn::rope::Params p, bool interleaved, cudaStream_
                       p.v_stride % W == 0 && p.qo_stride % W == 0 && p.ko_stride % W == 0;
     const int E = wide ? W : interleaved ? 2 : 1;
     p.items = interleaved ? p.d / E : p.rot / 2 / E + (p.d - p.rot) / E;
-    p.chunks = (p.all_heads + kHeads - 1) / kHeads;
-    const int per_token = p.items * p.chunks;
-    p.tokens_per_block = std::max(1, kThreads / per_token);
-    const dim3 grid((p.tokens + p.tokens_per_block - 1) / p.tokens_per_block);
+    p.per_token = p.items * ((p.all_heads + kHeads - 1) / kHeads);
+    p.tokens_per_block = std::max(1, kThreads / p.per_token);
+    // as many CTAs as are resident, which stride over the tokens
+    const int slices = (p.per_token + kThreads - 1) / kThreads;
+    const int groups = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
+    const dim3 grid(std::min(groups, std::max(1, sm_count_here() * ctas_of(interleaved) / slices)), slices);
     cudaError_t e;
     if (interleaved)
         e = wide ? launch_pdl(rope_kernel<T, W, true>, grid, dim3(kThreads), 0, s, p)
