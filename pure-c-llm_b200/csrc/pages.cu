@@ -22,7 +22,7 @@
 namespace attn {
 namespace pages {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;             // (256: 10.5 us, 1024: 9.8 us on the 2048-request step below)
 constexpr int kMaxSeq = 16384;            // 12 bytes each of shared memory
 
 struct Params {
@@ -42,30 +42,32 @@ __device__ __forceinline__ int sat_add(int a, int b) {
     return (int)min(s, 0x7fffffffu);
 }
 
-// Inclusive sums of `v` over the block's threads, on top of `carry` (the sum
-// so far, which becomes the sum with this block's).  Two barriers.
-__device__ __forceinline__ int block_scan(int v, int &carry, int *warp_sums) {
+// Sums of `a` and of `b` over the threads before this one; the block's totals
+// in total_a and total_b.  `warp_sums` holds two ints per warp.
+__device__ __forceinline__ void block_scan(int &a, int &b, int &total_a, int &total_b, int2 *warp_sums) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int s = v;
+    int x = a, y = b;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s = sat_add(s, u);
+        const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) { x = sat_add(x, u); y = sat_add(y, v); }
     }
-    if (lane == 31) warp_sums[warp] = s;
+    __syncthreads();                       // warp_sums may be written
+    if (lane == 31) warp_sums[warp] = make_int2(x, y);
     __syncthreads();
-    int w = lane < kThreads / 32 ? warp_sums[lane] : 0;
+    int2 w = lane < (int)blockDim.x / 32 ? warp_sums[lane] : make_int2(0, 0);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= o) w = sat_add(w, u);
+        const int u = __shfl_up_sync(0xffffffffu, w.x, o), v = __shfl_up_sync(0xffffffffu, w.y, o);
+        if (lane >= o) { w.x = sat_add(w.x, u); w.y = sat_add(w.y, v); }
     }
-    const int before = warp ? __shfl_sync(0xffffffffu, w, warp - 1) : 0;
-    const int total = __shfl_sync(0xffffffffu, w, 31);
-    const int r = sat_add(carry, sat_add(before, s));
-    carry = sat_add(carry, total);
-    __syncthreads();                       // warp_sums may be written again
-    return r;
+    total_a = __shfl_sync(0xffffffffu, w.x, 31);
+    total_b = __shfl_sync(0xffffffffu, w.y, 31);
+    // warps before, lanes before
+    const int wa = __shfl_sync(0xffffffffu, w.x, max(warp - 1, 0)), wb = __shfl_sync(0xffffffffu, w.y, max(warp - 1, 0));
+    const int la = __shfl_up_sync(0xffffffffu, x, 1), lb = __shfl_up_sync(0xffffffffu, y, 1);
+    a = sat_add(warp ? wa : 0, lane ? la : 0);
+    b = sat_add(warp ? wb : 0, lane ? lb : 0);
 }
 
 // the smallest i with sums[i] > x (sums ascending, n entries; n if none)
@@ -80,13 +82,13 @@ __device__ __forceinline__ int first_above(const int *sums, int n, int x) {
 }
 
 __global__ void __launch_bounds__(kThreads)
-page_plan_kernel(const Params p)
+page_plan_kernel(const __grid_constant__ Params p)
 {
     extern __shared__ int sums[];
     int *cu = sums;                        // new tokens up to and with request s
     int *need_sum = sums + p.n_seq;        // pages needed
     int *back_sum = need_sum + p.n_seq;    // pages returned
-    __shared__ int warp_sums[kThreads / 32];
+    __shared__ int2 warp_sums[kThreads / 32];
     __shared__ int s_used, s_refused;
     pdl_begin();                           // launched by launch_pdl
 
@@ -94,24 +96,38 @@ page_plan_kernel(const Params p)
     const int cap = p.max_pages << p.log_page;
     auto length = [&](int s) { return min(max(__ldg(p.lens + s), 0), cap); };
     auto pages_of = [&](long long tokens) { return (int)((tokens + page - 1) >> p.log_page); };
+    const int have_free = min(max(__ldg(p.free_count), 0), p.n_pages);
+    if (threadIdx.x == 0) s_refused = 0;
 
-    if (threadIdx.x == 0) { s_used = 0; s_refused = 0; }
-    int tokens = 0, returned = 0, needed = 0;
-    for (int s0 = 0; s0 < p.n_seq; s0 += kThreads) {
-        const int s = s0 + threadIdx.x;
-        int len = 0, nw = 0;
-        bool in = s < p.n_seq, ended = false;
-        if (in) { len = length(s); nw = __ldg(p.new_lens + s); ended = nw < 0; nw = max(nw, 0); }
-        const int c = block_scan(nw, tokens, warp_sums);
-        const int b = block_scan(ended ? pages_of(len) : 0, returned, warp_sums);
-        const long long end = (long long)len + nw;
-        const bool fits = in && !ended && (nw == 0 || (end <= cap && c <= p.max_tokens));
-        const int n = block_scan(fits ? pages_of(end) - pages_of(len) : 0, needed, warp_sums);
-        if (in) { cu[s] = c; back_sum[s] = b; need_sum[s] = n; }
+    // The lengths, side by side, and then: a thread sums up n_seq / threads
+    // requests that follow one another, the block the threads' sums.  What a
+    // request needs depends on the first of the sums.
+    for (int s = threadIdx.x; s < p.n_seq; s += blockDim.x) {
+        cu[s] = __ldg(p.new_lens + s);
+        need_sum[s] = length(s);
     }
     __syncthreads();
+    const int per = (p.n_seq + (int)blockDim.x - 1) / (int)blockDim.x;
+    const int s0 = min((int)threadIdx.x * per, p.n_seq), s1 = min(s0 + per, p.n_seq);
+    int c = 0, b = 0, n = 0, none = 0, tokens, returned, needed, ignored;
+    for (int s = s0; s < s1; s++) {
+        c = sat_add(c, max(cu[s], 0));
+        if (cu[s] < 0) b = sat_add(b, pages_of(need_sum[s]));
+    }
+    block_scan(c, b, tokens, returned, warp_sums);
+    for (int s = s0; s < s1; s++) {
+        const int len = need_sum[s], nw = cu[s];
+        const long long end = (long long)len + nw;
+        cu[s] = c = sat_add(c, max(nw, 0));
+        back_sum[s] = b = sat_add(b, nw < 0 ? pages_of(len) : 0);
+        const int need = nw > 0 && end <= cap && c <= p.max_tokens ? pages_of(end) - pages_of(len) : 0;
+        need_sum[s] = need;
+        n = sat_add(n, need);
+    }
+    block_scan(n, none, needed, ignored, warp_sums);
+    for (int s = s0; s < s1; s++) need_sum[s] = n = sat_add(n, need_sum[s]);
+    __syncthreads();
 
-    const int have_free = min(max(__ldg(p.free_count), 0), p.n_pages);
     const int avail = sat_add(have_free, returned);
     // a page of an ended request by its place among the returned ones
     auto returned_page = [&](int i) {
@@ -129,7 +145,9 @@ page_plan_kernel(const Params p)
     };
 
     // requests
-    const int tid = (int)(blockIdx.x * kThreads + threadIdx.x), total = (int)(gridDim.x * kThreads);
+    // (consecutive warps of the grid on different SMs: most outputs are short)
+    const int tid = (int)(((threadIdx.x >> 5) * gridDim.x + blockIdx.x) * 32 + (threadIdx.x & 31));
+    const int total = (int)(gridDim.x * blockDim.x);
     for (int s = tid; s < p.n_seq; s += total) {
         const int len = length(s), nw = __ldg(p.new_lens + s);
         p.lens_out[s] = nw < 0 ? 0 : served(s, len, nw) ? len + nw : len;
@@ -137,17 +155,9 @@ page_plan_kernel(const Params p)
     }
     // Pages taken: the need of the requests up to the last one that the list
     // reaches (every later need sum is larger, so the served ones come first).
-    {
-        const int k = first_above(need_sum, p.n_seq, avail);       // the first that the list does not reach
-        if (threadIdx.x == 0) s_used = k ? need_sum[k - 1] : 0;
-    }
-    if (blockIdx.x == 0) {
-        int refused = 0;
-        for (int s = threadIdx.x; s < p.n_seq; s += kThreads) {
-            const int nw = __ldg(p.new_lens + s);
-            refused += nw > 0 && !served(s, length(s), nw);
-        }
-        if (refused) atomicAdd(&s_refused, refused);
+    if (threadIdx.x == 0) {
+        const int reached = first_above(need_sum, p.n_seq, avail); // the first that the list does not reach
+        s_used = reached ? need_sum[reached - 1] : 0;
     }
     __syncthreads();
     const int used = s_used;
@@ -156,12 +166,21 @@ page_plan_kernel(const Params p)
         p.table[(long long)s * p.table_stride + pages_of(length(s)) + (i - need_before(s))] = list_page(avail - 1 - i);
     }
     for (int i = have_free + tid; i < min(avail - used, p.n_pages); i += total) p.free_pages[i] = returned_page(i - have_free);
-    if (tid == 0) {
-        p.cu_new[0] = 0;
-        p.counts[0] = min(avail - used, p.n_pages);
-        p.counts[1] = tokens;
-        p.counts[2] = s_refused;
-        p.counts[3] = used;
+    if (blockIdx.x == gridDim.x - 1) {
+        int refused = 0;
+        for (int s = threadIdx.x; s < p.n_seq; s += blockDim.x) {
+            const int nw = __ldg(p.new_lens + s);
+            refused += nw > 0 && !served(s, length(s), nw);
+        }
+        if (refused) atomicAdd(&s_refused, refused);
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            p.cu_new[0] = 0;
+            p.counts[0] = min(avail - used, p.n_pages);
+            p.counts[1] = tokens;
+            p.counts[2] = s_refused;
+            p.counts[3] = used;
+        }
     }
 
     // token rows
@@ -206,16 +225,18 @@ int launch_page_plan(const attn_page_shape *s, const int *lens, const int *new_l
     p.table_stride = s->table_stride ? s->table_stride : s->max_pages;
     p.n_seq = s->n_seq; p.max_pages = s->max_pages; p.max_tokens = s->max_tokens; p.n_pages = s->n_pages;
     p.log_page = __builtin_ctz((unsigned)s->page_size);
-    // A CTA for every 1024 token rows, or for as many pages as come back when an
-    // eighth of the tables does, up to one per SM (2048 requests of up to 8192
-    // tokens, 5 % ending: 20 us with the 2 CTAs of their 2048 rows, %STEP% us).
+    // A thread for every token row and request, and for as many pages as come
+    // back when an eighth of the tables does, up to one CTA per SM (2048
+    // requests of up to 8192 tokens, 5 % ending: 20 us with CTAs for their
+    // 2048 rows alone, 8.6 us).
     const long long back = std::min<long long>(s->n_pages, (long long)s->n_seq * s->max_pages) / 8;
-    const int grid = (int)std::max<long long>(1, std::min<long long>((std::max<long long>(s->max_tokens, back) + kThreads - 1) / kThreads,
-                                                                     sm_count_here()));
+    const long long work = std::max<long long>(std::max(s->max_tokens, s->n_seq), back);
+    const int threads = work <= 256 ? 256 : kThreads;
+    const int grid = (int)std::max<long long>(1, std::min<long long>((work + threads - 1) / threads, sm_count_here()));
     const size_t smem = (size_t)s->n_seq * 12;
     if (!ensure_smem_attr((const void *)page_plan_kernel, (size_t)kMaxSeq * 12))
         return set_error(ATTN_ERR_CUDA, "page plan: cannot set shared-memory size");
-    return check_pdl(launch_pdl(page_plan_kernel, dim3(grid), dim3(kThreads), smem, stream, p), "page_plan_kernel");
+    return check_pdl(launch_pdl(page_plan_kernel, dim3(grid), dim3(threads), smem, stream, p), "page_plan_kernel");
 }
 
 }  // namespace attn_host
