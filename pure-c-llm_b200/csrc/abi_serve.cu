@@ -177,7 +177,7 @@ int attn_rope_append_ex(const attn_rope_shape *s, const attn_paged_kv *cache, in
 static int check_prefix(const attn_prefix_shape *s, const attn_paged_kv *c, long long *rs) {
     if (!s) return set_error(ATTN_ERR_INVALID, "prefix decode: shape is NULL");
     if (s->n_seq < 0 || s->n_seq > 65535 || s->n_groups < 0 || s->n_groups > 65535 || s->heads < 1 || s->kv_heads < 1 ||
-        s->heads > 65535 || s->heads % s->kv_heads)
+        s->heads > 65535 || s->heads % s->kv_heads || (long long)s->n_seq * s->heads > (1 << 24))
         return set_error(ATTN_ERR_INVALID, "prefix decode: bad shape n_seq=%d n_groups=%d heads=%d kv_heads=%d",
                          s->n_seq, s->n_groups, s->heads, s->kv_heads);
     if (!head_dim_ok(s->head_dim))

@@ -51,6 +51,12 @@ __device__ __forceinline__ long long cache_row(const Params &p, const int *line,
 // The division of the work (prefix_decode.cu describes it)
 // ---------------------------------------------------------------------------
 constexpr int kEntries = 512;             // running sums of steps kept per CTA
+
+// a / b for a >= 0, b > 0: mostly in 32 bits, where a division is a quarter of
+// the instructions (the starts of the kernels are chains of them)
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
+}
 constexpr int kBegin = 1;                 // steps that the beginning and end of a segment count for
 
 // One part of the work.
@@ -173,8 +179,8 @@ struct Walk {
         const int teams = (int)min((long long)w.teams, total);
         l.steps = l.blocks = 0;
         if (team >= teams) return;
-        first = total * team / teams;
-        last = total * (team + 1) / teams;
+        first = quotient(total * team, teams);
+        last = quotient(total * (team + 1), teams);
         int lo = 0, hi = ceil_div(w.lines, w.per_entry);   // the last entry that begins at or before `first`
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -194,8 +200,8 @@ struct Walk {
                 s = 0;
                 s1 = -1;
                 if (n > 0 && at + n > first) {
-                    s = (int)((max(first, at) - at) / l.cost());
-                    s1 = (int)((min(last, at + n) - 1 - at) / l.cost());
+                    s = (int)quotient(max(first, at) - at, l.cost());
+                    s1 = (int)quotient(min(last, at + n) - 1 - at, l.cost());
                 }
             }
             const long long begin = at + (long long)s * l.cost() + kBegin;

@@ -147,8 +147,14 @@ prefix_rows_kernel(const __grid_constant__ Params p, const __grid_constant__ Par
     if (second) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// Joins the pieces of one query row: a CTA per (request, query head), its
-// warps taking the pieces in turn, a lane D/32 elements.
+// Joins the pieces of the query rows, a lane D/32 elements.  What counts is the
+// chain of dependent loads (lengths and first steps, then the pieces' m and l,
+// then their o), so each link's loads go out together: lane i takes piece i's
+// m and l, and the o's of kMany pieces are on their way at once.  With few rows
+// the four warps of a CTA share a row's pieces; with many, each takes a row
+// (8192 rows of 128: 35 us with four warps a row, 21 with one; 64 rows of 32
+// with some 20 pieces: 8 and 15 us).
+//
 // A slot of the tile kernel (w.half rows twice) holds, for a block of up to
 // w.half query rows, the pieces of its two warpgroups, which share the keys.
 struct Pieces {
@@ -157,17 +163,18 @@ struct Pieces {
     long long step;                       // rows between pieces
     int n;
 };
-constexpr int kMergeWarps = 4;
+constexpr int kMergeWarps = 4, kMany = 8;
 
+// `begin` and `total`: the line's first step and the part's steps.
 template <int D>
-__device__ __forceinline__ Pieces pieces_of(const Part &w, const Line &l, int line, int row, int hk) {
+__device__ __forceinline__ Pieces pieces_of(const Part &w, const Line &l, int row, int hk, long long begin, long long total) {
     Pieces r = {};
     if (l.steps == 0) return r;
     const int rb = row / w.seg_rows, hb = hk / w.head_block, hw = hk - hb * w.head_block;
-    const long long total = w.line_first[w.lines], teams = min((long long)w.teams, total);
-    const long long begin = w.line_first[line] + (long long)(rb * w.n_blocks + hb) * l.cost() + kBegin;
+    const long long teams = min((long long)w.teams, total);
+    begin += (long long)(rb * w.n_blocks + hb) * l.cost() + kBegin;
     // the team whose range [total t / teams, total (t + 1) / teams) holds a step
-    const int t0 = (int)(((begin + 1) * teams - 1) / total), t1 = (int)(((begin + l.steps) * teams - 1) / total);
+    const int t0 = (int)quotient((begin + 1) * teams - 1, total), t1 = (int)quotient((begin + l.steps) * teams - 1, total);
     const long long seg = (long long)(l.base + rb) * w.n_blocks + hb;
     const long long slot = ((seg + t0) * w.head_block + hw) * w.rows + row - rb * w.seg_rows;
     r.o = w.o + slot * D;
@@ -181,65 +188,98 @@ __device__ __forceinline__ Pieces pieces_of(const Part &w, const Line &l, int li
     return r;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool SHARED>   // SHARED: a row per CTA
 __global__ void __launch_bounds__(kMergeWarps * 32)
 prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Part own, const __grid_constant__ Part pre)
 {
     pdl_begin();                          // launched by launch_pdl
     constexpr int E = D / 32;
-    __shared__ float s_m[kMergeWarps], s_l[kMergeWarps], s_o[kMergeWarps][D];
-    const int s = blockIdx.y, h = blockIdx.x, hk = h / p.ratio, hr = h - hk * p.ratio;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    Pieces part[2];
-    part[0] = own.lines ? pieces_of<D>(own, line_of<false>(p, own, s), s, hr, hk) : Pieces{};
-    part[1] = Pieces{};
-    for (int g = 0; g < pre.lines; g++) {
-        const Line l = line_of<true>(p, pre, g);
-        if (s < l.first_req || (s - l.first_req) * p.ratio >= l.rows) continue;
-        part[1] = pieces_of<D>(pre, l, g, (s - l.first_req) * p.ratio + hr, hk);
-        break;
+    const int at = SHARED ? (int)blockIdx.x : (int)blockIdx.x * kMergeWarps + warp;
+    if (at >= p.n_seq * p.heads) return;
+    const int s = at / p.heads, h = at - s * p.heads, hk = h / p.ratio, hr = h - hk * p.ratio;
+
+    // the request's lines: its own and, by the lanes, 32 groups at a time
+    long long own_begin = 0, own_total = 0, pre_begin = 0, pre_total = 0;
+    Line own_line = {}, pre_line = {};
+    if (own.lines) {
+        own_begin = __ldcg(own.line_first + s);
+        own_total = __ldcg(own.line_first + own.lines);
+        own_line = line_of<false>(p, own, s);
     }
+    if (pre.lines) pre_total = __ldcg(pre.line_first + pre.lines);
+    for (int g0 = 0; g0 < pre.lines; g0 += 32) {
+        const int g = g0 + lane;
+        const bool in = g < pre.lines && s >= group_first(p, g) && s < group_first(p, g + 1);
+        const unsigned found = __ballot_sync(0xffffffffu, in);
+        if (found) {
+            const int mine = g0 + __ffs(found) - 1;
+            pre_begin = __ldcg(pre.line_first + mine);
+            pre_line = line_of<true>(p, pre, mine);
+            break;
+        }
+    }
+    const Pieces a = pieces_of<D>(own, own_line, hr, hk, own_begin, own_total);
+    const Pieces b = pieces_of<D>(pre, pre_line, (s - pre_line.first_req) * p.ratio + hr, hk, pre_begin, pre_total);
+
+    const int n = a.n + b.n;
     float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
     for (int i = 0; i < E; i++) o[i] = 0.f;
+    // piece j of the row; with SHARED, this warp's j-th
+    auto which = [&](int j) { return SHARED ? j * kMergeWarps + warp : j; };
+    for (int j0 = 0; which(j0) < n; j0 += 32) {
+        const int j = which(j0 + lane);
+        const float2 ml = j < a.n ? __ldcg(a.ml + j * a.step) : j < n ? __ldcg(b.ml + (j - a.n) * b.step) : make_float2(-INFINITY, 0.f);
+        const float mx = fmaxf(m, warp_max(ml.x));
+        if (mx == -INFINITY) continue;    // no valid row in these pieces
+        const float old = exp2f(m - mx), c = exp2f(ml.x - mx);
+        l = l * old + warp_sum(ml.y * c);
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const Pieces &r = part[k];
-        for (int j = warp; j < r.n; j += kMergeWarps) {
-            const float2 ml = __ldcg(r.ml + j * r.step);
-            float x[E];
+        for (int i = 0; i < E; i++) o[i] *= old;
+        m = mx;
+        for (int k0 = 0; k0 < 32 && which(j0 + k0) < n; k0 += kMany) {
+            float x[kMany][E];
 #pragma unroll
-            for (int i = 0; i < E; i++) x[i] = __ldcg(r.o + j * r.step * D + lane + 32 * i);
-            if (ml.x == -INFINITY) continue;          // no valid row in this piece
-            const float mx = fmaxf(m, ml.x), a = exp2f(m - mx), c = exp2f(ml.x - mx);
-            l = l * a + ml.y * c;
+            for (int k = 0; k < kMany; k++) {
+                const int q = which(j0 + k0 + k);
+                const float *from = (q < a.n ? a.o + q * a.step * D : b.o + (q - a.n) * b.step * D) + lane;
 #pragma unroll
-            for (int i = 0; i < E; i++) o[i] = o[i] * a + x[i] * c;
-            m = mx;
+                for (int i = 0; i < E; i++) x[k][i] = q < n ? __ldcg(from + 32 * i) : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < kMany; k++) {
+                // (a piece without a valid row has weight 0, and an o that may not have been written)
+                const float w = __shfl_sync(0xffffffffu, c, k0 + k);
+#pragma unroll
+                for (int i = 0; i < E; i++) o[i] = w > 0.f ? fmaf(x[k][i], w, o[i]) : o[i];
+            }
         }
     }
-    if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+    if constexpr (SHARED) {
+        __shared__ float s_m[kMergeWarps], s_l[kMergeWarps], s_o[kMergeWarps][D];
+        if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
 #pragma unroll
-    for (int i = 0; i < E; i++) s_o[warp][lane + 32 * i] = o[i];
-    __syncthreads();
-    float M = s_m[0];
+        for (int i = 0; i < E; i++) s_o[warp][lane + 32 * i] = o[i];
+        __syncthreads();
+        if (warp) return;
+        m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+        l = 0.f;
 #pragma unroll
-    for (int i = 1; i < kMergeWarps; i++) M = fmaxf(M, s_m[i]);
-    float c[kMergeWarps], L = 0.f;
+        for (int i = 0; i < E; i++) o[i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < kMergeWarps; i++) {
-        c[i] = s_m[i] == -INFINITY ? 0.f : exp2f(s_m[i] - M);
-        L += s_l[i] * c[i];
+        for (int k = 0; k < kMergeWarps; k++) {
+            const float c = s_m[k] == -INFINITY ? 0.f : exp2f(s_m[k] - m);
+            l += s_l[k] * c;
+#pragma unroll
+            for (int i = 0; i < E; i++) o[i] += s_o[k][lane + 32 * i] * c;
+        }
     }
-    if (threadIdx.x < D) {
-        float r = 0.f;
+    T *out = static_cast<T *>(p.out) + s * p.out_stride + (long long)h * D + lane;
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
 #pragma unroll
-        for (int i = 0; i < kMergeWarps; i++) r += s_o[i][threadIdx.x] * c[i];
-        static_cast<T *>(p.out)[s * p.out_stride + (long long)h * D + threadIdx.x] =
-            from_f32<T>(M == -INFINITY ? 0.f : r / L);
-    }
-    if (p.lse && threadIdx.x == 0)
-        p.lse[(long long)s * p.heads + h] = M == -INFINITY ? -INFINITY : (M + log2f(L)) * kLn2;
+    for (int i = 0; i < E; i++) out[32 * i] = from_f32<T>(o[i] * inv);
+    if (p.lse && lane == 0) p.lse[at] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 }  // namespace prefix
@@ -322,7 +362,11 @@ int run(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s) {
     if (L.pre.lines && (st = tile ? launch_prefix_tile(p, L.pre, D, s) : run_part<Pre, true, D, PRE_CTAS>(p, L.pre, 0, s)))
         return st;
     if (L.own.lines && (st = run_part<Own, false, D, OWN_CTAS>(p, L.own, L.pre.lines != 0, s))) return st;
-    return check_pdl(launch_pdl(prefix_merge_kernel<T, D>, dim3(p.heads, p.n_seq), dim3(kMergeWarps * 32), 0, s, p, L.own, L.pre),
+    const int rows = p.n_seq * p.heads;
+    const bool shared = rows < sm_count_here() * 16;
+    return check_pdl(launch_pdl(shared ? prefix_merge_kernel<T, D, true> : prefix_merge_kernel<T, D, false>,
+                                dim3(shared ? rows : (rows + kMergeWarps - 1) / kMergeWarps), dim3(kMergeWarps * 32), 0, s, p,
+                                L.own, L.pre),
                      "prefix_merge_kernel");
 }
 

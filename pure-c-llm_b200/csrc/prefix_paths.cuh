@@ -219,10 +219,11 @@ struct Bf16Path {
 #pragma unroll
                 for (int t = 0; t < NT; t++) mma_bf16(s[t][i], a, q[t][j][0], q[t][j][1]);
             }
+        // all tiles' maxima first, so that their exchanges overlap, and one vote
+        float neg[NT][2], alpha[NT][2];
+        bool grows = false;
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            float neg[2], alpha[2];
-            bool grows = false;
+        for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 float mx = -INFINITY;
@@ -234,27 +235,44 @@ struct Bf16Path {
                     }
                     mx = fmaxf(mx, fmaxf(s[t][i][e], s[t][i][e + 2]));
                 }
-                mx = fmaxf(m[t][e], keys_max(mx) * p.scale_log2);
-                neg[e] = mx == -INFINITY ? 0.f : -mx;
-                grows |= mx != m[t][e];
-                alpha[e] = ex2(m[t][e] + neg[e]);
-                m[t][e] = mx;
-                l[t][e] *= alpha[e];
-#pragma unroll
-                for (int i = 0; i < KM; i++) {
-                    s[t][i][e] = ex2(fmaf(s[t][i][e], p.scale_log2, neg[e]));
-                    s[t][i][e + 2] = ex2(fmaf(s[t][i][e + 2], p.scale_log2, neg[e]));
-                    l[t][e] += s[t][i][e] + s[t][i][e + 2];
-                }
+                neg[t][e] = mx;
             }
-            if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) neg[t][e] = fmaxf(neg[t][e], __shfl_xor_sync(0xffffffffu, neg[t][e], d));
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float mx = fmaxf(m[t][e], neg[t][e] * p.scale_log2);
+                grows |= mx != m[t][e];
+                neg[t][e] = mx == -INFINITY ? 0.f : -mx;
+                alpha[t][e] = ex2(m[t][e] + neg[t][e]);
+                m[t][e] = mx;
+            }
+        if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                l[t][0] *= alpha[t][0];
+                l[t][1] *= alpha[t][1];
 #pragma unroll
                 for (int j = 0; j < KS; j++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[t][j][e] *= alpha[e & 1];
+                    for (int e = 0; e < 4; e++) o[t][j][e] *= alpha[t][e & 1];
             }
+        }
 #pragma unroll
-            for (int i = 0; i < KM; i++)
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < KM; i++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[t][i][e] = ex2(fmaf(s[t][i][e], p.scale_log2, neg[t][e & 1]));
+                    l[t][e & 1] += s[t][i][e];
+                }
 #pragma unroll
                 for (int n = 0; n < 2; n++) {
                     if constexpr (NT == 1) {
@@ -265,7 +283,7 @@ struct Bf16Path {
                     }
                     hi[t][i][n] = transposed(hi[t][i][n]);
                 }
-        }
+            }
     }
     template <bool EDGE>
     __device__ __forceinline__ void values(const Params &, uint32_t st, unsigned mask) {
@@ -502,37 +520,54 @@ struct I8Path {
             }
             wscale = now;
         }
+        // all tiles' maxima first, so that their exchanges overlap, and one vote
         uint32_t pw[KM][NT][2];
+        float neg[NT], alpha[NT];
+        bool grows = false;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            float x[KM][2], mx = -INFINITY;
+            neg[t] = -INFINITY;
 #pragma unroll
             for (int i = 0; i < KM; i++)
 #pragma unroll
                 for (int n = 0; n < 2; n++) {
-                    x[i][n] = (s[t][i][2 * n] + s[t][i][2 * n + 1]) * qscale[t] * ks[i][n];
-                    if (EDGE && !(mask >> (16 * i + 8 * n + g) & 1)) x[i][n] = -INFINITY;
-                    mx = fmaxf(mx, x[i][n]);
+                    float x = (s[t][i][2 * n] + s[t][i][2 * n + 1]) * qscale[t] * ks[i][n];
+                    if (EDGE && !(mask >> (16 * i + 8 * n + g) & 1)) x = -INFINITY;
+                    s[t][i][2 * n] = x;
+                    neg[t] = fmaxf(neg[t], x);
                 }
-            mx = fmaxf(m[t], keys_max(mx));
-            const float neg = mx == -INFINITY ? 0.f : -mx;
-            if (__any_sync(0xffffffffu, mx != m[t])) {
-                const float a = ex2(m[t] + neg);
-                l[t] *= a;
-                scale_output(t, a);
-            }
+        }
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+            for (int t = 0; t < NT; t++) neg[t] = fmaxf(neg[t], __shfl_xor_sync(0xffffffffu, neg[t], d));
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const float mx = fmaxf(m[t], neg[t]);
+            grows |= mx != m[t];
+            neg[t] = mx == -INFINITY ? 0.f : -mx;
+            alpha[t] = ex2(m[t] + neg[t]);
             m[t] = mx;
+        }
+        if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                l[t] *= alpha[t];
+                scale_output(t, alpha[t]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++)
 #pragma unroll
             for (int i = 0; i < KM; i++)
 #pragma unroll
                 for (int n = 0; n < 2; n++) {
-                    const float e = ex2(x[i][n] + neg), w = e * (vs[i][n] * wscale);
+                    const float e = ex2(s[t][i][2 * n] + neg[t]), w = e * (vs[i][n] * wscale);
                     l[t] += e;
                     const __half hi = __float2half_rn(w);
                     const __half2 both = __halves2half2(hi, __float2half_rn(w - __half2float(hi)));
                     pw[i][t][n] = transposed(*reinterpret_cast<const uint32_t *>(&both));
                 }
-        }
 #pragma unroll
         for (int i = 0; i < KM; i++) {
 #pragma unroll
