@@ -29,9 +29,6 @@ __device__ __forceinline__ int checked_len(const Params &p, int len, int most) {
     return len;
 }
 __device__ __forceinline__ int own_len(const Params &p, int s) { return checked_len(p, __ldg(p.lens + s), p.max_len); }
-__device__ __forceinline__ int prefix_len(const Params &p, int g) {
-    return checked_len(p, __ldg(p.prefix_lens + g), p.max_prefix_len);
-}
 // first request of group g, within [0, n_seq]
 __device__ __forceinline__ int group_first(const Params &p, int g) {
     return min(max(__ldg(p.group_begin + g), 0), p.n_seq);
@@ -96,8 +93,9 @@ template <bool PRE>
 __device__ __forceinline__ Line line_of(const Params &p, const Part &w, int i) {
     Line l;
     if (PRE) {
+        const int len = __ldg(p.prefix_lens + i);            // on its way with the group's bounds
         group_blocks(p, w, i, l.first_req, l.rows, l.blocks, l.base);
-        l.keys = l.rows ? prefix_len(p, i) : 0;
+        l.keys = l.rows ? checked_len(p, len, p.max_prefix_len) : 0;
     } else {
         l.first_req = i;
         l.rows = p.ratio;

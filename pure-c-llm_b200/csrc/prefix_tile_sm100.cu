@@ -11,20 +11,20 @@
 // 256 query rows: with more than 128, warpgroup w takes rows [128 w, 128 w + 128)
 // of every step; with fewer, both take the same rows and every other step, and
 // the merge finds two pieces in the slot.  12 warps:
-//   warps 0-1   bring in Q rows and the keys' K and V rows.  A step whose 128
-//               keys all have rows is a few TMA boxes of a page's rows x 64 dims;
-//               at a line's end, with pages of fewer than 8 rows or outside the
-//               cache, and for Q, the lanes copy 16 bytes each into the same
+//   warp 0      K rows, warp 1 V rows.  A step whose 128 keys all have rows is a
+//               TMA box of 64 dims for each page (or 128 rows of one), a lane
+//               per box.  At a line's end, with pages of fewer than 8 rows or
+//               outside the cache, the lanes copy 16 bytes each into the same
 //               128-byte swizzled layout, with zeros for keys without a row, so
-//               that a probability of 0 never meets a NaN.  They report such a
-//               half (K or V of a step) when kLag more are on their way.  (All
-//               steps by lanes: 299 us for the prefixes above, the copying
-//               warps' instructions setting the pace.)
+//               that a probability of 0 never meets a NaN; they report such a
+//               half (K or V of a step) when their next one is on its way.
+//               (All steps by lanes: 299 us for the prefixes above, the copying
+//               instructions setting the pace.)
 //   warp 2      S_wu = Q_w K_u^T for the two halves u of a step's keys, M = 128,
 //               N = 64, both operands in shared memory
 //   warp 3      O_w += P_wu V_u (P from TMEM, V as it lies, MN-major)
 //   warps 4-7   softmax of warpgroup 0, warps 8-11 of warpgroup 1: a thread owns
-//               a row (a TMEM lane), keeps its maximum and sum, writes its bf16
+//               a row (a TMEM lane), brings it in, keeps its maximum and sum, writes its bf16
 //               probabilities to TMEM, and rescales O when the maximum grew by
 //               more than 2^8 (a stale one leaves P <= 256, and the piece's
 //               (m, l, o) stay consistent).  All exponentials on MUFU: lse is an
@@ -51,12 +51,13 @@ using namespace prefix;
 
 constexpr int BM = 128, BN = 128, BH = 64;   // query rows; keys of a step, of an S
 constexpr int kThreads = 384;
-constexpr int kLag = 2;                   // halves on their way when one is reported
-constexpr int kMasks = 8;                 // steps whose key masks are kept: more than the ring holds, and the one at work
+constexpr int kMasks = 8;                 // steps whose key masks are kept: more than K's ring holds, and the ones at work
 
 template <int D>
 struct Cfg {
-    static constexpr int SLOTS = D == 64 ? 8 : 5;             // ring of halves: K, V, K, ...
+    // rings of K and V tiles (V waits longer for its use); one ring for both would be ambiguous to parity
+    // waits once one of the two copying warps runs ahead of the other
+    static constexpr int KS = D == 64 ? 4 : 2, VS = D == 64 ? 4 : 3, SLOTS = KS + VS;
     static constexpr int TILE = BM * D * 2;                   // Q tile, K or V tile: D / 64 blocks of 128 rows x 128 bytes
     static constexpr int OFF_KV = 2 * TILE;
     static constexpr int OFF_BAR = OFF_KV + SLOTS * TILE;
@@ -68,7 +69,7 @@ __device__ __forceinline__ uint32_t col_s(int wg, int u) { return (uint32_t)(wg 
 template <int D> __device__ __forceinline__ uint32_t col_o(int wg) { return 4 * BH + (uint32_t)wg * D; }
 
 enum {
-    B_QF = 0, B_QE = 1,                   // Q copied; its last S finished
+    B_QF = 0, B_QE = 1,                   // Q there; its last S finished
     B_OF = 2,                             // per warpgroup: O read out
     B_SF = 4, B_PF = 8, B_OD = 12,        // per warpgroup and half (2 w + u): S ready; P written; PV finished
     B_FULL = 16, B_FREE = 24,             // per slot: copied; used
@@ -77,6 +78,11 @@ enum {
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+// Place of 16-byte piece ch of row r in a tile: block of 64 dims, row, piece XOR row % 8.
+__device__ __forceinline__ uint32_t tile_at(int r, int ch) {
+    return (uint32_t)((ch / 8) * BM * 128 + r * 128 + (((ch % 8) ^ (r & 7)) << 4));
 }
 
 template <int D>
@@ -97,7 +103,7 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        mbar_init(BAR(B_QF), 64);
+        mbar_init(BAR(B_QF), 256);
         mbar_init(BAR(B_QE), 1);
         for (int i = 0; i < 2; i++) mbar_init(BAR(B_OF + i), 128);
         for (int i = 0; i < 4; i++) {
@@ -106,7 +112,7 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             mbar_init(BAR(B_OD + i), 1);
         }
         for (int s = 0; s < C::SLOTS; s++) {
-            mbar_init(BAR(B_FULL + s), 64);
+            mbar_init(BAR(B_FULL + s), 32);
             mbar_init(BAR(B_FREE + s), 1);
         }
         *abort_flag = 0;
@@ -133,60 +139,25 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     // 384 x 168 registers at launch: 128 x 88 + 256 x 208
     if (warp < 4) regs_dec<88>();
     if (warp < 2) {
-        // ------------------------------------------------------------ copies
-        auto wait = [&](int b, int parity, int code) -> bool {
-            return __all_sync(0xffffffffu, mbar_wait(BAR(b), parity & 1, abort_flag, p.err, code));
-        };
-        int due[kLag] = {}, n_due = 0;        // barriers of the halves on their way, oldest first
-        auto report = [&](int b) {
-            fence_async_smem();           // this thread's copies, for the tensor cores
-            mbar_arrive(BAR(b));
-        };
-        auto copied = [&](int b) {
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (n_due == kLag) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
-                report(due[0]);
-#pragma unroll
-                for (int i = 0; i + 1 < kLag; i++) due[i] = due[i + 1];
-                due[kLag - 1] = b;
-            } else {
-#pragma unroll
-                for (int i = 0; i < kLag; i++)
-                    if (i == n_due) due[i] = b;
-                n_due++;
-            }
-        };
+        // ------------------------------------------------------------ K, V
+        const int kv = warp;
+        const CUtensorMap *map = kv ? &tv : &tk;
+        if (lane == 0) prefetch_tmap(map);
+        int due = -1;                     // slot of a half that the lanes have on its way
         auto flush = [&] {
+            if (due < 0) return;
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll
-            for (int i = 0; i < kLag; i++)
-                if (i < n_due) report(due[i]);
-            n_due = 0;
+            fence_async_smem();           // this thread's copies, for the tensor cores
+            mbar_arrive(BAR(B_FULL + due));
+            due = -1;
         };
-        const bool leader = elect_one();
-        constexpr int RPI = 32 / CPR;     // rows per copy instruction of a warp
+        constexpr int RPI = 32 / CPR;     // rows per copy instruction
         const int lr = lane / CPR, ch = lane % CPR;
-        // a 16-byte piece's place in a tile: 64-column block, row, piece XOR row % 8
-        auto place = [&](int r) { return (uint32_t)((ch / 8) * BM * 128 + r * 128 + (((ch % 8) ^ (r & 7)) << 4)); };
         bool ok = true;
-        int g = 0;                        // steps copied
-        for (int k = 0; ok && walk.next(x); k++) {
-            const bool two = x.rows > BM;
-            flush();                      // the S that frees Q may wait for what is due
-            if (k > 0 && !(ok = wait(B_QE, k - 1, 0x801))) break;
-            for (int t = 0; t < (two ? 2 : 1); t++)
-#pragma unroll 4
-                for (int r0 = 0; r0 < 64; r0 += RPI) {
-                    const int r = warp * 64 + r0 + lr, row = x.row0 + t * BM + r;
-                    const bool there = t * BM + r < x.rows;
-                    const int s = x.first_req + row / p.ratio, h = x.hb * p.ratio + row % p.ratio;
-                    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(p.q) +
-                                               (there ? s * p.q_stride + (long long)h * D : 0) + ch * 8;
-                    copy16(sQ + t * C::TILE + place(r), src, there);
-                }
-            copied(B_QF);
-            // cache rows of a step's 128 keys (-1: none), four per lane in both warps, read a step ahead
+        int g = 0;                        // steps
+        while (ok && walk.next(x)) {
+            const __nv_bfloat16 *from = static_cast<const __nv_bfloat16 *>(kv ? p.v : p.k) + (long long)x.hb * D + ch * 8;
+            // cache rows of a step's 128 keys (-1: none), four per lane, read a step ahead
             int next[4];
             auto look_up = [&](int j) {
 #pragma unroll
@@ -201,58 +172,52 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 unsigned valid[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
+                    row[i] = next[i];
                     valid[i] = __ballot_sync(0xffffffffu, next[i] >= 0);
-                    row[i] = max(next[i], 0);
                 }
                 look_up(j + 1);
                 const bool whole = boxes && (valid[0] & valid[1] & valid[2] & valid[3]) == 0xffffffffu;
+                const int ring = kv ? C::VS : C::KS, slot = kv ? C::KS + g % C::VS : g % C::KS;
+                const uint32_t to = sKV + slot * C::TILE;
+                if (g >= ring) {
+                    flush();              // nothing may stay due behind the wait
+                    ok = mbar_wait(BAR(B_FREE + slot), (g / ring + 1) & 1, abort_flag, p.err, 0x801 + kv);
+                    if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                }
+                if (kv == 0 && lane == 0) {
 #pragma unroll
-                for (int kv = 0; kv < 2; kv++) {
-                    const int half = 2 * g + kv, slot = half % C::SLOTS;
-                    const uint32_t to = sKV + slot * C::TILE;
-                    if (half >= C::SLOTS) {
-                        if (whole) flush();       // nothing may stay due behind the wait
-                        if (!(ok = wait(B_FREE + slot, half / C::SLOTS + 1, 0x802))) break;
+                    for (int i = 0; i < 4; i++) masks[g % kMasks * 4 + i] = valid[i];
+                }
+                __syncwarp();
+                if (whole) {
+                    const int rows = BN / boxes, key = lane * rows & 127;     // of lane n's box
+                    int r = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int y = __shfl_sync(0xffffffffu, row[i], key & 31);
+                        if (key >> 5 == i) r = y;
                     }
-                    if (kv == 0 && warp == 0 && lane == 0) {
+                    if (lane == 0) mbar_arrive_expect_tx(BAR(B_FULL + slot), C::TILE);
+                    else mbar_arrive(BAR(B_FULL + slot));
+                    __syncwarp();
+                    if (lane < boxes) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) masks[g % kMasks * 4 + i] = valid[i];
+                        for (int d = 0; d < D / 64; d++)
+                            tma_load_3d(to + d * BN * 128 + key * 128, map, BAR(B_FULL + slot), x.hb * D + 64 * d, r, 0);
                     }
                     __syncwarp();
-                    if (whole) {
-                        if (warp == 0) {
-                            if (leader) mbar_arrive_expect_tx(BAR(B_FULL + slot), C::TILE);
-                            __syncwarp();
-                            const int rows = BN / boxes;      // of a box
-                            for (int n = 0; n < boxes; n++) {
-                                const int key = n * rows;
-                                const int r = __shfl_sync(0xffffffffu, key < 64 ? (key < 32 ? row[0] : row[1]) : (key < 96 ? row[2] : row[3]), key & 31);
-                                if (leader) {
-#pragma unroll
-                                    for (int d = 0; d < D / 64; d++)
-                                        tma_load_3d(to + d * BN * 128 + key * 128, kv ? &tv : &tk, BAR(B_FULL + slot),
-                                                    x.hb * D + 64 * d, r, 0);
-                                }
-                                __syncwarp();
-                            }
-                        }
-                        if (warp != 0 || !leader) mbar_arrive(BAR(B_FULL + slot));
-                        __syncwarp();
-                        if (kv) flush();          // the query rows, behind the first step's boxes
-                        continue;
-                    }
-                    const __nv_bfloat16 *from = static_cast<const __nv_bfloat16 *>(kv ? p.v : p.k) + (long long)x.hb * D + ch * 8;
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-#pragma unroll 4
-                        for (int r0 = 0; r0 < 32; r0 += RPI) {
-                            const int r = __shfl_sync(0xffffffffu, warp ? row[2 + i] : row[i], r0 + lr);
-                            const bool there = (warp ? valid[2 + i] : valid[i]) >> (r0 + lr) & 1;
-                            copy16(to + place(warp * 64 + 32 * i + r0 + lr), from + (long long)r * p.row_stride, there);
-                        }
-                    copied(B_FULL + slot);
+                    continue;
                 }
-                if (!ok) break;
+                flush();
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll 4
+                    for (int r0 = 0; r0 < 32; r0 += RPI) {
+                        const int r = __shfl_sync(0xffffffffu, row[i], r0 + lr);
+                        copy16(to + tile_at(32 * i + r0 + lr, ch), from + (long long)max(r, 0) * p.row_stride, r >= 0);
+                    }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                due = slot;
             }
         }
         if (ok) flush();
@@ -270,8 +235,8 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             const bool two = x.rows > BM;
             if (!(ok = wait(B_QF, k, 0x811))) break;
             for (int j = x.a; ok && j < x.b; j++, g++) {
-                const int slot = 2 * g % C::SLOTS;
-                if (!(ok = wait(B_FULL + slot, 2 * g / C::SLOTS, 0x812))) break;
+                const int slot = g % C::KS;
+                if (!(ok = wait(B_FULL + slot, g / C::KS, 0x812))) break;
 #pragma unroll
                 for (int n = 0; n < 4; n++) {
                     const int u = n >> 1, wg = n & 1, b = 2 * wg + u;
@@ -314,8 +279,8 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         while (ok && walk.next(x)) {
             const bool two = x.rows > BM;
             for (int j = x.a; ok && j < x.b; j++, g++) {
-                const int slot = (2 * g + 1) % C::SLOTS;
-                if (!(ok = wait(B_FULL + slot, (2 * g + 1) / C::SLOTS, 0x821))) break;
+                const int slot = C::KS + g % C::VS;
+                if (!(ok = wait(B_FULL + slot, g / C::VS, 0x821))) break;
 #pragma unroll
                 for (int n = 0; n < 4; n++) {
                     const int u = n >> 1, wg = n & 1, b = 2 * wg + u;
@@ -349,8 +314,21 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16), tO = lanes + col_o<D>(wg);
         int g = 0, t = 0;                 // steps of the CTA; of this warpgroup
         bool ok = true;
-        while (ok && walk.next(x)) {
+        for (int k = 0; ok && walk.next(x); k++) {
             const bool two = x.rows > BM;
+            // this thread's query row (with up to 128 rows, warpgroup 0 brings them in for both)
+            if (k > 0) ok = mbar_wait(BAR(B_QE), (k - 1) & 1, abort_flag, p.err, 0x830);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            if (two || wg == 0) {
+                const int r = wg * BM + row, at = x.row0 + min(r, x.rows - 1);
+                const int s = x.first_req + at / p.ratio, h = x.hb * p.ratio + at % p.ratio;
+                const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(p.q) + s * p.q_stride + (long long)h * D;
+#pragma unroll
+                for (int c = 0; c < CPR; c++) copy16(sQ + wg * C::TILE + tile_at(row, c), src + 8 * c, r < x.rows);
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_async_smem();
+            }
+            mbar_arrive(BAR(B_QF));
             const int mine = two ? x.rows - wg * BM : x.rows;     // query rows of this warpgroup
             const bool idle = quad * 32 >= mine;                  // none of them in this warp: it only keeps step
             float m = -INFINITY, l = 0.f;
