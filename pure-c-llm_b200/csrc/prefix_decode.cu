@@ -59,7 +59,7 @@ __device__ __forceinline__ void run_piece(const Params &p, uint32_t ring, const 
     };
     bool next_valid;
     int next_row = row_of(a, next_valid), row = 0;
-    path.begin(p, first_req, row0, rows, hk);
+    path.begin(p, ring + SLOTS * Path::SLOT, first_req, row0, rows, hk);
     unsigned masks[AHEAD + 1];            // keys with a row, of this step and the ones in flight
     auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
     auto copy_k = [&](int step, int slot) {
@@ -111,10 +111,10 @@ __device__ __forceinline__ void run_piece(const Params &p, uint32_t ring, const 
 
 // Slots of a warp's ring: as many (an odd number) as CTAS rings of kWarps fit an SM, up to 7.
 template <class Path, int CTAS> struct Ring {
-    static constexpr int FIT = (CTAS == 1 ? 216 : 108) * 1024 / kWarps / Path::SLOT;
+    static constexpr int FIT = ((CTAS == 1 ? 216 : 108) * 1024 / kWarps - Path::SCRATCH) / Path::SLOT;
     static constexpr int SLOTS = FIT > 7 ? 7 : (FIT - 1) / 2 * 2 + 1;
-    static constexpr int BYTES = SLOTS * Path::SLOT;
-    static_assert(Path::SLOT % 128 == 0, "swizzled rows begin on 128 bytes");
+    static constexpr int BYTES = SLOTS * Path::SLOT + Path::SCRATCH;
+    static_assert(Path::SLOT % 128 == 0 && Path::SCRATCH % 128 == 0, "swizzled rows begin on 128 bytes");
 };
 
 // PRE: the groups' prefixes; otherwise the requests' own rows.  `second`: the

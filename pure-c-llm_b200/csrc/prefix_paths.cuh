@@ -166,14 +166,14 @@ __device__ __forceinline__ const T *query(const Params &p, int first_req, int ro
 // ---------------------------------------------------------------------------
 template <int D, int NT>
 struct Bf16Path {
-    static constexpr int ROWS = 8 * NT, KEYS = D <= 64 ? 32 : 16, LEAN = NT == 1;
+    static constexpr int ROWS = 8 * NT, KEYS = D <= 64 ? 32 : 16, LEAN = NT == 1, SCRATCH = 0;
     static constexpr int KM = KEYS / 16, KS = D / 16;         // 16-key tiles; 16-dim tiles
     static constexpr int PITCH = 2 * D, SLOT = KEYS * PITCH;
     uint32_t q[NT][KS][2], hi[NT][KM][2], lo[KM][2];          // queries; the step's probabilities
     float o[NT][KS][4], m[NT][2], l[NT][2];
     const char *kb, *vb;
 
-    __device__ __forceinline__ void begin(const Params &p, int first_req, int row0, int rows, int hk) {
+    __device__ __forceinline__ void begin(const Params &p, uint32_t, int first_req, int row0, int rows, int hk) {
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -365,7 +365,7 @@ __device__ __forceinline__ int exponent(float x) { return min(100, max(-100, (__
 
 template <int D, int NT>
 struct I8Path {
-    static constexpr int ROWS = 4 * NT, KEYS = 32, FOLD = 8, LEAN = NT == 1;
+    static constexpr int ROWS = 4 * NT, KEYS = 32, FOLD = 8, LEAN = NT == 1, SCRATCH = 0;
     static constexpr int KM = KEYS / 16, B64 = D / 64, REM = D % 64 != 0;
     static constexpr int KW = D / 16;                         // words of a K row per lane = k-steps = 16-dim tiles
     // a V slot holds its rows and both scales (K's are used with V's, once the code sums are there)
@@ -379,7 +379,7 @@ struct I8Path {
     int folded, head;
     const char *kb, *vb;
 
-    __device__ __forceinline__ void begin(const Params &p, int first_req, int row0, int rows, int hk) {
+    __device__ __forceinline__ void begin(const Params &p, uint32_t, int first_req, int row0, int rows, int hk) {
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -613,38 +613,57 @@ struct I8Path {
 // ---------------------------------------------------------------------------
 // fp32: fp32 FMAs on pairs, R query rows.
 //
-// LPK lanes share a key, each with E = D / LPK of its dims, so a score is a
-// dot product of E terms and log2(LPK) shuffles; each group of LPK lanes keeps
+// LPK lanes share a key, each with E = D / LPK of its dims, so a score is a dot
+// product of E terms and a sum over LPK lanes; each group of LPK lanes keeps
 // its own running softmax over its keys (every 32/LPK-th) and the groups join
 // once, in finish().  At most 4 R flops stand against a byte (R/2 of them), so
 // up to 8 rows the FMA pipe keeps up with the memory.
+//
+// SPREAD (8 rows): a step's R U scores of a group are summed by halving, a lane
+// handing on half of its values at each stage and keeping the other, so the
+// lanes end with R U / LPK scores each (8 / LPK of a row's lanes) instead of all
+// of them in every lane; each lane does the softmax of its own, and the
+// probabilities reach the group through a scratch of shared memory, as pairs.
+// (All scores in all lanes took 1,010 instructions a step of 8 keys at d 128,
+// 256 of them FMAs.)
 // ---------------------------------------------------------------------------
 template <int D, int R>
 struct F32Path {
     static constexpr int ROWS = R;
+    static constexpr bool SPREAD = R == 8;
     // 8 or 16 lanes read 128 bytes of a row together; q and o take 2 E R registers, 64 to 96
     static constexpr int LPK = R >= 4 && D > 32 ? 16 : 8, LEAN = R <= 4;
     static constexpr int E = D / LPK, W = E % 4 ? 2 : 4, N = E / W;   // floats per lane, per read, reads
     static constexpr int G = 32 / LPK;                        // keys at a time
     static constexpr int U = (D >= 96 ? 8 : D == 64 ? 16 : 32) / G;   // keys of a group per step
     static constexpr int KEYS = G * U, SLOT = KEYS * D * 4;
-    static_assert(KEYS <= 32 && LPK * E == D && N * W == E, "lane geometry");
+    static constexpr int L = SPREAD ? LPK / R : 1;            // lanes of a row
+    static constexpr int MINE = SPREAD ? U / L : U;           // scores of a row in a lane
+    static constexpr int M = SPREAD ? 1 : R;                  // rows whose m and l a lane keeps
+    static constexpr int SCRATCH = SPREAD ? G * R * U * 8 : 0;
+    static_assert(KEYS <= 32 && LPK * E == D && N * W == E && (!SPREAD || (LPK % R == 0 && MINE % 2 == 0)), "lane geometry");
     uint64_t q[R][E / 2], o[R][E / 2];
-    float m[R], l[R], x[R][U];                                // x: the step's scores, then probabilities
+    float m[M], l[M], x[SPREAD ? 1 : R][U];                   // x: the step's scores, then probabilities
+    uint32_t scratch;
     const char *kb, *vb;
 
     __device__ __forceinline__ static void read(uint64_t (&x)[E / 2], uint32_t at) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            if constexpr (W == 4)
-                asm volatile("ld.shared.v2.u64 {%0,%1}, [%2];" : "=l"(x[2 * i]), "=l"(x[2 * i + 1]) : "r"(at + i * LPK * 16) : "memory");
-            else
+            if constexpr (W == 4) {
+                pair(x[2 * i], x[2 * i + 1], at + i * LPK * 16);
+            } else {
                 asm volatile("ld.shared.u64 %0, [%1];" : "=l"(x[i]) : "r"(at + i * LPK * 8) : "memory");
+            }
         }
     }
-    __device__ __forceinline__ void begin(const Params &p, int first_req, int row0, int rows, int hk) {
+    __device__ __forceinline__ static void pair(uint64_t &a, uint64_t &b, uint32_t at) {
+        asm volatile("ld.shared.v2.u64 {%0,%1}, [%2];" : "=l"(a), "=l"(b) : "r"(at) : "memory");
+    }
+    __device__ __forceinline__ void begin(const Params &p, uint32_t scratch_, int first_req, int row0, int rows, int hk) {
         const int sub = (threadIdx.x & 31) % LPK;
         const uint64_t s2 = f2(p.scale_log2, p.scale_log2);
+        scratch = scratch_;
 #pragma unroll
         for (int r = 0; r < R; r++) {
             const float *a = query<float>(p, first_req, row0 + min(r, rows - 1), hk, D) + sub * W;
@@ -654,6 +673,9 @@ struct F32Path {
                 q[r][i] = fma2(f2(x.x, x.y), s2, 0ull);
                 o[r][i] = 0ull;
             }
+        }
+#pragma unroll
+        for (int r = 0; r < M; r++) {
             m[r] = -INFINITY;
             l[r] = 0.f;
         }
@@ -668,10 +690,15 @@ struct F32Path {
     __device__ __forceinline__ void copy_v(const Params &p, uint32_t st, int row) const {
         copy_rows<KEYS, D * 4, D * 4, AS_IS, RUNS>(st, vb, p.row_stride * 4, row);
     }
+    __device__ __forceinline__ void scale_output(int r, float a) {
+#pragma unroll
+        for (int i = 0; i < E / 2; i++) o[r][i] = fma2(o[r][i], f2(a, a), 0ull);
+    }
     template <bool EDGE>
     __device__ __forceinline__ void scores(const Params &, uint32_t st, unsigned mask) {
         const int lane = threadIdx.x & 31, g = lane / LPK;
         st += g * D * 4 + lane % LPK * W * 4;
+        float y[R * U];                   // score r U + u: this lane's part, then the sum
 #pragma unroll
         for (int u = 0; u < U; u++) {
             uint64_t k[E / 2];
@@ -683,35 +710,72 @@ struct F32Path {
                 for (int i = 0; i < E / 2; i++) a = fma2(q[r][i], k[i], a);
                 float lo, hi;
                 f2_split(a, lo, hi);
-                x[r][u] = lo + hi;
+                y[r * U + u] = lo + hi;
             }
         }
+        if constexpr (SPREAD) {
+            const int sub = lane % LPK;
 #pragma unroll
-        for (int d = LPK / 2; d > 0; d >>= 1)
+            for (int d = LPK / 2, n = R * U / 2; d > 0; d >>= 1, n >>= 1) {
+                const bool upper = sub & d;
 #pragma unroll
-            for (int r = 0; r < R; r++)
-#pragma unroll
-                for (int u = 0; u < U; u++) x[r][u] += __shfl_xor_sync(0xffffffffu, x[r][u], d);
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            float mx = m[r];
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                if (EDGE && !(mask >> (u * G + g) & 1)) x[r][u] = -INFINITY;
-                mx = fmaxf(mx, x[r][u]);
+                for (int i = 0; i < R * U / 2; i++) {
+                    if (i >= n) break;
+                    const float send = upper ? y[i] : y[i + n], keep = upper ? y[i + n] : y[i];
+                    y[i] = keep + __shfl_xor_sync(0xffffffffu, send, d);
+                }
             }
+            // now scores sub MINE + i: row sub / L, keys (sub % L) MINE + i of the group
+            float mx = m[0];
+#pragma unroll
+            for (int i = 0; i < MINE; i++) {
+                if (EDGE && !(mask >> (((sub % L) * MINE + i) * G + g) & 1)) y[i] = -INFINITY;
+                mx = fmaxf(mx, y[i]);
+            }
+#pragma unroll
+            for (int d = 1; d < L; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
             const float neg = mx == -INFINITY ? 0.f : -mx;
-            if (mx != m[r]) {
-                const float a = ex2(m[r] + neg);
-                l[r] *= a;
+            if (__any_sync(0xffffffffu, mx != m[0])) {
+                const float a = ex2(m[0] + neg);
+                l[0] *= a;
 #pragma unroll
-                for (int i = 0; i < E / 2; i++) o[r][i] = fma2(o[r][i], f2(a, a), 0ull);
-                m[r] = mx;
+                for (int r = 0; r < R; r++) scale_output(r, __shfl_sync(0xffffffffu, a, g * LPK + r * L));
+                m[0] = mx;
             }
+            const uint32_t to = scratch + (g * R * U + sub * MINE) * 8;
+            __syncwarp();                 // the last step's probabilities are read
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                x[r][u] = ex2(x[r][u] + neg);
-                l[r] += x[r][u];
+            for (int i = 0; i < MINE; i += 2) {
+                const float a = ex2(y[i] + neg), b = ex2(y[i + 1] + neg);
+                l[0] += a + b;
+                asm volatile("st.shared.v4.f32 [%0], {%1,%1,%2,%2};" ::"r"(to + i * 8), "f"(a), "f"(b) : "memory");
+            }
+            __syncwarp();
+        } else {
+#pragma unroll
+            for (int d = LPK / 2; d > 0; d >>= 1)
+#pragma unroll
+                for (int i = 0; i < R * U; i++) y[i] += __shfl_xor_sync(0xffffffffu, y[i], d);
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                float mx = m[r];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (EDGE && !(mask >> (u * G + g) & 1)) y[r * U + u] = -INFINITY;
+                    mx = fmaxf(mx, y[r * U + u]);
+                }
+                const float neg = mx == -INFINITY ? 0.f : -mx;
+                if (mx != m[r]) {
+                    const float a = ex2(m[r] + neg);
+                    l[r] *= a;
+                    scale_output(r, a);
+                    m[r] = mx;
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    x[r][u] = ex2(y[r * U + u] + neg);
+                    l[r] += x[r][u];
+                }
             }
         }
     }
@@ -719,37 +783,65 @@ struct F32Path {
     __device__ __forceinline__ void values(const Params &, uint32_t st, unsigned mask) {
         const int lane = threadIdx.x & 31, g = lane / LPK;
         st += g * D * 4 + lane % LPK * W * 4;
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            uint64_t v[E / 2];
+        auto value = [&](uint64_t (&v)[E / 2], int u) {
             read(v, st + u * G * D * 4);
             if (EDGE && !(mask >> (u * G + g) & 1)) {       // probability 0, and values that may be NaN
 #pragma unroll
                 for (int i = 0; i < E / 2; i++) v[i] = 0ull;
             }
+        };
+        if constexpr (SPREAD) {
 #pragma unroll
-            for (int r = 0; r < R; r++)
+            for (int u = 0; u < U; u += 2) {
+                uint64_t v[E / 2], w[E / 2];
+                value(v, u);
+                value(w, u + 1);
 #pragma unroll
-                for (int i = 0; i < E / 2; i++) o[r][i] = fma2(f2(x[r][u], x[r][u]), v[i], o[r][i]);
+                for (int r = 0; r < R; r++) {
+                    uint64_t a, b;
+                    pair(a, b, scratch + (g * R * U + r * U + u) * 8);
+#pragma unroll
+                    for (int i = 0; i < E / 2; i++) o[r][i] = fma2(b, w[i], fma2(a, v[i], o[r][i]));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                uint64_t v[E / 2];
+                value(v, u);
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int i = 0; i < E / 2; i++) o[r][i] = fma2(f2(x[r][u], x[r][u]), v[i], o[r][i]);
+            }
         }
     }
     __device__ __forceinline__ void finish(float *out, float2 *ml, int rows) {
-        const int lane = threadIdx.x & 31, sub = lane % LPK;
+        const int lane = threadIdx.x & 31, sub = lane % LPK, g = lane / LPK;
+        float a[M];
 #pragma unroll
-        for (int r = 0; r < R; r++) {
+        for (int r = 0; r < M; r++) {
             float mx = m[r];
 #pragma unroll
             for (int d = LPK; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            const float a = mx == -INFINITY ? 0.f : ex2(m[r] - mx);
-            float sum = l[r] * a;
+            a[r] = mx == -INFINITY ? 0.f : ex2(m[r] - mx);
+            float sum = l[r] * a[r];
+#pragma unroll
+            for (int d = 1; d < L; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
 #pragma unroll
             for (int d = LPK; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            const int row = SPREAD ? sub / L : r;
+            if (g == 0 && row < rows && (SPREAD ? sub % L == 0 : sub == 0)) ml[row] = make_float2(mx, sum);
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const float b = SPREAD ? __shfl_sync(0xffffffffu, a[0], g * LPK + r * L) : a[SPREAD ? 0 : r];
 #pragma unroll
             for (int i = 0; i < E / 2; i++) {
                 float lo, hi;
                 f2_split(o[r][i], lo, hi);
-                lo *= a;
-                hi *= a;
+                lo *= b;
+                hi *= b;
 #pragma unroll
                 for (int d = LPK; d < 32; d <<= 1) {
                     lo += __shfl_xor_sync(0xffffffffu, lo, d);
@@ -758,7 +850,6 @@ struct F32Path {
                 const int dim = i / (W / 2) * (LPK * W) + sub * W + i % (W / 2) * 2;
                 if (lane < LPK && r < rows) *reinterpret_cast<float2 *>(out + r * D + dim) = make_float2(lo, hi);
             }
-            if (lane == 0 && r < rows) ml[r] = make_float2(mx, sum);
         }
     }
 };
