@@ -347,16 +347,17 @@ int run_part(const attn::prefix::Params &p, const attn::prefix::Part &w, int sec
                      "prefix_rows_kernel");
 }
 
-template <class Own, class Pre, typename T, int D>
+template <class Own, class Pre, int D>
 int run(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s) {
     using namespace attn::prefix;
-    constexpr int OWN_CTAS = Own::LEAN ? 2 : 1, PRE_CTAS = 1;
+    using T = typename Own::Type;
+    constexpr int OWN_CTAS = Own::LEAN ? 2 : 1, PRE_CTAS = Pre::LEAN ? 2 : 1;
     // The tensor-core tiles take prefixes of bf16 caches from 32 query rows a
     // group on (counted on average: the groups' sizes are on the device).
     const bool tile = sizeof(T) == 2 && (D == 64 || D == 128) && p.n_groups &&
                       (long long)p.n_seq * p.ratio >= 32LL * p.n_groups;
     const Layout L = lay_out(p, D, Own::ROWS, Own::KEYS, sm_count_here() * OWN_CTAS, Pre::ROWS, Pre::KEYS,
-                             sm_count_here() * PRE_CTAS, tile, static_cast<char *>(ws));
+                             sm_count_here() * (tile ? 1 : PRE_CTAS), tile, static_cast<char *>(ws));
     if (need) { *need = L.bytes; return ATTN_OK; }
     int st;
     if (L.pre.lines && (st = tile ? launch_prefix_tile(p, L.pre, D, s) : run_part<Pre, true, D, PRE_CTAS>(p, L.pre, 0, s)))
@@ -370,27 +371,42 @@ int run(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s) {
                      "prefix_merge_kernel");
 }
 
+// Paths by the rows a part has: own rows have ratio of them (more than a path
+// holds make more blocks, which read the cache again); a prefix has those of
+// its group, counted on average, since the groups' sizes are on the device.
+template <class Own, int D>
+int run_pre(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s, long long rows) {
+    using namespace attn::prefix;
+    // as many rows as the registers hold (o takes D NT / 4 of them), where there are more than one tile's
+    constexpr bool BF16 = sizeof(typename Own::Type) == 2;
+    if constexpr (BF16) {
+        if (rows <= 8) return run<Own, Bf16Path<D, 1>, D>(p, ws, need, s);
+        return run<Own, Bf16Path<D, D == 32 ? 8 : D == 64 ? 4 : 2>, D>(p, ws, need, s);
+    } else {
+        if (rows <= 4) return run<Own, I8Path<D, 1>, D>(p, ws, need, s);
+        return run<Own, I8Path<D, D <= 64 ? 4 : 2>, D>(p, ws, need, s);
+    }
+}
+template <class Own, int D>
+int run_pre_f32(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s, long long rows) {
+    using namespace attn::prefix;
+    if (rows <= 4) return run<Own, F32Path<D, 4>, D>(p, ws, need, s);
+    return run<Own, F32Path<D, 8>, D>(p, ws, need, s);
+}
+
 template <int D>
 int run_d(const attn::prefix::Params &p, int kv_dtype, void *ws, size_t *need, cudaStream_t s) {
     using namespace attn::prefix;
-    // Tiles of query rows per warp: own rows as the request needs (more rows
-    // than two tiles hold make more blocks); for a prefix, K and V are read
-    // again for every block, so as many as the registers hold (o takes D NT / 4).
-    if (kv_dtype == ATTN_BF16) {
-        constexpr int N = D == 32 ? 8 : D == 64 ? 4 : 2;
-        return p.ratio <= 8 ? run<Bf16Path<D, 1>, Bf16Path<D, N>, __nv_bfloat16, D>(p, ws, need, s)
-                            : run<Bf16Path<D, 2>, Bf16Path<D, N>, __nv_bfloat16, D>(p, ws, need, s);
-    }
-    if (kv_dtype == ATTN_I8) {
-        constexpr int N = D <= 64 ? 4 : 2;
-        return p.ratio <= 4 ? run<I8Path<D, 1>, I8Path<D, N>, float, D>(p, ws, need, s)
-                            : run<I8Path<D, 2>, I8Path<D, N>, float, D>(p, ws, need, s);
-    }
-    // fp32: FMAs grow with the rows, so own rows take the request's, up to 8
-    if (p.ratio == 1) return run<F32Path<D, 1>, F32Path<D, 8>, float, D>(p, ws, need, s);
-    if (p.ratio == 2) return run<F32Path<D, 2>, F32Path<D, 8>, float, D>(p, ws, need, s);
-    if (p.ratio <= 4) return run<F32Path<D, 4>, F32Path<D, 8>, float, D>(p, ws, need, s);
-    return run<F32Path<D, 8>, F32Path<D, 8>, float, D>(p, ws, need, s);
+    const long long rows = p.n_groups ? ((long long)p.n_seq * p.ratio + p.n_groups - 1) / p.n_groups : 0;
+    if (kv_dtype == ATTN_BF16)
+        return p.ratio <= 8 ? run_pre<Bf16Path<D, 1>, D>(p, ws, need, s, rows) : run_pre<Bf16Path<D, 2>, D>(p, ws, need, s, rows);
+    if (kv_dtype == ATTN_I8)
+        return p.ratio <= 4 ? run_pre<I8Path<D, 1>, D>(p, ws, need, s, rows) : run_pre<I8Path<D, 2>, D>(p, ws, need, s, rows);
+    // fp32: FMAs grow with the rows, so own rows take the request's
+    if (p.ratio == 1) return run_pre_f32<F32Path<D, 1>, D>(p, ws, need, s, rows);
+    if (p.ratio == 2) return run_pre_f32<F32Path<D, 2>, D>(p, ws, need, s, rows);
+    if (p.ratio <= 4) return run_pre_f32<F32Path<D, 4>, D>(p, ws, need, s, rows);
+    return run_pre_f32<F32Path<D, 8>, D>(p, ws, need, s, rows);
 }
 
 int run_any(const attn::prefix::Params &p, int d, int kv_dtype, void *ws, size_t *need, cudaStream_t s) {

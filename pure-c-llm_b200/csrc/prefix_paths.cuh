@@ -166,6 +166,7 @@ __device__ __forceinline__ const T *query(const Params &p, int first_req, int ro
 // ---------------------------------------------------------------------------
 template <int D, int NT>
 struct Bf16Path {
+    using Type = __nv_bfloat16;           // of q and out
     static constexpr int ROWS = 8 * NT, KEYS = D <= 64 ? 32 : 16, LEAN = NT == 1, SCRATCH = 0;
     static constexpr int KM = KEYS / 16, KS = D / 16;         // 16-key tiles; 16-dim tiles
     static constexpr int PITCH = 2 * D, SLOT = KEYS * PITCH;
@@ -365,6 +366,7 @@ __device__ __forceinline__ int exponent(float x) { return min(100, max(-100, (__
 
 template <int D, int NT>
 struct I8Path {
+    using Type = float;
     static constexpr int ROWS = 4 * NT, KEYS = 32, FOLD = 8, LEAN = NT == 1, SCRATCH = 0;
     static constexpr int KM = KEYS / 16, B64 = D / 64, REM = D % 64 != 0;
     static constexpr int KW = D / 16;                         // words of a K row per lane = k-steps = 16-dim tiles
@@ -629,6 +631,7 @@ struct I8Path {
 // ---------------------------------------------------------------------------
 template <int D, int R>
 struct F32Path {
+    using Type = float;
     static constexpr int ROWS = R;
     static constexpr bool SPREAD = R == 8;
     // 8 or 16 lanes read 128 bytes of a row together; q and o take 2 E R registers, 64 to 96
