@@ -304,6 +304,11 @@ def test_rope_append(A, tokens, heads, kv_heads, d, rot, interleaved, kind, cach
 # ---------------------------------------------------------------------------
 # shared-prefix decode
 # ---------------------------------------------------------------------------
+def torch_equal(a, b):
+    import torch
+    return torch.equal(a, b)
+
+
 class PrefixCase:
     """Random tables over a cache whose unused rows are NaN (INT8: extreme scales) and whose unused table entries lie
     outside the cache."""
@@ -418,6 +423,31 @@ def test_prefix_group_sizes(A, kind, n, plen):
 def test_prefix_shared_heads(A, kind, d, ratio):
     c = PrefixCase(A, d + ratio, kind, d, 2 * ratio, 2, 16, [5, 9], [200, 70], np.random.RandomState(ratio).randint(0, 150, 14))
     c.check(*c.run())
+
+
+@pytest.mark.parametrize("d,heads,kv_heads,page", [(64, 8, 2, 16), (128, 8, 2, 64), (128, 4, 4, 4), (64, 16, 1, 8), (128, 16, 1, 128), (64, 4, 4, 1024)])
+@pytest.mark.parametrize("sizes,plens", [([70], [900]), ([33, 90], [385, 128]), ([2, 64, 1], [1, 2000, 127])])
+def test_prefix_tiles(A, d, heads, kv_heads, page, sizes, plens):
+    """bf16 groups of many query rows (the tensor-core tiles): blocks of 256 rows and of fewer than 128, steps that end
+    inside a tile, pages below and above a tile's rows."""
+    lens = np.random.RandomState(d + page).randint(0, 30, sum(sizes))
+    c = PrefixCase(A, d + sum(sizes), "bf16", d, heads, kv_heads, page, sizes, plens, lens)
+    out, lse = c.run()
+    c.check(out, lse)
+    again, l2 = c.run()
+    assert torch_equal(again, out) and torch_equal(l2, lse)
+
+
+def test_prefix_tiles_bad_page(A):
+    """A page outside the cache in the middle of a tile's keys: its rows are absent, and nothing is read there."""
+    c = PrefixCase(A, 21, "bf16", 128, 4, 1, 16, [40], [600], [3] * 40)
+    lost = set(range(int(c.ptable[0, 20]) * 16, int(c.ptable[0, 20]) * 16 + 16))
+    c.ptable = c.ptable.copy()
+    c.ptable[0, 20], keep = 2 ** 20, c.ptable[0, 20]
+    out, lse = c.run()
+    assert device_error(A) == 0x702
+    c.ptable[0, 20] = keep
+    c.check(out, lse, absent=lost)
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -545,3 +575,15 @@ def test_serving_calls_are_captured_in_a_graph(A):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want) and float(out.abs().sum()) > 0
+
+
+@pytest.mark.parametrize("cache", ["f32", "int8"])
+def test_serving_example(A, cache):
+    """The example's loop: projection, plan, append and decode together; fp32 arithmetic, the repository's 1e-5."""
+    import importlib.util
+    import os
+    from conftest import ROOT
+    spec = importlib.util.spec_from_file_location("serve_shared_prefix", os.path.join(ROOT, "examples", "serve_shared_prefix.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    assert m.main(requests=6, prompt=130, steps=21, cache=cache) < 1e-5
