@@ -60,17 +60,17 @@ constexpr int kBegin = 1;                 // steps that the beginning and end of
 struct Part {
     float *o;                             // pieces: [slot][heads of the block][rows][D]
     float2 *ml;                           //         [slot][heads of the block][rows] (m in base 2, l)
-    long long *line_first;                // first step of each line, and the total
-    int lines, per_entry;                 // lines, lines per entry of the running sums
+    long long *line_first;                // first step of each line, the total, and the steps of a team
+    int lines, per_entry, entries;        // lines, lines per entry of the running sums, entries
     int head_block, n_blocks;             // key heads per team, their blocks
     int splits, teams;                    // teams per CTA, in all
     int blocks;                           // blocks of query rows of an own line
-    int seg_rows, rows;                   // query rows of a block, of a slot
-    int keys;                             // keys of a step
+    int log_rows, rows;                   // query rows of a block (2^log_rows), of a slot
+    int log_keys;                         // keys of a step (2^log_keys)
     int half;                             // see Pieces (0: one piece per slot)
 };
 
-__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+__device__ __forceinline__ int ceil_shift(int a, int log_b) { return (a + (1 << log_b) - 1) >> log_b; }
 
 // Query rows of a group and their blocks, and the index of the first block: an
 // ascending numbering without a sum over the groups before.
@@ -78,8 +78,8 @@ __device__ __forceinline__ void group_blocks(const Params &p, const Part &w, int
                                              int &blocks, int &base) {
     first_req = group_first(p, g);
     rows = max(group_first(p, g + 1) - first_req, 0) * p.ratio;
-    blocks = ceil_div(rows, w.seg_rows);
-    base = first_req * p.ratio / w.seg_rows + g;
+    blocks = ceil_shift(rows, w.log_rows);
+    base = (first_req * p.ratio >> w.log_rows) + g;
 }
 
 struct Line {
@@ -103,17 +103,19 @@ __device__ __forceinline__ Line line_of(const Params &p, const Part &w, int i) {
         l.base = i * w.blocks;
         l.keys = own_len(p, i);
     }
-    l.steps = ceil_div(l.keys, w.keys);
+    l.steps = ceil_shift(l.keys, w.log_keys);
     return l;
 }
 
 // Running sums of the lines' costs, one per entry of w.per_entry lines, in
 // sums[0 .. entries], by all threads of the CTA; CTA 0 also writes each line's
-// own for the merge.  Returns the total.
+// own for the merge.  Returns the steps of a team: team t takes steps
+// [t n, (t + 1) n), so none between a segment's first and last is without a
+// piece, and a step's team is one division.
 template <bool PRE>
 __device__ __forceinline__ long long sum_lines(const Params &p, const Part &w, long long *sums, long long *warp_sums) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int entries = ceil_div(w.lines, w.per_entry);
+    const int entries = w.entries;
     long long carry = 0;
     for (int e0 = 0; e0 < entries; e0 += (int)blockDim.x) {
         const int e = e0 + threadIdx.x;
@@ -140,6 +142,7 @@ __device__ __forceinline__ long long sum_lines(const Params &p, const Part &w, l
     if (threadIdx.x == 0) sums[0] = 0;
     __syncthreads();
     const long long total = entries ? sums[entries] : 0;
+    const long long of_team = max(quotient(total + w.teams - 1, w.teams), 1LL);
     if (blockIdx.x == 0) {
         for (int e = threadIdx.x; e < entries; e += blockDim.x) {
             long long at = sums[e];
@@ -148,9 +151,12 @@ __device__ __forceinline__ long long sum_lines(const Params &p, const Part &w, l
                 at += line_of<PRE>(p, w, i).total(w);
             }
         }
-        if (threadIdx.x == 0) w.line_first[w.lines] = total;
+        if (threadIdx.x == 0) {
+            w.line_first[w.lines] = total;
+            w.line_first[w.lines + 1] = of_team;
+        }
     }
-    return total;
+    return of_team;
 }
 
 // Steps [a, b) of a segment: keys of a page-table line against query rows
@@ -161,9 +167,7 @@ struct Piece {
     int keys, a, b, first_req, row0, rows, hb;
 };
 
-// The pieces of team `team`'s range [total t / teams, total (t + 1) / teams).
-// No more teams than steps, so that none between a segment's first and last is
-// without a piece.
+// The pieces of team `team`'s range.
 template <bool PRE>
 struct Walk {
     const Params &p;
@@ -172,14 +176,17 @@ struct Walk {
     int i = 0, s = 0, s1 = -1, team;
     Line l;
 
-    __device__ __forceinline__ Walk(const Params &p_, const Part &w_, const long long *sums, long long total, int team_)
+    __device__ __forceinline__ Walk(const Params &p_, const Part &w_, const long long *sums, long long of_team, int team_)
         : p(p_), w(w_), team(team_) {
-        const int teams = (int)min((long long)w.teams, total);
         l.steps = l.blocks = 0;
-        if (team >= teams) return;
-        first = quotient(total * team, teams);
-        last = quotient(total * (team + 1), teams);
-        int lo = 0, hi = ceil_div(w.lines, w.per_entry);   // the last entry that begins at or before `first`
+        const long long total = w.entries ? sums[w.entries] : 0;
+        first = of_team * team;
+        last = min(first + of_team, total);
+        if (first >= last) {
+            last = 0;
+            return;
+        }
+        int lo = 0, hi = w.entries;       // the last entry that begins at or before `first`
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (sums[mid] <= first) lo = mid;
@@ -198,14 +205,14 @@ struct Walk {
                 s = 0;
                 s1 = -1;
                 if (n > 0 && at + n > first) {
-                    s = (int)quotient(max(first, at) - at, l.cost());
-                    s1 = (int)quotient(min(last, at + n) - 1 - at, l.cost());
+                    s = first > at ? (int)quotient(first - at, l.cost()) : 0;
+                    s1 = last < at + n ? (int)quotient(last - 1 - at, l.cost()) : l.blocks * w.n_blocks - 1;
                 }
             }
             const long long begin = at + (long long)s * l.cost() + kBegin;
             x.a = (int)(max(first, begin) - begin);
             x.b = (int)(min(last, begin + l.steps) - begin);
-            const int rb = s / w.n_blocks;
+            const int rb = w.n_blocks == 1 ? s : s / w.n_blocks;
             x.hb = s - rb * w.n_blocks;
             s++;
             if (x.a >= x.b) continue;     // the range holds the segment's beginning alone
@@ -213,8 +220,8 @@ struct Walk {
             x.table = PRE ? p.prefix_table + (long long)i * p.max_prefix_pages : p.block_table + (long long)i * p.max_pages;
             x.keys = l.keys;
             x.first_req = l.first_req;
-            x.row0 = rb * w.seg_rows;
-            x.rows = min(l.rows - x.row0, w.seg_rows);
+            x.row0 = rb << w.log_rows;
+            x.rows = min(l.rows - x.row0, 1 << w.log_rows);
             return true;
         }
     }

@@ -59,7 +59,7 @@ __device__ __forceinline__ void run_piece(const Params &p, uint32_t ring, const 
     };
     bool next_valid;
     int next_row = row_of(a, next_valid), row = 0;
-    path.begin(p, ring + SLOTS * Path::SLOT, first_req, row0, rows, hk);
+    path.place(p, hk);
     unsigned masks[AHEAD + 1];            // keys with a row, of this step and the ones in flight
     auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
     auto copy_k = [&](int step, int slot) {
@@ -89,6 +89,7 @@ __device__ __forceinline__ void run_piece(const Params &p, uint32_t ring, const 
         masks[i] = copy_k(a + i, 2 * i);
         copy_v(a + i, 2 * i + 1);
     }
+    path.begin(p, ring + SLOTS * Path::SLOT, first_req, row0, rows, hk);      // the queries, behind the first copies
     int at = 0;                           // slot of this step's K
     for (int step = a; step < b; step++) {
         const int after = at + 1 == SLOTS ? 0 : at + 1, before = at ? at - 1 : SLOTS - 1;
@@ -132,11 +133,11 @@ prefix_rows_kernel(const __grid_constant__ Params p, const __grid_constant__ Par
     if (!second) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    const long long total = sum_lines<PRE>(p, w, sums, warp_sums);
+    const long long of_team = sum_lines<PRE>(p, w, sums, warp_sums);
     const int warp = threadIdx.x >> 5;
     const uint32_t ring = sm100::smem_u32(ring_bytes) + warp * R::BYTES;
     const int team_warp = warp % w.head_block, team = warp / w.head_block * (int)gridDim.x + (int)blockIdx.x;
-    Walk<PRE> walk(p, w, sums, total, team);
+    Walk<PRE> walk(p, w, sums, of_team, team);
     for (Piece x; walk.next(x);) {
         const int hk = x.hb * w.head_block + team_warp;
         if (hk >= p.kv_heads) continue;
@@ -165,23 +166,21 @@ struct Pieces {
 };
 constexpr int kMergeWarps = 4, kMany = 8;
 
-// `begin` and `total`: the line's first step and the part's steps.
+// `begin`: the line's first step; `of_team`: steps of a team.
 template <int D>
-__device__ __forceinline__ Pieces pieces_of(const Part &w, const Line &l, int row, int hk, long long begin, long long total) {
+__device__ __forceinline__ Pieces pieces_of(const Part &w, const Line &l, int row, int hk, long long begin, long long of_team) {
     Pieces r = {};
     if (l.steps == 0) return r;
-    const int rb = row / w.seg_rows, hb = hk / w.head_block, hw = hk - hb * w.head_block;
-    const long long teams = min((long long)w.teams, total);
+    const int rb = row >> w.log_rows, hb = w.n_blocks == 1 ? 0 : hk / w.head_block, hw = hk - hb * w.head_block;
     begin += (long long)(rb * w.n_blocks + hb) * l.cost() + kBegin;
-    // the team whose range [total t / teams, total (t + 1) / teams) holds a step
-    const int t0 = (int)quotient((begin + 1) * teams - 1, total), t1 = (int)quotient((begin + l.steps) * teams - 1, total);
+    const int t0 = (int)quotient(begin, of_team), t1 = (int)quotient(begin + l.steps - 1, of_team);
     const long long seg = (long long)(l.base + rb) * w.n_blocks + hb;
-    const long long slot = ((seg + t0) * w.head_block + hw) * w.rows + row - rb * w.seg_rows;
+    const long long slot = ((seg + t0) * w.head_block + hw) * w.rows + row - (rb << w.log_rows);
     r.o = w.o + slot * D;
     r.ml = w.ml + slot;
     r.step = (long long)w.head_block * w.rows;
     r.n = t1 - t0 + 1;
-    if (w.half && l.rows - rb * w.seg_rows <= w.half) {      // two pieces in each slot, one behind the other
+    if (w.half && l.rows - (rb << w.log_rows) <= w.half) {      // two pieces in each slot, one behind the other
         r.step = w.half;
         r.n *= 2;
     }
@@ -195,19 +194,19 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
     pdl_begin();                          // launched by launch_pdl
     constexpr int E = D / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int at = SHARED ? (int)blockIdx.x : (int)blockIdx.x * kMergeWarps + warp;
-    if (at >= p.n_seq * p.heads) return;
-    const int s = at / p.heads, h = at - s * p.heads, hk = h / p.ratio, hr = h - hk * p.ratio;
+    const int h = (int)blockIdx.x * (SHARED ? 1 : kMergeWarps) + (SHARED ? 0 : warp), s = blockIdx.y;
+    if (h >= p.heads) return;
+    const int hk = p.ratio == 1 ? h : h / p.ratio, hr = h - hk * p.ratio;
 
     // the request's lines: its own and, by the lanes, 32 groups at a time
-    long long own_begin = 0, own_total = 0, pre_begin = 0, pre_total = 0;
+    long long own_begin = 0, own_team = 1, pre_begin = 0, pre_team = 1;
     Line own_line = {}, pre_line = {};
     if (own.lines) {
         own_begin = __ldcg(own.line_first + s);
-        own_total = __ldcg(own.line_first + own.lines);
+        own_team = __ldcg(own.line_first + own.lines + 1);
         own_line = line_of<false>(p, own, s);
     }
-    if (pre.lines) pre_total = __ldcg(pre.line_first + pre.lines);
+    if (pre.lines) pre_team = __ldcg(pre.line_first + pre.lines + 1);
     for (int g0 = 0; g0 < pre.lines; g0 += 32) {
         const int g = g0 + lane;
         const bool in = g < pre.lines && s >= group_first(p, g) && s < group_first(p, g + 1);
@@ -219,8 +218,8 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
             break;
         }
     }
-    const Pieces a = pieces_of<D>(own, own_line, hr, hk, own_begin, own_total);
-    const Pieces b = pieces_of<D>(pre, pre_line, (s - pre_line.first_req) * p.ratio + hr, hk, pre_begin, pre_total);
+    const Pieces a = pieces_of<D>(own, own_line, hr, hk, own_begin, own_team);
+    const Pieces b = pieces_of<D>(pre, pre_line, (s - pre_line.first_req) * p.ratio + hr, hk, pre_begin, pre_team);
 
     const int n = a.n + b.n;
     float m = -INFINITY, l = 0.f, o[E];
@@ -279,7 +278,7 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
     const float inv = m == -INFINITY ? 0.f : 1.f / l;
 #pragma unroll
     for (int i = 0; i < E; i++) out[32 * i] = from_f32<T>(o[i] * inv);
-    if (p.lse && lane == 0) p.lse[at] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+    if (p.lse && lane == 0) p.lse[(long long)s * p.heads + h] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 }  // namespace prefix
@@ -313,19 +312,28 @@ Layout lay_out(const attn::prefix::Params &p, int d, int own_rows, int own_keys,
         if (!lines) return;
         w.lines = lines;
         w.per_entry = (lines + kEntries - 1) / kEntries;
-        w.n_blocks = pre && tile ? p.kv_heads : (p.kv_heads + kWarps - 1) / kWarps;
-        w.head_block = (p.kv_heads + w.n_blocks - 1) / w.n_blocks;
-        w.splits = pre && tile ? 1 : kWarps / w.head_block;
+        w.entries = (lines + w.per_entry - 1) / w.per_entry;
+        // Key heads per team: adjacent ones, in blocks that leave as few of a CTA's warps idle as may be.
+        int best = 0;
+        for (int n = pre && tile ? p.kv_heads : (p.kv_heads + kWarps - 1) / kWarps; n <= p.kv_heads; n++) {
+            const int block = (p.kv_heads + n - 1) / n, splits = pre && tile ? 1 : kWarps / block;
+            const int used = p.kv_heads * splits * 1000 / n;          // warps at work, in thousandths
+            if (used <= best) continue;
+            best = used;
+            w.n_blocks = n;
+            w.head_block = block;
+            w.splits = splits;
+        }
         w.teams = grid * w.splits;
-        w.seg_rows = seg_rows;
-        w.keys = keys;
+        w.log_rows = __builtin_ctz((unsigned)seg_rows);
+        w.log_keys = __builtin_ctz((unsigned)keys);
         w.blocks = (p.ratio + seg_rows - 1) / seg_rows;
         const long long all_rows = (long long)p.n_seq * p.ratio;
         w.rows = pre && tile ? seg_rows : (int)std::min<long long>(pre ? all_rows : p.ratio, seg_rows);
         w.half = pre && tile ? 128 : 0;
         const long long blocks = pre ? all_rows / seg_rows + lines : (long long)lines * w.blocks;
         const size_t slots = (size_t)(blocks * w.n_blocks + w.teams) * w.head_block * w.rows;
-        w.line_first = reinterpret_cast<long long *>(take(((size_t)lines + 1) * 8));
+        w.line_first = reinterpret_cast<long long *>(take(((size_t)lines + 2) * 8));
         w.ml = reinterpret_cast<float2 *>(take(slots * 8));
         w.o = reinterpret_cast<float *>(take(slots * d * 4));
     };
@@ -366,7 +374,7 @@ int run(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s) {
     const int rows = p.n_seq * p.heads;
     const bool shared = rows < sm_count_here() * 16;
     return check_pdl(launch_pdl(shared ? prefix_merge_kernel<T, D, true> : prefix_merge_kernel<T, D, false>,
-                                dim3(shared ? rows : (rows + kMergeWarps - 1) / kMergeWarps), dim3(kMergeWarps * 32), 0, s, p,
+                                dim3(shared ? p.heads : (p.heads + kMergeWarps - 1) / kMergeWarps, p.n_seq), dim3(kMergeWarps * 32), 0, s, p,
                                 L.own, L.pre),
                      "prefix_merge_kernel");
 }

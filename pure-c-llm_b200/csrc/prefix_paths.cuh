@@ -2,8 +2,8 @@
 // head, for bf16, INT8 and fp32 caches (prefix_decode.cu runs them).
 //
 // A path holds up to ROWS query rows and their running (m, l, o), and takes
-// KEYS cache rows a step, K and V each in a slot of shared memory: copy_k() and
-// copy_v() start the copies, scores() and values() fold them in, finish()
+// KEYS cache rows a step, K and V each in a slot of shared memory: place() finds
+// the head, begin() reads the queries, copy_k() and copy_v() start the copies, scores() and values() fold them in, finish()
 // writes the state.  LEAN paths hold few enough registers for two CTAs per SM.
 // Row i of a block is query head hk * ratio + (row0 + i) % ratio of request
 // first_req + (row0 + i) / ratio.
@@ -189,6 +189,8 @@ struct Bf16Path {
             m[t][0] = m[t][1] = -INFINITY;
             l[t][0] = l[t][1] = 0.f;
         }
+    }
+    __device__ __forceinline__ void place(const Params &p, int hk) {
         kb = static_cast<const char *>(p.k) + (long long)hk * D * 2;
         vb = static_cast<const char *>(p.v) + (long long)hk * D * 2;
     }
@@ -415,6 +417,8 @@ struct I8Path {
         }
         wscale = 0.f;
         folded = 0;
+    }
+    __device__ __forceinline__ void place(const Params &p, int hk) {
         head = hk;
         kb = static_cast<const char *>(p.k) + (long long)hk * D;
         vb = static_cast<const char *>(p.v) + (long long)hk * D;
@@ -682,6 +686,8 @@ struct F32Path {
             m[r] = -INFINITY;
             l[r] = 0.f;
         }
+    }
+    __device__ __forceinline__ void place(const Params &p, int hk) {
         kb = static_cast<const char *>(p.k) + (long long)hk * D * 4;
         vb = static_cast<const char *>(p.v) + (long long)hk * D * 4;
     }

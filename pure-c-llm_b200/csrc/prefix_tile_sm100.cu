@@ -128,8 +128,8 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     // (the sums lie where the query rows come after the next barrier)
     long long *sums = reinterpret_cast<long long *>(sb);
     static_assert((kEntries + 1 + 32) * 8 <= 2 * C::TILE, "sums in the query tiles");
-    const long long total = sum_lines<true>(p, w, sums, sums + kEntries + 1);
-    Walk<true> walk(p, w, sums, total, (int)blockIdx.x);
+    const long long of_team = sum_lines<true>(p, w, sums, sums + kEntries + 1);
+    Walk<true> walk(p, w, sums, of_team, (int)blockIdx.x);
     Piece x;
     tc_fence_before();
     __syncthreads();
