@@ -166,14 +166,17 @@ struct Pieces {
 };
 constexpr int kMergeWarps = 4, kMany = 8;
 
-// `begin`: the line's first step; `of_team`: steps of a team.
+// First step of the row's segment in the order of all steps.
+__device__ __forceinline__ long long segment_begin(const Part &w, const Line &l, int row, int hk, long long line_begin) {
+    const int rb = row >> w.log_rows, hb = w.n_blocks == 1 ? 0 : hk / w.head_block;
+    return line_begin + (long long)(rb * w.n_blocks + hb) * l.cost() + kBegin;
+}
+// The pieces of a row, from teams t0 .. t1.
 template <int D>
-__device__ __forceinline__ Pieces pieces_of(const Part &w, const Line &l, int row, int hk, long long begin, long long of_team) {
+__device__ __forceinline__ Pieces pieces_of(const Part &w, const Line &l, int row, int hk, int t0, int t1) {
     Pieces r = {};
     if (l.steps == 0) return r;
     const int rb = row >> w.log_rows, hb = w.n_blocks == 1 ? 0 : hk / w.head_block, hw = hk - hb * w.head_block;
-    begin += (long long)(rb * w.n_blocks + hb) * l.cost() + kBegin;
-    const int t0 = (int)quotient(begin, of_team), t1 = (int)quotient(begin + l.steps - 1, of_team);
     const long long seg = (long long)(l.base + rb) * w.n_blocks + hb;
     const long long slot = ((seg + t0) * w.head_block + hw) * w.rows + row - (rb << w.log_rows);
     r.o = w.o + slot * D;
@@ -218,8 +221,14 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
             break;
         }
     }
-    const Pieces a = pieces_of<D>(own, own_line, hr, hk, own_begin, own_team);
-    const Pieces b = pieces_of<D>(pre, pre_line, (s - pre_line.first_req) * p.ratio + hr, hk, pre_begin, pre_team);
+    // teams of the first and last step of both segments: four divisions, one in each of four lanes
+    const int pre_row = (s - pre_line.first_req) * p.ratio + hr;
+    const long long x = segment_begin(own, own_line, hr, hk, own_begin), y = segment_begin(pre, pre_line, pre_row, hk, pre_begin);
+    const int k = lane & 3;
+    const int team = (int)quotient(max((k < 2 ? x : y) + (k & 1 ? (k < 2 ? own_line.steps : pre_line.steps) - 1 : 0), 0LL),
+                                   k < 2 ? own_team : pre_team);
+    const Pieces a = pieces_of<D>(own, own_line, hr, hk, __shfl_sync(0xffffffffu, team, 0), __shfl_sync(0xffffffffu, team, 1));
+    const Pieces b = pieces_of<D>(pre, pre_line, pre_row, hk, __shfl_sync(0xffffffffu, team, 2), __shfl_sync(0xffffffffu, team, 3));
 
     const int n = a.n + b.n;
     float m = -INFINITY, l = 0.f, o[E];
