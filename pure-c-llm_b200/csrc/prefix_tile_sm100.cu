@@ -5,7 +5,7 @@
 // With r rows a prefix costs r flops per byte, so past about 250 rows the
 // tensor cores bound it and not HBM; mma.sync, at a quarter of their rate,
 // already from 64 (two 32768-row prefixes of 512 rows each, 8 x 128: 957 us on
-// mma.sync, %TILE% us here).
+// mma.sync, 147 us here: 880 TFLOP/s).
 //
 // One CTA per SM walks its range of steps (prefix.cuh) of 128 keys.  A slot is
 // 256 query rows: with more than 128, warpgroup w takes rows [128 w, 128 w + 128)
