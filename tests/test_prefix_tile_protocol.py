@@ -95,8 +95,6 @@ def _roles(pieces, ring, lose=None, boxes=lambda g: False, grows=lambda: False):
         def softmax(w):
             g, t = 0, 0
             for k, (n, two) in enumerate(pieces):
-                if k:
-                    yield W("QE", k)
                 yield A("QF")
                 steps = mine(n, two, w)
                 for j in steps:
@@ -107,6 +105,7 @@ def _roles(pieces, ring, lose=None, boxes=lambda g: False, grows=lambda: False):
                             yield W(("OD", w, 1 - u), t + u)
                         yield A(("PF", w, u))
                     t += 1
+                yield W("QE", k + 1)      # O is turned over where Q was
                 if steps:
                     yield W(("OD", w, 0), t)
                     yield W(("OD", w, 1), t)
