@@ -316,13 +316,19 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         bool ok = true;
         for (int k = 0; ok && walk.next(x); k++) {
             const bool two = x.rows > BM;
-            // this thread's query row (with up to 128 rows, warpgroup 0 brings them in for both)
+            // the warp's 32 query rows, CPR lanes a row (with up to 128 rows, warpgroup 0 brings them in for both);
+            // a lane to a row, 16 bytes of 32 rows an instruction, took 2.5 us instead of 1.1
             if (two || wg == 0) {
+                constexpr int RPI = 32 / CPR;
                 const int r = wg * BM + row, at = x.row0 + min(r, x.rows - 1);
                 const int s = x.first_req + at / p.ratio, h = x.hb * p.ratio + at % p.ratio;
-                const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(p.q) + s * p.q_stride + (long long)h * D;
+                const long long mine = s * p.q_stride + (long long)h * D;
 #pragma unroll
-                for (int c = 0; c < CPR; c++) copy16(sQ + wg * C::TILE + tile_at(row, c), src + 8 * c, r < x.rows);
+                for (int r0 = 0; r0 < 32; r0 += RPI) {
+                    const int n = r0 + lane / CPR, to = quad * 32 + n, ch = lane % CPR;
+                    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(p.q) + __shfl_sync(0xffffffffu, mine, n) + 8 * ch;
+                    copy16(sQ + wg * C::TILE + tile_at(to, ch), src, wg * BM + to < x.rows);
+                }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 fence_async_smem();
             }
