@@ -5,7 +5,7 @@
 // With r rows a prefix costs r flops per byte, so past about 250 rows the
 // tensor cores bound it and not HBM; mma.sync, at a quarter of their rate,
 // already from 64 (two 32768-row prefixes of 512 rows each, 8 x 128: 957 us on
-// mma.sync, 147 us here: 880 TFLOP/s).
+// mma.sync, 143 us here, merge included: 900 TFLOP/s).
 //
 // One CTA per SM walks its range of steps (prefix.cuh) of 128 keys.  A slot is
 // 256 query rows: with more than 128, warpgroup w takes rows [128 w, 128 w + 128)
@@ -336,15 +336,17 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             const int mine = two ? x.rows - wg * BM : x.rows;     // query rows of this warpgroup
             const bool idle = quad * 32 >= mine;                  // none of them in this warp: it only keeps step
             float m = -INFINITY, l = 0.f;
-            bool any = false;
+            bool any = false, ready = false;
             for (int j = x.a; ok && j < x.b; j++) {
                 if (!two && ((j - x.a) & 1) != wg) continue;
 #pragma unroll 1
                 for (int u = 0; u < 2; u++) {
                     const int b = 2 * wg + u;
                     const uint32_t tS = lanes + col_s(wg, u);
-                    ok = mbar_wait(BAR(B_SF + b), t & 1, abort_flag, p.err, 0x831 + u);
-                    if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                    if (!__all_sync(0xffffffffu, ready)) {
+                        ok = mbar_wait(BAR(B_SF + b), t & 1, abort_flag, p.err, 0x831 + u);
+                        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                    }
                     tc_fence_after();
                     if (!idle) {
                         uint32_t s[BH];
@@ -412,6 +414,8 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                                 tmem_st32(tO + c0, o);
                             }
                         }
+                        // the next half's S, looked for while P is on its way to TMEM (after it: 146.5 us for the prefixes above, and 143)
+                        ready = mbar_test_wait(BAR(B_SF + 2 * wg + 1 - u), (t + u) & 1);
                         tmem_wait_st();
                         tc_fence_before();
                     }
