@@ -33,7 +33,10 @@
 // at d 128).  S_w1 is formed while S_w0 is in the softmax, so a warpgroup does
 // not wait for its own products.  (With 128 keys in one S per warpgroup the
 // chain softmax, PV, next S took 5,300 cycles a step, of which the exponentials
-// of both warpgroups are 2,048.)
+// of both warpgroups are 2,048; with P in halves but S in one product 171 us, the
+// warpgroup waiting for its last PV and the S after it.  One warp for both products
+// in a fixed order: 217 us, its own instructions and waits take 1,730 cycles a pair;
+// four, one per product and warpgroup: no faster than two.)
 //
 // Every wait is bounded; a timeout records a code in the device error word and
 // raises a CTA-wide flag, on which all roles fall through to the teardown.
@@ -430,7 +433,7 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             if (!(ok = __all_sync(0xffffffffu, ok))) break;
             // The piece: this warpgroup's half of the slot.  A warp turns 32 dims of its 32 rows
             // over in what was the place of their queries and writes them 128 bytes at a time.
-            // (Each thread writing its own row, 512 bytes apart: 6 us for a piece instead of 2.)
+            // (Each thread writing its own row, 512 bytes apart: 6.4 us from a piece's last P to the next piece, 3.4 so.)
             const long long at = x.slot * w.rows + wg * BM + row;
             if (any) {
                 ok = mbar_wait(BAR(B_OD + 2 * wg), (t - 1) & 1, abort_flag, p.err, 0x835) &&
