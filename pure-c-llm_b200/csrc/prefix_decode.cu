@@ -232,6 +232,7 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
 
     const int n = a.n + b.n;
     float m = -INFINITY, l = 0.f, o[E];
+    bool bad = false;                     // a sum that is no number, also of a piece without a maximum (all its scores are none)
 #pragma unroll
     for (int i = 0; i < E; i++) o[i] = 0.f;
     // piece j of the row; with SHARED, this warp's j-th
@@ -240,6 +241,7 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
         const int j = which(j0 + lane);
         const float2 ml = j < a.n ? __ldcg(a.ml + j * a.step) : j < n ? __ldcg(b.ml + (j - a.n) * b.step) : make_float2(-INFINITY, 0.f);
         const float mx = fmaxf(m, warp_max(ml.x));
+        bad |= ml.y != ml.y;
         if (mx == -INFINITY) continue;    // no valid row in these pieces
         const float old = exp2f(m - mx), c = exp2f(ml.x - mx);
         l = l * old + warp_sum(ml.y * c);
@@ -264,9 +266,11 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
             }
         }
     }
+    bad = __any_sync(0xffffffffu, bad);
     if constexpr (SHARED) {
+        __shared__ bool s_bad[kMergeWarps];
         __shared__ float s_m[kMergeWarps], s_l[kMergeWarps], s_o[kMergeWarps][D];
-        if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+        if (lane == 0) { s_m[warp] = m; s_l[warp] = l; s_bad[warp] = bad; }
 #pragma unroll
         for (int i = 0; i < E; i++) s_o[warp][lane + 32 * i] = o[i];
         __syncthreads();
@@ -279,11 +283,13 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
         for (int k = 0; k < kMergeWarps; k++) {
             const float c = s_m[k] == -INFINITY ? 0.f : exp2f(s_m[k] - m);
             l += s_l[k] * c;
+            bad |= s_bad[k];
 #pragma unroll
             for (int i = 0; i < E; i++) o[i] += s_o[k][lane + 32 * i] * c;
         }
     }
     T *out = static_cast<T *>(p.out) + s * p.out_stride + (long long)h * D + lane;
+    if (bad) m = l = NAN;
     const float inv = m == -INFINITY ? 0.f : 1.f / l;
 #pragma unroll
     for (int i = 0; i < E; i++) out[32 * i] = from_f32<T>(o[i] * inv);

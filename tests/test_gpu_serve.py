@@ -464,6 +464,32 @@ def test_prefix_none(A, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("ratio", [1, 2, 4])
+@pytest.mark.parametrize("sizes,plen,no_group", [([], 0, 5), ([5], 300, 0), ([40], 300, 0)])
+def test_prefix_not_numbers(A, kind, ratio, sizes, plen, no_group):
+    """What is no number in a query, a key or a value shows in its own outputs, and only there."""
+    n = sum(sizes) + no_group
+    c = PrefixCase(A, 14, kind, 64, 3 * ratio, 3, 16, sizes, [plen] * len(sizes), ([70, 200, 40, 33, 64] * n)[:n], no_group=no_group)
+    row = [c.rows_of(s)[plen:] for s in range(5)]
+    c.q[0, 5] = float("nan")                      # head 0
+    c.q[1, 64 * (3 * ratio - 1)] = float("inf")   # the last head
+    if kind == "int8":
+        c.ks[row[2][7], 1] = float("nan")         # key head 1
+        c.vs[row[3][32], 2] = float("nan")        # key head 2
+    else:
+        c.kc[row[2][7], 64 + 9] = float("nan")
+        c.vc[row[3][32], 128:192] = float("nan")
+    out, lse = c.run()
+    o = out.view(n, 3 * ratio, 64)
+    bad = {(0, 0), (1, 3 * ratio - 1)} | {(2, ratio + i) for i in range(ratio)} | {(3, 2 * ratio + i) for i in range(ratio)}
+    for s in range(n):
+        for h in range(3 * ratio):
+            assert (not o[s, h].isfinite().any()) if (s, h) in bad else o[s, h].isfinite().all(), (s, h)
+            assert bool(lse[s, h].isfinite()) == ((s, h) not in bad or s == 3), (s, h)
+    c.check(out, lse, only=[4])
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_prefix_sharp_scores(A, kind):
     """Scores of many hundreds: the largest key alone counts, and nothing overflows."""
     c = PrefixCase(A, 11, kind, 64, 4, 4, 16, [6], [700], [0, 10, 300, 1, 64, 65], q_std=300.0)
