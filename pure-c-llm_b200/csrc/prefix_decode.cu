@@ -424,7 +424,9 @@ int run_d(const attn::prefix::Params &p, int kv_dtype, void *ws, size_t *need, c
     if (kv_dtype == ATTN_BF16)
         return p.ratio <= 8 ? run_pre<Bf16Path<D, 1>, D>(p, ws, need, s, rows) : run_pre<Bf16Path<D, 2>, D>(p, ws, need, s, rows);
     if (kv_dtype == ATTN_I8)
-        return p.ratio <= 4 ? run_pre<I8Path<D, 1>, D>(p, ws, need, s, rows) : run_pre<I8Path<D, 2>, D>(p, ws, need, s, rows);
+        return p.ratio <= 2   ? run_pre<I8Digits<D>, D>(p, ws, need, s, rows)
+               : p.ratio <= 4 ? run_pre<I8Path<D, 1>, D>(p, ws, need, s, rows)
+                              : run_pre<I8Path<D, 2>, D>(p, ws, need, s, rows);
     // fp32: FMAs grow with the rows, so own rows take the request's
     if (p.ratio == 1) return run_pre_f32<F32Path<D, 1>, D>(p, ws, need, s, rows);
     if (p.ratio == 2) return run_pre_f32<F32Path<D, 2>, D>(p, ws, need, s, rows);

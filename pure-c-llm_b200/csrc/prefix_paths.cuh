@@ -617,6 +617,241 @@ struct I8Path {
 };
 
 // ---------------------------------------------------------------------------
+// INT8 codes, 2 query rows: both products in integers, so no code is converted.
+//
+// A query and a weight p * vscale become integers of 30 bits, the row's largest
+// element in [2^29, 2^30) and a weight 1 at 2^29 (the power of two that keeps
+// weights under 2 as above), and go in as four signed digits of base 256,
+// columns 4 r to 4 r + 3 of the tile from the highest down.  The sums are exact:
+// under 2^21 of a score's digits, and 2^19 a step of an output's, for FOLD steps.
+// Lane (g, c) has the pair of digits 2 (c & 1) of row c / 2, and the two lanes
+// of a row exchange theirs.  Not numbers: a query's makes the score's scale one,
+// a vscale's the output.
+//
+// The weights of keys g and g + 8 share the 16-bit elements of the transposition,
+// so a lane's word of 4 keys is 2c, 2c + 8, 2c + 1, 2c + 9, and of V four words
+// (4 keys, 4 dims) turn into it with 8 byte permutations.
+// (64 requests with up to 8192 rows, 16 x 64: 117 us a call, 129 with two f16 parts
+// and converted codes; more query rows would need a second tile of digits.)
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// x, |x| <= 2^30, as four signed bytes of base 256
+__device__ __forceinline__ uint32_t digits(int x) { return ((uint32_t)x + 0x00808080u) ^ 0x00808080u; }
+
+template <int D>
+struct I8Digits : I8Path<D, 1> {
+    using Base = I8Path<D, 1>;
+    using Base::B64;
+    using Base::KM;
+    using Base::KW;
+    using Base::OFF_S;
+    using Base::REM;
+    using Base::SWAP;
+    using Base::VP;
+    static constexpr int ROWS = 2, FOLD = 64;
+    uint32_t q[KW];
+    float s[KM][2];                                           // the step's code sums
+    int o[KW][4];
+    float f[KW][2], m, l, qscale, wscale, bad;
+    int folded;
+
+    __device__ __forceinline__ void begin(const Params &p, uint32_t, int first_req, int row0, int rows, int hk) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        const float *a = query<float>(p, first_req, row0 + min(g >> 2, rows - 1), hk, D);
+        float4 x[KW];
+        float amax = 0.f, poison = 0.f;
+#pragma unroll
+        for (int j = 0; j < KW; j++) {
+            // word j of this lane: 16 codes of each 64 dims, then 8 of the last 32
+            const int dim = j < 4 * B64 ? 64 * (j / 4) + 16 * c + 4 * (j % 4) : 64 * B64 + 8 * c + 4 * (j - 4 * B64);
+            x[j] = __ldg(reinterpret_cast<const float4 *>(a + dim));
+            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w))));
+            poison += x[j].x * 0.f + x[j].y * 0.f + (x[j].z * 0.f + x[j].w * 0.f);
+        }
+        amax = quad_max(amax);
+        poison += __shfl_xor_sync(0xffffffffu, poison, 1);
+        poison += __shfl_xor_sync(0xffffffffu, poison, 2);
+        const int e = amax > 0.f ? 29 - max((__float_as_int(amax) >> 23) - 127, -97) : 0;      // both powers are numbers
+        const float up = pow2i(e);
+        qscale = __shfl_sync(0xffffffffu, p.scale_log2 * pow2i(-e) + poison, 16 * (c >> 1));   // of row c / 2
+        const uint32_t digit = 3 - (g & 3);
+#pragma unroll
+        for (int j = 0; j < KW; j++) {
+            const uint32_t d0 = digits(__float2int_rn(x[j].x * up)), d1 = digits(__float2int_rn(x[j].y * up));
+            const uint32_t d2 = digits(__float2int_rn(x[j].z * up)), d3 = digits(__float2int_rn(x[j].w * up));
+            const uint32_t pick = digit | (4 + digit) << 4;
+            q[j] = prmt(prmt(d0, d1, pick), prmt(d2, d3, pick), 0x5410);
+#pragma unroll
+            for (int n = 0; n < 4; n++) o[j][n] = 0;
+            f[j][0] = f[j][1] = 0.f;
+        }
+        m = -INFINITY;
+        l = wscale = bad = 0.f;
+        folded = 0;
+    }
+    __device__ __forceinline__ void fold() {
+#pragma unroll
+        for (int j = 0; j < KW; j++)
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                f[j][n] += fmaf((float)o[j][2 * n], 256.f, (float)o[j][2 * n + 1]);
+                o[j][2 * n] = o[j][2 * n + 1] = 0;
+            }
+        folded = 0;
+    }
+    __device__ __forceinline__ void scale_output(float a) {
+        fold();
+#pragma unroll
+        for (int j = 0; j < KW; j++) {
+            f[j][0] *= a;
+            f[j][1] *= a;
+        }
+    }
+    template <bool EDGE>
+    __device__ __forceinline__ void scores(const Params &, uint32_t st, unsigned) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        const uint32_t kst = st + g * D, swap = SWAP ? (g & 1) * 64 : 0;
+        const float mine = c & 1 ? 1.f : 65536.f, others = c & 1 ? 65536.f : 1.f;
+#pragma unroll
+        for (int i = 0; i < KM; i++) {
+            uint32_t w[2][KW];                                // codes of keys g and g + 8
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const uint32_t at = kst + (16 * i + 8 * n) * D;
+#pragma unroll
+                for (int x = 0; x < B64; x++) {
+                    const uint4 k = lds16(at + 64 * x + 16 * c + (x & 1 ? -swap : swap));
+                    w[n][4 * x] = k.x; w[n][4 * x + 1] = k.y; w[n][4 * x + 2] = k.z; w[n][4 * x + 3] = k.w;
+                }
+                if constexpr (REM) {
+                    const uint2 k = lds8(at + 64 * B64 + 8 * c);
+                    w[n][4 * B64] = k.x; w[n][4 * B64 + 1] = k.y;
+                }
+            }
+            int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < KW; j += 2) mma_s8(sum, w[0][j], w[1][j], w[0][j + 1], w[1][j + 1], q[j], q[j + 1]);
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const float x = (float)(sum[2 * n] * 256 + sum[2 * n + 1]);
+                s[i][n] = fmaf(__shfl_xor_sync(0xffffffffu, x, 1), others, x * mine);
+            }
+        }
+    }
+    template <bool EDGE>
+    __device__ __forceinline__ void values(const Params &, uint32_t st, unsigned mask) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        const uint32_t vst = st + 2 * c * VP, v8 = 8 * g ^ c << 5, v4 = 4 * g ^ c << 5;
+        // scales of the lane's keys: g, g + 8 of each 16; absent keys' scales are not numbers to go by
+        float vs[KM][2], big = 0.f, mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < KM; i++)
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const int key = 16 * i + 8 * n + g;
+                const bool there = !EDGE || (mask >> key & 1);
+                const float ks = __uint_as_float(lds4(st + OFF_S + key * 4));
+                vs[i][n] = __uint_as_float(lds4(st + OFF_S + 128 + key * 4));
+                if (!there) vs[i][n] = 0.f;
+                big = fmaxf(big, fabsf(vs[i][n]));
+                bad = fmaf(vs[i][n], 0.f, bad);
+                s[i][n] = there ? s[i][n] * qscale * ks : -INFINITY;
+                mx = fmaxf(mx, s[i][n]);
+            }
+        // weights' scale: the power of two over the largest vscale so far
+        if (__any_sync(0xffffffffu, big > 0.f && (wscale == 0.f || big * wscale >= 2.f))) {
+            const float now = pow2i(-exponent(keys_max(big)));
+            if (wscale != 0.f) scale_output(now / wscale);
+            wscale = now;
+        }
+        mx = fmaxf(m, keys_max(mx));
+        const float neg = mx == -INFINITY ? 0.f : -mx, alpha = ex2(m + neg);
+        if (__any_sync(0xffffffffu, mx != m)) {
+            l *= alpha;
+            scale_output(alpha);
+        }
+        m = mx;
+        uint32_t w[KM];
+#pragma unroll
+        for (int i = 0; i < KM; i++) {
+            uint32_t d[2];
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const float e = ex2(s[i][n] + neg);
+                l += e;
+                d[n] = digits(__float2int_rn(e * (vs[i][n] * wscale) * 536870912.f));
+            }
+            w[i] = transposed(prmt(d[0], d[1], c & 1 ? 0x4051 : 0x6273));
+        }
+        // 4 dims of 4 keys to 4 keys of each dim
+        auto turn = [](uint32_t (&x)[4], uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
+            const uint32_t a = prmt(v0, v2, 0x5140), b = prmt(v1, v3, 0x5140), e = prmt(v0, v2, 0x7362), h = prmt(v1, v3, 0x7362);
+            x[0] = prmt(a, b, 0x5410); x[1] = prmt(a, b, 0x7632); x[2] = prmt(e, h, 0x5410); x[3] = prmt(e, h, 0x7632);
+        };
+        static_assert(KM == 2, "a step is one product's depth");
+#pragma unroll
+        for (int x = 0; x < B64; x++) {
+            uint2 v[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+                    v[i][n] = lds8(vst + (i * 16 + (n >> 1) * 8) * VP + v_at<VP>(n & 1, x & 1 ? v8 ^ 64 : v8, x / 2 * 128));
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                uint32_t y[2][4];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    if (h == 0) turn(y[i], v[i][0].x, v[i][1].x, v[i][2].x, v[i][3].x);
+                    else turn(y[i], v[i][0].y, v[i][1].y, v[i][2].y, v[i][3].y);
+                }
+                mma_s8(o[4 * x + 2 * h], y[0][0], y[0][1], y[1][0], y[1][1], w[0], w[1]);
+                mma_s8(o[4 * x + 2 * h + 1], y[0][2], y[0][3], y[1][2], y[1][3], w[0], w[1]);
+            }
+        }
+        if constexpr (REM) {
+            uint32_t v[4], y[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+                    v[n] = lds4(vst + (i * 16 + (n >> 1) * 8) * VP + v_at<VP>(n & 1, B64 ? v4 ^ 64 : v4, 0));
+                turn(y[i], v[0], v[1], v[2], v[3]);
+            }
+            mma_s8(o[4 * B64], y[0][0], y[0][1], y[1][0], y[1][1], w[0], w[1]);
+            mma_s8(o[4 * B64 + 1], y[0][2], y[0][3], y[1][2], y[1][3], w[0], w[1]);
+        }
+        if (++folded == FOLD) fold();
+    }
+    __device__ __forceinline__ void finish(float *out, float2 *ml, int rows) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        fold();
+        const float down = wscale == 0.f ? 0.f : 1.f / wscale * 1.862645149230957e-9f;      // 2^-29
+        const float sum = keys_sum(l), nan = keys_sum(bad);
+        const float mine = c & 1 ? 1.f : 65536.f, others = c & 1 ? 65536.f : 1.f;
+#pragma unroll
+        for (int j = 0; j < KW; j++)
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+                f[j][n] = fmaf(__shfl_xor_sync(0xffffffffu, f[j][n], 1), others, f[j][n] * mine) * down + nan;
+        const int row = c >> 1;
+        if (row >= rows) return;
+        if (g == 0 && !(c & 1)) ml[row] = make_float2(m, sum);
+        // tile j's rows g and g + 8 are dims 2j and 2j + 1 (of 8, or 4) of the lane's; the two lanes take turns
+#pragma unroll
+        for (int j = 0; j < KW; j += 2) {
+            if ((j / 2 & 1) != (c & 1)) continue;
+            const int dim = j < 4 * B64 ? 64 * (j / 4) + 8 * g + 2 * (j % 4) : 64 * B64 + 4 * g;
+            *reinterpret_cast<float4 *>(out + row * D + dim) = make_float4(f[j][0], f[j][1], f[j + 1][0], f[j + 1][1]);
+        }
+    }
+};
+
+// ---------------------------------------------------------------------------
 // fp32: fp32 FMAs on pairs, R query rows.
 //
 // LPK lanes share a key, each with E = D / LPK of its dims, so a score is a dot

@@ -463,6 +463,21 @@ def test_prefix_none(A, kind):
     c.check(*c.run(workspace=None))
 
 
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("ratio", [1, 2, 4])
+def test_prefix_int8_largest_codes(A, d, ratio):
+    """Codes of -128 and 127 and equal scores over many rows: the largest sums a piece can hold."""
+    import torch
+    c = PrefixCase(A, d, "int8", d, ratio, 1, 64, [], [], [50000, 4097], no_group=2)
+    c.q.fill_(-1.0)
+    for x, s, x64, code in ((c.kc, c.ks, c.k64, -128), (c.vc, c.vs, c.v64, 127)):
+        x.fill_(code)
+        x[::3, 1::2] = -code - 1
+        s.copy_(torch.where(s.isnan(), s, torch.full_like(s, 2.0 ** -9)))
+        x64[:] = x.cpu().numpy().astype(np.float64) * 2.0 ** -9
+    c.check(*c.run())
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("ratio", [1, 2, 4])
 @pytest.mark.parametrize("sizes,plen,no_group", [([], 0, 5), ([5], 300, 0), ([40], 300, 0)])
