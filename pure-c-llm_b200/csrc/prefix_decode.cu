@@ -423,6 +423,7 @@ int run_d(const attn::prefix::Params &p, int kv_dtype, void *ws, size_t *need, c
     const long long rows = p.n_groups ? ((long long)p.n_seq * p.ratio + p.n_groups - 1) / p.n_groups : 0;
     if (kv_dtype == ATTN_BF16)
         return p.ratio <= 8 ? run_pre<Bf16Path<D, 1>, D>(p, ws, need, s, rows) : run_pre<Bf16Path<D, 2>, D>(p, ws, need, s, rows);
+    // INT8: two rows fill a tile of digits (8192 own rows of 8 x 128: 114 us a call, 117 in f16 parts; 32 x 32: 175 and 190)
     if (kv_dtype == ATTN_I8)
         return p.ratio <= 2   ? run_pre<I8Digits<D>, D>(p, ws, need, s, rows)
                : p.ratio <= 4 ? run_pre<I8Path<D, 1>, D>(p, ws, need, s, rows)

@@ -4,7 +4,8 @@
 // A path holds up to ROWS query rows and their running (m, l, o), and takes
 // KEYS cache rows a step, K and V each in a slot of shared memory: place() finds
 // the head, begin() reads the queries, copy_k() and copy_v() start the copies,
-// scores() and values() fold them in, finish() writes the state.  LEAN paths hold few enough registers for two CTAs per SM.
+// scores() and values() fold them in, finish() writes the state.  LEAN paths hold
+// few enough registers for two CTAs per SM.
 // Row i of a block is query head hk * ratio + (row0 + i) % ratio of request
 // first_req + (row0 + i) / ratio.
 //

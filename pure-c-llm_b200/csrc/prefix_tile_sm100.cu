@@ -23,8 +23,9 @@
 //   warp 2      S_wu = Q_w K_u^T for the two halves u of a step's keys, M = 128,
 //               N = 64, both operands in shared memory
 //   warp 3      O_w += P_wu V_u (P from TMEM, V as it lies, MN-major)
-//   warps 4-7   softmax of warpgroup 0, warps 8-11 of warpgroup 1: a thread owns
-//               a row (a TMEM lane), brings it in, keeps its maximum and sum, writes its bf16
+//   warps 4-7   softmax of warpgroup 0, warps 8-11 of warpgroup 1: a warp
+//               brings 32 query rows in, a thread keeps the maximum and sum of its row
+//               (a TMEM lane), writes its bf16
 //               probabilities to TMEM, and rescales O when the maximum grew by
 //               more than 2^8 (a stale one leaves P <= 256, and the piece's
 //               (m, l, o) stay consistent).  All exponentials on MUFU: lse is an
