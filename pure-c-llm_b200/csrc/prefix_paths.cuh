@@ -336,11 +336,15 @@ struct Bf16Path {
 // INT8 codes, 4 NT query rows: the same products in f16, in which a code is
 // exact.
 //
-// A query and a weight p * vscale go in as two f16 parts, columns 2 r and
+// A query and a weight w = p * vscale go in as two f16 parts, columns 2 r and
 // 2 r + 1 of the row's tile, whose results are added: 22 bits of each.  The
 // query row is first scaled by a power of two that puts its largest element in
-// [2^7, 2^8), the weights by one, kept for the piece, that keeps them under 2,
-// so the second parts stay above f16's smallest numbers.  A code c becomes f16
+// [2^7, 2^8), a row's weights by one that puts the largest of them so far in
+// [2^14, 2^15), so the second parts stay above f16's smallest numbers (a weight
+// 2^-17 of the largest keeps its 22 bits, any other 2^-39 of the largest).  The
+// largest weight and not the largest vscale sets that power: a row with a wide
+// vscale and no probability would take the bits of all others.  It follows the
+// weights down when the maximum of the scores grows.  A code c becomes f16
 // as the low byte of 1024 + (c + 128) minus 1152, all exact.  The tensor core
 // rounds its sums towards zero, which drifts over a long piece, so every
 // FOLD steps the output sums move to fp32 registers.
@@ -364,8 +368,17 @@ __device__ __forceinline__ void f16_parts(float a, float b, uint32_t &hi, uint32
 }
 // 2^e as a float, e in [-126, 127]
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
-// exponent of x > 0, within [-100, 100]
-__device__ __forceinline__ int exponent(float x) { return min(100, max(-100, (__float_as_int(x) >> 23 & 255) - 127)); }
+// exponent of x >= 0, within [-97, 127]
+__device__ __forceinline__ int exponent(float x) { return min(127, max(-97, (__float_as_int(x) >> 23) - 127)); }
+// Is a weight at or past the next power of two above the row's largest so far?
+__device__ __forceinline__ bool outgrows(float weight, float top) {
+    return weight > __int_as_float(__float_as_int(top) | 0x007fffff);
+}
+// What the sums of weights are multiplied by when the row's largest weight
+// becomes `now`, and the weights before lose the factor alpha.
+__device__ __forceinline__ float rescaling(float alpha, float top, float now) {
+    return alpha * pow2i(min(127, max(-126, exponent(top) - exponent(now))));
+}
 
 template <int D, int NT>
 struct I8Path {
@@ -380,7 +393,7 @@ struct I8Path {
     float s[NT][KM][4];                                       // the step's code sums
     float o[NT][KW][4], f[NT][KW][2], m[NT], l[NT];
     float qscale[NT];                                         // scale log2(e) / the query row's power of two
-    float wscale;                                             // the weights' power of two
+    float top[NT];                                            // the row's largest weight |p vscale|
     int folded, head;
     const char *kb, *vb;
 
@@ -414,9 +427,8 @@ struct I8Path {
                 f[t][j][0] = f[t][j][1] = 0.f;
             }
             m[t] = -INFINITY;
-            l[t] = 0.f;
+            l[t] = top[t] = 0.f;
         }
-        wscale = 0.f;
         folded = 0;
     }
     __device__ __forceinline__ void place(const Params &p, int hk) {
@@ -507,7 +519,7 @@ struct I8Path {
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
         const uint32_t vst = st + 2 * c * VP, v8 = 8 * g ^ c << 5, v4 = 4 * g ^ c << 5;
         // scales of the lane's keys: g, g + 8 of each 16; absent keys' scales are not numbers to go by
-        float ks[KM][2], vs[KM][2], big = 0.f;
+        float ks[KM][2], vs[KM][2];
 #pragma unroll
         for (int i = 0; i < KM; i++)
 #pragma unroll
@@ -516,20 +528,10 @@ struct I8Path {
                 ks[i][n] = __uint_as_float(lds4(st + OFF_S + key * 4));
                 vs[i][n] = __uint_as_float(lds4(st + OFF_S + 128 + key * 4));
                 if (EDGE && !(mask >> key & 1)) vs[i][n] = 0.f;
-                big = fmaxf(big, fabsf(vs[i][n]));
             }
-        // weights' scale: the power of two over the largest vscale so far
-        if (__any_sync(0xffffffffu, big > 0.f && (wscale == 0.f || big * wscale >= 2.f))) {
-            const float now = pow2i(-exponent(keys_max(big)));
-            if (wscale != 0.f) {
-#pragma unroll
-                for (int t = 0; t < NT; t++) scale_output(t, now / wscale);
-            }
-            wscale = now;
-        }
         // all tiles' maxima first, so that their exchanges overlap, and one vote
         uint32_t pw[KM][NT][2];
-        float neg[NT], alpha[NT];
+        float neg[NT], alpha[NT], big[NT];
         bool grows = false;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -555,26 +557,44 @@ struct I8Path {
             neg[t] = mx == -INFINITY ? 0.f : -mx;
             alpha[t] = ex2(m[t] + neg[t]);
             m[t] = mx;
-        }
-        if (__any_sync(0xffffffffu, grows)) {
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                l[t] *= alpha[t];
-                scale_output(t, alpha[t]);
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < NT; t++)
+            l[t] *= alpha[t];
+            big[t] = 0.f;
 #pragma unroll
             for (int i = 0; i < KM; i++)
 #pragma unroll
                 for (int n = 0; n < 2; n++) {
-                    const float e = ex2(s[t][i][2 * n] + neg[t]), w = e * (vs[i][n] * wscale);
+                    const float e = ex2(s[t][i][2 * n] + neg[t]);
                     l[t] += e;
+                    s[t][i][2 * n] = e * vs[i][n];
+                    big[t] = fmaxf(big[t], fabsf(s[t][i][2 * n]));
+                }
+            grows |= outgrows(big[t], top[t]);
+        }
+        if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+                for (int t = 0; t < NT; t++) big[t] = fmaxf(big[t], __shfl_xor_sync(0xffffffffu, big[t], d));
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const float now = fmaxf(top[t] * alpha[t], big[t]);
+                scale_output(t, rescaling(alpha[t], top[t], now));
+                top[t] = now;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const float wscale = pow2i(14 - exponent(top[t]));
+#pragma unroll
+            for (int i = 0; i < KM; i++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const float w = s[t][i][2 * n] * wscale;
                     const __half hi = __float2half_rn(w);
                     const __half2 both = __halves2half2(hi, __float2half_rn(w - __half2float(hi)));
                     pw[i][t][n] = transposed(*reinterpret_cast<const uint32_t *>(&both));
                 }
+        }
 #pragma unroll
         for (int i = 0; i < KM; i++) {
 #pragma unroll
@@ -599,10 +619,9 @@ struct I8Path {
     __device__ __forceinline__ void finish(float *out, float2 *ml, int rows) {
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
         fold();
-        const float down = wscale == 0.f ? 0.f : 1.f / wscale;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            const float sum = keys_sum(l[t]);
+            const float sum = keys_sum(l[t]), down = pow2i(exponent(top[t]) - 14);
             const int row = 4 * t + c;
             if (row >= rows) continue;
             if (g == 0) ml[row] = make_float2(m[t], sum);
@@ -621,9 +640,9 @@ struct I8Path {
 // INT8 codes, 2 query rows: both products in integers, so no code is converted.
 //
 // A query and a weight p * vscale become integers of 30 bits, the row's largest
-// element in [2^29, 2^30) and a weight 1 at 2^29 (the power of two that keeps
-// weights under 2 as above), and go in as four signed digits of base 256,
-// columns 4 r to 4 r + 3 of the tile from the highest down.  The sums are exact:
+// element and its largest weight so far (as above) in [2^29, 2^30), and go in as
+// four signed digits of base 256, columns 4 r to 4 r + 3 of the tile from the
+// highest down.  The sums are exact:
 // under 2^21 of a score's digits, and 2^19 a step of an output's, for FOLD steps.
 // Lane (g, c) has the pair of digits 2 (c & 1) of row c / 2, and the two lanes
 // of a row exchange theirs.  Not numbers: a query's makes the score's scale one,
@@ -657,7 +676,7 @@ struct I8Digits : I8Path<D, 1> {
     uint32_t q[KW];
     float s[KM][2];                                           // the step's code sums
     int o[KW][4];
-    float f[KW][2], m, l, qscale, wscale, bad;
+    float f[KW][2], m, l, qscale, top, bad;
     int folded;
 
     __device__ __forceinline__ void begin(const Params &p, uint32_t, int first_req, int row0, int rows, int hk) {
@@ -691,7 +710,7 @@ struct I8Digits : I8Path<D, 1> {
             f[j][0] = f[j][1] = 0.f;
         }
         m = -INFINITY;
-        l = wscale = bad = 0.f;
+        l = top = bad = 0.f;
         folded = 0;
     }
     __device__ __forceinline__ void fold() {
@@ -748,7 +767,7 @@ struct I8Digits : I8Path<D, 1> {
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
         const uint32_t vst = st + 2 * c * VP, v8 = 8 * g ^ c << 5, v4 = 4 * g ^ c << 5;
         // scales of the lane's keys: g, g + 8 of each 16; absent keys' scales are not numbers to go by
-        float vs[KM][2], big = 0.f, mx = -INFINITY;
+        float vs[KM][2], mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < KM; i++)
 #pragma unroll
@@ -758,34 +777,36 @@ struct I8Digits : I8Path<D, 1> {
                 const float ks = __uint_as_float(lds4(st + OFF_S + key * 4));
                 vs[i][n] = __uint_as_float(lds4(st + OFF_S + 128 + key * 4));
                 if (!there) vs[i][n] = 0.f;
-                big = fmaxf(big, fabsf(vs[i][n]));
                 bad = fmaf(vs[i][n], 0.f, bad);
                 s[i][n] = there ? s[i][n] * qscale * ks : -INFINITY;
                 mx = fmaxf(mx, s[i][n]);
             }
-        // weights' scale: the power of two over the largest vscale so far
-        if (__any_sync(0xffffffffu, big > 0.f && (wscale == 0.f || big * wscale >= 2.f))) {
-            const float now = pow2i(-exponent(keys_max(big)));
-            if (wscale != 0.f) scale_output(now / wscale);
-            wscale = now;
-        }
         mx = fmaxf(m, keys_max(mx));
         const float neg = mx == -INFINITY ? 0.f : -mx, alpha = ex2(m + neg);
-        if (__any_sync(0xffffffffu, mx != m)) {
-            l *= alpha;
-            scale_output(alpha);
+        float big = 0.f;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < KM; i++)
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const float e = ex2(s[i][n] + neg);
+                l += e;
+                vs[i][n] *= e;
+                big = fmaxf(big, fabsf(vs[i][n]));
+            }
+        if (__any_sync(0xffffffffu, mx != m || outgrows(big, top))) {
+            const float now = fmaxf(top * alpha, keys_max(big));
+            scale_output(rescaling(alpha, top, now));
+            top = now;
         }
         m = mx;
+        const float wscale = pow2i(29 - exponent(top));
         uint32_t w[KM];
 #pragma unroll
         for (int i = 0; i < KM; i++) {
             uint32_t d[2];
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const float e = ex2(s[i][n] + neg);
-                l += e;
-                d[n] = digits(__float2int_rn(e * (vs[i][n] * wscale) * 536870912.f));
-            }
+            for (int n = 0; n < 2; n++) d[n] = digits(__float2int_rn(vs[i][n] * wscale));
             w[i] = transposed(prmt(d[0], d[1], c & 1 ? 0x4051 : 0x6273));
         }
         // 4 dims of 4 keys to 4 keys of each dim
@@ -831,8 +852,7 @@ struct I8Digits : I8Path<D, 1> {
     __device__ __forceinline__ void finish(float *out, float2 *ml, int rows) {
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
         fold();
-        const float down = wscale == 0.f ? 0.f : 1.f / wscale * 1.862645149230957e-9f;      // 2^-29
-        const float sum = keys_sum(l), nan = keys_sum(bad);
+        const float down = pow2i(exponent(top) - 29), sum = keys_sum(l), nan = keys_sum(bad);
         const float mine = c & 1 ? 1.f : 65536.f, others = c & 1 ? 65536.f : 1.f;
 #pragma unroll
         for (int j = 0; j < KW; j++)

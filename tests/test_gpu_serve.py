@@ -478,6 +478,51 @@ def test_prefix_int8_largest_codes(A, d, ratio):
     c.check(*c.run())
 
 
+def scores_bound(c, s):
+    """out of request s in 64 bits and its bound, key by key: with delta_j = 2^-21 (1 + scale sum|q k_j|) a probability is
+    off by the factor 1 +- 2 delta_j, and so is the sum it is divided by: 2 sum p delta |v| + 2 sum p delta . sum p |v|.
+    (A key without a probability adds nothing, however wide its value is.)"""
+    rows, d, r = c.rows_of(s), c.d, c.heads // c.kv_heads
+    q = c.q[s].double().cpu().numpy().reshape(c.heads, d)
+    out, tol = np.zeros((c.heads, d)), np.zeros((c.heads, d))
+    for h in range(c.heads):
+        k, v = (x[rows][:, h // r * d:(h // r + 1) * d] for x in (c.k64, c.v64))
+        x = k @ q[h] / np.sqrt(d)
+        p = np.exp(x - x.max())
+        p /= p.sum()
+        delta = 2.0 ** -21 * (1 + np.abs(k) @ np.abs(q[h]) / np.sqrt(d))
+        out[h] = p @ v
+        tol[h] = 2 * (p * delta) @ np.abs(v) + 2 * (p @ delta) * (p @ np.abs(v)) + len(rows) * 2.0 ** -126 * np.abs(v).max()
+    return out.ravel(), tol.ravel()
+
+
+@pytest.mark.parametrize("spread", [1e3, 1e4, 1e6])
+@pytest.mark.parametrize("d,ratio", [(32, 1), (64, 1), (64, 2), (96, 2), (128, 1), (64, 4), (128, 4), (32, 8), (64, 8)])
+@pytest.mark.parametrize("sizes,plen,mixed", [([], 0, False), ([3], 300, False), ([20], 300, False), ([6], 300, True)])
+def test_prefix_int8_wide_value_scales(A, d, ratio, sizes, plen, mixed, spread):
+    """Value scales far apart: every 16th row's is `spread` times the others' and its scores are too low to count, so it may
+    not cost the others their bits; `mixed` spreads the scales evenly in their logarithm instead."""
+    n = max(5, sum(sizes))
+    c = PrefixCase(A, d + ratio, "int8", d, 2 * ratio, 2, 16, sizes, [plen] * len(sizes), ([70, 200, 40, 33, 64] * n)[:n], no_group=n - sum(sizes))
+    r = np.random.RandomState(d)
+    if mixed:
+        wide = np.exp(r.uniform(0, np.log(spread), c.v64.shape[0]))
+    else:
+        wide = np.where(np.arange(c.v64.shape[0]) % 16 == 5, spread, 1.0)
+        c.q[:, ::d] = 300.0                       # dim 0 of every head: code -127 in a wide row, 0 in the others
+        codes = np.where(wide > 1, -127, 0).astype(np.int8)
+        for j in range(2):
+            c.kc[:, j * d] = dev(codes)
+            c.k64[:, j * d] = codes * np.nan_to_num(c.ks[:, j].double().cpu().numpy())
+    c.vs *= dev(wide.astype(np.float32))[:, None]
+    c.v64 = c.vc.double().cpu().numpy() * np.repeat(np.nan_to_num(c.vs.double().cpu().numpy()), d, 1)
+    out, _ = c.run()
+    for s in range(n):
+        want, tol = scores_bound(c, s)
+        err = np.abs(out[s].double().cpu().numpy() - want)
+        assert (err <= tol).all(), (s, (err / tol).max())
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("ratio", [1, 2, 4])
 @pytest.mark.parametrize("sizes,plen,no_group", [([], 0, 5), ([5], 300, 0), ([40], 300, 0)])
