@@ -453,7 +453,8 @@ ATTN_API int attn_rope_ex(const attn_rope_shape *s, int dtype, const float *tabl
 
 /* The serving form: q turned into q_out; k turned and v as it is written to
  * cache row slot_map[t] (a DEVICE array; a token whose slot is outside the
- * cache, -1 say, writes nothing there).  dtype ATTN_F32 into an ATTN_F32 or
+ * cache, -1 say, writes nothing there, and its position, which may be past the
+ * table where attn_page_plan_ex refused the token, is not reported).  dtype ATTN_F32 into an ATTN_F32 or
  * ATTN_I8 cache (quantised per (token, head) as attn_kv_quantize_int8 does),
  * ATTN_BF16 into an ATTN_BF16 cache.  Slots of a call must differ from one
  * another. */

@@ -46,11 +46,16 @@ struct Params {
     float sign;                           // -1: transpose
 };
 
-// Row of the table of token t.
-__device__ __forceinline__ int position_of(const Params &p, int t) {
+// Does a slot lie in the cache?  (Without a slot map every token has its row.)
+__device__ __forceinline__ bool in_cache(const Params &p, long long row) { return !p.slots || (row >= 0 && row < p.rows); }
+
+// Row of the table of token t.  A position outside it is reported, unless the
+// token has no place in the cache (slot `row`): a request that the page plan
+// refuses at its table's end asks for just such positions.
+__device__ __forceinline__ int position_of(const Params &p, int t, long long row) {
     int pos = p.positions ? __ldg(p.positions + t) : t % p.seq_len;
     if ((unsigned)pos >= (unsigned)p.max_pos) {
-        atomicExch(p.err, 0x701);
+        if (in_cache(p, row)) atomicExch(p.err, 0x701);
         pos = pos < 0 ? 0 : p.max_pos - 1;
     }
     return pos;
@@ -133,15 +138,15 @@ rope_kernel(const __grid_constant__ Params p)
 
     const int stride = (int)gridDim.x * p.tokens_per_block;
     int t = (int)blockIdx.x * p.tokens_per_block + tl;
-    auto position = [&](int t) { return turns && t < p.tokens ? position_of(p, t) : 0; };
     auto slot = [&](int t) { return p.slots && t < p.tokens ? __ldg(p.slots + t) : (long long)t; };
-    int next_pos = position(t);
+    auto position = [&](int t, long long row) { return turns && t < p.tokens ? position_of(p, t, row) : 0; };
     long long next_row = slot(t);
+    int next_pos = position(t, next_row);
     for (; t < p.tokens; t += stride) {
         const int pos = next_pos;
-        const long long row = !p.slots || (next_row >= 0 && next_row < p.rows) ? next_row : -1;
-        next_pos = position(t + stride);
+        const long long row = in_cache(p, next_row) ? next_row : -1;
         next_row = slot(t + stride);
+        next_pos = position(t + stride, next_row);
         float c[C], s[C];
         if (turns) {
             const float *cs = p.table + ((long long)pos * half + item * C) * 2;
@@ -224,11 +229,11 @@ rope_append_i8_kernel(const __grid_constant__ Params p, int interleaved, float *
     const int r = (int)(unit % per_token), h = r % p.kv_heads;
     const bool is_v = r >= p.kv_heads;
     const long long row = __ldg(p.slots + t);
-    if (row < 0 || row >= p.rows) return;
+    if (!in_cache(p, row)) return;
     const float *src = is_v ? static_cast<const float *>(p.v) + t * p.v_stride + (long long)h * D
                             : static_cast<const float *>(p.k) + t * p.k_stride + (long long)h * D;
     const int half = p.rot / 2;
-    const int pos = is_v || !p.rot ? 0 : position_of(p, t);
+    const int pos = is_v || !p.rot ? 0 : position_of(p, t, row);
     float x[E];
     float amax = 1e-8f;
 #pragma unroll
@@ -388,7 +393,6 @@ int launch_rope_append(const attn_rope_shape *s, const attn_paged_kv *c, int dty
     const int st = check_pdl(e, "rope_append_i8_kernel");
     if (st) return st;
     p.k = p.v = nullptr;                  // q alone
-    p.slots = nullptr;
     p.kv_heads = 0;
     p.all_heads = p.q_heads;
     p.k_out = p.v_out = nullptr;

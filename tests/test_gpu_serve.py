@@ -301,6 +301,47 @@ def test_rope_append(A, tokens, heads, kv_heads, d, rot, interleaved, kind, cach
         assert (c[mask] == 77).all()
 
 
+@pytest.mark.parametrize("kind,cache", [("f32", "f32"), ("bf16", "bf16"), ("f32", "int8")])
+@pytest.mark.parametrize("rot", [32, 6])
+def test_rope_append_after_a_refusal(A, kind, cache, rot):
+    """A request at the end of its table is refused one token more, whose position is past a rotary table of the cache's
+    length: no error is reported, and the other requests' tokens go where they should.  A token that has a slot and
+    such a position is reported."""
+    import torch
+    page, d, heads = 4, 32, 2
+    lens, new = np.array([8, 2, 0, 7], np.int32), np.array([2, 1, 3, 1], np.int32)
+    table = np.array([[0, 1], [2, -1], [-1, -1], [3, 4]], np.int32)
+    shape = A.PageShape(4, page, 2, 8, 8, 0)
+    plan = A.page_outputs(shape)
+    A.page_plan_t(shape, dev(lens), dev(new), dev(np.array([5, 6, 7, 0, 0, 0, 0, 0], np.int32)), dev(np.array([3], np.int32)), dev(table), plan)
+    slots, positions = plan["slot_map"].cpu().numpy(), plan["positions"].cpu().numpy()
+    assert slots.tolist() == [-1, -1, 10, 28, 29, 30, 19, -1] and positions.tolist() == [8, 9, 2, 0, 1, 2, 7, 0]
+    q, k, v, _, angles = rope_case(A, 5, 8, heads, heads, d, rot, kind, max_pos=8)
+    dt = torch.int8 if cache == "int8" else q.dtype
+    kc, vc = (torch.full((32, heads * d), 77, dtype=dt, device="cuda") for _ in range(2))
+    ks, vs = ((torch.full((32, heads), -1.0, device="cuda") for _ in range(2)) if cache == "int8" else (None, None))
+    rshape = A.RopeShape(8, 0, heads, heads, d, rot, 0, 8, 0, 0, 0, 0, 0)
+    paged, q_out = A.PageCache.of(kc, vc, ks, vs), torch.empty_like(q)
+    device_error(A)
+    A.rope_append_t(rshape, paged, dev(angles), plan["positions"], plan["slot_map"], q, k, v, q_out)
+    assert device_error(A) == 0
+    at = slots[slots >= 0]
+    want = R.rope(k.float().cpu().numpy(), heads, angles, np.minimum(positions, 7), rot, 0)[slots >= 0]
+    got = kc[dev(at)].float().cpu().numpy().astype(np.float64)
+    if cache == "int8":
+        step = np.repeat(ks[dev(at)].cpu().numpy().astype(np.float64), d, 1)
+        assert (np.abs(got * step - want) <= 0.5 * step * (1 + 2.0 ** -12)).all()      # half a code, and rounding
+        assert torch.equal(vc[dev(at)], A.quantize_int8_t(v, heads)[0][dev(slots >= 0)])
+    else:
+        rope_close(kc[dev(at)], k, want, heads, rot, kind)
+        assert torch.equal(vc[dev(at)], v[dev(slots >= 0)])
+    others = np.setdiff1d(np.arange(32), at)
+    assert (kc[dev(others)] == 77).all() and (vc[dev(others)] == 77).all()
+    plan["positions"][3] = 8
+    A.rope_append_t(rshape, paged, dev(angles), plan["positions"], plan["slot_map"], q, k, v, q_out)
+    assert device_error(A) == 0x701
+
+
 # ---------------------------------------------------------------------------
 # shared-prefix decode
 # ---------------------------------------------------------------------------
