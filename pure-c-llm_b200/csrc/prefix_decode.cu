@@ -201,22 +201,23 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
     if (h >= p.heads) return;
     const int hk = p.ratio == 1 ? h : h / p.ratio, hr = h - hk * p.ratio;
 
-    // the request's lines: its own and, by the lanes, 32 groups at a time
+    // The request's lines: its own and, by the lanes, 32 groups at a time.  A
+    // part whose bound is 0 has no launch of its own; its lengths are checked here.
     long long own_begin = 0, own_team = 1, pre_begin = 0, pre_team = 1;
-    Line own_line = {}, pre_line = {};
+    const Line own_line = line_of<false>(p, own, s);
+    Line pre_line = {};
     if (own.lines) {
         own_begin = __ldcg(own.line_first + s);
         own_team = __ldcg(own.line_first + own.lines + 1);
-        own_line = line_of<false>(p, own, s);
     }
     if (pre.lines) pre_team = __ldcg(pre.line_first + pre.lines + 1);
-    for (int g0 = 0; g0 < pre.lines; g0 += 32) {
+    for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
         const int g = g0 + lane;
-        const bool in = g < pre.lines && s >= group_first(p, g) && s < group_first(p, g + 1);
+        const bool in = g < p.n_groups && s >= group_first(p, g) && s < group_first(p, g + 1);
         const unsigned found = __ballot_sync(0xffffffffu, in);
         if (found) {
             const int mine = g0 + __ffs(found) - 1;
-            pre_begin = __ldcg(pre.line_first + mine);
+            if (pre.lines) pre_begin = __ldcg(pre.line_first + mine);
             pre_line = line_of<true>(p, pre, mine);
             break;
         }

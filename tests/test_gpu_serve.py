@@ -642,6 +642,27 @@ def test_prefix_bad_pages_and_lengths(A, kind):
     c.check(out, None)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_prefix_lengths_past_a_bound_of_zero(A, kind):
+    """A part whose bound is 0 has no rows, and lengths above the bound are reported all the same: own rows, a prefix,
+    and neither of them; not the prefix of a group without requests."""
+    c = PrefixCase(A, 15, kind, 64, 2, 2, 16, [2, 0, 1], [40, 7, 0], [9, 0, 30])
+    device_error(A)
+    full, lens, plens = (c.shape.max_len, c.shape.max_prefix_len), c.lens, c.plens
+    for own, prefix, code in ((0, full[1], 0x703), (full[0], 0, 0x703), (0, 0, 0x703), (full[0], full[1], 0)):
+        c.shape.max_len, c.shape.max_prefix_len = own, prefix
+        c.lens, c.plens = lens, plens
+        out, lse = c.run()
+        assert device_error(A) == code, (own, prefix)
+        c.lens, c.plens = np.minimum(lens, own), np.minimum(plens, prefix)
+        c.check(out, lse)
+    c.shape.max_len, c.shape.max_prefix_len, c.lens, c.plens = full[0], 0, lens, np.array([0, 7, 0], np.int32)
+    out, lse = c.run()
+    assert device_error(A) == 0
+    c.plens = 0 * plens
+    c.check(out, lse)
+
+
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
 def test_prefix_cache_past_32_bits(A, kind):
     """Rows whose element offsets pass 2^31."""
