@@ -244,7 +244,8 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
         const float mx = fmaxf(m, warp_max(ml.x));
         bad |= ml.y != ml.y;
         if (mx == -INFINITY) continue;    // no valid row in these pieces
-        const float old = exp2f(m - mx), c = exp2f(ml.x - mx);
+        const bool rows = ml.x != -INFINITY;
+        const float old = exp2f(m - mx), c = rows ? exp2f(ml.x - mx) : 0.f;
         l = l * old + warp_sum(ml.y * c);
 #pragma unroll
         for (int i = 0; i < E; i++) o[i] *= old;
@@ -260,10 +261,11 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
             }
 #pragma unroll
             for (int k = 0; k < kMany; k++) {
-                // (a piece without a valid row has weight 0, and an o that may not have been written)
-                const float w = __shfl_sync(0xffffffffu, c, k0 + k);
+                // A piece without a valid row has an o that may not have been written; one whose weight is 0
+                // because its scores are low still hands on a value that is no number.
+                const float w = __shfl_sync(0xffffffffu, rows ? c : -1.f, k0 + k);
 #pragma unroll
-                for (int i = 0; i < E; i++) o[i] = w > 0.f ? fmaf(x[k][i], w, o[i]) : o[i];
+                for (int i = 0; i < E; i++) o[i] = w >= 0.f ? fmaf(x[k][i], w, o[i]) : o[i];
             }
         }
     }

@@ -591,6 +591,25 @@ def test_prefix_not_numbers(A, kind, ratio, sizes, plen, no_group):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("ratio", [1, 4])
+@pytest.mark.parametrize("n", [5, 40])
+def test_prefix_value_not_a_number_without_weight(A, kind, ratio, n):
+    """A prefix of one row whose value is no number, and whose score is so low that its weight is 0 beside the own rows':
+    it shows all the same, in its own key head alone."""
+    c = PrefixCase(A, 16, kind, 64, 2 * ratio, 2, 16, [n], [1], ([70, 0, 40, 33, 300] * n)[:n])
+    c.q.fill_(4.0)
+    row = c.rows_of(0)[0]
+    if kind == "int8":
+        c.kc[row] = -127
+        c.ks[row], c.vs[row, 1] = 0.5, float("nan")
+    else:
+        c.kc[row], c.vc[row, 64:] = -60.0, float("nan")
+    out, lse = c.run()
+    o = out.view(n, 2, ratio, 64).isfinite()
+    assert o[:, 0].all() and not o[:, 1].any() and lse.isfinite().all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_prefix_sharp_scores(A, kind):
     """Scores of many hundreds: the largest key alone counts, and nothing overflows."""
     c = PrefixCase(A, 11, kind, 64, 4, 4, 16, [6], [700], [0, 10, 300, 1, 64, 65], q_std=300.0)
