@@ -86,9 +86,16 @@ struct Line {
     int keys, steps, blocks;              // blocks of query rows
     int first_req, rows, base;            // of the line's query rows; index of its first block
     // cost of a segment, and of the line, in steps
-    __device__ int cost() const { return steps + kBegin; }
+    __host__ __device__ int cost() const { return steps + kBegin; }
     __device__ long long total(const Part &w) const { return steps ? (long long)cost() * blocks * w.n_blocks : 0; }
 };
+// First step of a query row's segment in the order of all steps, for a row of
+// the line that begins at line_begin; 0 in a part that the call does not have.
+__host__ __device__ __forceinline__ long long segment_begin(const Part &w, const Line &l, int row, int hk, long long line_begin) {
+    if (!w.lines) return 0;
+    const int rb = row >> w.log_rows, hb = w.n_blocks == 1 ? 0 : hk / w.head_block;
+    return line_begin + (long long)(rb * w.n_blocks + hb) * l.cost() + kBegin;
+}
 template <bool PRE>
 __device__ __forceinline__ Line line_of(const Params &p, const Part &w, int i) {
     Line l;

@@ -166,11 +166,6 @@ struct Pieces {
 };
 constexpr int kMergeWarps = 4, kMany = 8;
 
-// First step of the row's segment in the order of all steps.
-__device__ __forceinline__ long long segment_begin(const Part &w, const Line &l, int row, int hk, long long line_begin) {
-    const int rb = row >> w.log_rows, hb = w.n_blocks == 1 ? 0 : hk / w.head_block;
-    return line_begin + (long long)(rb * w.n_blocks + hb) * l.cost() + kBegin;
-}
 // The pieces of a row, from teams t0 .. t1.
 template <int D>
 __device__ __forceinline__ Pieces pieces_of(const Part &w, const Line &l, int row, int hk, int t0, int t1) {
