@@ -344,8 +344,8 @@ ATTN_API int attn_kv_cache_append(attn_kv_cache *c, int layer, int pos,
  * each new token takes), attn_rope_append_ex (positions turned into Q and K,
  * K and V written to those rows) and attn_prefix_decode_ex (one query token
  * per request over the rows its group shares and its own).
- * None of these allocates, except attn_prefix_decode_ex without a workspace;
- * all run on the caller's stream and may be captured in a graph.
+ * All run on the caller's stream; none allocates, and all may be captured in a
+ * graph, except attn_prefix_decode_ex without a workspace of the caller's.
  * ---------------------------------------------------------------------- */
 /* A cache of `rows` token rows.  Page p of a P-token page size is rows
  * [p*P, (p+1)*P); row r of head h starts at element r*row_stride + h*d, as in
@@ -499,7 +499,9 @@ ATTN_API size_t attn_prefix_decode_workspace_bytes(const attn_prefix_shape *s, c
  * bf16: bf16 products, probabilities rounded to bf16, fp32 sums and statistics.
  * A NaN in a query or a row that is read gives NaN in the outputs it reaches.
  * workspace (256-byte aligned) may be NULL: the library's own per-device
- * buffer, grown on demand; calls that use it must not overlap on the GPU. */
+ * buffer, grown on demand; calls that use it must not overlap on the GPU, and
+ * while the stream is captured it is refused (ATTN_ERR_WORKSPACE), because a
+ * graph would outlive the buffer. */
 ATTN_API int attn_prefix_decode_ex(const attn_prefix_shape *s, const attn_paged_kv *cache,
                 const void *q, const int *group_begin, const int *prefix_table,
                 const int *prefix_lens, const int *block_table, const int *lens, void *out,

@@ -236,8 +236,15 @@ int attn_prefix_decode_ex(const attn_prefix_shape *s, const attn_paged_kv *cache
         if (workspace_bytes < need || !aligned(workspace, 256))
             return set_error(ATTN_ERR_WORKSPACE, "prefix decode: workspace needs %zu bytes (256-byte aligned), got %zu",
                              need, workspace_bytes);
-    } else if (!(workspace = library_workspace(4, need, cs))) {
-        return set_error(ATTN_ERR_NOMEM, "prefix decode: cannot allocate %zu-byte workspace", need);
+    } else {
+        // A graph would keep the address of a buffer that a later, larger call replaces.
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        const cudaError_t e = cudaStreamIsCapturing(cs, &capture);
+        if (e != cudaSuccess) (void)cudaGetLastError();
+        if (capture != cudaStreamCaptureStatusNone || e == cudaErrorStreamCaptureImplicit)
+            return set_error(ATTN_ERR_WORKSPACE, "prefix decode: a graph needs a workspace of the caller's (%zu bytes)", need);
+        if (!(workspace = library_workspace(4, need, cs)))
+            return set_error(ATTN_ERR_NOMEM, "prefix decode: cannot allocate %zu-byte workspace", need);
     }
     attn::prefix::Params p = {};
     p.q = q; p.k = cache->k; p.v = cache->v; p.kscale = cache->kscale; p.vscale = cache->vscale;

@@ -744,6 +744,34 @@ def test_serving_calls_are_captured_in_a_graph(A):
     assert torch.equal(out, want) and float(out.abs().sum()) > 0
 
 
+def prefix_call(A, c, q, out, lse, workspace):
+    """A call on device arrays made beforehand, as a captured one needs."""
+    group = (dev(c.begin), dev(c.ptable), dev(c.plens))
+    own = (dev(c.table), dev(c.lens))
+    return lambda: A.prefix_decode_t(c.shape, c.cache, q, *group, *own, out, lse=lse, workspace=workspace)
+
+
+def test_prefix_without_a_workspace_is_refused_in_a_graph(A):
+    """The library's buffer may move, and a graph would keep its address: refused while capturing, and the capture goes on."""
+    import torch
+    c = PrefixCase(A, 17, "f32", 64, 4, 2, 16, [3], [100], [20, 0, 40])
+    want, wl = c.run(workspace=None)
+    out, lse = torch.zeros_like(want), torch.zeros_like(wl)
+    work = torch.empty(A.prefix_decode_workspace_bytes(c.shape, c.cache), dtype=torch.uint8, device="cuda")
+    refused, taken = (prefix_call(A, c, c.q, out, lse, w) for w in (None, work))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(A.AttnError, match="workspace") as e:
+            refused()
+        taken()
+    assert e.value.status == A.ERR_WORKSPACE
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(lse, wl)
+    again, _ = c.run(workspace=None)
+    assert torch.equal(again, want)
+
+
 @pytest.mark.parametrize("cache", ["f32", "int8"])
 def test_serving_example(A, cache):
     """The example's loop: projection, plan, append and decode together; fp32 arithmetic, the repository's 1e-5."""
