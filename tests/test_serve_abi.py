@@ -1,6 +1,8 @@
 """Refusals of the serving entry points: argument checks run before any CUDA call."""
 import ctypes
 
+import pytest
+
 import attn_b200 as A
 
 P = 1 << 20                                      # an aligned stand-in address
@@ -114,3 +116,165 @@ def test_prefix_decode_refusals():
     assert decode(shape, kv(), ws=P, ws_bytes=1) == A.ERR_WORKSPACE
     assert decode(shape, kv(), ws=P + 16, ws_bytes=1 << 30) == A.ERR_WORKSPACE
     assert decode(A.PrefixShape(**{**ok, "n_seq": 0}), kv()) == A.OK
+
+
+# ---------------------------------------------------------------------------
+# the torch forms: each tensor is held against the shape beside it
+# ---------------------------------------------------------------------------
+class Given:
+    """A stand-in for a CUDA tensor: what the checks look at, at an address that is never read."""
+
+    def __init__(self, tensor, is_cuda=True):
+        self.t, self.is_cuda, self.device = tensor, is_cuda, "cuda:0" if is_cuda else "cpu"
+        self.dtype, self.shape = tensor.dtype, tensor.shape
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+class Reached(Exception):
+    pass
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """Calls that pass the checks end with Reached and not in the library."""
+    def stop(*args):
+        raise Reached
+
+    class Lib:
+        def __getattr__(self, name):
+            return stop
+    monkeypatch.setattr(A, "lib", Lib())
+    monkeypatch.setattr(A, "_stream", lambda: 0)
+
+
+def refused(call, given, bad, error):
+    with pytest.raises(error) as e:
+        call(**{**given, **bad})
+    assert next(iter(bad)) in str(e.value), str(e.value)
+
+
+def each_refused(call, given, optional=()):
+    """Every tensor on its own: of another type, too short, on the host."""
+    import torch
+    with pytest.raises(Reached):
+        call(**given)
+    for name, g in given.items():
+        other = torch.int64 if g.dtype == torch.int32 else torch.int32 if g.dtype == torch.int64 else torch.float64
+        if name != "q" and name != "workspace":
+            refused(call, given, {name: Given(g.t.to(other))}, TypeError)
+        refused(call, given, {name: Given(g.t, is_cuda=False)}, ValueError)
+        if name != "workspace":
+            refused(call, given, {name: Given(g.t[:-1])}, ValueError)
+            if g.numel() > 1:
+                refused(call, given, {name: Given(torch.empty((2 * g.shape[0],) + g.shape[1:], dtype=g.dtype)[::2])}, ValueError)
+        if name in optional:
+            with pytest.raises(Reached):
+                call(**{**given, name: None})
+
+
+def ints(*shape, dtype=None):
+    import torch
+    return Given(torch.zeros(shape, dtype=dtype or torch.int32))
+
+
+def test_page_plan_tensors(calls):
+    import torch
+    shape = A.PageShape(4, 16, 8, 32, 64, 0)
+    given = dict(lens=ints(4), new_lens=ints(4), pos_base=ints(4), free_pages=ints(64), free_count=ints(1), block_table=ints(4, 8),
+                 cu_new=ints(5), positions=ints(32), token_seq=ints(32), counts=ints(4), slot_map=ints(32, dtype=torch.int64), lens_out=ints(4))
+
+    def call(**kw):
+        out = {k: kw[k] for k in ("cu_new", "positions", "token_seq", "counts", "slot_map")}
+        A.page_plan_t(shape, kw["lens"], kw["new_lens"], kw["free_pages"], kw["free_count"], kw["block_table"], {**out, "lens": kw["lens_out"]},
+                      pos_base=kw["pos_base"])
+    lens_out = given.pop("lens_out")
+    each_refused(lambda **kw: call(lens_out=lens_out, **kw), given, optional=("pos_base", "token_seq"))
+    with pytest.raises(TypeError, match="lens"):
+        call(**given, lens_out=ints(4, dtype=torch.int64))
+    with pytest.raises(ValueError, match="lens"):
+        call(**given, lens_out=ints(3))
+    given["lens_out"], shape.table_stride = lens_out, 11  # a table inside a wider one
+    with pytest.raises(ValueError, match="block_table"):
+        call(**given)
+    for table in (ints(4, 11), Given(torch.zeros((4, 11), dtype=torch.int32)[:, 2:10])):
+        with pytest.raises(Reached):
+            call(**{**given, "block_table": table})
+
+
+def test_rope_tensors(calls):
+    import torch
+    shape = A.RopeShape(6, 0, 4, 2, 32, 32, 0, 16, 0, 0, 0, 0, 0)
+    f = dict(dtype=torch.float32)
+    given = dict(table=Given(torch.zeros((16, 16, 2))), positions=ints(6), q=ints(6, 128, **f), k=ints(6, 64, **f), q_out=ints(6, 128, **f),
+                 k_out=ints(6, 64, **f))
+
+    def call(**kw):
+        A.rope_t(shape, kw["table"], kw["positions"], kw["q"], kw["k"], kw["q_out"], kw["k_out"])
+    each_refused(call, given, optional=("positions", "k", "k_out"))
+    refused(call, given, {"k": ints(6, 64, dtype=torch.bfloat16)}, TypeError)
+    refused(call, given, {"q": Given(torch.zeros((6, 200))[:, :128])}, ValueError)          # its stride is not the shape's
+    refused(call, given, {"q": ints(6, 256, **f)}, ValueError)
+    for q in (ints(6, 4, 32, **f), ints(24, 32, **f), ints(9, 128, **f)):     # the same memory in other shapes, and more of it
+        with pytest.raises(Reached):
+            call(**{**given, "q": q})
+    shape.q_row_stride = 200
+    with pytest.raises(Reached):
+        call(**{**given, "q": Given(torch.zeros((6, 200))[:, 30:158])})
+
+
+def test_rope_append_tensors(calls):
+    import torch
+    shape = A.RopeShape(6, 0, 4, 2, 32, 32, 0, 16, 0, 0, 0, 0, 0)
+    f = dict(dtype=torch.float32)
+    given = dict(table=Given(torch.zeros((16, 16, 2))), positions=ints(6), slot_map=ints(6, dtype=torch.int64), q=ints(6, 128, **f),
+                 k=ints(6, 64, **f), v=ints(6, 64, **f), q_out=ints(6, 128, **f))
+    cache = A.PageCache.of(ints(32, 64, **f), ints(32, 64, **f))
+
+    def call(kv=cache, **kw):
+        A.rope_append_t(shape, kv, kw["table"], kw["positions"], kw["slot_map"], kw["q"], kw["k"], kw["v"], kw["q_out"])
+    each_refused(call, given, optional=("positions",))
+    narrow = A.PageCache.of(*(Given(torch.zeros((32, 96))[:, :32]) for _ in range(2)))
+    codes = [ints(32, 64, dtype=torch.int8) for _ in range(2)]
+    other = A.PageCache.of(*codes, *(Given(torch.zeros(32, 4)) for _ in range(2)))
+    for kv, word in ((narrow, "rows of 32"), (other, "scales of 4")):
+        with pytest.raises(ValueError, match=word):
+            call(kv=kv, **given)
+
+
+def test_page_cache_tensors():
+    import torch
+    f = dict(dtype=torch.float32)
+    k, scale, codes = ints(8, 64, **f), ints(8, 2, **f), ints(8, 64, dtype=torch.int8)
+    A.PageCache.of(k, k)
+    A.PageCache.of(codes, codes, scale, scale)
+    for bad in ((k, ints(8, 64, dtype=torch.bfloat16)), (k, ints(7, 64, **f)), (k, Given(k.t, is_cuda=False)), (ints(512, **f),) * 2,
+                (codes, codes), (codes, codes, scale, None), (codes, codes, scale, ints(7, 2, **f)), (codes, codes, scale, ints(8, 3, **f))):
+        with pytest.raises(ValueError):
+            A.PageCache.of(*bad)
+    for bad in ((codes, codes, scale, ints(8, 2, dtype=torch.float64)), (ints(8, 64, dtype=torch.float64),) * 2):
+        with pytest.raises(TypeError):
+            A.PageCache.of(*bad)
+
+
+def test_prefix_decode_tensors(calls):
+    import torch
+    shape = A.PrefixShape(4, 2, 4, 2, 32, A.BF16, 16, 3, 5, 48, 80, 0, 0, 0.0)
+    b = dict(dtype=torch.bfloat16)
+    given = dict(q=ints(4, 128, **b), group_begin=ints(3), prefix_table=ints(2, 3), prefix_lens=ints(2), block_table=ints(4, 5), lens=ints(4),
+                 out=ints(4, 128, **b), lse=ints(4, 4, dtype=torch.float32), workspace=ints(64, dtype=torch.uint8))
+    cache = A.PageCache.of(ints(32, 64, **b), ints(32, 64, **b))
+
+    def call(**kw):
+        A.prefix_decode_t(shape, cache, kw["q"], kw["group_begin"], kw["prefix_table"], kw["prefix_lens"], kw["block_table"], kw["lens"],
+                          kw["out"], lse=kw["lse"], workspace=kw["workspace"])
+    each_refused(call, given, optional=("lse", "workspace"))
+    refused(call, given, {"q": ints(4, 128, dtype=torch.float32)}, TypeError)
+    refused(call, given, {"block_table": ints(4, 6)}, ValueError)                          # its lines are not max_pages apart
+    with pytest.raises(ValueError, match="rows of 64"):
+        shape.kv_heads = 4
+        call(**given)
+    shape.kv_heads, shape.n_groups = 2, 0
+    with pytest.raises(Reached):
+        call(**{**given, "group_begin": None, "prefix_table": None, "prefix_lens": None})
