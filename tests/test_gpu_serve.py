@@ -782,3 +782,14 @@ def test_serving_example(A, cache):
     m = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(m)
     assert m.main(requests=6, prompt=130, steps=21, cache=cache) < 1e-5
+
+
+def test_serving_example_uses_the_prompts_attention(A, monkeypatch):
+    """What the prompt attends to reaches the requests, and an output that is no number reaches the example's result."""
+    import runpy
+    import os
+    from conftest import ROOT
+    m = runpy.run_path(os.path.join(ROOT, "examples", "serve_shared_prefix.py"))
+    forward = A.forward_t
+    monkeypatch.setattr(A, "forward_t", lambda *a, **kw: (forward(*a, **kw)[0] * float("nan"), None))
+    assert not m["main"](requests=2, prompt=20, steps=3) < 1e-5
