@@ -708,6 +708,84 @@ def test_prefix_cache_past_32_bits(A, kind):
     assert torch.equal(out, want) and torch.equal(lse, wl)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("sizes", [[224] + [1] * 32, [0, 1, 2, 0, 3, 5] * 15, [1] * 70])
+def test_prefix_many_groups(A, kind, sizes):
+    """More groups than a warp looks through at once, empty ones and one that has most of the requests."""
+    r = np.random.RandomState(len(sizes))
+    n = sum(sizes) + 3
+    c = PrefixCase(A, 18, kind, 32, 4, 2, 16, sizes, r.randint(0, 90, len(sizes)), r.randint(0, 20, n), no_group=3)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [6, 70])
+def test_prefix_call_in_a_graph(A, kind, n):
+    """A call with a prefix (own rows' launch beside the prefix's) between other work on the stream, captured and replayed
+    with other queries and lengths: the same bits as the calls one by one."""
+    import torch
+    c = PrefixCase(A, 19, kind, 64, 4, 2, 16, [n // 2, n - n // 2], [300, 90], np.random.RandomState(n).randint(0, 60, n))
+    queries = [dev(synth.normal(40 + i, tuple(c.q.shape)), c.q.dtype) for i in range(3)]
+    lengths = [dev(np.minimum(c.lens, m).astype(np.int32)) for m in (60, 31, 7)]
+    q, lens, out = torch.empty_like(c.q), torch.empty_like(lengths[0]), torch.empty_like(c.q)
+    lse, twice = torch.empty((n, 4), device="cuda"), torch.empty_like(c.q)
+    work = torch.empty(A.prefix_decode_workspace_bytes(c.shape, c.cache), dtype=torch.uint8, device="cuda")
+    group, table, given = (dev(c.begin), dev(c.ptable), dev(c.plens)), dev(c.table), (torch.empty_like(c.q), torch.empty_like(lens))
+
+    def step():
+        q.copy_(given[0])
+        lens.copy_(given[1])
+        A.prefix_decode_t(c.shape, c.cache, q, *group, table, lens, out, lse=lse, workspace=work)
+        torch.mul(out, 2, out=twice)
+        q.zero_()                         # the next call's inputs may be written as soon as this one is over
+        lens.zero_()
+
+    want = []
+    for x in zip(queries, lengths):
+        for to, src in zip(given, x):
+            to.copy_(src)
+        step()
+        want.append((twice.clone(), lse.clone()))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+        step()
+    for x, (w, wl) in zip(zip(queries, lengths), want):
+        for to, src in zip(given, x):
+            to.copy_(src)
+        twice.zero_()
+        lse.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(twice, w) and torch.equal(lse, wl)
+    c.q, c.lens = queries[0], lengths[0].cpu().numpy()
+    c.check(want[0][0] / 2, want[0][1])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_prefix_calls_on_two_streams(A, kind):
+    """Two calls at a time, each on its stream with its workspace: the same bits as alone."""
+    import torch
+    cases = [PrefixCase(A, 20 + i, kind, 64, 4, 2, 16, [n], [plen], np.random.RandomState(n).randint(0, 300, n))
+             for i, (n, plen) in enumerate(((40, 700), (9, 2000)))]
+    want = [c.run() for c in cases]
+    outs = [(torch.empty_like(w), torch.empty_like(l)) for w, l in want]
+    calls = [prefix_call(A, c, c.q, *o, torch.empty(A.prefix_decode_workspace_bytes(c.shape, c.cache), dtype=torch.uint8, device="cuda"))
+             for c, o in zip(cases, outs)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for o in outs:
+            o[0].fill_(float("nan"))
+        torch.cuda.synchronize()
+        for call, stream in zip(calls, streams):
+            with torch.cuda.stream(stream):
+                call()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o[0], w[0]) and torch.equal(o[1], w[1])
+
+
 def test_serving_calls_are_captured_in_a_graph(A):
     """plan, append and decode in one CUDA graph, replayed: the same results as the calls."""
     import torch
