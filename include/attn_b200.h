@@ -496,7 +496,7 @@ ATTN_API size_t attn_prefix_decode_workspace_bytes(const attn_prefix_shape *s, c
  * [0, max] is clamped and records 0x703 in the device error word; a page
  * outside the cache records 0x702 and its rows count as absent.  fp32 and INT8
  * caches: fp32 arithmetic or products of exact parts with fp32 or integer sums;
- * bf16: bf16 products, probabilities rounded to bf16, fp32 sums and statistics.
+ * bf16: bf16 products, probabilities in two bf16 parts, fp32 sums and statistics.
  * A NaN in a query or a row that is read gives NaN in the outputs it reaches.
  * workspace (256-byte aligned) may be NULL: the library's own per-device
  * buffer, grown on demand; calls that use it must not overlap on the GPU, and

@@ -22,16 +22,18 @@
 //               instructions setting the pace.)
 //   warp 2      S_wu = Q_w K_u^T for the two halves u of a step's keys, M = 128,
 //               N = 64, both operands in shared memory
-//   warp 3      O_w += P_wu V_u (P from TMEM, V as it lies, MN-major)
+//   warp 3      O_w += P_wu V_u (P in two bf16 parts from TMEM, V as it lies, MN-major)
 //   warps 4-7   softmax of warpgroup 0, warps 8-11 of warpgroup 1: a warp
 //               brings 32 query rows in, a thread keeps the maximum and sum of its row
-//               (a TMEM lane), writes its bf16
-//               probabilities to TMEM, and rescales O when the maximum grew by
+//               (a TMEM lane), writes its probabilities to TMEM, and rescales O when the maximum grew by
 //               more than 2^8 (a stale one leaves P <= 256, and the piece's
 //               (m, l, o) stay consistent).  All exponentials on MUFU: lse is an
 //               output.
-// TMEM: four S of 64 columns, each overwritten by its P, and two O (512 columns
-// at d 128).  S_w1 is formed while S_w0 is in the softmax, so a warpgroup does
+// A probability goes in as two bf16 parts, its rounding and the rest, which leaves
+// no error but that of rounding the output (one part: 1.4 times it).  The second
+// product and its packing cost documents 297 -> 321 us and chat 54.5 -> 57.
+// TMEM: four S of 64 columns, each overwritten by the two parts of its P, and two
+// O (512 columns at d 128).  S_w1 is formed while S_w0 is in the softmax, so a warpgroup does
 // not wait for its own products.  (With 128 keys in one S per warpgroup the
 // chain softmax, PV, next S took 5,300 cycles a step, of which the exponentials
 // of both warpgroups are 2,048; with P in halves but S in one product 171 us, the
@@ -297,8 +299,8 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                     if (leader) {
                         const uint64_t vd = sw128_desc(sKV + slot * C::TILE + u * BH * 128, BM * 128, 1024);
 #pragma unroll
-                        for (int kk = 0; kk < BH / 16; kk++)      // 16 keys: 8 columns of P, 2 KB of V
-                            mma_bf16_ts(tmem + col_o<D>(wg), tmem + col_s(wg, u) + kk * 8, vd + 128 * kk, id, !first || kk > 0);
+                        for (int kk = 0; kk < 2 * BH / 16; kk++)  // 16 keys: 8 columns of a part of P, 2 KB of V
+                            mma_bf16_ts(tmem + col_o<D>(wg), tmem + col_s(wg, u) + kk * 8, vd + 128 * (kk % (BH / 16)), id, !first || kk > 0);
                         mma_commit(BAR(B_OD + b));
                     }
                     __syncwarp();
@@ -387,7 +389,7 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                         const float neg = m == -INFINITY ? 0.f : -m;
                         const uint64_t scale2 = f2(p.scale_log2, p.scale_log2), neg2 = f2(neg, neg);
                         uint64_t l2[4] = {0ull, 0ull, 0ull, 0ull};
-                        uint32_t pk[32];
+                        uint32_t hi[32], lo[32];
 #pragma unroll
                         for (int c = 0; c < 32; c++) {
                             float e, f;
@@ -395,14 +397,15 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                             e = ex2(e);
                             f = ex2(f);
                             l2[c & 3] = add2(l2[c & 3], f2(e, f));
-                            pk[c] = pack_bf16(e, f);
+                            bf16_parts(e, f, hi[c], lo[c]);
                         }
                         {
                             float e, f;
                             f2_split(add2(add2(l2[0], l2[1]), add2(l2[2], l2[3])), e, f);
                             l += e + f;
                         }
-                        tmem_st32(tS, pk);                        // over S, which is in registers
+                        tmem_st32(tS, hi);                        // over S, which is in registers
+                        tmem_st32(tS + 32, lo);
                         if (__any_sync(0xffffffffu, any && grow)) {
                             // O is the previous half's product's until that is done
                             ok = mbar_wait(BAR(B_OD + 2 * wg + 1 - u), (t - 1 + u) & 1, abort_flag, p.err, 0x833 + u);

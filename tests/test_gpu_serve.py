@@ -479,6 +479,21 @@ def test_prefix_tiles(A, d, heads, kv_heads, page, sizes, plens):
     assert torch_equal(again, out) and torch_equal(l2, lse)
 
 
+@pytest.mark.parametrize("d,heads,kv_heads", [(32, 4, 4), (64, 4, 4), (96, 6, 2), (128, 4, 2)])
+@pytest.mark.parametrize("n,plen", [(3, 50), (12, 700), (20, 3), (40, 9), (70, 900), (140, 65)])
+def test_prefix_bf16_error_is_the_outputs_rounding(A, d, heads, kv_heads, n, plen):
+    """The same precision whatever the group's size: rounding the output (2^-8 of it), a probability's second part (2^-17 of
+    it) and the scores (4 delta) are all there is between a bf16 result and the 64-bit one."""
+    c = PrefixCase(A, d + n, "bf16", d, heads, kv_heads, 16, [n], [plen], np.random.RandomState(n).randint(0, 20, n))
+    out, _ = c.run()
+    for s in range(0, n, 3):
+        rows = c.rows_of(s)
+        want, _, weight, reach = R.prefix_decode(c.q[s].double().cpu().numpy(), c.k64[rows], c.v64[rows], heads, kv_heads, 1 / np.sqrt(d))
+        tol = 2.0 ** -8 * np.abs(want) + (2.0 ** -17 + 4 * 2.0 ** -21 * (1 + np.repeat(reach, d))) * weight
+        err = np.abs(out[s].double().cpu().numpy() - want)
+        assert (err <= tol).all(), (s, (err / tol).max())
+
+
 def test_prefix_tiles_bad_page(A):
     """A page outside the cache in the middle of a tile's keys: its rows are absent, and nothing is read there."""
     c = PrefixCase(A, 21, "bf16", 128, 4, 1, 16, [40], [600], [3] * 40)
