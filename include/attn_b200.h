@@ -410,7 +410,12 @@ ATTN_API int attn_page_plan_ex(const attn_page_shape *s, const int *lens, const 
  *   ATTN_ROPE_RAMP    by wavelength: a pair that turns more than `fast` times
  *                     within trained_len tokens keeps f_i, one that turns less
  *                     than `slow` times takes f_i / factor, and between them
- *                     the two are mixed linearly in the pair's index
+ *                     the two are mixed linearly in the pair's index, between
+ *                     the indices (no whole numbers) where a pair turns just
+ *                     `fast` and just `slow` times.  A checkpoint trained with
+ *                     another mixture (bounds rounded to whole pairs, or linear
+ *                     in the number of turns) brings its own table:
+ *                     attn_rope_ex takes any
  * Every table entry is multiplied by `magnitude` (0: 1). */
 enum { ATTN_ROPE_PLAIN = 0, ATTN_ROPE_LINEAR = 1, ATTN_ROPE_BASE = 2, ATTN_ROPE_RAMP = 3 };
 typedef struct {
@@ -455,7 +460,8 @@ ATTN_API int attn_rope_ex(const attn_rope_shape *s, int dtype, const float *tabl
  * cache row slot_map[t] (a DEVICE array; a token whose slot is outside the
  * cache, -1 say, writes nothing there, and its position, which may be past the
  * table where attn_page_plan_ex refused the token, is not reported).  dtype ATTN_F32 into an ATTN_F32 or
- * ATTN_I8 cache (quantised per (token, head) as attn_kv_quantize_int8 does),
+ * ATTN_I8 cache (quantised per (token, head) as attn_kv_quantize_int8 does: a
+ * NaN among a head's elements becomes a code like any other, -127),
  * ATTN_BF16 into an ATTN_BF16 cache.  Slots of a call must differ from one
  * another. */
 ATTN_API int attn_rope_append_ex(const attn_rope_shape *s, const attn_paged_kv *cache, int dtype,
@@ -483,8 +489,10 @@ typedef struct {
 ATTN_API size_t attn_prefix_decode_workspace_bytes(const attn_prefix_shape *s, const attn_paged_kv *cache);
 
 /* Decodes one query token per request over the rows of its group's prefix and
- * its own rows, as one softmax: out = sum_j softmax_j(scale q.k_j) v_j.  The
- * prefix is read once for all requests of a group.
+ * its own rows, as one softmax: out = sum_j softmax_j(scale q.k_j) v_j.  A
+ * prefix is read once for each block of its group's query rows (requests x
+ * heads/kv_heads), not for each request; a block has up to 4 to 256 rows, more
+ * where the groups have more on average.
  *   group_begin[n_groups+1] (DEVICE, ascending): group g is requests
  *     [group_begin[g], group_begin[g+1]); a request of no group has no prefix.
  *   prefix_table[n_groups][max_prefix_pages], prefix_lens[n_groups],
@@ -497,7 +505,8 @@ ATTN_API size_t attn_prefix_decode_workspace_bytes(const attn_prefix_shape *s, c
  * outside the cache records 0x702 and its rows count as absent.  fp32 and INT8
  * caches: fp32 arithmetic or products of exact parts with fp32 or integer sums;
  * bf16: bf16 products, probabilities in two bf16 parts, fp32 sums and statistics.
- * A NaN in a query or a row that is read gives NaN in the outputs it reaches.
+ * A NaN in a query or a row that is read gives NaN in the outputs it reaches (in
+ * an ATTN_I8 cache a NaN can be in a scale only).
  * workspace (256-byte aligned) may be NULL: the library's own per-device
  * buffer, grown on demand; calls that use it must not overlap on the GPU, and
  * while the stream is captured it is refused (ATTN_ERR_WORKSPACE), because a

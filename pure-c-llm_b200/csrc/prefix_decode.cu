@@ -374,7 +374,9 @@ int run(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s) {
     using T = typename Own::Type;
     constexpr int OWN_CTAS = Own::LEAN ? 2 : 1, PRE_CTAS = Pre::LEAN ? 2 : 1;
     // The tensor-core tiles take prefixes of bf16 caches from 32 query rows a
-    // group on (counted on average: the groups' sizes are on the device).
+    // group on (counted on average: the groups' sizes are on the device).  A call
+    // on an 8192-row prefix in us, warps and tiles, 8 x 128: 24 rows 30.4 and 28.5, 32 rows
+    // 32.2 and 29.0, 64 rows 40.2 and 32.0; 16 x 64: 31.9 and 32.1, 33.1 and 32.7, 39.6 and 35.0.
     const bool tile = sizeof(T) == 2 && (D == 64 || D == 128) && p.n_groups &&
                       (long long)p.n_seq * p.ratio >= 32LL * p.n_groups;
     const Layout L = lay_out(p, D, Own::ROWS, Own::KEYS, sm_count_here() * OWN_CTAS, Pre::ROWS, Pre::KEYS,
@@ -398,7 +400,11 @@ int run(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s) {
 template <class Own, int D>
 int run_pre(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s, long long rows) {
     using namespace attn::prefix;
-    // as many rows as the registers hold (o takes D NT / 4 of them), where there are more than one tile's
+    // As many rows as the registers hold (o takes D NT / 4 of them), where there are more than one tile's.
+    // A call on an 8192-row prefix in us, one tile and several: bf16 8 x 128: 8 rows 27.9 and 24.9, 16 rows
+    // 27.5 and 26.1, 48 rows 39.0 and 36.4; 16 x 64: 23.3 and 25.0, 25.6 and 29.9, 38.1 and 38.1.  INT8 8 x 128:
+    // 4 rows 25.1 and 23.4, 8 rows 24.5 and 24.6, 16 rows 28.4 and 27.2; 16 x 64: 20.3 and 24.9, 22.4 and 26.4,
+    // 31.8 and 30.7.  (One tile a piece reads the rows again for each 8, or 4, query rows, from L2 mostly.)
     constexpr bool BF16 = sizeof(typename Own::Type) == 2;
     if constexpr (BF16) {
         if (rows <= 8) return run<Own, Bf16Path<D, 1>, D>(p, ws, need, s);
@@ -411,6 +417,8 @@ int run_pre(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t 
 template <class Own, int D>
 int run_pre_f32(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s, long long rows) {
     using namespace attn::prefix;
+    // 4 rows a piece and 8, in us on an 8192-row prefix: 12 x 128: 4 rows 43.6 and 36.4, 5 rows 55.2 and 36.7;
+    // 16 x 64: 31.1 and 33.0, 37.2 and 33.0
     if (rows <= 4) return run<Own, F32Path<D, 4>, D>(p, ws, need, s);
     return run<Own, F32Path<D, 8>, D>(p, ws, need, s);
 }
@@ -421,7 +429,7 @@ int run_d(const attn::prefix::Params &p, int kv_dtype, void *ws, size_t *need, c
     const long long rows = p.n_groups ? ((long long)p.n_seq * p.ratio + p.n_groups - 1) / p.n_groups : 0;
     if (kv_dtype == ATTN_BF16)
         return p.ratio <= 8 ? run_pre<Bf16Path<D, 1>, D>(p, ws, need, s, rows) : run_pre<Bf16Path<D, 2>, D>(p, ws, need, s, rows);
-    // INT8: two rows fill a tile of digits (8192 own rows of 8 x 128: 114 us a call, 117 in f16 parts; 32 x 32: 175 and 190)
+    // INT8: two rows fill a tile of digits (8192 own rows of 8 x 128: 110 us a call, 116 in f16 parts; 32 x 32: 173 and 188)
     if (kv_dtype == ATTN_I8)
         return p.ratio <= 2   ? run_pre<I8Digits<D>, D>(p, ws, need, s, rows)
                : p.ratio <= 4 ? run_pre<I8Path<D, 1>, D>(p, ws, need, s, rows)

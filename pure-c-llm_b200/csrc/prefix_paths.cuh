@@ -646,7 +646,7 @@ struct I8Path {
 // The weights of keys g and g + 8 share the 16-bit elements of the transposition,
 // so a lane's word of 4 keys is 2c, 2c + 8, 2c + 1, 2c + 9, and of V four words
 // (4 keys, 4 dims) turn into it with 8 byte permutations.
-// (64 requests with up to 8192 rows, 16 x 64: 117 us a call, 129 with two f16 parts
+// (64 requests with up to 8192 rows, 16 x 64: 117 us a call, 126 with two f16 parts
 // and converted codes; more query rows would need a second tile of digits.)
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {

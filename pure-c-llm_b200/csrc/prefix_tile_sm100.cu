@@ -4,8 +4,10 @@
 //
 // With r rows a prefix costs r flops per byte, so past about 250 rows the
 // tensor cores bound it and not HBM; mma.sync, at a quarter of their rate,
-// already from 64 (two 32768-row prefixes of 512 rows each, 8 x 128: 957 us on
-// mma.sync, 143 us here, merge included: 900 TFLOP/s).
+// already from 64 (two 32768-row prefixes of 512 rows each, 8 x 128, called with
+// one own row a request: 174 us, merge included: 742 TFLOP/s; 957 us on mma.sync
+// with probabilities in one part).  The times in brackets below were taken with
+// one part too, when the same call took 143 us.
 //
 // One CTA per SM walks its range of steps (prefix.cuh) of 128 keys.  A slot is
 // 256 query rows: with more than 128, warpgroup w takes rows [128 w, 128 w + 128)
@@ -18,8 +20,7 @@
 //               128-byte swizzled layout, with zeros for keys without a row, so
 //               that a probability of 0 never meets a NaN; they report such a
 //               half (K or V of a step) when their next one is on its way.
-//               (All steps by lanes: 299 us for the prefixes above, the copying
-//               instructions setting the pace.)
+//               (All steps by lanes: 299 us, the copying instructions setting the pace.)
 //   warp 2      S_wu = Q_w K_u^T for the two halves u of a step's keys, M = 128,
 //               N = 64, both operands in shared memory
 //   warp 3      O_w += P_wu V_u (P in two bf16 parts from TMEM, V as it lies, MN-major)
@@ -31,7 +32,7 @@
 //               output.
 // A probability goes in as two bf16 parts, its rounding and the rest, which leaves
 // no error but that of rounding the output (one part: 1.4 times it).  The second
-// product and its packing cost documents 297 -> 321 us and chat 54.5 -> 57.
+// product and its packing took that call from 143 to 174 us.
 // TMEM: four S of 64 columns, each overwritten by the two parts of its P, and two
 // O (512 columns at d 128).  S_w1 is formed while S_w0 is in the softmax, so a warpgroup does
 // not wait for its own products.  (With 128 keys in one S per warpgroup the
@@ -421,7 +422,7 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                                 tmem_st32(tO + c0, o);
                             }
                         }
-                        // the next half's S, looked for while P is on its way to TMEM (after it: 146.5 us for the prefixes above, and 143)
+                        // the next half's S, looked for while P is on its way to TMEM (P in one part: 143 us so, 146.5 after it)
                         ready = mbar_test_wait(BAR(B_SF + 2 * wg + 1 - u), (t + u) & 1);
                         tmem_wait_st();
                         tc_fence_before();
