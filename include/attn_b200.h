@@ -364,7 +364,8 @@ typedef struct {
     int page_size;              /* tokens per page: a power of two, <= 1024    */
     int max_pages;              /* block_table columns                         */
     int max_tokens;             /* rows of slot_map, positions and token_seq   */
-    int n_pages;                /* entries of free_pages                       */
+    int n_pages;                /* entries of free_pages: all pages there are
+                                   (what comes back past them is lost)         */
     int table_stride;           /* ints between block_table rows (0: max_pages) */
 } attn_page_shape;
 

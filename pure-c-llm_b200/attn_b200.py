@@ -228,6 +228,12 @@ def _dtype_code(t):
     raise TypeError(f"unsupported dtype {t.dtype}")
 
 
+def _device() -> int:
+    """Number of torch's current device."""
+    import torch
+    return torch._C._cuda_getDevice()
+
+
 def _stream():
     """Handle of torch's current stream on the current device."""
     import torch
@@ -345,17 +351,17 @@ class PageCache(PagedKV):
         kv = I8 if k.dtype == torch.int8 else _dtype_code(k)
         if v.dtype != k.dtype or v.shape != k.shape or v.stride() != k.stride() or k.dim() != 2 or k.stride(1) != 1:
             raise ValueError("k and v must have one type, shape and layout, with dense rows")
-        if not (k.is_cuda and v.is_cuda):
-            raise ValueError("k and v must be CUDA tensors")
+        if not k.is_cuda or v.device != k.device:
+            raise ValueError("k and v must be CUDA tensors of one device")
         if kv == I8:
             for x in (kscale, vscale):
                 if x is None or x.dim() != 2 or x.shape != (k.shape[0], kscale.shape[1]) or not x.is_contiguous():
                     raise ValueError("an int8 cache needs dense kscale and vscale of (rows, kv_heads)")
-                if x.dtype != torch.float32 or not x.is_cuda:
-                    raise TypeError("kscale and vscale must be fp32 CUDA tensors")
+                if x.dtype != torch.float32 or x.device != k.device:
+                    raise TypeError("kscale and vscale must be fp32 tensors of the cache's device")
         c = cls(kv, k.shape[0], k.stride(0), k.data_ptr(), v.data_ptr(), _ptr(kscale), _ptr(vscale))
         c.tensors = (k, v, kscale, vscale)
-        c.width, c.scale_heads = k.shape[1], kscale.shape[1] if kv == I8 else None
+        c.device, c.width, c.scale_heads = k.get_device(), k.shape[1], kscale.shape[1] if kv == I8 else None
         return c
 
 
@@ -364,18 +370,19 @@ def _ptr(t):
 
 
 # The shapes of these calls stand beside their tensors, so each tensor is looked at: what the library reads and writes
-# by a shape has to lie within it.  (In one pass over few attributes: it counts in calls of a few microseconds.)
-def _dense(*given):
-    """(name, tensor, dtype, elements): the tensor (None: not given) is a dense CUDA tensor of so many elements or more."""
+# by a shape has to lie within it, on the current device.  (In one pass over few attributes: it counts in calls of a
+# few microseconds.)
+def _dense(device, *given):
+    """(name, tensor, dtype, elements): the tensor (None: not given) is a dense one of so many elements or more."""
     for name, t, dtype, n in given:
-        if t is not None and (t.dtype is not dtype or not t.is_contiguous() or t.numel() < n or not t.is_cuda):
+        if t is not None and (t.dtype is not dtype or not t.is_contiguous() or t.numel() < n or t.get_device() != device):
             if t.dtype is not dtype:
                 raise TypeError(f"{name} is {t.dtype}, not {dtype}")
-            raise ValueError(f"{name}, {tuple(t.shape)} of strides {t.stride()} on {t.device}, is not {n} dense elements on a GPU")
+            raise ValueError(f"{name}, {tuple(t.shape)} of strides {t.stride()} on {t.device}, is not {n} dense elements on device {device}")
 
 
-def _rows(dtype, name, t, rows, width, stride):
-    """t (None: not given) is a CUDA tensor of dtype with `rows` rows of `width` elements, `stride` apart (0: width), as
+def _rows(device, dtype, name, t, rows, width, stride):
+    """t (None: not given) is a tensor of dtype with `rows` rows of `width` elements, `stride` apart (0: width), as
     (rows, width) or, where it is dense, in any shape whose last dimension lies within a row."""
     if t is None:
         return
@@ -385,13 +392,16 @@ def _rows(dtype, name, t, rows, width, stride):
     fits = len(shape) == 2 and shape[0] >= rows and shape[1] >= width and steps[1] == 1 and (steps[0] == stride or rows == 1) or \
         rows <= 0 or width <= 0 or \
         stride == width and t.is_contiguous() and t.numel() >= rows * width and shape[-1] <= width
-    if not (fits and t.is_cuda):
-        raise ValueError(f"{name}, {tuple(shape)} of strides {steps} on {t.device}, is not {rows} rows of {width}, {stride} apart, on a GPU")
+    if not fits or t.get_device() != device:
+        raise ValueError(f"{name}, {tuple(shape)} of strides {steps} on {t.device}, is not {rows} rows of {width}, {stride} apart, "
+                         f"on device {device}")
 
 
-def _cache_holds(cache, kv_heads, head_dim):
+def _cache_holds(device, cache, kv_heads, head_dim):
     """The tensors of a PageCache hold rows of these heads (a PagedKV of bare addresses cannot be looked at)."""
     if isinstance(cache, PageCache):
+        if cache.device != device:
+            raise ValueError(f"the cache is on device {cache.device}, not {device}")
         if cache.width < kv_heads * head_dim:
             raise ValueError(f"cache rows of {cache.width} elements hold no {kv_heads} heads of {head_dim}")
         if cache.scale_heads not in (None, kv_heads):
@@ -413,12 +423,12 @@ def page_plan_t(shape: PageShape, lens, new_lens, free_pages, free_count, block_
     entries of block_table and the returned pages in free_pages; out["lens"] and out["counts"][:1] are the next step's
     lens and free_count."""
     import torch
-    n, rows, i32 = shape.n_seq, shape.max_tokens, torch.int32
-    _dense(("lens", lens, i32, n), ("new_lens", new_lens, i32, n), ("pos_base", pos_base, i32, n), ("free_pages", free_pages, i32, shape.n_pages),
+    on, n, rows, i32 = _device(), shape.n_seq, shape.max_tokens, torch.int32
+    _dense(on, ("lens", lens, i32, n), ("new_lens", new_lens, i32, n), ("pos_base", pos_base, i32, n), ("free_pages", free_pages, i32, shape.n_pages),
            ("free_count", free_count, i32, 1), ("out['lens']", out["lens"], i32, n), ("out['cu_new']", out["cu_new"], i32, n + 1),
            ("out['slot_map']", out["slot_map"], torch.int64, rows), ("out['positions']", out["positions"], i32, rows),
            ("out['token_seq']", out.get("token_seq"), i32, rows), ("out['counts']", out["counts"], i32, 4))
-    _rows(i32, "block_table", block_table, n, shape.max_pages, shape.table_stride)
+    _rows(on, i32, "block_table", block_table, n, shape.max_pages, shape.table_stride)
     check(lib.attn_page_plan_ex(shape, lens.data_ptr(), new_lens.data_ptr(), _ptr(pos_base), free_pages.data_ptr(),
                                 free_count.data_ptr(), block_table.data_ptr(), out["lens"].data_ptr(),
                                 out["cu_new"].data_ptr(), out["slot_map"].data_ptr(), out["positions"].data_ptr(),
@@ -437,12 +447,12 @@ def rope_table_t(config: RopeConfig, device="cuda"):
 def rope_t(shape: RopeShape, table, positions, q, k, q_out, k_out, transpose=False):
     """attn_rope_ex on (tokens, heads * d) fp32 or bf16 tensors; positions int32 or None; k and k_out may be None."""
     import torch
-    n, d, dtype = shape.tokens, shape.head_dim, q.dtype
-    _dense(("table", table, torch.float32, shape.max_pos * shape.rot_dim), ("positions", positions, torch.int32, n))
-    _rows(dtype, "q", q, n, shape.heads * d, shape.q_row_stride)
-    _rows(dtype, "k", k, n, shape.kv_heads * d, shape.k_row_stride)
-    _rows(dtype, "q_out", q_out, n, shape.heads * d, shape.q_out_row_stride)
-    _rows(dtype, "k_out", k_out, n, shape.kv_heads * d, shape.k_out_row_stride)
+    on, n, d, dtype = _device(), shape.tokens, shape.head_dim, q.dtype
+    _dense(on, ("table", table, torch.float32, shape.max_pos * shape.rot_dim), ("positions", positions, torch.int32, n))
+    _rows(on, dtype, "q", q, n, shape.heads * d, shape.q_row_stride)
+    _rows(on, dtype, "k", k, n, shape.kv_heads * d, shape.k_row_stride)
+    _rows(on, dtype, "q_out", q_out, n, shape.heads * d, shape.q_out_row_stride)
+    _rows(on, dtype, "k_out", k_out, n, shape.kv_heads * d, shape.k_out_row_stride)
     check(lib.attn_rope_ex(shape, _dtype_code(q), _ptr(table), _ptr(positions), q.data_ptr(), _ptr(k),
                            q_out.data_ptr(), _ptr(k_out), int(transpose), _stream()))
     return q_out, k_out
@@ -451,14 +461,14 @@ def rope_t(shape: RopeShape, table, positions, q, k, q_out, k_out, transpose=Fal
 def rope_append_t(shape: RopeShape, cache: PagedKV, table, positions, slot_map, q, k, v, q_out):
     """attn_rope_append_ex: positions int32 or None, slot_map int64."""
     import torch
-    n, d, heads, dtype = shape.tokens, shape.head_dim, shape.kv_heads, q.dtype
-    _dense(("table", table, torch.float32, shape.max_pos * shape.rot_dim), ("positions", positions, torch.int32, n),
+    on, n, d, heads, dtype = _device(), shape.tokens, shape.head_dim, shape.kv_heads, q.dtype
+    _dense(on, ("table", table, torch.float32, shape.max_pos * shape.rot_dim), ("positions", positions, torch.int32, n),
            ("slot_map", slot_map, torch.int64, n))
-    _rows(dtype, "q", q, n, shape.heads * d, shape.q_row_stride)
-    _rows(dtype, "k", k, n, heads * d, shape.k_row_stride)
-    _rows(dtype, "v", v, n, heads * d, shape.v_row_stride)
-    _rows(dtype, "q_out", q_out, n, shape.heads * d, shape.q_out_row_stride)
-    _cache_holds(cache, heads, d)
+    _rows(on, dtype, "q", q, n, shape.heads * d, shape.q_row_stride)
+    _rows(on, dtype, "k", k, n, heads * d, shape.k_row_stride)
+    _rows(on, dtype, "v", v, n, heads * d, shape.v_row_stride)
+    _rows(on, dtype, "q_out", q_out, n, shape.heads * d, shape.q_out_row_stride)
+    _cache_holds(on, cache, heads, d)
     check(lib.attn_rope_append_ex(shape, cache, _dtype_code(q), _ptr(table), _ptr(positions), slot_map.data_ptr(),
                                   q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), _stream()))
     return q_out
@@ -473,17 +483,17 @@ def prefix_decode_t(shape: PrefixShape, cache: PagedKV, q, group_begin, prefix_t
     """attn_prefix_decode_ex: q and out (n_seq, heads * d); tables and lengths int32; group_begin, prefix_table and
     prefix_lens may be None when shape.n_groups is 0."""
     import torch
-    n, groups, heads, d, i32 = shape.n_seq, shape.n_groups, shape.heads, shape.head_dim, torch.int32
+    on, n, groups, heads, d, i32 = _device(), shape.n_seq, shape.n_groups, shape.heads, shape.head_dim, torch.int32
     dtype = torch.bfloat16 if shape.dtype == BF16 else torch.float32
-    _dense(("lens", lens, i32, n), ("lse", lse, torch.float32, n * heads),
+    _dense(on, ("lens", lens, i32, n), ("lse", lse, torch.float32, n * heads),
            ("workspace", workspace, workspace.dtype if workspace is not None else None, 0))
     if groups > 0:
-        _dense(("group_begin", group_begin, i32, groups + 1), ("prefix_lens", prefix_lens, i32, groups))
-        _rows(i32, "prefix_table", prefix_table, groups, shape.max_prefix_pages, 0)
-    _rows(i32, "block_table", block_table, n, shape.max_pages, 0)
-    _rows(dtype, "q", q, n, heads * d, shape.q_row_stride)
-    _rows(dtype, "out", out, n, heads * d, shape.out_row_stride)
-    _cache_holds(cache, shape.kv_heads, d)
+        _dense(on, ("group_begin", group_begin, i32, groups + 1), ("prefix_lens", prefix_lens, i32, groups))
+        _rows(on, i32, "prefix_table", prefix_table, groups, shape.max_prefix_pages, 0)
+    _rows(on, i32, "block_table", block_table, n, shape.max_pages, 0)
+    _rows(on, dtype, "q", q, n, heads * d, shape.q_row_stride)
+    _rows(on, dtype, "out", out, n, heads * d, shape.out_row_stride)
+    _cache_holds(on, cache, shape.kv_heads, d)
     check(lib.attn_prefix_decode_ex(shape, cache, q.data_ptr(), _ptr(group_begin), _ptr(prefix_table),
                                     _ptr(prefix_lens), block_table.data_ptr(), lens.data_ptr(), out.data_ptr(),
                                     _ptr(lse), _ptr(workspace),

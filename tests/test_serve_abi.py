@@ -124,9 +124,9 @@ def test_prefix_decode_refusals():
 class Given:
     """A stand-in for a CUDA tensor: what the checks look at, at an address that is never read."""
 
-    def __init__(self, tensor, is_cuda=True):
-        self.t, self.is_cuda, self.device = tensor, is_cuda, "cuda:0" if is_cuda else "cpu"
-        self.dtype, self.shape = tensor.dtype, tensor.shape
+    def __init__(self, tensor, device=0):
+        self.t, self.is_cuda, self.device = tensor, device >= 0, f"cuda:{device}" if device >= 0 else "cpu"
+        self.dtype, self.shape, self.get_device = tensor.dtype, tensor.shape, lambda: device
 
     def __getattr__(self, name):
         return getattr(self.t, name)
@@ -147,6 +147,7 @@ def calls(monkeypatch):
             return stop
     monkeypatch.setattr(A, "lib", Lib())
     monkeypatch.setattr(A, "_stream", lambda: 0)
+    monkeypatch.setattr(A, "_device", lambda: 0)
 
 
 def refused(call, given, bad, error):
@@ -156,7 +157,7 @@ def refused(call, given, bad, error):
 
 
 def each_refused(call, given, optional=()):
-    """Every tensor on its own: of another type, too short, on the host."""
+    """Every tensor on its own: of another type, too short, on the host, on another GPU."""
     import torch
     with pytest.raises(Reached):
         call(**given)
@@ -164,7 +165,8 @@ def each_refused(call, given, optional=()):
         other = torch.int64 if g.dtype == torch.int32 else torch.int32 if g.dtype == torch.int64 else torch.float64
         if name != "q" and name != "workspace":
             refused(call, given, {name: Given(g.t.to(other))}, TypeError)
-        refused(call, given, {name: Given(g.t, is_cuda=False)}, ValueError)
+        for device in (-1, 1):
+            refused(call, given, {name: Given(g.t, device)}, ValueError)
         if name != "workspace":
             refused(call, given, {name: Given(g.t[:-1])}, ValueError)
             if g.numel() > 1:
@@ -238,7 +240,8 @@ def test_rope_append_tensors(calls):
     narrow = A.PageCache.of(*(Given(torch.zeros((32, 96))[:, :32]) for _ in range(2)))
     codes = [ints(32, 64, dtype=torch.int8) for _ in range(2)]
     other = A.PageCache.of(*codes, *(Given(torch.zeros(32, 4)) for _ in range(2)))
-    for kv, word in ((narrow, "rows of 32"), (other, "scales of 4")):
+    away = A.PageCache.of(*(Given(torch.zeros(32, 64), 1) for _ in range(2)))
+    for kv, word in ((narrow, "rows of 32"), (other, "scales of 4"), (away, "device 1")):
         with pytest.raises(ValueError, match=word):
             call(kv=kv, **given)
 
@@ -249,11 +252,11 @@ def test_page_cache_tensors():
     k, scale, codes = ints(8, 64, **f), ints(8, 2, **f), ints(8, 64, dtype=torch.int8)
     A.PageCache.of(k, k)
     A.PageCache.of(codes, codes, scale, scale)
-    for bad in ((k, ints(8, 64, dtype=torch.bfloat16)), (k, ints(7, 64, **f)), (k, Given(k.t, is_cuda=False)), (ints(512, **f),) * 2,
+    for bad in ((k, ints(8, 64, dtype=torch.bfloat16)), (k, ints(7, 64, **f)), (k, Given(k.t, -1)), (k, Given(k.t, 1)), (ints(512, **f),) * 2,
                 (codes, codes), (codes, codes, scale, None), (codes, codes, scale, ints(7, 2, **f)), (codes, codes, scale, ints(8, 3, **f))):
         with pytest.raises(ValueError):
             A.PageCache.of(*bad)
-    for bad in ((codes, codes, scale, ints(8, 2, dtype=torch.float64)), (ints(8, 64, dtype=torch.float64),) * 2):
+    for bad in ((codes, codes, scale, ints(8, 2, dtype=torch.float64)), (codes, codes, scale, Given(scale.t, 1)), (ints(8, 64, dtype=torch.float64),) * 2):
         with pytest.raises(TypeError):
             A.PageCache.of(*bad)
 
