@@ -18,7 +18,7 @@ int launch_rope_append(const attn_rope_shape *s, const attn_paged_kv *c, int dty
                        void *q_out, int *err, cudaStream_t stream);
 size_t prefix_decode_workspace(const attn_prefix_shape *s, int kv_dtype);
 int launch_prefix_decode(const attn::prefix::Params &p, int d, int kv_dtype, void *ws, cudaStream_t s);
-void *library_workspace(int which, size_t bytes, cudaStream_t s);
+void *library_workspace(int which, size_t bytes, cudaStream_t s);      // slot 4: the prefix decode's pieces
 int *device_error_ptr();
 
 static bool aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
