@@ -469,6 +469,44 @@ ATTN_API int attn_rope_append_ex(const attn_rope_shape *s, const attn_paged_kv *
                 const float *table, const int *positions, const long long *slot_map,
                 const void *q, const void *k, const void *v, void *q_out, attn_stream_t stream);
 
+/* Root-mean-square norm of each head of Q and K, as models with normed queries
+ * and keys have it before the rotation: x becomes x * w / sqrt(mean(x^2) + eps)
+ * over the head_dim elements of a head.  (Weights kept as an offset from 1 are
+ * passed with the 1 added.) */
+typedef struct {
+    const float *q_weight, *k_weight;   /* DEVICE, head_dim floats each, shared
+                                           by the heads (NULL: ones)           */
+    float eps;                          /* >= 0                                */
+} attn_head_norm;
+
+/* attn_rope_ex of the normed heads, in one pass: q_out, k_out = the heads of q,
+ * k normed, weighted and turned, fp32 arithmetic, rounded once.  rot_dim 0
+ * norms alone.  q may be q_out and k may be k_out; k and k_out may be NULL. */
+ATTN_API int attn_norm_rope_ex(const attn_rope_shape *s, const attn_head_norm *n, int dtype, const float *table,
+                const int *positions, const void *q, const void *k, void *q_out, void *k_out,
+                attn_stream_t stream);
+
+/* Its gradients, from the forward's inputs q, k and the gradients dq_out,
+ * dk_out of its outputs: dq, dk (SET; their rows lie as those of q and k, the
+ * others as those of q_out and k_out) and, where wanted, the weights' gradients
+ * dq_weight, dk_weight (head_dim floats, summed over tokens and heads; NULL:
+ * not wanted; accumulate = 1 adds to them, 0 sets them).  dq may be dq_out or q
+ * where the row strides of the two are the same, dk likewise; k, dk_out and dk
+ * may all be NULL (a dk_weight is then as over no tokens).  The same result on
+ * every run.  `workspace` (256-byte aligned) is needed when a weight's gradient
+ * is wanted, and only then. */
+ATTN_API size_t attn_norm_rope_bwd_workspace_bytes(const attn_rope_shape *s);
+ATTN_API int attn_norm_rope_bwd_ex(const attn_rope_shape *s, const attn_head_norm *n, int dtype, const float *table,
+                const int *positions, const void *q, const void *k, const void *dq_out, const void *dk_out,
+                void *dq, void *dk, float *dq_weight, float *dk_weight, int accumulate,
+                void *workspace, size_t workspace_bytes, attn_stream_t stream);
+
+/* attn_rope_append_ex of the normed heads: q normed and turned into q_out, k
+ * normed and turned and v as it is written to the cache. */
+ATTN_API int attn_norm_rope_append_ex(const attn_rope_shape *s, const attn_head_norm *n, const attn_paged_kv *cache,
+                int dtype, const float *table, const int *positions, const long long *slot_map,
+                const void *q, const void *k, const void *v, void *q_out, attn_stream_t stream);
+
 typedef struct {
     int n_seq;                  /* requests, one query token each, <= 65535    */
     int n_groups;               /* groups that share a prefix (0: none)        */

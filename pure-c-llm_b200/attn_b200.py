@@ -82,6 +82,10 @@ class RopeShape(ctypes.Structure):
                 ("k_out_row_stride", ctypes.c_longlong)]
 
 
+class HeadNormPtrs(ctypes.Structure):
+    _fields_ = [("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("eps", ctypes.c_float)]
+
+
 class PrefixShape(ctypes.Structure):
     _fields_ = [("n_seq", ctypes.c_int), ("n_groups", ctypes.c_int), ("heads", ctypes.c_int),
                 ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("dtype", ctypes.c_int),
@@ -130,6 +134,10 @@ SIGNATURES = {
     "attn_rope_table_ex": (I, [ctypes.POINTER(RopeConfig), P, P]),
     "attn_rope_ex": (I, [ctypes.POINTER(RopeShape), I, P, P, P, P, P, P, I, P]),
     "attn_rope_append_ex": (I, [ctypes.POINTER(RopeShape), ctypes.POINTER(PagedKV), I, P, P, P, P, P, P, P, P]),
+    "attn_norm_rope_ex": (I, [ctypes.POINTER(RopeShape), ctypes.POINTER(HeadNormPtrs), I, P, P, P, P, P, P, P]),
+    "attn_norm_rope_bwd_workspace_bytes": (SZ, [ctypes.POINTER(RopeShape)]),
+    "attn_norm_rope_bwd_ex": (I, [ctypes.POINTER(RopeShape), ctypes.POINTER(HeadNormPtrs), I] + [P] * 10 + [I, P, SZ, P]),
+    "attn_norm_rope_append_ex": (I, [ctypes.POINTER(RopeShape), ctypes.POINTER(HeadNormPtrs), ctypes.POINTER(PagedKV), I] + [P] * 8),
     "attn_prefix_decode_workspace_bytes": (SZ, [ctypes.POINTER(PrefixShape), ctypes.POINTER(PagedKV)]),
     "attn_prefix_decode_ex": (I, [ctypes.POINTER(PrefixShape), ctypes.POINTER(PagedKV), P, P, P, P, P, P, P, P, P, SZ, P]),
     "attn_shard_range": (I, [LL, I, I, ctypes.POINTER(LL), ctypes.POINTER(LL)]),
@@ -471,6 +479,83 @@ def rope_append_t(shape: RopeShape, cache: PagedKV, table, positions, slot_map, 
     _cache_holds(on, cache, heads, d)
     check(lib.attn_rope_append_ex(shape, cache, _dtype_code(q), _ptr(table), _ptr(positions), slot_map.data_ptr(),
                                   q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), _stream()))
+    return q_out
+
+
+class HeadNorm(HeadNormPtrs):
+    """Norm of each head of Q and K (attn_head_norm) over weight tensors, which it keeps alive: head_dim fp32 each, or
+    None for ones."""
+
+    @classmethod
+    def of(cls, q_weight=None, k_weight=None, eps=1e-6):
+        n = cls(_ptr(q_weight), _ptr(k_weight), eps)
+        n.tensors = (q_weight, k_weight)
+        return n
+
+
+def _norm_holds(device, norm, head_dim):
+    """The weights of a HeadNorm have a head's elements (those of bare addresses cannot be looked at)."""
+    import torch
+    if isinstance(norm, HeadNorm):
+        _dense(device, ("q_weight", norm.tensors[0], torch.float32, head_dim), ("k_weight", norm.tensors[1], torch.float32, head_dim))
+
+
+def norm_rope_t(shape: RopeShape, norm: HeadNormPtrs, table, positions, q, k, q_out, k_out):
+    """attn_norm_rope_ex on (tokens, heads * d) fp32 or bf16 tensors; positions int32 or None; k and k_out may be None."""
+    import torch
+    on, n, d, dtype = _device(), shape.tokens, shape.head_dim, q.dtype
+    _dense(on, ("table", table, torch.float32, shape.max_pos * shape.rot_dim), ("positions", positions, torch.int32, n))
+    _norm_holds(on, norm, d)
+    _rows(on, dtype, "q", q, n, shape.heads * d, shape.q_row_stride)
+    _rows(on, dtype, "k", k, n, shape.kv_heads * d, shape.k_row_stride)
+    _rows(on, dtype, "q_out", q_out, n, shape.heads * d, shape.q_out_row_stride)
+    _rows(on, dtype, "k_out", k_out, n, shape.kv_heads * d, shape.k_out_row_stride)
+    check(lib.attn_norm_rope_ex(shape, norm, _dtype_code(q), _ptr(table), _ptr(positions), q.data_ptr(), _ptr(k),
+                                q_out.data_ptr(), _ptr(k_out), _stream()))
+    return q_out, k_out
+
+
+def norm_rope_bwd_workspace_bytes(shape: RopeShape) -> int:
+    return lib.attn_norm_rope_bwd_workspace_bytes(shape)
+
+
+def norm_rope_bwd_t(shape: RopeShape, norm: HeadNormPtrs, table, positions, q, k, dq_out, dk_out, dq, dk, dq_weight=None,
+                    dk_weight=None, accumulate=False, workspace=None):
+    """attn_norm_rope_bwd_ex: dq and dk lie as q and k, dq_out and dk_out as the forward's outputs.  With weight
+    gradients and no workspace, one is allocated."""
+    import torch
+    on, n, d, dtype = _device(), shape.tokens, shape.head_dim, q.dtype
+    _dense(on, ("table", table, torch.float32, shape.max_pos * shape.rot_dim), ("positions", positions, torch.int32, n),
+           ("dq_weight", dq_weight, torch.float32, d), ("dk_weight", dk_weight, torch.float32, d),
+           ("workspace", workspace, workspace.dtype if workspace is not None else None, 0))
+    _norm_holds(on, norm, d)
+    for name, t, heads, stride in (("q", q, shape.heads, shape.q_row_stride), ("k", k, shape.kv_heads, shape.k_row_stride),
+                                   ("dq_out", dq_out, shape.heads, shape.q_out_row_stride), ("dk_out", dk_out, shape.kv_heads, shape.k_out_row_stride),
+                                   ("dq", dq, shape.heads, shape.q_row_stride), ("dk", dk, shape.kv_heads, shape.k_row_stride)):
+        _rows(on, dtype, name, t, n, heads * d, stride)
+    if workspace is None and (dq_weight is not None or dk_weight is not None):
+        workspace = torch.empty(norm_rope_bwd_workspace_bytes(shape), dtype=torch.uint8, device=q.device)
+    check(lib.attn_norm_rope_bwd_ex(shape, norm, _dtype_code(q), _ptr(table), _ptr(positions), q.data_ptr(), _ptr(k),
+                                    dq_out.data_ptr(), _ptr(dk_out), dq.data_ptr(), _ptr(dk), _ptr(dq_weight), _ptr(dk_weight),
+                                    int(accumulate), _ptr(workspace),
+                                    workspace.numel() * workspace.element_size() if workspace is not None else 0, _stream()))
+    return dq, dk, dq_weight, dk_weight
+
+
+def norm_rope_append_t(shape: RopeShape, norm: HeadNormPtrs, cache: PagedKV, table, positions, slot_map, q, k, v, q_out):
+    """attn_norm_rope_append_ex: positions int32 or None, slot_map int64."""
+    import torch
+    on, n, d, heads, dtype = _device(), shape.tokens, shape.head_dim, shape.kv_heads, q.dtype
+    _dense(on, ("table", table, torch.float32, shape.max_pos * shape.rot_dim), ("positions", positions, torch.int32, n),
+           ("slot_map", slot_map, torch.int64, n))
+    _norm_holds(on, norm, d)
+    _rows(on, dtype, "q", q, n, shape.heads * d, shape.q_row_stride)
+    _rows(on, dtype, "k", k, n, heads * d, shape.k_row_stride)
+    _rows(on, dtype, "v", v, n, heads * d, shape.v_row_stride)
+    _rows(on, dtype, "q_out", q_out, n, shape.heads * d, shape.q_out_row_stride)
+    _cache_holds(on, cache, heads, d)
+    check(lib.attn_norm_rope_append_ex(shape, norm, cache, _dtype_code(q), _ptr(table), _ptr(positions), slot_map.data_ptr(),
+                                       q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), _stream()))
     return q_out
 
 

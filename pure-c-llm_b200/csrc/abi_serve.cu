@@ -5,6 +5,7 @@
 
 #include "common.cuh"
 #include "prefix.cuh"
+#include "serve_checks.cuh"
 
 namespace attn_host {
 int launch_page_plan(const attn_page_shape *s, const int *lens, const int *new_lens, const int *pos_base,
@@ -16,38 +17,19 @@ int launch_rope(const attn_rope_shape *s, int dtype, const float *table, const i
 int launch_rope_append(const attn_rope_shape *s, const attn_paged_kv *c, int dtype, const float *table,
                        const int *positions, const long long *slots, const void *q, const void *k, const void *v,
                        void *q_out, int *err, cudaStream_t stream);
+int launch_norm_rope(const attn_rope_shape *s, const attn_head_norm *n, int dtype, const float *table, const int *positions, const void *q,
+                     const void *k, void *q_out, void *k_out, int *err, cudaStream_t stream);
+size_t norm_rope_bwd_workspace(const attn_rope_shape *s);
+int launch_norm_rope_bwd(const attn_rope_shape *s, const attn_head_norm *n, int dtype, const float *table, const int *positions, const void *q,
+                         const void *k, const void *dq_out, const void *dk_out, void *dq, void *dk, float *dq_weight, float *dk_weight,
+                         int accumulate, void *ws, int *err, cudaStream_t stream);
+int launch_norm_rope_append(const attn_rope_shape *s, const attn_head_norm *n, const attn_paged_kv *c, int dtype, const float *table,
+                            const int *positions, const long long *slots, const void *q, const void *k, const void *v, void *q_out, int *err,
+                            cudaStream_t stream);
 size_t prefix_decode_workspace(const attn_prefix_shape *s, int kv_dtype);
 int launch_prefix_decode(const attn::prefix::Params &p, int d, int kv_dtype, void *ws, cudaStream_t s);
 void *library_workspace(int which, size_t bytes, cudaStream_t s);      // slot 4: the prefix decode's pieces
 int *device_error_ptr();
-
-static bool aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
-static bool head_dim_ok(int d) { return d == 32 || d == 64 || d == 96 || d == 128; }
-static bool page_size_ok(int n) { return n >= 1 && n <= 1024 && (n & (n - 1)) == 0; }
-static bool overlap(const void *a, size_t na, const void *b, size_t nb) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return x < y + nb && y < x + na;
-}
-
-// Checks of a paged cache for kv_heads heads of d; the row stride in elements.
-static int check_cache(const attn_paged_kv *c, int kv_heads, int d, long long *row_stride, const char *who) {
-    if (!c) return set_error(ATTN_ERR_INVALID, "%s: cache is NULL", who);
-    if (c->kv_dtype != ATTN_F32 && c->kv_dtype != ATTN_BF16 && c->kv_dtype != ATTN_I8)
-        return set_error(ATTN_ERR_UNSUPPORTED, "%s: kv_dtype %d not supported", who, c->kv_dtype);
-    const long long hd = (long long)kv_heads * d;
-    const int unit = c->kv_dtype == ATTN_F32 ? 4 : c->kv_dtype == ATTN_BF16 ? 8 : 16;
-    *row_stride = c->row_stride ? c->row_stride : hd;
-    if (*row_stride < hd || *row_stride % unit)
-        return set_error(ATTN_ERR_INVALID, "%s: cache row_stride %lld must be >= kv_heads*d=%lld and a multiple of %d",
-                         who, *row_stride, hd, unit);
-    if (c->rows < 0) return set_error(ATTN_ERR_INVALID, "%s: cache of %lld rows", who, c->rows);
-    if (!c->k || !c->v || !aligned(c->k, 16) || !aligned(c->v, 16))
-        return set_error(ATTN_ERR_INVALID, "%s: cache k and v must be 16-byte aligned and not NULL", who);
-    if (c->kv_dtype == ATTN_I8 && (!c->kscale || !c->vscale || !aligned(c->kscale, 4) || !aligned(c->vscale, 4)))
-        return set_error(ATTN_ERR_INVALID, "%s: an INT8 cache needs kscale and vscale", who);
-    return ATTN_OK;
-}
-
 }  // namespace attn_host
 
 using namespace attn_host;
@@ -169,6 +151,95 @@ int attn_rope_append_ex(const attn_rope_shape *s, const attn_paged_kv *cache, in
     if (!err) return set_error(ATTN_ERR_CUDA, "rope append: no device error word");
     return launch_rope_append(s, cache, dtype, table, positions, slot_map, q, k, v, q_out, err,
                               reinterpret_cast<cudaStream_t>(stream));
+}
+
+// ---------------------------------------------------------------------------
+// normed heads, turned
+// ---------------------------------------------------------------------------
+static int check_norm(const attn_head_norm *n) {
+    if (!n) return set_error(ATTN_ERR_INVALID, "norm rope: norm is NULL");
+    if (!(n->eps >= 0.f) || n->eps > 1e30f) return set_error(ATTN_ERR_INVALID, "norm rope: eps %g", (double)n->eps);
+    if (!aligned(n->q_weight, 4) || !aligned(n->k_weight, 4)) return set_error(ATTN_ERR_INVALID, "norm rope: misaligned weights");
+    return ATTN_OK;
+}
+
+// Row strides of q and k, and of their outputs (or gradients): the same where two tensors are one.
+static bool strides_differ(const attn_rope_shape *s, bool of_q) {
+    const long long w = (long long)(of_q ? s->heads : s->kv_heads) * s->head_dim;
+    const long long in = of_q ? s->q_row_stride : s->k_row_stride, out = of_q ? s->q_out_row_stride : s->k_out_row_stride;
+    return (in ? in : w) != (out ? out : w);
+}
+
+int attn_norm_rope_ex(const attn_rope_shape *s, const attn_head_norm *n, int dtype, const float *table, const int *positions,
+                      const void *q, const void *k, void *q_out, void *k_out, attn_stream_t stream) {
+    int st = check_rope(s, dtype, table, positions);
+    if (st || (st = check_norm(n))) return st;
+    if (s->tokens == 0) return ATTN_OK;
+    const size_t e = dtype == ATTN_F32 ? 4 : 2;
+    if (!q || !q_out || !k != !k_out) return set_error(ATTN_ERR_INVALID, "norm rope: NULL tensor pointer");
+    if (!aligned(q, e) || !aligned(k, e) || !aligned(q_out, e) || !aligned(k_out, e))
+        return set_error(ATTN_ERR_INVALID, "norm rope: tensors must be %zu-byte aligned", e);
+    if ((q == q_out && strides_differ(s, true)) || (k && k == k_out && strides_differ(s, false)))
+        return set_error(ATTN_ERR_INVALID, "norm rope: in place, the strides of input and output must be the same");
+    int *err = device_error_ptr();
+    if (!err) return set_error(ATTN_ERR_CUDA, "norm rope: no device error word");
+    return launch_norm_rope(s, n, dtype, table, positions, q, k, q_out, k_out, err, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t attn_norm_rope_bwd_workspace_bytes(const attn_rope_shape *s) {
+    if (!s || s->tokens < 0 || s->tokens > (1 << 30) || s->heads < 1 || s->heads > 65535 || s->kv_heads < 1 || s->kv_heads > 65535 ||
+        !head_dim_ok(s->head_dim))
+        return 0;
+    return norm_rope_bwd_workspace(s);
+}
+
+int attn_norm_rope_bwd_ex(const attn_rope_shape *s, const attn_head_norm *n, int dtype, const float *table, const int *positions,
+                          const void *q, const void *k, const void *dq_out, const void *dk_out, void *dq, void *dk, float *dq_weight,
+                          float *dk_weight, int accumulate, void *workspace, size_t workspace_bytes, attn_stream_t stream) {
+    int st = check_rope(s, dtype, table, positions);
+    if (st || (st = check_norm(n))) return st;
+    const size_t e = dtype == ATTN_F32 ? 4 : 2;
+    if (s->tokens && (!q || !dq_out || !dq || !k != !dk_out || !k != !dk))
+        return set_error(ATTN_ERR_INVALID, "norm rope backward: NULL tensor pointer");
+    const void *const tensors[] = {q, k, dq_out, dk_out, dq, dk};
+    for (const void *t : tensors)
+        if (!aligned(t, e)) return set_error(ATTN_ERR_INVALID, "norm rope backward: tensors must be %zu-byte aligned", e);
+    if (!aligned(dq_weight, 4) || !aligned(dk_weight, 4))
+        return set_error(ATTN_ERR_INVALID, "norm rope backward: misaligned weight gradients");
+    if ((dq && dq == dq_out && strides_differ(s, true)) || (dk && dk == dk_out && strides_differ(s, false)))
+        return set_error(ATTN_ERR_INVALID, "norm rope backward: in place, the strides of input and output must be the same");
+    if (dq_weight || dk_weight) {
+        const size_t need = norm_rope_bwd_workspace(s);
+        if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
+            return set_error(ATTN_ERR_WORKSPACE, "norm rope backward: weight gradients need a workspace of %zu bytes (256-byte aligned), got %zu",
+                             need, workspace ? workspace_bytes : 0);
+    }
+    int *err = device_error_ptr();
+    if (!err) return set_error(ATTN_ERR_CUDA, "norm rope backward: no device error word");
+    return launch_norm_rope_bwd(s, n, dtype, table, positions, q, k, dq_out, dk_out, dq, dk, dq_weight, dk_weight, accumulate ? 1 : 0,
+                                workspace, err, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int attn_norm_rope_append_ex(const attn_rope_shape *s, const attn_head_norm *n, const attn_paged_kv *cache, int dtype, const float *table,
+                             const int *positions, const long long *slot_map, const void *q, const void *k, const void *v, void *q_out,
+                             attn_stream_t stream) {
+    int st = check_rope(s, dtype, table, positions);
+    if (st || (st = check_norm(n))) return st;
+    long long rs;
+    if ((st = check_cache(cache, s->kv_heads, s->head_dim, &rs, "norm rope append"))) return st;
+    if ((dtype == ATTN_BF16) != (cache->kv_dtype == ATTN_BF16))
+        return set_error(ATTN_ERR_UNSUPPORTED, "norm rope append: dtype %d into a cache of dtype %d", dtype, cache->kv_dtype);
+    if (s->tokens == 0) return ATTN_OK;
+    const size_t e = dtype == ATTN_F32 ? 4 : 2;
+    if (!q || !k || !v || !q_out || !slot_map) return set_error(ATTN_ERR_INVALID, "norm rope append: NULL pointer");
+    if (!aligned(q, e) || !aligned(k, e) || !aligned(v, e) || !aligned(q_out, e) || !aligned(slot_map, 8))
+        return set_error(ATTN_ERR_INVALID, "norm rope append: tensors must be %zu-byte aligned, slot_map 8-byte", e);
+    if (q == q_out && strides_differ(s, true))
+        return set_error(ATTN_ERR_INVALID, "norm rope append: in place, the strides of q and q_out must be the same");
+    int *err = device_error_ptr();
+    if (!err) return set_error(ATTN_ERR_CUDA, "norm rope append: no device error word");
+    return launch_norm_rope_append(s, n, cache, dtype, table, positions, slot_map, q, k, v, q_out, err,
+                                   reinterpret_cast<cudaStream_t>(stream));
 }
 
 // ---------------------------------------------------------------------------
