@@ -556,6 +556,101 @@ ATTN_API int attn_prefix_decode_ex(const attn_prefix_shape *s, const attn_paged_
                 float *lse, void *workspace, size_t workspace_bytes, attn_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Drafted token trees over a paged cache (speculative decoding): a step checks
+ * several drafted tokens of a request at once, of which one path is kept.
+ * Draft 0 of a request is its last sampled token (or any first row), and each
+ * other one descends from an earlier one, so a path's indexes ascend.  A step:
+ *   attn_page_plan_ex       new_lens = the drafts: their cache rows
+ *   attn_tree_plan_ex       positions by depth, and who sees whom
+ *   per layer: project, attn_rope_append_ex or attn_norm_rope_append_ex,
+ *   attn_tree_decode_ex     every draft over prefix, context and its ancestors
+ *   (the caller compares the model's answers with the drafts)
+ *   attn_tree_commit_ex     the accepted path's rows moved together, all layers;
+ *                           its lens_out and counts are the next step's lens
+ *                           and free_count
+ * None allocates; all may be captured in a graph.
+ * ---------------------------------------------------------------------- */
+/* cu_rows[n_seq+1]: request s's drafts are token rows [cu_rows[s], cu_rows[s+1])
+ * (the page plan's cu_new; ends are clamped to n_rows, the rows of the other
+ * arrays).  parents[r]: the parent's index within the request, less than the
+ * draft's own, or -1.  positions[r], as the page plan leaves them: that of each
+ * request's first row is read.  Written, for the requests' rows alone:
+ *   positions_out[r] (may be positions): the first row's position + the draft's
+ *     depth (0 for a draft without a parent);
+ *   masks[r][mask_words]: bit j % 32 of word j / 32 is set where draft j is
+ *     draft r or an ancestor of it.
+ * mask_words is 1 to 32, n_seq at most 65535.  A parent that is no earlier
+ * draft counts as -1 and records 0x704 in the device error word; drafts past
+ * 32 * mask_words get an empty mask and depth 0 and record 0x705. */
+ATTN_API int attn_tree_plan_ex(int n_seq, int n_rows, int mask_words, const int *cu_rows, const int *parents,
+                const int *positions, int *positions_out, uint32_t *masks, attn_stream_t stream);
+
+typedef struct {
+    int n_seq;                  /* requests, <= 65535                          */
+    int n_rows;                 /* token rows of q, out, lse and masks:
+                                   n_rows * heads <= 2^24                      */
+    int n_groups;               /* groups that share a prefix (0: none)        */
+    int heads, kv_heads;        /* as in attn_prefix_shape, and below          */
+    int head_dim;
+    int dtype;
+    int page_size;
+    int max_prefix_pages;
+    int max_pages;
+    int max_prefix_len;         /* upper bounds of prefix_lens and lens        */
+    int max_len;
+    int max_nodes;              /* upper bound of lens - ctx_lens, <= 1024     */
+    int mask_words;             /* words of a row of masks, <= 32 and at least
+                                   max_nodes / 32 (0 where masks is NULL)      */
+    long long q_row_stride, out_row_stride;
+    float scale;
+} attn_tree_shape;
+
+/* Bytes of device workspace attn_tree_decode_ex needs (by the shape, the
+ * cache's type and the device's number of SMs). */
+ATTN_API size_t attn_tree_decode_workspace_bytes(const attn_tree_shape *s, const attn_paged_kv *cache);
+
+/* Each token row of request s attends, as one softmax, to the rows of its
+ * group's prefix, to the first ctx_lens[s] rows of block_table[s] and to those
+ * of the rows ctx_lens[s] + j, below lens[s], for which its mask has bit j
+ * (masks NULL: j up to the row's index in the request).  A row that a token
+ * does not see may hold anything.  lens[s] = ctx_lens[s] for a request whose
+ * drafts have no rows (refused by the page plan): the page plan's lens and
+ * lens_out are ctx_lens and lens.
+ *   cu_rows[n_seq+1] (DEVICE, ascending): the requests' rows of q and out; ends
+ *   are clamped to n_rows, and rows of no request are left as they are.
+ *   group_begin[n_groups+1] (ascending): group g is requests [group_begin[g],
+ *   group_begin[g+1]).  Prefixes, tables, lse, clamped lengths and error codes
+ *   0x702 and 0x703, arithmetic and NaN as in attn_prefix_decode_ex.  A row that
+ *   sees nothing gets out = 0 and lse = -inf.  A prefix, and a context, is read once for each
+ *   block of up to 4 to 256 query rows (token rows x heads/kv_heads).
+ * workspace: 256-byte aligned, of the size above; calls that may overlap on the
+ * GPU need one each. */
+ATTN_API int attn_tree_decode_ex(const attn_tree_shape *s, const attn_paged_kv *cache, const void *q, const int *cu_rows,
+                const int *ctx_lens, const int *lens, const uint32_t *masks, const int *group_begin,
+                const int *prefix_table, const int *prefix_lens, const int *block_table, void *out, float *lse,
+                void *workspace, size_t workspace_bytes, attn_stream_t stream);
+
+/* Keeps, of every request's drafts, the path that ends at draft leaf[s] (-1:
+ * none): the drafts in the leaf's mask (masks NULL: drafts 0 .. leaf[s]) go, in
+ * their order, to rows ctx_lens[s], ctx_lens[s] + 1, ... in each of the n_layers
+ * caches (a HOST array, at most ATTN_MAX_LAYERS, all of one type; K, V and
+ * scales), whose rows follow block_table.  Of the page shape, max_tokens is the
+ * rows of masks.  Written besides:
+ *   lens_out[n_seq]: ctx_lens + the drafts kept (lens where there were none);
+ *   free_pages past *free_count: the pages behind the kept rows, in request and
+ *     page order (what passes n_pages entries is lost);
+ *   counts[4]: the free pages after it, the drafts kept, the requests that kept
+ *     none, the pages handed back.
+ * A leaf that is no drafted row of its request keeps nothing and, unless the
+ * request has no drafted rows, records 0x706 in the device error word; a page
+ * outside a cache records 0x702 and its rows stay where they are.  lens_out and
+ * counts must not overlap lens, ctx_lens, leaf and free_count. */
+ATTN_API int attn_tree_commit_ex(const attn_page_shape *s, int n_layers, const attn_paged_kv *caches, int kv_heads, int head_dim,
+                const int *cu_rows, const int *ctx_lens, const int *lens, const int *leaf, const uint32_t *masks,
+                int mask_words, const int *block_table, int *free_pages, const int *free_count, int *lens_out,
+                int *counts, attn_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Multi-GPU partitioning by (batch x head) units
  * ---------------------------------------------------------------------- */
 /* Contiguous split of n_units over `world` ranks: rank gets [*begin, *end). */

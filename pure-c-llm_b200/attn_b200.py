@@ -95,6 +95,14 @@ class PrefixShape(ctypes.Structure):
                 ("scale", ctypes.c_float)]
 
 
+class TreeShape(ctypes.Structure):
+    _fields_ = [("n_seq", ctypes.c_int), ("n_rows", ctypes.c_int), ("n_groups", ctypes.c_int), ("heads", ctypes.c_int),
+                ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("dtype", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("max_prefix_pages", ctypes.c_int), ("max_pages", ctypes.c_int), ("max_prefix_len", ctypes.c_int),
+                ("max_len", ctypes.c_int), ("max_nodes", ctypes.c_int), ("mask_words", ctypes.c_int),
+                ("q_row_stride", ctypes.c_longlong), ("out_row_stride", ctypes.c_longlong), ("scale", ctypes.c_float)]
+
+
 class Split(ctypes.Structure):
     _fields_ = [("batch0", ctypes.c_int), ("batch", ctypes.c_int), ("head0", ctypes.c_int),
                 ("heads", ctypes.c_int), ("nb", ctypes.c_int), ("nh", ctypes.c_int)]
@@ -140,6 +148,10 @@ SIGNATURES = {
     "attn_norm_rope_append_ex": (I, [ctypes.POINTER(RopeShape), ctypes.POINTER(HeadNormPtrs), ctypes.POINTER(PagedKV), I] + [P] * 8),
     "attn_prefix_decode_workspace_bytes": (SZ, [ctypes.POINTER(PrefixShape), ctypes.POINTER(PagedKV)]),
     "attn_prefix_decode_ex": (I, [ctypes.POINTER(PrefixShape), ctypes.POINTER(PagedKV), P, P, P, P, P, P, P, P, P, SZ, P]),
+    "attn_tree_plan_ex": (I, [I, I, I, P, P, P, P, P, P]),
+    "attn_tree_decode_workspace_bytes": (SZ, [ctypes.POINTER(TreeShape), ctypes.POINTER(PagedKV)]),
+    "attn_tree_decode_ex": (I, [ctypes.POINTER(TreeShape), ctypes.POINTER(PagedKV)] + [P] * 12 + [SZ, P]),
+    "attn_tree_commit_ex": (I, [ctypes.POINTER(PageShape), I, ctypes.POINTER(PagedKV), I, I] + [P] * 5 + [I] + [P] * 6),
     "attn_shard_range": (I, [LL, I, I, ctypes.POINTER(LL), ctypes.POINTER(LL)]),
     "attn_shard_lpt": (I, [P, I, I, I, P, P]),
     "attn_gather_permute": (I, [P, P, I, I, I, I, I, I, P]),
@@ -585,3 +597,76 @@ def prefix_decode_t(shape: PrefixShape, cache: PagedKV, q, group_begin, prefix_t
                                     workspace.numel() * workspace.element_size() if workspace is not None else 0,
                                     _stream()))
     return out
+
+
+# ---------------------------------------------------------------------------
+# drafted token trees
+# ---------------------------------------------------------------------------
+def tree_plan_t(cu_rows, parents, positions, positions_out, masks):
+    """attn_tree_plan_ex: int32 tensors; cu_rows (n_seq + 1), masks (rows, words), the others (rows).  positions_out may
+    be positions."""
+    import torch
+    on, i32, rows = _device(), torch.int32, parents.numel()
+    if masks.dim() != 2:
+        raise ValueError(f"masks, {tuple(masks.shape)}, is not (rows, words)")
+    _dense(on, ("cu_rows", cu_rows, i32, 1), ("parents", parents, i32, 0), ("positions", positions, i32, rows),
+           ("positions_out", positions_out, i32, rows), ("masks", masks, i32, rows * masks.shape[1]))
+    check(lib.attn_tree_plan_ex(cu_rows.numel() - 1, rows, masks.shape[1], cu_rows.data_ptr(), parents.data_ptr(), positions.data_ptr(),
+                                positions_out.data_ptr(), masks.data_ptr(), _stream()))
+    return positions_out, masks
+
+
+def tree_decode_workspace_bytes(shape: TreeShape, cache: PagedKV) -> int:
+    return lib.attn_tree_decode_workspace_bytes(shape, cache)
+
+
+def tree_decode_t(shape: TreeShape, cache: PagedKV, q, cu_rows, ctx_lens, lens, masks, block_table, out, lse=None, group_begin=None,
+                  prefix_table=None, prefix_lens=None, workspace=None):
+    """attn_tree_decode_ex: q and out (n_rows, heads * d); masks (n_rows, mask_words) int32 or None; tables and lengths
+    int32; the groups' tensors may be None when shape.n_groups is 0.  Without a workspace one is allocated."""
+    import torch
+    on, n, rows, groups, heads, d, i32 = _device(), shape.n_seq, shape.n_rows, shape.n_groups, shape.heads, shape.head_dim, torch.int32
+    dtype = torch.bfloat16 if shape.dtype == BF16 else torch.float32
+    _dense(on, ("cu_rows", cu_rows, i32, n + 1), ("ctx_lens", ctx_lens, i32, n), ("lens", lens, i32, n),
+           ("masks", masks, i32, rows * shape.mask_words), ("lse", lse, torch.float32, rows * heads),
+           ("workspace", workspace, workspace.dtype if workspace is not None else None, 0))
+    if groups > 0:
+        _dense(on, ("group_begin", group_begin, i32, groups + 1), ("prefix_lens", prefix_lens, i32, groups))
+        _rows(on, i32, "prefix_table", prefix_table, groups, shape.max_prefix_pages, 0)
+    _rows(on, i32, "block_table", block_table, n, shape.max_pages, 0)
+    _rows(on, dtype, "q", q, rows, heads * d, shape.q_row_stride)
+    _rows(on, dtype, "out", out, rows, heads * d, shape.out_row_stride)
+    _cache_holds(on, cache, shape.kv_heads, d)
+    if workspace is None:
+        workspace = torch.empty(tree_decode_workspace_bytes(shape, cache), dtype=torch.uint8, device=q.device)
+    check(lib.attn_tree_decode_ex(shape, cache, q.data_ptr(), cu_rows.data_ptr(), ctx_lens.data_ptr(), lens.data_ptr(), _ptr(masks),
+                                  _ptr(group_begin), _ptr(prefix_table), _ptr(prefix_lens), block_table.data_ptr(), out.data_ptr(),
+                                  _ptr(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream()))
+    return out
+
+
+def cache_array(caches):
+    """The caches of a model's layers, as tree_commit_t takes them (it keeps them alive)."""
+    a = (PagedKV * len(caches))(*caches)
+    a.caches = tuple(caches)
+    return a
+
+
+def tree_commit_t(shape: PageShape, caches, kv_heads: int, head_dim: int, cu_rows, ctx_lens, lens, leaf, masks, block_table, free_pages,
+                  free_count, lens_out, counts):
+    """attn_tree_commit_ex: caches by cache_array; int32 tensors; masks (rows, words) or None (chains, of up to 1024)."""
+    import torch
+    on, n, i32 = _device(), shape.n_seq, torch.int32
+    if masks is not None and masks.dim() != 2:
+        raise ValueError(f"masks, {tuple(masks.shape)}, is not (rows, words)")
+    words = masks.shape[1] if masks is not None else 32
+    _dense(on, ("cu_rows", cu_rows, i32, n + 1), ("ctx_lens", ctx_lens, i32, n), ("lens", lens, i32, n), ("leaf", leaf, i32, n),
+           ("masks", masks, i32, shape.max_tokens * words), ("free_pages", free_pages, i32, shape.n_pages), ("free_count", free_count, i32, 1),
+           ("lens_out", lens_out, i32, n), ("counts", counts, i32, 4))
+    _rows(on, i32, "block_table", block_table, n, shape.max_pages, shape.table_stride)
+    for cache in getattr(caches, "caches", ()):
+        _cache_holds(on, cache, kv_heads, head_dim)
+    check(lib.attn_tree_commit_ex(shape, len(caches), caches, kv_heads, head_dim, cu_rows.data_ptr(), ctx_lens.data_ptr(), lens.data_ptr(),
+                                  leaf.data_ptr(), _ptr(masks), words, block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+                                  lens_out.data_ptr(), counts.data_ptr(), _stream()))
+    return lens_out, counts

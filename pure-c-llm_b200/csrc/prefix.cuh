@@ -1,5 +1,6 @@
-// prefix.cuh -- what the kernels of attn_prefix_decode_ex share: the call's
-// arguments on the device, and the walk through a page table.
+// prefix.cuh -- what the kernels of attn_prefix_decode_ex and
+// attn_tree_decode_ex share: the call's arguments on the device, and the walk
+// through a page table.
 #pragma once
 #include "common.cuh"
 
@@ -19,6 +20,10 @@ struct Params {
     int log_page, n_pages;
     int max_prefix_pages, max_pages, max_prefix_len, max_len;
     float scale_log2;                                 // scale * log2(e)
+    // attn_tree_decode_ex (n_seq: query tokens, of n_req requests)
+    const int *row_begin, *ctx_lens;                  // first query token of each request; rows before its drafts
+    const uint32_t *masks;
+    int n_req, max_nodes, mask_words;
 };
 
 __device__ __forceinline__ int checked_len(const Params &p, int len, int most) {
@@ -29,8 +34,17 @@ __device__ __forceinline__ int checked_len(const Params &p, int len, int most) {
     return len;
 }
 __device__ __forceinline__ int own_len(const Params &p, int s) { return checked_len(p, __ldg(p.lens + s), p.max_len); }
-// first request of group g, within [0, n_seq]
+// What the lines of a part are: the requests' own rows, each with one query
+// token; the groups' prefixes; or the groups' prefixes and then the requests'
+// contexts, of requests with several query tokens (drafts).
+enum Lines { OWN, PREFIX, TREES };
+
+// first query token of request r, within [0, n_seq]
+__device__ __forceinline__ int row_first(const Params &p, int r) { return min(max(__ldg(p.row_begin + r), 0), p.n_seq); }
+// first query token of group g, within [0, n_seq]
+template <int LINES>
 __device__ __forceinline__ int group_first(const Params &p, int g) {
+    if constexpr (LINES == TREES) return row_first(p, min(max(__ldg(p.group_begin + g), 0), p.n_req));
     return min(max(__ldg(p.group_begin + g), 0), p.n_seq);
 }
 
@@ -68,23 +82,25 @@ struct Part {
     int log_rows, rows;                   // query rows of a block (2^log_rows), of a slot
     int log_keys;                         // keys of a step (2^log_keys)
     int half;                             // see Pieces (0: one piece per slot)
+    long long after;                      // TREES: rows of the prefixes' pieces
 };
 
 __device__ __forceinline__ int ceil_shift(int a, int log_b) { return (a + (1 << log_b) - 1) >> log_b; }
 
-// Query rows of a group and their blocks, and the index of the first block: an
-// ascending numbering without a sum over the groups before.
-__device__ __forceinline__ void group_blocks(const Params &p, const Part &w, int g, int &first_req, int &rows,
-                                             int &blocks, int &base) {
-    first_req = group_first(p, g);
-    rows = max(group_first(p, g + 1) - first_req, 0) * p.ratio;
+// Query rows of line i, the query tokens [first, next), and their blocks, and
+// the index of the first block: an ascending numbering without a sum over the
+// lines before.
+__device__ __forceinline__ void line_blocks(const Params &p, const Part &w, int i, int first, int next, int &rows,
+                                            int &blocks, int &base) {
+    rows = max(next - first, 0) * p.ratio;
     blocks = ceil_shift(rows, w.log_rows);
-    base = (first_req * p.ratio >> w.log_rows) + g;
+    base = (first * p.ratio >> w.log_rows) + i;
 }
 
 struct Line {
     int keys, steps, blocks;              // blocks of query rows
-    int first_req, rows, base;            // of the line's query rows; index of its first block
+    int first_req, rows, base;            // of the line's query rows (first query token); index of its first block
+    bool prefix;                          // TREES
     // cost of a segment, and of the line, in steps
     __host__ __device__ int cost() const { return steps + kBegin; }
     __device__ long long total(const Part &w) const { return steps ? (long long)cost() * blocks * w.n_blocks : 0; }
@@ -96,13 +112,20 @@ __host__ __device__ __forceinline__ long long segment_begin(const Part &w, const
     const int rb = row >> w.log_rows, hb = w.n_blocks == 1 ? 0 : hk / w.head_block;
     return line_begin + (long long)(rb * w.n_blocks + hb) * l.cost() + kBegin;
 }
-template <bool PRE>
+template <int LINES>
 __device__ __forceinline__ Line line_of(const Params &p, const Part &w, int i) {
     Line l;
-    if (PRE) {
+    l.prefix = LINES == PREFIX || (LINES == TREES && i < p.n_groups);
+    if (l.prefix) {
         const int len = __ldg(p.prefix_lens + i);            // on its way with the group's bounds
-        group_blocks(p, w, i, l.first_req, l.rows, l.blocks, l.base);
+        l.first_req = group_first<LINES>(p, i);
+        line_blocks(p, w, i, l.first_req, group_first<LINES>(p, i + 1), l.rows, l.blocks, l.base);
         l.keys = l.rows ? checked_len(p, len, p.max_prefix_len) : 0;
+    } else if (LINES == TREES) {
+        const int r = i - p.n_groups, len = __ldg(p.ctx_lens + r);
+        l.first_req = row_first(p, r);
+        line_blocks(p, w, r, l.first_req, row_first(p, r + 1), l.rows, l.blocks, l.base);
+        l.keys = l.rows ? checked_len(p, len, p.max_len) : 0;
     } else {
         l.first_req = i;
         l.rows = p.ratio;
@@ -119,7 +142,7 @@ __device__ __forceinline__ Line line_of(const Params &p, const Part &w, int i) {
 // own for the merge.  Returns the steps of a team: team t takes steps
 // [t n, (t + 1) n), so none between a segment's first and last is without a
 // piece, and a step's team is one division.
-template <bool PRE>
+template <int LINES>
 __device__ __forceinline__ long long sum_lines(const Params &p, const Part &w, long long *sums, long long *warp_sums) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int entries = w.entries;
@@ -129,7 +152,7 @@ __device__ __forceinline__ long long sum_lines(const Params &p, const Part &w, l
         long long v = 0;
         if (e < entries)
             for (int i = e * w.per_entry; i < min((e + 1) * w.per_entry, w.lines); i++)
-                v += line_of<PRE>(p, w, i).total(w);
+                v += line_of<LINES>(p, w, i).total(w);
         long long s = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -155,7 +178,7 @@ __device__ __forceinline__ long long sum_lines(const Params &p, const Part &w, l
             long long at = sums[e];
             for (int i = e * w.per_entry; i < min((e + 1) * w.per_entry, w.lines); i++) {
                 w.line_first[i] = at;
-                at += line_of<PRE>(p, w, i).total(w);
+                at += line_of<LINES>(p, w, i).total(w);
             }
         }
         if (threadIdx.x == 0) {
@@ -170,12 +193,41 @@ __device__ __forceinline__ long long sum_lines(const Params &p, const Part &w, l
 // [row0, row0 + rows) of the line, for block hb of key heads.
 struct Piece {
     const int *table;
-    long long slot;
+    long long at;                         // its first row on the workspace
     int keys, a, b, first_req, row0, rows, hb;
+    int apart;                            // rows between its key heads' states, or its two halves (Part::half)
 };
 
+// Where the pieces of a segment lie on the workspace: team t's at row
+// first + t * step, `apart` rows for each key head of the block (tiles: for
+// each of the two halves).  As segments and teams ascend together, no two
+// pieces meet.
+//   OWN, PREFIX: slots of w.rows rows for each key head.
+//   TREES: a request's few rows would leave most of a slot empty, so its
+//   pieces take as many rows as they have, behind those of the tokens before.
+//   With half, where a block of up to w.half rows has two states, a prefix
+//   takes w.half rows more for that, and a request's rows count twice.
+struct Place { long long first, step; int apart; };
+template <int LINES>
+__host__ __device__ __forceinline__ Place place_of(const Params &p, const Part &w, const Line &l, int rb, int hb) {
+    Place x;
+    x.step = (long long)w.head_block * w.rows;
+    if constexpr (LINES != TREES) {
+        x.first = ((long long)(l.base + rb) * w.n_blocks + hb) * x.step;
+        x.apart = w.half ? w.half : w.rows;
+        return x;
+    }
+    const int left = l.rows - (rb << w.log_rows), rows = left < 1 << w.log_rows ? left : 1 << w.log_rows;
+    const long long row = (long long)l.first_req * p.ratio + (rb << w.log_rows);
+    const int times = w.half && rows <= w.half ? 2 : 1;
+    x.apart = w.half && times == 1 ? w.half : rows;
+    const long long before = l.prefix ? row + (long long)w.half * (l.base - (l.first_req * p.ratio >> w.log_rows)) : row * (w.half ? 2 : 1);
+    x.first = (l.prefix ? 0 : w.after) + (before * w.n_blocks + (long long)hb * rows * times) * w.head_block;
+    return x;
+}
+
 // The pieces of team `team`'s range.
-template <bool PRE>
+template <int LINES>
 struct Walk {
     const Params &p;
     const Part &w;
@@ -207,7 +259,7 @@ struct Walk {
             while (s > s1) {              // the next line that the range meets, and its segments in the range
                 at += l.total(w);
                 if (++i >= w.lines || at >= last) { i = w.lines; at = last; l.steps = 0; return false; }
-                l = line_of<PRE>(p, w, i);
+                l = line_of<LINES>(p, w, i);
                 const long long n = l.total(w);
                 s = 0;
                 s1 = -1;
@@ -223,8 +275,11 @@ struct Walk {
             x.hb = s - rb * w.n_blocks;
             s++;
             if (x.a >= x.b) continue;     // the range holds the segment's beginning alone
-            x.slot = (long long)(l.base + rb) * w.n_blocks + x.hb + team;
-            x.table = PRE ? p.prefix_table + (long long)i * p.max_prefix_pages : p.block_table + (long long)i * p.max_pages;
+            const Place at = place_of<LINES>(p, w, l, rb, x.hb);
+            x.at = at.first + team * at.step;
+            x.apart = at.apart;
+            x.table = l.prefix ? p.prefix_table + (long long)i * p.max_prefix_pages
+                               : p.block_table + (long long)(LINES == TREES ? i - p.n_groups : i) * p.max_pages;
             x.keys = l.keys;
             x.first_req = l.first_req;
             x.row0 = rb << w.log_rows;

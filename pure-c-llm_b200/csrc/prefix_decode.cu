@@ -21,132 +21,11 @@
 // copies its rows through a ring of its own in shared memory, from which the
 // lanes read them in the layout that the arithmetic takes (prefix_paths.cuh),
 // and meets no other warp until the merge.
-#include <algorithm>
-
 #include "prefix.cuh"
-#include "prefix_paths.cuh"
+#include "prefix_rows.cuh"
 
 namespace attn {
 namespace prefix {
-
-constexpr int kWarps = 8;
-
-// One warp's piece: steps [a, b) of a line for the query rows of one block and
-// one key head.  The ring holds SLOTS halves of steps (K, V, K, ...): AHEAD
-// whole steps are in flight beside the half at work.
-template <class Path, int SLOTS>
-__device__ __forceinline__ void run_piece(const Params &p, uint32_t ring, const int *table, int keys, int a, int b,
-                                          int first_req, int row0, int rows, int hk, float *o, float2 *ml) {
-    static_assert(SLOTS % 2 == 1 && SLOTS >= 3, "ring");
-    constexpr int AHEAD = SLOTS / 2;
-    constexpr unsigned all = Path::KEYS == 32 ? 0xffffffffu : (1u << (Path::KEYS & 31)) - 1;
-    const int lane = threadIdx.x & 31;
-    const bool runs = p.log_page >= 4;
-    Path path;
-    // Cache row of this lane's key of a step: bad pages and keys past the line
-    // have no valid row.  In pages of 16 rows or more, a run of 16 keys is
-    // copied from its first key's row, which keys past the line do not decide.
-    auto row_of = [&](int step, bool &valid) {
-        const int t = step * Path::KEYS + lane;
-        valid = lane < Path::KEYS && t < keys && step < b;
-        int row = 0;
-        if (valid) {
-            const long long r = cache_row(p, table, t);
-            valid = r >= 0;
-            row = max((int)r, 0);
-        }
-        return row;
-    };
-    bool next_valid;
-    int next_row = row_of(a, next_valid), row = 0;
-    path.place(p, hk);
-    unsigned masks[AHEAD + 1];            // keys with a row, of this step and the ones in flight
-    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-    auto copy_k = [&](int step, int slot) {
-        row = next_row;
-        if (step < b) {
-            if (runs) path.template copy_k<true>(p, ring + slot * Path::SLOT, row);
-            else path.template copy_k<false>(p, ring + slot * Path::SLOT, row);
-        }
-        commit();
-        const unsigned mask = __ballot_sync(0xffffffffu, next_valid);
-        next_row = row_of(step + 1, next_valid);
-        return mask;
-    };
-    auto copy_v = [&](int step, int slot) {
-        if (step < b) {
-            if (runs) path.template copy_v<true>(p, ring + slot * Path::SLOT, row);
-            else path.template copy_v<false>(p, ring + slot * Path::SLOT, row);
-        }
-        commit();
-    };
-    auto wait = [] {
-        asm volatile("cp.async.wait_group %0;" ::"n"(SLOTS - 1) : "memory");
-        __syncwarp();                     // every lane's copies of the half are there
-    };
-#pragma unroll
-    for (int i = 0; i < AHEAD; i++) {
-        masks[i] = copy_k(a + i, 2 * i);
-        copy_v(a + i, 2 * i + 1);
-    }
-    path.begin(p, ring + SLOTS * Path::SLOT, first_req, row0, rows, hk);      // the queries, behind the first copies
-    int at = 0;                           // slot of this step's K
-    for (int step = a; step < b; step++) {
-        const int after = at + 1 == SLOTS ? 0 : at + 1, before = at ? at - 1 : SLOTS - 1;
-        masks[AHEAD] = copy_k(step + AHEAD, before);
-        wait();
-        if (masks[0] == all) path.template scores<false>(p, ring + at * Path::SLOT, all);
-        else path.template scores<true>(p, ring + at * Path::SLOT, masks[0]);
-        __syncwarp();                     // K's slot may be copied over
-        copy_v(step + AHEAD, at);
-        wait();
-        if (masks[0] == all) path.template values<false>(p, ring + after * Path::SLOT, all);
-        else path.template values<true>(p, ring + after * Path::SLOT, masks[0]);
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < AHEAD; i++) masks[i] = masks[i + 1];
-        at = after + 1 == SLOTS ? 0 : after + 1;
-    }
-    path.finish(o, ml, rows);
-}
-
-// Slots of a warp's ring: as many (an odd number) as CTAS rings of kWarps fit an SM, up to 7.
-template <class Path, int CTAS> struct Ring {
-    static constexpr int FIT = ((CTAS == 1 ? 216 : 108) * 1024 / kWarps - Path::SCRATCH) / Path::SLOT;
-    static constexpr int SLOTS = FIT > 7 ? 7 : (FIT - 1) / 2 * 2 + 1;
-    static constexpr int BYTES = SLOTS * Path::SLOT + Path::SCRATCH;
-    static_assert(Path::SLOT % 128 == 0 && Path::SCRATCH % 128 == 0, "swizzled rows begin on 128 bytes");
-};
-
-// PRE: the groups' prefixes; otherwise the requests' own rows.  `second`: the
-// launch before this one is the prefix part's, which has waited for the work
-// before it when this one may start; the two run side by side, and this one
-// ends after both.
-template <class Path, bool PRE, int D, int CTAS>
-__global__ void __launch_bounds__(kWarps * 32, CTAS)
-prefix_rows_kernel(const __grid_constant__ Params p, const __grid_constant__ Part w, int second)
-{
-    using R = Ring<Path, CTAS>;
-    extern __shared__ __align__(128) uint8_t ring_bytes[];
-    __shared__ long long sums[kEntries + 1];
-    __shared__ long long warp_sums[32];
-    if (!second) asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-    const long long of_team = sum_lines<PRE>(p, w, sums, warp_sums);
-    const int warp = threadIdx.x >> 5;
-    const uint32_t ring = sm100::smem_u32(ring_bytes) + warp * R::BYTES;
-    const int team_warp = warp % w.head_block, team = warp / w.head_block * (int)gridDim.x + (int)blockIdx.x;
-    Walk<PRE> walk(p, w, sums, of_team, team);
-    for (Piece x; walk.next(x);) {
-        const int hk = x.hb * w.head_block + team_warp;
-        if (hk >= p.kv_heads) continue;
-        const long long slot = x.slot * w.head_block + team_warp;
-        run_piece<Path, R::SLOTS>(p, ring, x.table, x.keys, x.a, x.b, x.first_req, x.row0, x.rows, hk,
-                                  w.o + slot * w.rows * D, w.ml + slot * w.rows);
-    }
-    if (second) asm volatile("griddepcontrol.wait;" ::: "memory");
-}
 
 // Joins the pieces of the query rows, a lane D/32 elements.  What counts is the
 // chain of dependent loads (lengths and first steps, then the pieces' m and l,
@@ -167,18 +46,18 @@ struct Pieces {
 constexpr int kMergeWarps = 4, kMany = 8;
 
 // The pieces of a row, from teams t0 .. t1.
-template <int D>
-__device__ __forceinline__ Pieces pieces_of(const Part &w, const Line &l, int row, int hk, int t0, int t1) {
+template <int LINES, int D>
+__device__ __forceinline__ Pieces pieces_of(const Params &p, const Part &w, const Line &l, int row, int hk, int t0, int t1) {
     Pieces r = {};
     if (l.steps == 0) return r;
     const int rb = row >> w.log_rows, hb = w.n_blocks == 1 ? 0 : hk / w.head_block, hw = hk - hb * w.head_block;
-    const long long seg = (long long)(l.base + rb) * w.n_blocks + hb;
-    const long long slot = ((seg + t0) * w.head_block + hw) * w.rows + row - (rb << w.log_rows);
-    r.o = w.o + slot * D;
-    r.ml = w.ml + slot;
-    r.step = (long long)w.head_block * w.rows;
+    const Place x = place_of<LINES>(p, w, l, rb, hb);
+    const long long at = x.first + t0 * x.step + (w.half ? 0 : (long long)hw * x.apart) + row - (rb << w.log_rows);
+    r.o = w.o + at * D;
+    r.ml = w.ml + at;
+    r.step = x.step;
     r.n = t1 - t0 + 1;
-    if (w.half && l.rows - (rb << w.log_rows) <= w.half) {      // two pieces in each slot, one behind the other
+    if (w.half && l.rows - (rb << w.log_rows) <= w.half) {      // two pieces of a team's, one behind the other
         r.step = w.half;
         r.n *= 2;
     }
@@ -199,7 +78,7 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
     // The request's lines: its own and, by the lanes, 32 groups at a time.  A
     // part whose bound is 0 has no launch of its own; its lengths are checked here.
     long long own_begin = 0, own_team = 1, pre_begin = 0, pre_team = 1;
-    const Line own_line = line_of<false>(p, own, s);
+    const Line own_line = line_of<OWN>(p, own, s);
     Line pre_line = {};
     if (own.lines) {
         own_begin = __ldcg(own.line_first + s);
@@ -208,12 +87,12 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
     if (pre.lines) pre_team = __ldcg(pre.line_first + pre.lines + 1);
     for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
         const int g = g0 + lane;
-        const bool in = g < p.n_groups && s >= group_first(p, g) && s < group_first(p, g + 1);
+        const bool in = g < p.n_groups && s >= group_first<PREFIX>(p, g) && s < group_first<PREFIX>(p, g + 1);
         const unsigned found = __ballot_sync(0xffffffffu, in);
         if (found) {
             const int mine = g0 + __ffs(found) - 1;
             if (pre.lines) pre_begin = __ldcg(pre.line_first + mine);
-            pre_line = line_of<true>(p, pre, mine);
+            pre_line = line_of<PREFIX>(p, pre, mine);
             break;
         }
     }
@@ -223,8 +102,8 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
     const int k = lane & 3;
     const int team = (int)quotient(max((k < 2 ? x : y) + (k & 1 ? (k < 2 ? own_line.steps : pre_line.steps) - 1 : 0), 0LL),
                                    k < 2 ? own_team : pre_team);
-    const Pieces a = pieces_of<D>(own, own_line, hr, hk, __shfl_sync(0xffffffffu, team, 0), __shfl_sync(0xffffffffu, team, 1));
-    const Pieces b = pieces_of<D>(pre, pre_line, pre_row, hk, __shfl_sync(0xffffffffu, team, 2), __shfl_sync(0xffffffffu, team, 3));
+    const Pieces a = pieces_of<OWN, D>(p, own, own_line, hr, hk, __shfl_sync(0xffffffffu, team, 0), __shfl_sync(0xffffffffu, team, 1));
+    const Pieces b = pieces_of<PREFIX, D>(p, pre, pre_line, pre_row, hk, __shfl_sync(0xffffffffu, team, 2), __shfl_sync(0xffffffffu, team, 3));
 
     const int n = a.n + b.n;
     float m = -INFINITY, l = 0.f, o[E];
@@ -299,8 +178,6 @@ prefix_merge_kernel(const __grid_constant__ Params p, const __grid_constant__ Pa
 
 namespace attn_host {
 
-int sm_count_here();
-bool ensure_smem_attr(const void *func, size_t bytes);
 int launch_prefix_tile(const attn::prefix::Params &p, const attn::prefix::Part &w, int d, cudaStream_t s);
 
 namespace {
@@ -323,27 +200,10 @@ Layout lay_out(const attn::prefix::Params &p, int d, int own_rows, int own_keys,
     };
     auto part = [&](Part &w, int lines, int seg_rows, int keys, int grid, bool pre) {
         if (!lines) return;
-        w.lines = lines;
-        w.per_entry = (lines + kEntries - 1) / kEntries;
-        w.entries = (lines + w.per_entry - 1) / w.per_entry;
-        // Key heads per team: adjacent ones, in blocks that leave as few of a CTA's warps idle as may be.
-        int best = 0;
-        for (int n = pre && tile ? p.kv_heads : (p.kv_heads + kWarps - 1) / kWarps; n <= p.kv_heads; n++) {
-            const int block = (p.kv_heads + n - 1) / n, splits = pre && tile ? 1 : kWarps / block;
-            const int used = p.kv_heads * splits * 1000 / n;          // warps at work, in thousandths
-            if (used <= best) continue;
-            best = used;
-            w.n_blocks = n;
-            w.head_block = block;
-            w.splits = splits;
-        }
-        w.teams = grid * w.splits;
-        w.log_rows = __builtin_ctz((unsigned)seg_rows);
-        w.log_keys = __builtin_ctz((unsigned)keys);
+        divide_part(w, p, lines, seg_rows, keys, grid, pre && tile);
         w.blocks = (p.ratio + seg_rows - 1) / seg_rows;
         const long long all_rows = (long long)p.n_seq * p.ratio;
         w.rows = pre && tile ? seg_rows : (int)std::min<long long>(pre ? all_rows : p.ratio, seg_rows);
-        w.half = pre && tile ? 128 : 0;
         const long long blocks = pre ? all_rows / seg_rows + lines : (long long)lines * w.blocks;
         const size_t slots = (size_t)(blocks * w.n_blocks + w.teams) * w.head_block * w.rows;
         w.line_first = reinterpret_cast<long long *>(take(((size_t)lines + 2) * 8));
@@ -354,18 +214,6 @@ Layout lay_out(const attn::prefix::Params &p, int d, int own_rows, int own_keys,
     part(r.pre, p.max_prefix_len ? p.n_groups : 0, tile ? 256 : pre_rows, tile ? 128 : pre_keys, pre_grid, true);
     r.bytes = std::max<size_t>(off, 256);
     return r;
-}
-
-template <class Path, bool PRE, int D, int CTAS>
-int run_part(const attn::prefix::Params &p, const attn::prefix::Part &w, int second, cudaStream_t s) {
-    using namespace attn::prefix;
-    using R = Ring<Path, CTAS>;
-    const auto kernel = prefix_rows_kernel<Path, PRE, D, CTAS>;
-    const int warps = w.splits * w.head_block;
-    if (!ensure_smem_attr((const void *)kernel, (size_t)R::BYTES * kWarps))
-        return set_error(ATTN_ERR_CUDA, "prefix decode: cannot set shared-memory size");
-    return check_pdl(launch_pdl(kernel, dim3(w.teams / w.splits), dim3(warps * 32), (size_t)R::BYTES * warps, s, p, w, second),
-                     "prefix_rows_kernel");
 }
 
 template <class Own, class Pre, int D>
@@ -383,9 +231,9 @@ int run(const attn::prefix::Params &p, void *ws, size_t *need, cudaStream_t s) {
                              sm_count_here() * (tile ? 1 : PRE_CTAS), tile, static_cast<char *>(ws));
     if (need) { *need = L.bytes; return ATTN_OK; }
     int st;
-    if (L.pre.lines && (st = tile ? launch_prefix_tile(p, L.pre, D, s) : run_part<Pre, true, D, PRE_CTAS>(p, L.pre, 0, s)))
+    if (L.pre.lines && (st = tile ? launch_prefix_tile(p, L.pre, D, s) : run_part<Pre, PREFIX, D, PRE_CTAS>(p, L.pre, 0, s)))
         return st;
-    if (L.own.lines && (st = run_part<Own, false, D, OWN_CTAS>(p, L.own, L.pre.lines != 0, s))) return st;
+    if (L.own.lines && (st = run_part<Own, OWN, D, OWN_CTAS>(p, L.own, L.pre.lines != 0, s))) return st;
     const int rows = p.n_seq * p.heads;
     const bool shared = rows < sm_count_here() * 16;
     return check_pdl(launch_pdl(shared ? prefix_merge_kernel<T, D, true> : prefix_merge_kernel<T, D, false>,

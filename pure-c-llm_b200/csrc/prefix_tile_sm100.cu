@@ -1,6 +1,7 @@
-// prefix_tile_sm100.cu -- the prefix part of attn_prefix_decode_ex on the
-// Blackwell tensor cores, for bf16 caches whose groups have many query rows
-// (requests x query heads per key head).
+// prefix_tile_sm100.cu -- the prefix part of attn_prefix_decode_ex, and the
+// prefixes and contexts of attn_tree_decode_ex, on the Blackwell tensor cores,
+// for bf16 caches whose groups (or drafts) have many query rows (query tokens x
+// query heads per key head).
 //
 // With r rows a prefix costs r flops per byte, so past about 250 rows the
 // tensor cores bound it and not HBM; mma.sync, at a quarter of their rate,
@@ -92,7 +93,7 @@ __device__ __forceinline__ uint32_t tile_at(int r, int ch) {
     return (uint32_t)((ch / 8) * BM * 128 + r * 128 + (((ch % 8) ^ (r & 7)) << 4));
 }
 
-template <int D>
+template <int D, int LINES>
 __global__ void __launch_bounds__(kThreads, 1)
 prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                    const __grid_constant__ Params p, const __grid_constant__ Part w, int boxes)
@@ -135,8 +136,8 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     // (the sums lie where the query rows come after the next barrier)
     long long *sums = reinterpret_cast<long long *>(sb);
     static_assert((kEntries + 1 + 32) * 8 <= 2 * C::TILE, "sums in the query tiles");
-    const long long of_team = sum_lines<true>(p, w, sums, sums + kEntries + 1);
-    Walk<true> walk(p, w, sums, of_team, (int)blockIdx.x);
+    const long long of_team = sum_lines<LINES>(p, w, sums, sums + kEntries + 1);
+    Walk<LINES> walk(p, w, sums, of_team, (int)blockIdx.x);
     Piece x;
     tc_fence_before();
     __syncthreads();
@@ -439,7 +440,7 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             // The piece: this warpgroup's half of the slot.  A warp turns 32 dims of its 32 rows
             // over in what was the place of their queries and writes them 128 bytes at a time.
             // (Each thread writing its own row, 512 bytes apart: 6.4 us from a piece's last P to the next piece, 3.4 so.)
-            const long long at = x.slot * w.rows + wg * BM + row;
+            const long long at = x.at + wg * x.apart + row;
             if (any) {
                 ok = mbar_wait(BAR(B_OD + 2 * wg), (t - 1) & 1, abort_flag, p.err, 0x835) &&
                      mbar_wait(BAR(B_OD + 2 * wg + 1), (t - 1) & 1, abort_flag, p.err, 0x836);
@@ -516,10 +517,10 @@ static bool cache_map(CUtensorMap *m, const void *ptr, int cols, long long rows,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D>
+template <int D, int LINES>
 static int launch_d(const attn::prefix::Params &p, const attn::prefix::Part &w, cudaStream_t s) {
     using namespace attn::ptile;
-    if (!ensure_smem_attr((const void *)prefix_tile_kernel<D>, Cfg<D>::SMEM))
+    if (!ensure_smem_attr((const void *)prefix_tile_kernel<D, LINES>, Cfg<D>::SMEM))
         return set_error(ATTN_ERR_CUDA, "prefix decode: cannot set shared-memory size");
     // A step is BN / box boxes; a box of the swizzled layout begins on 8 rows.
     CUtensorMap tk = {}, tv = {};
@@ -527,13 +528,16 @@ static int launch_d(const attn::prefix::Params &p, const attn::prefix::Part &w, 
     const long long rows = (long long)p.n_pages << p.log_page;
     const bool maps = box >= 8 && cache_map(&tk, p.k, p.kv_heads * D, rows, p.row_stride, box) &&
                       cache_map(&tv, p.v, p.kv_heads * D, rows, p.row_stride, box);
-    return check_pdl(launch_pdl(prefix_tile_kernel<D>, dim3(w.teams), dim3(kThreads), Cfg<D>::SMEM, s, tk, tv, p, w,
+    return check_pdl(launch_pdl(prefix_tile_kernel<D, LINES>, dim3(w.teams), dim3(kThreads), Cfg<D>::SMEM, s, tk, tv, p, w,
                                 maps ? BN / box : 0),
                      "prefix_tile_kernel");
 }
 
 int launch_prefix_tile(const attn::prefix::Params &p, const attn::prefix::Part &w, int d, cudaStream_t s) {
-    return d == 64 ? launch_d<64>(p, w, s) : launch_d<128>(p, w, s);
+    return d == 64 ? launch_d<64, attn::prefix::PREFIX>(p, w, s) : launch_d<128, attn::prefix::PREFIX>(p, w, s);
+}
+int launch_tree_tile(const attn::prefix::Params &p, const attn::prefix::Part &w, int d, cudaStream_t s) {
+    return d == 64 ? launch_d<64, attn::prefix::TREES>(p, w, s) : launch_d<128, attn::prefix::TREES>(p, w, s);
 }
 
 }  // namespace attn_host
