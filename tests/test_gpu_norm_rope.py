@@ -190,16 +190,15 @@ def test_strided_views(A, kind, offset):
     c.check_backward(dk, None, c.k, c.gk, 2, c.kw, pos)
     for t in (out, grads):
         assert (t[:, :offset] == 5).all() and (t[:, offset + 256:offset + 300] == 5).all() and (t[:, offset + 428:] == 5).all()
-    alone, da, daw, none = torch.empty_like(c.q), torch.empty_like(c.q), torch.empty_like(dqw), torch.full_like(dqw, 2.0)
+    alone, daw, none = torch.empty_like(c.q), torch.empty_like(dqw), torch.full_like(dqw, 2.0)
     shape = c.shape(13, q_row_stride=st)
     A.norm_rope_t(shape, c.norm, dev(c.table), None, q, None, alone, None)
-    assert torch.equal(alone, qo)
+    c.check_forward(alone, c.q, 4, c.qw, pos)     # (aligned rows may go another way than unaligned ones: not the same bits)
     g = c.gq
     dw = wide(torch.zeros_like(c.q))[1]
     A.norm_rope_bwd_t(shape, c.norm, dev(c.table), None, q, None, g, None, dw, None, daw, none)
     c.check_backward(dw, daw, c.q, c.gq, 4, c.qw, pos)
     assert (none == 0).all()                      # the sum over no tokens
-    del da
 
 
 def test_without_weights_and_other_inputs(A):
