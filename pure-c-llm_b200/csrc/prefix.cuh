@@ -69,6 +69,9 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
     return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
 }
 constexpr int kBegin = 1;                 // steps that the beginning and end of a segment count for
+// TREES by tiles: a step of more than 128 query rows costs that many of fewer
+// rows, whose prefixes and contexts the teams get alike; and a beginning and end
+constexpr int kFullStep = 2, kTileBegin = 3;
 
 // One part of the work.
 struct Part {
@@ -101,16 +104,18 @@ struct Line {
     int keys, steps, blocks;              // blocks of query rows
     int first_req, rows, base;            // of the line's query rows (first query token); index of its first block
     bool prefix;                          // TREES
-    // cost of a segment, and of the line, in steps
-    __host__ __device__ int cost() const { return steps + kBegin; }
+    int weight = 1, begin = kBegin;       // cost of a step, and of a segment's beginning and end
+    // cost of a segment, and of the line
+    __host__ __device__ int cost() const { return steps * weight + begin; }
     __device__ long long total(const Part &w) const { return steps ? (long long)cost() * blocks * w.n_blocks : 0; }
 };
-// First step of a query row's segment in the order of all steps, for a row of
-// the line that begins at line_begin; 0 in a part that the call does not have.
+// First step of a query row's segment in the order of all steps (by their
+// costs), for a row of the line that begins at line_begin; 0 in a part that the
+// call does not have.
 __host__ __device__ __forceinline__ long long segment_begin(const Part &w, const Line &l, int row, int hk, long long line_begin) {
     if (!w.lines) return 0;
     const int rb = row >> w.log_rows, hb = w.n_blocks == 1 ? 0 : hk / w.head_block;
-    return line_begin + (long long)(rb * w.n_blocks + hb) * l.cost() + kBegin;
+    return line_begin + (long long)(rb * w.n_blocks + hb) * l.cost() + l.begin;
 }
 template <int LINES>
 __device__ __forceinline__ Line line_of(const Params &p, const Part &w, int i) {
@@ -134,6 +139,10 @@ __device__ __forceinline__ Line line_of(const Params &p, const Part &w, int i) {
         l.keys = own_len(p, i);
     }
     l.steps = ceil_shift(l.keys, w.log_keys);
+    if (LINES == TREES && w.half) {
+        l.weight = l.rows > w.half ? kFullStep : 1;
+        l.begin = kTileBegin;
+    }
     return l;
 }
 
@@ -172,7 +181,8 @@ __device__ __forceinline__ long long sum_lines(const Params &p, const Part &w, l
     if (threadIdx.x == 0) sums[0] = 0;
     __syncthreads();
     const long long total = entries ? sums[entries] : 0;
-    const long long of_team = max(quotient(total + w.teams - 1, w.teams), 1LL);
+    // (no fewer than a step costs: else a team between a segment's first and last would be without one)
+    const long long of_team = max(quotient(total + w.teams - 1, w.teams), LINES == TREES ? (long long)kFullStep : 1LL);
     if (blockIdx.x == 0) {
         for (int e = threadIdx.x; e < entries; e += blockDim.x) {
             long long at = sums[e];
@@ -268,9 +278,14 @@ struct Walk {
                     s1 = last < at + n ? (int)quotient(last - 1 - at, l.cost()) : l.blocks * w.n_blocks - 1;
                 }
             }
-            const long long begin = at + (long long)s * l.cost() + kBegin;
+            // a step is the team's that its first unit of cost is
+            const long long begin = at + (long long)s * l.cost() + l.begin;
             x.a = (int)(max(first, begin) - begin);
-            x.b = (int)(min(last, begin + l.steps) - begin);
+            x.b = (int)(min(last, begin + (long long)l.steps * l.weight) - begin);
+            if (LINES == TREES && l.weight > 1) {
+                x.a = (x.a + l.weight - 1) / l.weight;
+                x.b = (x.b + l.weight - 1) / l.weight;
+            }
             const int rb = w.n_blocks == 1 ? s : s / w.n_blocks;
             x.hb = s - rb * w.n_blocks;
             s++;

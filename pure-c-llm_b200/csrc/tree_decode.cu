@@ -16,7 +16,7 @@
 namespace attn {
 namespace prefix {
 
-constexpr int kJoinWarps = 4, kMany = 8, kKeys = 4;
+constexpr int kJoinWarps = 8;
 
 // The request of query token r (the last whose tokens begin at or before r),
 // or -1 where it has none.  By a warp, 32 probes at a time.
@@ -64,21 +64,38 @@ __device__ __forceinline__ Pieces pieces_of(const Params &p, const Part &w, cons
 template <typename KV> struct Out { using Type = float; };
 template <> struct Out<__nv_bfloat16> { using Type = __nv_bfloat16; };
 
-// One query row (token x head) per warp; SHARED: per CTA, whose warps share its
-// pieces and drafted rows.
+// Four consecutive elements as floats, and back.
+__device__ __forceinline__ float4 four(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+__device__ __forceinline__ float4 four(const __nv_bfloat16 *p) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(p);
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                       __uint_as_float(w.y & 0xffff0000u));
+}
+__device__ __forceinline__ float4 four(const int8_t *p) {
+    const char4 c = *reinterpret_cast<const char4 *>(p);
+    return make_float4(c.x, c.y, c.z, c.w);
+}
+
+// A warp takes one query token and four adjacent query heads, eight lanes a
+// head: lane i has elements 4 i .. 4 i + 3 of every 32.  A score is then three
+// exchanges for all four heads, and each lane keeps its head's maximum and sum,
+// so weights need none.  SHARED: the warps of a CTA share that, each taking some
+// of the drafted rows and pieces.
 template <typename KV, int D, bool SHARED>
-__global__ void __launch_bounds__(kJoinWarps * 32)
+__global__ void __launch_bounds__(kJoinWarps * 32, 2)
 tree_join_kernel(const __grid_constant__ Params p, const __grid_constant__ Part w)
 {
     pdl_begin();                          // launched by launch_pdl
     using T = typename Out<KV>::Type;
-    constexpr int E = D / 32;
+    constexpr int C = D / 32, KB = 4;     // elements of a lane, in fours; drafted rows, and pieces, at once
     constexpr bool I8 = sizeof(KV) == 1;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int r = blockIdx.x, h = (int)blockIdx.y * (SHARED ? 1 : kJoinWarps) + (SHARED ? 0 : warp);
-    if (h >= p.heads) return;
+    const int r = blockIdx.x;
+    const int unit = (int)blockIdx.y * (SHARED ? 1 : kJoinWarps) + (SHARED ? 0 : warp);
+    if (r >= row_first(p, p.n_req) || 4 * unit >= p.heads) return;
     const int req = request_of(p, r);
     if (req < 0) return;
+    const int h = min(4 * unit + lane / 8, p.heads - 1), mine = lane % 8 * 4;      // (idle lanes repeat the last head)
     const int hk = p.ratio == 1 ? h : h / p.ratio, hr = h - hk * p.ratio;
 
     const Line ctx = line_of<TREES>(p, w, p.n_groups + req);
@@ -93,31 +110,46 @@ tree_join_kernel(const __grid_constant__ Params p, const __grid_constant__ Part 
         const bool in = g < p.n_groups && r >= group_first<TREES>(p, g) && r < group_first<TREES>(p, g + 1);
         const unsigned found = __ballot_sync(0xffffffffu, in);
         if (found) {
-            const int mine = g0 + __ffs(found) - 1;
-            if (w.lines) pre_begin = __ldcg(w.line_first + mine);
-            pre = line_of<TREES>(p, w, mine);
+            const int at = g0 + __ffs(found) - 1;
+            if (w.lines) pre_begin = __ldcg(w.line_first + at);
+            pre = line_of<TREES>(p, w, at);
             break;
         }
     }
-    const int ctx_row = (r - ctx.first_req) * p.ratio + hr, pre_row = (r - pre.first_req) * p.ratio + hr;
-    // teams of the first and last step of both segments: four divisions, one in each of four lanes
-    const long long x = segment_begin(w, ctx, ctx_row, hk, ctx_begin), y = segment_begin(w, pre, pre_row, hk, pre_begin);
-    const int k = lane & 3;
-    const int mine = (int)quotient(max((k < 2 ? x : y) + (k & 1 ? (k < 2 ? ctx.steps : pre.steps) - 1 : 0), 0LL), team);
-    const Pieces a = pieces_of<D>(p, w, ctx, ctx_row, hk, __shfl_sync(0xffffffffu, mine, 0), __shfl_sync(0xffffffffu, mine, 1));
-    const Pieces b = pieces_of<D>(p, w, pre, pre_row, hk, __shfl_sync(0xffffffffu, mine, 2), __shfl_sync(0xffffffffu, mine, 3));
-
-    float m = -INFINITY, l = 0.f, o[E];
-    bool bad = false;                     // a score or a sum that is no number
-#pragma unroll
-    for (int i = 0; i < E; i++) o[i] = 0.f;
-
-    // the drafted rows that the token sees, kKeys at a time
     const int drafts = checked_len(p, checked_len(p, __ldg(p.lens + req), p.max_len) - ctx.keys, p.max_nodes);
-    float q[E];
-    const T *query = static_cast<const T *>(p.q) + r * p.q_stride + (long long)h * D + lane;
+
+    float4 q[C], o[C];
+    float m = -INFINITY, l = 0.f;
+    const T *query = static_cast<const T *>(p.q) + r * p.q_stride + (long long)h * D + mine;
 #pragma unroll
-    for (int i = 0; i < E; i++) q[i] = to_f32(query[32 * i]);
+    for (int c = 0; c < C; c++) {
+        q[c] = four(query + 32 * c);
+        o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    auto add = [&](int c, float f, float4 v) {
+        o[c].x = fmaf(f, v.x, o[c].x);
+        o[c].y = fmaf(f, v.y, o[c].y);
+        o[c].z = fmaf(f, v.z, o[c].z);
+        o[c].w = fmaf(f, v.w, o[c].w);
+    };
+    // Takes in maxima x (-inf: none) with sums s; x becomes the weights.
+    auto fold = [&](float (&x)[KB], const float (&s)[KB]) {
+        float mx = m;
+#pragma unroll
+        for (int i = 0; i < KB; i++) mx = fmaxf(mx, x[i]);
+        const float old = mx == m ? 1.f : exp2f(m - mx);
+        l *= old;
+#pragma unroll
+        for (int c = 0; c < C; c++) o[c] = make_float4(o[c].x * old, o[c].y * old, o[c].z * old, o[c].w * old);
+        m = mx;
+#pragma unroll
+        for (int i = 0; i < KB; i++) {
+            x[i] = x[i] == -INFINITY ? 0.f : exp2f(x[i] - mx);
+            l = fmaf(x[i], s[i], l);
+        }
+    };
+
+    // the drafted rows that the token sees
     const int *table = p.block_table + (long long)req * p.max_pages;
     int seen = 0;
     for (int j0 = 0; j0 < drafts; j0 += 32) {
@@ -126,122 +158,133 @@ tree_join_kernel(const __grid_constant__ Params p, const __grid_constant__ Part 
                                 : last >= 31 ? 0xffffffffu : last < 0 ? 0u : (2u << last) - 1;
         if (drafts - j0 < 32) bits &= (1u << (drafts - j0)) - 1;
         while (bits) {
-            long long row[kKeys];
+            int row[KB];
+            bool any = false;
 #pragma unroll
-            for (int i = 0; i < kKeys; i++) {
+            for (int i = 0; i < KB; i++) {
                 row[i] = -1;
                 while (bits) {
                     const int j = __ffs(bits) - 1;
                     bits &= bits - 1;
                     if (SHARED && (seen++ % kJoinWarps) != warp) continue;
-                    row[i] = cache_row(p, table, ctx.keys + j0 + j);
+                    row[i] = (int)cache_row(p, table, ctx.keys + j0 + j);
+                    any = true;
                     break;
                 }
             }
-            float s[kKeys], v[kKeys][E], mx = m;
+            if (!any) continue;
+            float4 v[KB][C];
+            float x[KB], one[KB];
 #pragma unroll
-            for (int i = 0; i < kKeys; i++) {
-                const long long at = max(row[i], 0LL) * p.row_stride + (long long)hk * D + lane;
-                s[i] = 0.f;
+            for (int i = 0; i < KB; i++) {
+                x[i] = 0.f;
+                one[i] = 1.f;
+                const long long at = max(row[i], 0) * p.row_stride + (long long)hk * D + mine;
 #pragma unroll
-                for (int e = 0; e < E; e++) {
-                    if constexpr (I8) {
-                        s[i] = fmaf(q[e], (float)static_cast<const int8_t *>(p.k)[at + 32 * e], s[i]);
-                        v[i][e] = (float)static_cast<const int8_t *>(p.v)[at + 32 * e];
-                    } else {
-                        s[i] = fmaf(q[e], to_f32(static_cast<const KV *>(p.k)[at + 32 * e]), s[i]);
-                        v[i][e] = to_f32(static_cast<const KV *>(p.v)[at + 32 * e]);
-                    }
+                for (int c = 0; c < C; c++) {
+                    if (row[i] < 0) continue;
+                    const float4 k = four(static_cast<const KV *>(p.k) + at + 32 * c);
+                    v[i][c] = four(static_cast<const KV *>(p.v) + at + 32 * c);
+                    x[i] = fmaf(q[c].x, k.x, fmaf(q[c].y, k.y, fmaf(q[c].z, k.z, fmaf(q[c].w, k.w, x[i]))));
                 }
             }
 #pragma unroll
-            for (int i = 0; i < kKeys; i++) {
-                s[i] = warp_sum(s[i]) * p.scale_log2;
-                if constexpr (I8) s[i] *= p.kscale[max(row[i], 0LL) * p.kv_heads + hk];
-                if (row[i] < 0) s[i] = -INFINITY;
-                bad |= s[i] != s[i];
-                mx = fmaxf(mx, s[i]);
+            for (int k = 1; k < 8; k *= 2)
+#pragma unroll
+                for (int i = 0; i < KB; i++) x[i] += __shfl_xor_sync(0xffffffffu, x[i], k);
+            float vscale[KB];
+#pragma unroll
+            for (int i = 0; i < KB; i++) {
+                x[i] *= p.scale_log2;
+                if constexpr (I8) {
+                    const long long at = (long long)max(row[i], 0) * p.kv_heads + hk;
+                    x[i] *= __ldg(p.kscale + at);
+                    vscale[i] = __ldg(p.vscale + at);
+                }
+                if (row[i] < 0) x[i] = -INFINITY;
             }
-            if (mx == -INFINITY) continue;
-            const float old = exp2f(m - mx);
-            l *= old;
+            fold(x, one);
 #pragma unroll
-            for (int e = 0; e < E; e++) o[e] *= old;
-            m = mx;
-#pragma unroll
-            for (int i = 0; i < kKeys; i++) {
+            for (int i = 0; i < KB; i++) {
                 if (row[i] < 0) continue;
-                float c = exp2f(s[i] - m);
-                l += c;
-                if constexpr (I8) c *= p.vscale[row[i] * p.kv_heads + hk];
+                if constexpr (I8) x[i] *= vscale[i];
 #pragma unroll
-                for (int e = 0; e < E; e++) o[e] = fmaf(c, v[i][e], o[e]);
+                for (int c = 0; c < C; c++) add(c, x[i], v[i][c]);
             }
         }
     }
 
-    // the pieces
-    const int n = a.n + b.n;
-    auto which = [&](int j) { return SHARED ? j * kJoinWarps + warp : j; };
-    for (int j0 = 0; which(j0) < n; j0 += 32) {
-        const int j = which(j0 + lane);
-        const float2 ml = j < a.n ? __ldcg(a.ml + a.at(j)) : j < n ? __ldcg(b.ml + b.at(j - a.n)) : make_float2(-INFINITY, 0.f);
-        const float mx = fmaxf(m, warp_max(ml.x));
-        bad |= ml.y != ml.y;
-        if (mx == -INFINITY) continue;    // no valid row in these pieces
-        const bool rows = ml.x != -INFINITY;
-        const float old = exp2f(m - mx), c = rows ? exp2f(ml.x - mx) : 0.f;
-        l = l * old + warp_sum(ml.y * c);
+    // the pieces of the two lines
+    auto join = [&](const Line &line, long long begin) {
+        if (line.steps == 0) return;
+        const int row = (r - line.first_req) * p.ratio + hr;
+        const long long first = segment_begin(w, line, row, hk, begin);
+        const int t0 = (int)quotient(max(first, 0LL), team), t1 = (int)quotient(max(first + (long long)(line.steps - 1) * line.weight, 0LL), team);
+        const Pieces a = pieces_of<D>(p, w, line, row, hk, t0, t1);
+        int most = a.n;                   // of the four heads
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 8));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 16));
+        for (int j0 = SHARED ? warp * KB : 0; j0 < most; j0 += KB * (SHARED ? kJoinWarps : 1)) {
+            float x[KB], s[KB];
+            float4 v[KB][C];
 #pragma unroll
-        for (int i = 0; i < E; i++) o[i] *= old;
-        m = mx;
-        for (int k0 = 0; k0 < 32 && which(j0 + k0) < n; k0 += kMany) {
-            float z[kMany][E];
+            for (int i = 0; i < KB; i++) {
+                const int j = j0 + i;
+                const long long at = j < a.n ? a.at(j) : 0;
+                const float2 ml = j < a.n ? __ldcg(a.ml + at) : make_float2(-INFINITY, 0.f);
+                x[i] = ml.x;
+                s[i] = ml.y;
 #pragma unroll
-            for (int k = 0; k < kMany; k++) {
-                const int q = which(j0 + k0 + k);
-                const float *from = (q < a.n ? a.o + a.at(q) * D : b.o + b.at(q - a.n) * D) + lane;
-#pragma unroll
-                for (int i = 0; i < E; i++) z[k][i] = q < n ? __ldcg(from + 32 * i) : 0.f;
+                for (int c = 0; c < C; c++)
+                    v[i][c] = j < a.n ? __ldcg(reinterpret_cast<const float4 *>(a.o + at * D + mine + 32 * c)) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
+            bool there[KB];
 #pragma unroll
-            for (int k = 0; k < kMany; k++) {
-                // A piece without a valid row has an o that may not have been written; one whose weight is 0
-                // because its scores are low still hands on a value that is no number.
-                const float f = __shfl_sync(0xffffffffu, rows ? c : -1.f, k0 + k);
+            for (int i = 0; i < KB; i++) there[i] = x[i] != -INFINITY;
+            fold(x, s);
+            // A piece without a valid row has an o that may not have been written; one whose weight is 0 because its
+            // scores are low still hands on a value that is no number.
 #pragma unroll
-                for (int i = 0; i < E; i++) o[i] = f >= 0.f ? fmaf(z[k][i], f, o[i]) : o[i];
-            }
+            for (int i = 0; i < KB; i++)
+                if (there[i]) {
+#pragma unroll
+                    for (int c = 0; c < C; c++) add(c, x[i], v[i][c]);
+                }
         }
-    }
-    bad = __any_sync(0xffffffffu, bad);
+    };
+    join(ctx, ctx_begin);
+    join(pre, pre_begin);
+
     if constexpr (SHARED) {
-        __shared__ bool s_bad[kJoinWarps];
-        __shared__ float s_m[kJoinWarps], s_l[kJoinWarps], s_o[kJoinWarps][D];
-        if (lane == 0) { s_m[warp] = m; s_l[warp] = l; s_bad[warp] = bad; }
+        __shared__ float2 s_ml[kJoinWarps][4];
+        __shared__ float4 s_o[kJoinWarps][C][32];
+        if (lane % 8 == 0) s_ml[warp][lane / 8] = make_float2(m, l);
 #pragma unroll
-        for (int i = 0; i < E; i++) s_o[warp][lane + 32 * i] = o[i];
+        for (int c = 0; c < C; c++) s_o[warp][c][lane] = o[c];
         __syncthreads();
         if (warp) return;
-        m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-        l = 0.f;
+        for (int k0 = 1; k0 < kJoinWarps; k0 += KB) {
+            float x[KB], s[KB];
 #pragma unroll
-        for (int i = 0; i < E; i++) o[i] = 0.f;
+            for (int i = 0; i < KB; i++) {
+                const float2 ml = k0 + i < kJoinWarps ? s_ml[k0 + i][lane / 8] : make_float2(-INFINITY, 0.f);
+                x[i] = ml.x;
+                s[i] = ml.y;
+            }
+            fold(x, s);
 #pragma unroll
-        for (int k = 0; k < kJoinWarps; k++) {
-            const float c = s_m[k] == -INFINITY ? 0.f : exp2f(s_m[k] - m);
-            l += s_l[k] * c;
-            bad |= s_bad[k];
+            for (int i = 0; i < KB; i++)
 #pragma unroll
-            for (int i = 0; i < E; i++) o[i] += s_o[k][lane + 32 * i] * c;
+                for (int c = 0; c < C; c++)
+                    if (k0 + i < kJoinWarps) add(c, x[i], s_o[k0 + i][c][lane]);
         }
     }
-    T *out = static_cast<T *>(p.out) + r * p.out_stride + (long long)h * D + lane;
-    if (bad) m = l = NAN;
-    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    if (4 * unit + lane / 8 >= p.heads) return;
+    T *out = static_cast<T *>(p.out) + r * p.out_stride + (long long)h * D + mine;
+    const float inv = l != l ? NAN : m == -INFINITY ? 0.f : 1.f / l;
 #pragma unroll
-    for (int i = 0; i < E; i++) out[32 * i] = from_f32<T>(o[i] * inv);
-    if (p.lse && lane == 0) p.lse[(long long)r * p.heads + h] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+    for (int c = 0; c < C; c++) store4(out + 32 * c, make_float4(o[c].x * inv, o[c].y * inv, o[c].z * inv, o[c].w * inv));
+    if (p.lse && lane % 8 == 0) p.lse[(long long)r * p.heads + h] = l != l ? NAN : m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 }  // namespace prefix
@@ -282,9 +325,10 @@ size_t lay_out(Part &w, const Params &p, int d, int seg_rows, int keys, int grid
 template <typename KV, int D>
 int join(const Params &p, const Part &w, cudaStream_t s) {
     using namespace attn::prefix;
-    const bool shared = p.n_seq * p.heads < sm_count_here() * 16;
+    const int units = (p.heads + 3) / 4;
+    const bool shared = (long long)p.n_seq * units < 8LL * sm_count_here();
     return check_pdl(launch_pdl(shared ? tree_join_kernel<KV, D, true> : tree_join_kernel<KV, D, false>,
-                                dim3(p.n_seq, shared ? p.heads : (p.heads + kJoinWarps - 1) / kJoinWarps), dim3(kJoinWarps * 32), 0, s, p, w),
+                                dim3(p.n_seq, shared ? units : (units + kJoinWarps - 1) / kJoinWarps), dim3(kJoinWarps * 32), 0, s, p, w),
                      "tree_join_kernel");
 }
 
