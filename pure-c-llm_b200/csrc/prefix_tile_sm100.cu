@@ -60,6 +60,10 @@ using namespace prefix;
 constexpr int BM = 128, BN = 128, BH = 64;   // query rows; keys of a step, of an S
 constexpr int kThreads = 384;
 constexpr int kMasks = 8;                 // steps whose key masks are kept: more than K's ring holds, and the ones at work
+// Pieces of which the K warp has told the others: it is as many ahead of them as K's ring has slots, and two.  (Each warp
+// walking by itself kept the walk's state in the softmax's registers, which spilled: 8 % on the long prefixes of drafts.)
+constexpr int kQueue = 16;
+struct __align__(16) Queued { long long at; int a, b, first_req, row0, rows, hb, apart; };       // rows 0: no more
 
 template <int D>
 struct Cfg {
@@ -67,10 +71,14 @@ struct Cfg {
     // waits once one of the two copying warps runs ahead of the other
     static constexpr int KS = D == 64 ? 4 : 2, VS = D == 64 ? 4 : 3, SLOTS = KS + VS;
     static constexpr int TILE = BM * D * 2;                   // Q tile, K or V tile: D / 64 blocks of 128 rows x 128 bytes
-    static constexpr int OFF_KV = 2 * TILE;
+    // The places of two query tiles, each also of what both warpgroups turn over of O (16 KB a warpgroup)
+    static constexpr int QTILE = TILE > 32768 ? TILE : 32768;
+    static constexpr int OFF_KV = 2 * QTILE;
     static constexpr int OFF_BAR = OFF_KV + SLOTS * TILE;
-    static constexpr int OFF_MASK = OFF_BAR + 320;
-    static constexpr int SMEM = OFF_MASK + kMasks * 16 + 1024;
+    static constexpr int OFF_MASK = OFF_BAR + 416;           // (barriers, the TMEM address, the abort flag)
+    static constexpr int OFF_QUEUE = OFF_MASK + kMasks * 16;
+    static constexpr int SMEM = OFF_QUEUE + kQueue * (int)sizeof(Queued) + 1024;
+    static_assert(SMEM <= 232448, "shared memory of a CTA");
 };
 // TMEM columns
 __device__ __forceinline__ uint32_t col_s(int wg, int u) { return (uint32_t)(wg * 2 + u) * BH; }
@@ -81,7 +89,10 @@ enum {
     B_OF = 2,                             // per warpgroup: O read out
     B_SF = 4, B_PF = 8, B_OD = 12,        // per warpgroup and half (2 w + u): S ready; P written; PV finished
     B_FULL = 16, B_FREE = 24,             // per slot: copied; used
-    B_COUNT = 32
+    B_VE = 32,                            // a step's V rows that come as some boxes are there
+    B_TD = 33,                            // a piece's O is out: the query tiles' places are free of it
+    B_PQ = 34,                            // per place of the queue: a piece is there
+    B_COUNT = B_PQ + kQueue
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
@@ -105,14 +116,18 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     uint8_t *sb = smem_raw + (base - raw);
     const uint32_t sQ = base, sKV = base + C::OFF_KV, bar0 = base + C::OFF_BAR;
 #define BAR(i) (bar0 + 8u * (uint32_t)(i))
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sb + C::OFF_BAR + 256);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(sb + C::OFF_BAR + 260);
+    static_assert(8 * B_COUNT <= 400, "barriers");
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sb + C::OFF_BAR + 400);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(sb + C::OFF_BAR + 404);
     volatile uint32_t *masks = reinterpret_cast<volatile uint32_t *>(sb + C::OFF_MASK);   // [step % kMasks][4]: keys with a row
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(BAR(B_QF), 256);
         mbar_init(BAR(B_QE), 1);
+        mbar_init(BAR(B_VE), 1);
+        mbar_init(BAR(B_TD), 256);
+        for (int i = 0; i < kQueue; i++) mbar_init(BAR(B_PQ + i), 1);
         for (int i = 0; i < 2; i++) mbar_init(BAR(B_OF + i), 128);
         for (int i = 0; i < 4; i++) {
             mbar_init(BAR(B_SF + i), 2);
@@ -135,10 +150,19 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // (the sums lie where the query rows come after the next barrier)
     long long *sums = reinterpret_cast<long long *>(sb);
-    static_assert((kEntries + 1 + 32) * 8 <= 2 * C::TILE, "sums in the query tiles");
+    static_assert((kEntries + 1 + 32) * 8 <= 2 * C::QTILE, "sums in the query tiles");
     const long long of_team = sum_lines<LINES>(p, w, sums, sums + kEntries + 1);
-    Walk<LINES> walk(p, w, sums, of_team, (int)blockIdx.x);
-    Piece x;
+    Walk<LINES> walk(p, w, sums, of_team, (int)blockIdx.x);      // (of the copying warps)
+    volatile Queued *queue = reinterpret_cast<volatile Queued *>(sb + C::OFF_QUEUE);
+    Queued x;
+    // Piece k, for the other warps; false where there is none, or on a timeout.
+    auto piece = [&](int k, Queued &y) {
+        const bool ok = mbar_wait(BAR(B_PQ + k % kQueue), (k / kQueue) & 1, abort_flag, p.err, 0x805);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        const volatile Queued &q = queue[k % kQueue];
+        y.at = q.at; y.a = q.a; y.b = q.b; y.first_req = q.first_req; y.row0 = q.row0; y.rows = q.rows; y.hb = q.hb; y.apart = q.apart;
+        return y.rows > 0;
+    };
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -151,19 +175,49 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const int kv = warp;
         const CUtensorMap *map = kv ? &tv : &tk;
         if (lane == 0) prefetch_tmap(map);
-        int due = -1;                     // slot of a half that the lanes have on its way
+        int due = -1;                     // slot of a half that is on its way and not reported
+        int edges = 0;                    // halves of V that came as some boxes
+        bool boxed = false;               // the due half is one of them, without the keys `absent`
+        unsigned absent[4];
+        bool ok = true;
         auto flush = [&] {
             if (due < 0) return;
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            if (boxed) {
+                // zeros for the keys without a row, over what a page holds behind its last key: a probability of 0
+                // must not meet a NaN
+                ok = ok && mbar_wait(BAR(B_VE), edges & 1, abort_flag, p.err, 0x804);
+                ok = __all_sync(0xffffffffu, ok);
+                edges++;
+                if (!ok) return;
+                const uint32_t to = sKV + due * C::TILE;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (!absent[i]) continue;
+                    for (int r = lane / CPR; r < 32; r += 32 / CPR)
+                        if (absent[i] >> r & 1)
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(to + tile_at(32 * i + r, lane % CPR)), "r"(0) : "memory");
+                }
+                boxed = false;
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
             fence_async_smem();           // this thread's copies, for the tensor cores
             mbar_arrive(BAR(B_FULL + due));
             due = -1;
         };
         constexpr int RPI = 32 / CPR;     // rows per copy instruction
         const int lr = lane / CPR, ch = lane % CPR;
-        bool ok = true;
-        int g = 0;                        // steps
-        while (ok && walk.next(x)) {
+        auto tell = [&](int k, const Piece &x, int rows) {
+            if (kv == 0 && lane == 0) {
+                volatile Queued &q = queue[k % kQueue];
+                q.at = x.at; q.a = x.a; q.b = x.b; q.first_req = x.first_req; q.row0 = x.row0; q.rows = rows; q.hb = x.hb; q.apart = x.apart;
+                mbar_arrive(BAR(B_PQ + k % kQueue));
+            }
+        };
+        int g = 0, k = 0;                 // steps, pieces
+        Piece x;
+        for (; ok && walk.next(x); k++) {
+            tell(k, x, x.rows);
             const __nv_bfloat16 *from = static_cast<const __nv_bfloat16 *>(kv ? p.v : p.k) + (long long)x.hb * D + ch * 8;
             // cache rows of a step's 128 keys (-1: none), four per lane, read a step ahead
             int next[4];
@@ -184,11 +238,12 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                     valid[i] = __ballot_sync(0xffffffffu, next[i] >= 0);
                 }
                 look_up(j + 1);
-                const bool whole = boxes && (valid[0] & valid[1] & valid[2] & valid[3]) == 0xffffffffu;
+                const bool whole = (valid[0] & valid[1] & valid[2] & valid[3]) == 0xffffffffu;
                 const int ring = kv ? C::VS : C::KS, slot = kv ? C::KS + g % C::VS : g % C::KS;
                 const uint32_t to = sKV + slot * C::TILE;
                 if (g >= ring) {
                     flush();              // nothing may stay due behind the wait
+                    if (!ok) break;
                     ok = mbar_wait(BAR(B_FREE + slot), (g / ring + 1) & 1, abort_flag, p.err, 0x801 + kv);
                     if (!(ok = __all_sync(0xffffffffu, ok))) break;
                 }
@@ -197,26 +252,40 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                     for (int i = 0; i < 4; i++) masks[g % kMasks * 4 + i] = valid[i];
                 }
                 __syncwarp();
-                if (whole) {
+                if (boxes) {
+                    // A box for each page that there is (its first key's row): of K as it comes, since scores of keys
+                    // without a row are masked; of V, where some have none, with zeros in their place before it is reported
                     const int rows = BN / boxes, key = lane * rows & 127;     // of lane n's box
-                    int r = 0;
+                    int r = -1;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int y = __shfl_sync(0xffffffffu, row[i], key & 31);
                         if (key >> 5 == i) r = y;
                     }
-                    if (lane == 0) mbar_arrive_expect_tx(BAR(B_FULL + slot), C::TILE);
-                    else mbar_arrive(BAR(B_FULL + slot));
+                    const bool mine = lane < boxes && r >= 0, edge = kv && !whole;
+                    const int bytes = __popc(__ballot_sync(0xffffffffu, mine)) * rows * D * 2;
+                    if (edge) flush();
+                    if (!ok) break;
+                    const uint32_t bar = edge ? BAR(B_VE) : BAR(B_FULL + slot);
+                    if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+                    else if (!edge) mbar_arrive(bar);
                     __syncwarp();
-                    if (lane < boxes) {
+                    if (mine) {
 #pragma unroll
                         for (int d = 0; d < D / 64; d++)
-                            tma_load_3d(to + d * BN * 128 + key * 128, map, BAR(B_FULL + slot), x.hb * D + 64 * d, r, 0);
+                            tma_load_3d(to + d * BN * 128 + key * 128, map, bar, x.hb * D + 64 * d, r, 0);
                     }
                     __syncwarp();
+                    if (edge) {
+                        due = slot;
+                        boxed = true;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) absent[i] = ~valid[i];
+                    }
                     continue;
                 }
                 flush();
+                if (!ok) break;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
 #pragma unroll 4
@@ -228,6 +297,8 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 due = slot;
             }
         }
+        x = {};
+        tell(k, x, 0);
         if (ok) flush();
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == 2) {
@@ -239,8 +310,12 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         constexpr uint32_t id = idesc_bf16(BM, BH, 0, 0);
         int g = 0, t[2] = {0, 0};         // steps; steps per warpgroup
         bool ok = true;
-        for (int k = 0; ok && walk.next(x); k++) {
+        int place = 0;                    // of a single query tile (as in the softmax)
+        bool single = false;
+        for (int k = 0; ok && piece(k, x); k++) {
             const bool two = x.rows > BM;
+            place = !two && single ? 1 - place : 0;
+            single = !two;
             if (!(ok = wait(B_QF, k, 0x811))) break;
             for (int j = x.a; ok && j < x.b; j++, g++) {
                 const int slot = g % C::KS;
@@ -254,7 +329,7 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                     if (!ok) break;
                     tc_fence_after();
                     if (leader) {
-                        const uint64_t qd = sw128_desc(sQ + (two ? wg : 0) * C::TILE, 16, 1024);
+                        const uint64_t qd = sw128_desc(sQ + (two ? wg : place) * C::QTILE, 16, 1024);
                         const uint64_t kd = sw128_desc(sKV + slot * C::TILE + u * BH * 128, 16, 1024);
 #pragma unroll
                         for (int kk = 0; kk < D / 16; kk++) {   // 32 bytes on per step, a block of 16 KB on per 64 dims
@@ -284,7 +359,7 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         constexpr uint32_t id = idesc_bf16(BM, D, 0, 1);
         int g = 0, t[2] = {0, 0}, done[2] = {0, 0};   // steps; steps and pieces per warpgroup
         bool ok = true;
-        while (ok && walk.next(x)) {
+        for (int k = 0; ok && piece(k, x); k++) {
             const bool two = x.rows > BM;
             for (int j = x.a; ok && j < x.b; j++, g++) {
                 const int slot = C::KS + g % C::VS;
@@ -322,25 +397,37 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16), tO = lanes + col_o<D>(wg);
         int g = 0, t = 0;                 // steps of the CTA; of this warpgroup
         bool ok = true;
-        for (int k = 0; ok && walk.next(x); k++) {
-            const bool two = x.rows > BM;
-            // the warp's 32 query rows, CPR lanes a row (with up to 128 rows, warpgroup 0 brings them in for both);
-            // a lane to a row, 16 bytes of 32 rows an instruction, took 2.5 us instead of 1.1
-            if (two || wg == 0) {
-                constexpr int RPI = 32 / CPR;
-                const int r = wg * BM + row, at = x.row0 + min(r, x.rows - 1);
-                const int s = x.first_req + at / p.ratio, h = x.hb * p.ratio + at % p.ratio;
-                const long long mine = s * p.q_stride + (long long)h * D;
+        // the warp's 32 query rows of a piece, CPR lanes a row, to the tile at `place`
+        // (a lane to a row, 16 bytes of 32 rows an instruction, took 2.5 us instead of 1.1)
+        auto copy_queries = [&](const Queued &y, int place) {
+            constexpr int RPI = 32 / CPR;
+            const int r = y.rows > BM ? wg * BM + row : row, at = y.row0 + min(r, y.rows - 1);
+            const int s = y.first_req + at / p.ratio, h = y.hb * p.ratio + at % p.ratio;
+            const long long from = s * p.q_stride + (long long)h * D;
 #pragma unroll
-                for (int r0 = 0; r0 < 32; r0 += RPI) {
-                    const int n = r0 + lane / CPR, to = quad * 32 + n, ch = lane % CPR;
-                    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(p.q) + __shfl_sync(0xffffffffu, mine, n) + 8 * ch;
-                    copy16(sQ + wg * C::TILE + tile_at(to, ch), src, wg * BM + to < x.rows);
-                }
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                fence_async_smem();
+            for (int r0 = 0; r0 < 32; r0 += RPI) {
+                const int n = r0 + lane / CPR, to = quad * 32 + n, ch = lane % CPR;
+                const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(p.q) + __shfl_sync(0xffffffffu, from, n) + 8 * ch;
+                copy16(sQ + place * C::QTILE + tile_at(to, ch), src, r - row + to < y.rows);
             }
+        };
+        auto queries_there = [&] {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_async_smem();
             mbar_arrive(BAR(B_QF));
+        };
+        // Query tiles.  A piece of more than 128 rows has both places, warpgroup w place w, for its queries and later its
+        // O.  A smaller one has one place, whose queries warpgroup 0 brings in for both; where two such pieces follow one
+        // another they take turns, so the second one's queries come while the first one's O goes out.
+        int place = 0;
+        bool ahead = false;               // x's queries have come with the piece before
+        bool more = piece(0, x);
+        for (int k = 0; ok && more; k++) {
+            const bool two = x.rows > BM;
+            if (!ahead) {
+                if (two || wg == 0) copy_queries(x, two ? wg : place);
+                queries_there();
+            }
             const int mine = two ? x.rows - wg * BM : x.rows;     // query rows of this warpgroup
             const bool idle = quad * 32 >= mine;                  // none of them in this warp: it only keeps step
             float m = -INFINITY, l = 0.f;
@@ -435,8 +522,18 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             }
             if (!ok) break;
             g += x.b - x.a;
+            Queued y;                     // the next piece
+            more = piece(k + 1, y);
+            ahead = more && !two && y.rows <= BM;
+            if (ahead && wg == 0) {
+                // the other place: warpgroup 1 has taken O of the piece before this one out through it
+                ok = k == 0 || mbar_wait(BAR(B_TD), (k - 1) & 1, abort_flag, p.err, 0x837);
+                if (!(ok = __all_sync(0xffffffffu, ok))) break;
+                copy_queries(y, 1 - place);
+            }
             ok = mbar_wait(BAR(B_QE), k & 1, abort_flag, p.err, 0x830);
             if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            if (ahead && wg == 1) mbar_arrive(BAR(B_QF));     // (behind the queries of this piece, which QE followed)
             // The piece: this warpgroup's half of the slot.  A warp turns 32 dims of its 32 rows
             // over in what was the place of their queries and writes them 128 bytes at a time.
             // (Each thread writing its own row, 512 bytes apart: 6.4 us from a piece's last P to the next piece, 3.4 so.)
@@ -445,6 +542,9 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 ok = mbar_wait(BAR(B_OD + 2 * wg), (t - 1) & 1, abort_flag, p.err, 0x835) &&
                      mbar_wait(BAR(B_OD + 2 * wg + 1), (t - 1) & 1, abort_flag, p.err, 0x836);
                 if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            }
+            if (ahead && wg == 0) queries_there();
+            if (any) {
                 tc_fence_after();
                 if (!idle) {
 #pragma unroll
@@ -452,7 +552,7 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                         uint32_t o[32];
                         tmem_ld32(tO + c0, o);
                         tmem_wait_ld();
-                        float4 *turn = reinterpret_cast<float4 *>(sb + wg * C::TILE + quad * 32 * 128);
+                        float4 *turn = reinterpret_cast<float4 *>(sb + (two ? wg * C::QTILE : place * C::QTILE + wg * 16384) + quad * 32 * 128);
 #pragma unroll
                         for (int c = 0; c < 8; c++)
                             turn[lane * 8 + (c ^ (lane & 7))] = make_float4(__uint_as_float(o[4 * c]), __uint_as_float(o[4 * c + 1]),
@@ -472,6 +572,14 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 mbar_arrive(BAR(B_OF + wg));      // the next piece's first product may overwrite O
             }
             if (row < mine) w.ml[at] = make_float2(m, l);
+            mbar_arrive(BAR(B_TD));
+            // both places next: the other warpgroup may still be taking its O out through this one's
+            if (more && !two && y.rows > BM) {
+                ok = mbar_wait(BAR(B_TD), k & 1, abort_flag, p.err, 0x838);
+                if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            }
+            place = ahead ? 1 - place : 0;
+            x = y;
         }
     }
 
