@@ -646,9 +646,14 @@ def tree_decode_t(shape: TreeShape, cache: PagedKV, q, cu_rows, ctx_lens, lens, 
 
 
 def cache_array(caches):
-    """The caches of a model's layers, as tree_commit_t takes them (it keeps them alive)."""
+    """The caches of a model's layers, as tree_commit_t takes them (it keeps them alive): PageCaches of one device and
+    one number of heads, or PagedKVs of bare addresses."""
     a = (PagedKV * len(caches))(*caches)
     a.caches = tuple(caches)
+    held = [c for c in caches if isinstance(c, PageCache)]
+    if len({(c.device, c.scale_heads) for c in held}) > 1:
+        raise ValueError("the caches are on different devices, or of different key heads")
+    a.narrowest = min(held, key=lambda c: c.width) if held else None
     return a
 
 
@@ -664,8 +669,7 @@ def tree_commit_t(shape: PageShape, caches, kv_heads: int, head_dim: int, cu_row
            ("masks", masks, i32, shape.max_tokens * words), ("free_pages", free_pages, i32, shape.n_pages), ("free_count", free_count, i32, 1),
            ("lens_out", lens_out, i32, n), ("counts", counts, i32, 4))
     _rows(on, i32, "block_table", block_table, n, shape.max_pages, shape.table_stride)
-    for cache in getattr(caches, "caches", ()):
-        _cache_holds(on, cache, kv_heads, head_dim)
+    _cache_holds(on, getattr(caches, "narrowest", None), kv_heads, head_dim)
     check(lib.attn_tree_commit_ex(shape, len(caches), caches, kv_heads, head_dim, cu_rows.data_ptr(), ctx_lens.data_ptr(), lens.data_ptr(),
                                   leaf.data_ptr(), _ptr(masks), words, block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
                                   lens_out.data_ptr(), counts.data_ptr(), _stream()))

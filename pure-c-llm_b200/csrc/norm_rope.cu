@@ -18,14 +18,21 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace attn {
 namespace nrope {
 
 constexpr int kThreads = 256;
 constexpr int kHeads = 4, kHeadsBwd = 2;  // heads of a group
-constexpr int kCtas = 2;                  // per SM, that the registers leave
-constexpr int direct_ctas(bool pairs) { return pairs ? 3 : 2; }
+constexpr int kCtas = 2;                  // of kThreads per SM, that the registers leave
+// The direct kernels' heads of a group and CTAs per SM.  Forward, 32749 tokens of 32/8 x 128 in bf16 with 4 heads and 3
+// CTAs 157 us, 4 and 4 (spilling) 177, 8 and 2 177, 4 and 2 220; 4096 of 12/12 x 128 in fp32 with 3 and 3 19.7 us,
+// 4 and 3 22.2, 2 and 3 20.3.  Backward with the next token's loads on their way while this one's are worked on, 2 CTAs:
+// fp32 with 2 heads 34.1 us (without 36.2; 3 heads 42.1, 3 CTAs 55), 8192 of 16/4 x 64 in bf16 with 4 heads 23 us (without 29.8).
+constexpr int direct_heads(size_t element) { return element == 2 ? 4 : 3; }
+constexpr int direct_ctas(bool codes) { return codes ? 2 : 3; }
+constexpr int direct_heads_bwd(size_t element) { return element == 2 ? 4 : 2; }
 
 struct Params {
     const void *q, *k, *v;                // inputs of the forward pass
@@ -45,6 +52,7 @@ struct Params {
     int heads[3];                         // of q, k and v
     int chunks[3];                        // groups of them
     int lanes, per_token, tokens_per_block;   // lanes of a group; threads of a token
+    int threads;                          // of a CTA
     int items, turned;                    // direct kernels: items of a head, those that turn
     float eps, inv_d;
 };
@@ -77,14 +85,43 @@ __device__ __forceinline__ bool in_cache(const Params &p, long long row) { retur
 
 // Row of the table of token t; as in rope.cu, a position outside it is
 // reported unless the token has no place in the cache.
-__device__ __forceinline__ int position_of(const Params &p, int t, long long row) {
-    int pos = p.positions ? __ldg(p.positions + t) : t % p.seq_len;
+__device__ __forceinline__ int checked_position(const Params &p, int pos, long long row) {
     if ((unsigned)pos >= (unsigned)p.max_pos) {
         if (in_cache(p, row)) atomicExch(p.err, 0x701);
         pos = pos < 0 ? 0 : p.max_pos - 1;
     }
     return pos;
 }
+__device__ __forceinline__ int position_of(const Params &p, int t, long long row) {
+    return checked_position(p, p.positions ? __ldg(p.positions + t) : t % p.seq_len, row);
+}
+// Positions of tokens first, first + stride, ...: each one asked for a token
+// before its use, and looked at when it is used.
+struct Positions {
+    int next, step;
+    __device__ __forceinline__ Positions(const Params &p, int t, int stride, bool wanted) {
+        next = step = 0;
+        if (!wanted) return;
+        if (p.positions) {
+            if (t < p.tokens) next = __ldg(p.positions + t);
+        } else {
+            next = t % p.seq_len;
+            step = stride % p.seq_len;
+        }
+    }
+    // this token's; asks for that of token t
+    __device__ __forceinline__ int advance(const Params &p, int t, bool wanted) {
+        const int pos = next;
+        if (!wanted) return pos;
+        if (p.positions) {
+            if (t < p.tokens) next = __ldg(p.positions + t);
+        } else {
+            next += step;
+            if (next >= p.seq_len) next -= p.seq_len;
+        }
+        return pos;
+    }
+};
 
 // 16 bytes of elements as they lie in memory, and as floats.  WIDE: addresses
 // are multiples of 16 bytes; otherwise of an element.
@@ -236,7 +273,7 @@ norm_rope_kernel(const __grid_constant__ Params p)
     using V = Vec<T, WIDE>;
     constexpr int E = V::E;
     extern __shared__ float exchange[];   // d floats per group
-    const Place x = place_of<kHeads>(p, (int)blockIdx.y * kThreads + (int)threadIdx.x);
+    const Place x = place_of<kHeads>(p, (int)(blockIdx.y * blockDim.x + threadIdx.x));
     if (!x.there) return;
     const int e0 = x.item * E;
     const bool there = e0 < p.d;          // lanes past the head take part in the sums alone
@@ -299,12 +336,13 @@ norm_rope_kernel(const __grid_constant__ Params p)
 
 // Each CTA's part of the weights' gradients: the groups' sums of a column, in
 // the order of the groups.  sums: d floats of each group, at their columns.
+template <int HEADS>
 __device__ __forceinline__ void write_partial(const Params &p, const float *sums) {
-    for (int col = threadIdx.x; col < 2 * p.d; col += kThreads) {
+    for (int col = threadIdx.x; col < 2 * p.d; col += p.threads) {
         const int kind = col >= p.d, e = col - kind * p.d;
         float sum = 0.f;
-        for (int u = 0; u < kThreads; u += p.lanes) {
-            const Place y = place_of<kHeadsBwd>(p, (int)blockIdx.y * kThreads + u);
+        for (int u = 0; u < p.threads; u += p.lanes) {
+            const Place y = place_of<HEADS>(p, (int)blockIdx.y * p.threads + u);
             if (y.there && y.kind == kind) sum += sums[u / p.lanes * p.d + e];
         }
         p.partial[((long long)blockIdx.y * gridDim.x + blockIdx.x) * 2 * p.d + col] = sum;
@@ -320,7 +358,7 @@ norm_rope_bwd_kernel(const __grid_constant__ Params p)
     using V = Vec<T, WIDE>;
     constexpr int E = V::E;
     extern __shared__ float exchange[];   // d floats per group
-    const Place x = place_of<kHeadsBwd>(p, (int)blockIdx.y * kThreads + (int)threadIdx.x);
+    const Place x = place_of<kHeadsBwd>(p, (int)(blockIdx.y * blockDim.x + threadIdx.x));
     const int e0 = x.item * E;
     const bool there = x.there && e0 < p.d;
     float *row_buf = exchange + threadIdx.x / p.lanes * p.d;
@@ -385,313 +423,375 @@ norm_rope_bwd_kernel(const __grid_constant__ Params p)
         for (int i = 0; i < E; i++) row_buf[e0 + i] = dw[i];
     }
     __syncthreads();
-    write_partial(p, exchange);
+    write_partial<kHeadsBwd>(p, exchange);
 }
 
 // ---------------------------------------------------------------------------
 // The direct kernels: both elements of every pair in one lane, so nothing is
-// exchanged but the sums.  Rotation in halves: an item is 16 bytes of the first
-// half and the 16 bytes rot/2 behind them, or 16 bytes that do not turn;
-// interleaved: 16 bytes.
+// exchanged but the sums.  A lane has four elements of a head (rotation
+// interleaved), or four of the first half and the four rot/2 behind them, or
+// four that do not turn; the arithmetic is in packed pairs of floats.
 // ---------------------------------------------------------------------------
-template <bool PAIRS, int E> struct Item {
-    static constexpr int C = PAIRS ? E / 2 : E;               // pairs of an item
+using sm100::f2;
+using sm100::f2_split;
+using sm100::fma2;
+using sm100::mul2;
+
+// Four elements as they lie in memory, and as two packed pairs of floats.
+template <typename T> struct Four;
+template <> struct Four<float> {
+    float4 raw;
+    __device__ __forceinline__ void zero() { raw = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ void load(const float *p) { raw = *reinterpret_cast<const float4 *>(p); }
+    __device__ __forceinline__ void store(float *p) const { *reinterpret_cast<float4 *>(p) = raw; }
+    __device__ __forceinline__ void get(uint64_t (&x)[2]) const { x[0] = f2(raw.x, raw.y); x[1] = f2(raw.z, raw.w); }
+    __device__ __forceinline__ void set(const uint64_t (&x)[2]) { f2_split(x[0], raw.x, raw.y); f2_split(x[1], raw.z, raw.w); }
+};
+template <> struct Four<__nv_bfloat16> {
+    uint2 raw;
+    __device__ __forceinline__ void zero() { raw = make_uint2(0, 0); }
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { raw = *reinterpret_cast<const uint2 *>(p); }
+    __device__ __forceinline__ void store(__nv_bfloat16 *p) const { *reinterpret_cast<uint2 *>(p) = raw; }
+    __device__ __forceinline__ void get(uint64_t (&x)[2]) const {
+        x[0] = f2(__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u));
+        x[1] = f2(__uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u));
+    }
+    __device__ __forceinline__ void set(const uint64_t (&x)[2]) {
+        float a, b;
+        f2_split(x[0], a, b);
+        raw.x = sm100::pack_bf16(a, b);
+        f2_split(x[1], a, b);
+        raw.y = sm100::pack_bf16(a, b);
+    }
+};
+__device__ __forceinline__ uint64_t swapped(uint64_t x) {
+    float a, b;
+    f2_split(x, a, b);
+    return f2(b, a);
+}
+__device__ __forceinline__ float sum_of(uint64_t x) {
+    float a, b;
+    f2_split(x, a, b);
+    return a + b;
+}
+// 1 / sqrt(x): the approximation and one step of Newton's, within 2^-23.  (The
+// rounded one is some 20 instructions.)  Of 0 and infinity as it is.
+__device__ __forceinline__ float inverse_root(float x) {
+    const float r = rsqrtf(x), better = r * fmaf(-0.5f * x * r, r, 1.5f);
+    return x > 0.f && x < INFINITY ? better : r;
+}
+
+// An item's place in the head, and cosines and sines of its pairs, packed:
+// interleaved (c0, c0), (c1, c1) and (-s0, s0), (-s1, s1); in halves c0 c1,
+// c2 c3 and s0 s1, s2 s3.
+template <bool PAIRS> struct Item {
     int off;                              // of its first element in the head
     bool turns;
     __device__ __forceinline__ Item(const Params &p, int item) {
         turns = item < p.turned;
-        off = PAIRS || turns ? item * E : p.rot + (item - p.turned) * E;
+        off = PAIRS || turns ? item * 4 : p.rot + (item - p.turned) * 4;
     }
-    // cosines and sines of its pairs
-    __device__ __forceinline__ void angles(const Params &p, int pos, int item, float (&c)[C], float (&s)[C]) const {
-        const float4 *row = reinterpret_cast<const float4 *>(p.table + ((long long)pos * (p.rot / 2) + item * C) * 2);
-#pragma unroll
-        for (int i = 0; i < C; i += 2) {
-            const float4 x = __ldg(row + i / 2);
-            c[i] = x.x; s[i] = x.y; c[i + 1] = x.z; s[i + 1] = x.w;
+    __device__ __forceinline__ void angles(const Params &p, int pos, int item, uint64_t (&c)[2], uint64_t (&s)[2]) const {
+        const float4 *row = reinterpret_cast<const float4 *>(p.table + ((long long)pos * (p.rot / 2) + item * (PAIRS ? 2 : 4)) * 2);
+        const float4 x = __ldg(row);
+        if constexpr (PAIRS) {
+            c[0] = f2(x.x, x.x); s[0] = f2(-x.y, x.y);
+            c[1] = f2(x.z, x.z); s[1] = f2(-x.w, x.w);
+        } else {
+            const float4 y = __ldg(row + 1);
+            c[0] = f2(x.x, x.z); s[0] = f2(x.y, x.w);
+            c[1] = f2(y.x, y.z); s[1] = f2(y.y, y.w);
         }
     }
 };
+__device__ __forceinline__ uint64_t negated(uint64_t x) { return x ^ 0x8000000080000000ull; }
 
-template <typename T, bool PAIRS, bool CODES>
-__global__ void __launch_bounds__(kThreads, direct_ctas(PAIRS))
+// Weights of both kinds in shared memory (by all threads, before a barrier).
+__device__ __forceinline__ void bring_weights(const Params &p, float (&weights)[2][128]) {
+    for (int i = threadIdx.x; i < 2 * p.d; i += (int)blockDim.x) {
+        const int kind = i >= p.d, e = i - kind * p.d;
+        const float *from = kind ? p.k_weight : p.q_weight;
+        weights[kind][e] = from ? __ldg(from + e) : 1.f;
+    }
+}
+__device__ __forceinline__ void pairs_of(const float *p, uint64_t (&x)[2]) {
+    const float4 v = *reinterpret_cast<const float4 *>(p);
+    x[0] = f2(v.x, v.y);
+    x[1] = f2(v.z, v.w);
+}
+
+template <typename T, int D, bool PAIRS, bool CODES>
+__global__ void __launch_bounds__(kThreads, direct_ctas(CODES))
 norm_rope_direct_kernel(const __grid_constant__ Params p)
 {
     pdl_begin();                          // launched by launch_pdl
-    using V = Vec<T, true>;
-    constexpr int E = V::E, C = Item<PAIRS, E>::C;
-    __shared__ float weights[2][128];
-    for (int i = threadIdx.x; i < 2 * p.d; i += kThreads) {
-        const float *from = i < p.d ? p.q_weight : p.k_weight;
-        weights[i >= p.d][i < p.d ? i : i - p.d] = from ? __ldg(from + (i < p.d ? i : i - p.d)) : 1.f;
-    }
+    constexpr int H = direct_heads(sizeof(T));
+    __shared__ __align__(16) float weights[2][128];
+    bring_weights(p, weights);
     __syncthreads();
-    const Place x = place_of<kHeads>(p, (int)blockIdx.y * kThreads + (int)threadIdx.x);
+    const Place x = place_of<H>(p, (int)(blockIdx.y * blockDim.x + threadIdx.x));
     if (!x.there) return;
-    const Item<PAIRS, E> item(p, x.item);
-    const bool there = x.item < p.items, turns = item.turns && x.kind < 2;
-    const int half = p.rot / 2;
-    const float *weight = weights[x.kind & 1] + (there ? item.off : 0), *weight2 = weight + (!PAIRS && item.turns ? half : 0);
-
-    const int in_row = x.head * p.d + item.off;
-    const T *from = static_cast<const T *>(x.kind == 0 ? p.q : x.kind == 1 ? p.k : p.v) + in_row;
-    const long long from_stride = x.kind == 0 ? p.q_stride : x.kind == 1 ? p.k_stride : p.v_stride;
-    const long long to_stride = x.kind == 0 ? p.qo_stride : p.ko_stride;
-    void *to = x.kind == 0 ? p.q_out : x.kind == 1 ? p.k_out : p.v_out;
-    const bool second = !PAIRS && item.turns;                // a second vector (V's heads are cut up alike)
+    const Item<PAIRS> item(p, x.item);
+    const bool there = x.item < p.items, turns = item.turns && x.kind < 2 && there;
+    const bool second = !PAIRS && item.turns && there;       // a second vector (V's heads are cut up alike)
+    const int half = p.rot / 2, n = there ? x.n : 0;
 
     const int stride = (int)gridDim.x * p.tokens_per_block;
     int t = (int)blockIdx.x * p.tokens_per_block + x.token;
-    auto slot_of = [&](int t) { return p.slots && t < p.tokens ? __ldg(p.slots + t) : (long long)t; };
-    auto pos_of = [&](int t, long long slot) { return turns && there && t < p.tokens ? position_of(p, t, slot) : 0; };
-    long long next_slot = slot_of(t);
-    int next_pos = pos_of(t, next_slot);
-    for (; t < p.tokens; t += stride) {
-        const long long slot = next_slot;
-        const int pos = next_pos;
-        next_slot = slot_of(t + stride);
-        next_pos = pos_of(t + stride, next_slot);
-        if (x.kind > 0 && !in_cache(p, slot)) continue;       // (the whole group)
-        V a[kHeads], b[kHeads];
-        const T *src = from + t * from_stride;
+    const int in_row = x.head * D + item.off;
+    const long long from_stride = x.kind == 0 ? p.q_stride : x.kind == 1 ? p.k_stride : p.v_stride;
+    const long long to_stride = x.kind == 0 ? p.qo_stride : p.ko_stride;
+    const T *src = static_cast<const T *>(x.kind == 0 ? p.q : x.kind == 1 ? p.k : p.v) + in_row + t * from_stride;
+    void *to = x.kind == 0 ? p.q_out : x.kind == 1 ? p.k_out : p.v_out;
+    Positions positions(p, t, stride, turns);
+    long long next_slot = p.slots && t < p.tokens ? __ldg(p.slots + t) : 0;
+    for (; t < p.tokens; t += stride, src += stride * from_stride) {
+        const long long slot = p.slots ? next_slot : t;
+        const bool skip = x.kind > 0 && !in_cache(p, slot);   // (the whole group)
+        Four<T> a[H], b[H];
 #pragma unroll
-        for (int h = 0; h < kHeads; h++) {
-            a[h].raw = b[h].raw = make_uint4(0, 0, 0, 0);
-            if (h < x.n && there) {
-                a[h].load(src + h * p.d);
-                if (second) b[h].load(src + h * p.d + half);
+        for (int h = 0; h < H; h++) {
+            a[h].zero();
+            b[h].zero();
+            if (h < n && !skip) {
+                a[h].load(src + h * D);
+                if (second) b[h].load(src + h * D + half);
             }
         }
+        if (p.slots && t + stride < p.tokens) next_slot = __ldg(p.slots + t + stride);
+        const int pos = positions.advance(p, t + stride, turns);
+        if (skip) continue;
         const long long at = (x.kind == 0 ? (long long)t : slot) * to_stride + in_row;
+        T *dst = static_cast<T *>(to) + at;
         if (!CODES && x.kind == 2) {
 #pragma unroll
-            for (int h = 0; h < kHeads; h++)
-                if (h < x.n && there) {
-                    a[h].store(static_cast<T *>(to) + at + h * p.d);
-                    if (second) b[h].store(static_cast<T *>(to) + at + h * p.d + half);
+            for (int h = 0; h < H; h++)
+                if (h < n) {
+                    a[h].store(dst + h * D);
+                    if (second) b[h].store(dst + h * D + half);
                 }
             continue;
         }
-        // a pair (u, v) becomes r (u wc - v vs, v vc + u ws): the weights go into the angles, for all heads
-        float wc[C], ws[C], vc[C], vs[C];
-        if (x.kind < 2) {
-            float c[C], s[C];
-#pragma unroll
-            for (int i = 0; i < C; i++) { c[i] = 1.f; s[i] = 0.f; }
-            if (turns && there) item.angles(p, pos, x.item, c, s);
-#pragma unroll
-            for (int i = 0; i < C; i++) {
-                const float w = weight[PAIRS ? 2 * i : i], v = PAIRS ? weight[2 * i + 1] : weight2[i];
-                wc[i] = w * c[i]; ws[i] = w * s[i]; vc[i] = v * c[i]; vs[i] = v * s[i];
-            }
-        }
-        float r[kHeads];
+        float r[H];
+        // The weights go into the angles, for all heads: in halves (u, v) becomes r (u wc - v vs, v vc + u ws), interleaved
+        // (u, v) becomes r ((u, v) (wc, vc) + (v, u) (-vs, ws)).
+        uint64_t wc[2], vs[2], vc[2], ws[2];
         if (x.kind < 2) {
 #pragma unroll
-            for (int h = 0; h < kHeads; h++) {
-                float u[E], v[E];
+            for (int h = 0; h < H; h++) {
+                uint64_t u[2], sum;
                 a[h].get(u);
-                r[h] = 0.f;
-#pragma unroll
-                for (int i = 0; i < E; i++) r[h] = fmaf(u[i], u[i], r[h]);
+                sum = fma2(u[1], u[1], mul2(u[0], u[0]));
                 if constexpr (!PAIRS) {
-                    b[h].get(v);
+                    b[h].get(u);
+                    sum = fma2(u[1], u[1], fma2(u[0], u[0], sum));
+                }
+                r[h] = sum_of(sum);
+            }
+            uint64_t c[2] = {f2(1.f, 1.f), f2(1.f, 1.f)}, s[2] = {0, 0};
+            if (turns) item.angles(p, checked_position(p, pos, slot), x.item, c, s);
+            const float *weight = weights[x.kind] + (there ? item.off : 0);
+            uint64_t w[2];
+            pairs_of(weight, w);
+            if constexpr (PAIRS) {
 #pragma unroll
-                    for (int i = 0; i < E; i++) r[h] = fmaf(v[i], v[i], r[h]);
+                for (int i = 0; i < 2; i++) { wc[i] = mul2(w[i], c[i]); vs[i] = mul2(swapped(w[i]), s[i]); }
+            } else {
+                uint64_t v[2] = {0, 0};
+                if (second) pairs_of(weight + half, v);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    wc[i] = mul2(w[i], c[i]); ws[i] = mul2(w[i], s[i]);
+                    vc[i] = mul2(v[i], c[i]); vs[i] = negated(mul2(v[i], s[i]));
                 }
             }
             group_sums(r, p, x.mask);
 #pragma unroll
-            for (int h = 0; h < kHeads; h++) r[h] = __frsqrt_rn(fmaf(r[h], p.inv_d, p.eps));
+            for (int h = 0; h < H; h++) r[h] = inverse_root(fmaf(r[h], p.inv_d, p.eps));
         }
 #pragma unroll
-        for (int h = 0; h < kHeads; h++) {
-            if (h >= x.n) break;
-            float u[E], v[E];
+        for (int h = 0; h < H; h++) {
+            uint64_t u[2], v[2];
             a[h].get(u);
             b[h].get(v);
             if (x.kind < 2) {
+                const uint64_t rr = f2(r[h], r[h]);
                 if constexpr (PAIRS) {
 #pragma unroll
-                    for (int i = 0; i < C; i++) {
-                        const float y = u[2 * i], z = u[2 * i + 1];
-                        u[2 * i] = r[h] * (turns ? fmaf(y, wc[i], -(z * vs[i])) : y * wc[i]);
-                        u[2 * i + 1] = r[h] * (turns ? fmaf(z, vc[i], y * ws[i]) : z * vc[i]);
+                    for (int i = 0; i < 2; i++) {
+                        const uint64_t y = mul2(u[i], wc[i]);
+                        u[i] = mul2(turns ? fma2(swapped(u[i]), vs[i], y) : y, rr);
                     }
                 } else {                  // (what does not turn has no v, and sines of 0)
 #pragma unroll
-                    for (int i = 0; i < C; i++) {
-                        const float y = u[i], z = v[i];
-                        u[i] = r[h] * fmaf(y, wc[i], -(z * vs[i]));
-                        v[i] = r[h] * fmaf(z, vc[i], y * ws[i]);
+                    for (int i = 0; i < 2; i++) {
+                        const uint64_t y = u[i], z = v[i];
+                        u[i] = mul2(fma2(z, vs[i], mul2(y, wc[i])), rr);
+                        v[i] = mul2(fma2(y, ws[i], mul2(z, vc[i])), rr);
                     }
                 }
             }
-            if (CODES && x.kind > 0) {
-                float amax = 1e-8f;
+            if constexpr (CODES) {
+                if (x.kind > 0) {
+                    float y[4], z[4], amax = 1e-8f;
 #pragma unroll
-                for (int i = 0; i < E; i++) amax = fmaxf(amax, fabsf(u[i]));
-                if (second) {
+                    for (int i = 0; i < 2; i++) {
+                        f2_split(u[i], y[2 * i], y[2 * i + 1]);
+                        f2_split(v[i], z[2 * i], z[2 * i + 1]);
+                    }
 #pragma unroll
-                    for (int i = 0; i < E; i++) amax = fmaxf(amax, fabsf(v[i]));
+                    for (int i = 0; i < 4; i++) amax = fmaxf(amax, fmaxf(fabsf(y[i]), second ? fabsf(z[i]) : 0.f));
+                    const float scale = __fdiv_rn(group_max(amax, p, x.mask), 127.0f), inv = __fdiv_rn(1.0f, scale);
+                    if (h >= n) continue;
+                    int8_t *codes = static_cast<int8_t *>(to) + at + h * D;
+                    *reinterpret_cast<uint32_t *>(codes) = codes_of(y, inv);
+                    if (second) *reinterpret_cast<uint32_t *>(codes + half) = codes_of(z, inv);
+                    if (x.item == 0) (x.kind == 1 ? p.kscale : p.vscale)[slot * p.heads[x.kind] + x.head + h] = scale;
+                    continue;
                 }
-                const float scale = __fdiv_rn(group_max(amax, p, x.mask), 127.0f), inv = __fdiv_rn(1.0f, scale);
-                if constexpr (CODES) {
-                    int8_t *dst = static_cast<int8_t *>(to) + at + h * p.d;
-                    if (there) *reinterpret_cast<uint32_t *>(dst) = codes_of(u, inv);
-                    if (there && second) *reinterpret_cast<uint32_t *>(dst + half) = codes_of(v, inv);
-                }
-                if (x.item == 0) (x.kind == 1 ? p.kscale : p.vscale)[slot * p.heads[x.kind] + x.head + h] = scale;
-            } else if (there) {
+            }
+            if (h < n) {
                 a[h].set(u);
-                a[h].store(static_cast<T *>(to) + at + h * p.d);
+                a[h].store(dst + h * D);
                 if (second) {
                     b[h].set(v);
-                    b[h].store(static_cast<T *>(to) + at + h * p.d + half);
+                    b[h].store(dst + h * D + half);
                 }
             }
         }
     }
 }
 
-template <typename T, bool PAIRS>
-__global__ void __launch_bounds__(kThreads, 2)
+template <typename T, int D, bool PAIRS>
+__global__ void __launch_bounds__(kThreads, kCtas)
 norm_rope_bwd_direct_kernel(const __grid_constant__ Params p)
 {
     pdl_begin();                          // launched by launch_pdl
-    using V = Vec<T, true>;
-    constexpr int E = V::E, C = Item<PAIRS, E>::C;
+    constexpr int H = direct_heads_bwd(sizeof(T));
     extern __shared__ float sums[];       // d floats per group
-    __shared__ float weights[2][128];
-    for (int i = threadIdx.x; i < 2 * p.d; i += kThreads) {
-        const float *from = i < p.d ? p.q_weight : p.k_weight;
-        weights[i >= p.d][i < p.d ? i : i - p.d] = from ? __ldg(from + (i < p.d ? i : i - p.d)) : 1.f;
-    }
+    __shared__ __align__(16) float weights[2][128];
+    bring_weights(p, weights);
     __syncthreads();
-    const Place x = place_of<kHeadsBwd>(p, (int)blockIdx.y * kThreads + (int)threadIdx.x);
-    const Item<PAIRS, E> item(p, x.item);
-    const bool there = x.there && x.item < p.items, second = !PAIRS && item.turns;
-    const int half = p.rot / 2;
-    const float *weight = weights[x.kind & 1] + (there ? item.off : 0), *weight2 = weight + (second ? half : 0);
-    const int in_row = x.head * p.d + item.off;
-    const T *from = static_cast<const T *>(x.kind == 0 ? p.q : p.k) + in_row;
-    const T *grad = static_cast<const T *>(x.kind == 0 ? p.dq_out : p.dk_out) + in_row;
-    T *to = static_cast<T *>(x.kind == 0 ? p.dq : p.dk) + in_row;
-    const long long from_stride = x.kind == 0 ? p.q_stride : p.k_stride, grad_stride = x.kind == 0 ? p.qo_stride : p.ko_stride;
-    const int last = x.there ? p.tokens : 0;
-    float dw[E], dv[E];                   // of the item's first and second vector
-#pragma unroll
-    for (int i = 0; i < E; i++) dw[i] = dv[i] = 0.f;
-
-    const int stride = (int)gridDim.x * p.tokens_per_block;
+    const Place x = place_of<H>(p, (int)(blockIdx.y * blockDim.x + threadIdx.x));
+    const Item<PAIRS> item(p, x.item);
+    const bool there = x.there && x.item < p.items, turns = item.turns && there, second = !PAIRS && turns;
+    const int half = p.rot / 2, n = there ? x.n : 0;
+    const int last = x.there ? p.tokens : 0, stride = (int)gridDim.x * p.tokens_per_block;
     int t = (int)blockIdx.x * p.tokens_per_block + x.token;
-    auto pos_of = [&](int t) { return item.turns && there && t < last ? position_of(p, t, t) : 0; };
-    int next_pos = pos_of(t);
-    for (; t < last; t += stride) {
-        const int pos = next_pos;
-        next_pos = pos_of(t + stride);
-        V xa[kHeadsBwd], xb[kHeadsBwd], ga[kHeadsBwd], gb[kHeadsBwd];
+    const int in_row = x.head * D + item.off;
+    const long long from_stride = x.kind == 0 ? p.q_stride : p.k_stride, grad_stride = x.kind == 0 ? p.qo_stride : p.ko_stride;
+    const T *from = static_cast<const T *>(x.kind == 0 ? p.q : p.k) + in_row + t * from_stride;
+    const T *grad = static_cast<const T *>(x.kind == 0 ? p.dq_out : p.dk_out) + in_row + t * grad_stride;
+    T *to = static_cast<T *>(x.kind == 0 ? p.dq : p.dk) + in_row + t * from_stride;
+    uint64_t w[2], v[2] = {0, 0};         // weights of the two vectors
+    const float *weight = weights[x.kind & 1] + (there ? item.off : 0);
+    pairs_of(weight, w);
+    if (second) pairs_of(weight + half, v);
+    uint64_t dw[2] = {0, 0}, dv[2] = {0, 0};
+
+    // the next token's loads are on their way while this one's are worked on
+    Four<T> next_xa[H], next_xb[H], next_ga[H], next_gb[H];
+    Positions positions(p, t, stride, turns && x.there);
+    auto bring = [&](int t) {
 #pragma unroll
-        for (int h = 0; h < kHeadsBwd; h++) {
-            xa[h].raw = xb[h].raw = ga[h].raw = gb[h].raw = make_uint4(0, 0, 0, 0);
-            if (h < x.n && there) {
-                xa[h].load(from + t * from_stride + h * p.d);
-                ga[h].load(grad + t * grad_stride + h * p.d);
+        for (int h = 0; h < H; h++) {
+            next_xa[h].zero(); next_xb[h].zero(); next_ga[h].zero(); next_gb[h].zero();
+            if (h < n && t < last) {
+                next_xa[h].load(from + h * D);
+                next_ga[h].load(grad + h * D);
                 if (second) {
-                    xb[h].load(from + t * from_stride + h * p.d + half);
-                    gb[h].load(grad + t * grad_stride + h * p.d + half);
+                    next_xb[h].load(from + h * D + half);
+                    next_gb[h].load(grad + h * D + half);
                 }
             }
         }
-        float c[C], s[C];
+    };
+    bring(t);
+    for (; t < last; t += stride, to += stride * from_stride) {
+        Four<T> xa[H], xb[H], ga[H], gb[H];
 #pragma unroll
-        for (int i = 0; i < C; i++) { c[i] = 1.f; s[i] = 0.f; }
-        if (item.turns && there) item.angles(p, pos, x.item, c, s);
-        // the gradient turned back: (g c + g' s, g' c - g s)
-        auto back = [&](const V &ra, const V &rb, float (&g)[E], float (&f)[E]) {
-            ra.get(g);
+        for (int h = 0; h < H; h++) { xa[h] = next_xa[h]; xb[h] = next_xb[h]; ga[h] = next_ga[h]; gb[h] = next_gb[h]; }
+        from += stride * from_stride;
+        grad += stride * grad_stride;
+        const int pos = positions.advance(p, t + stride, turns);
+        bring(t + stride);
+        uint64_t c[2] = {f2(1.f, 1.f), f2(1.f, 1.f)}, s[2] = {0, 0};
+        if (turns) item.angles(p, checked_position(p, pos, t), x.item, c, s);
+        // the gradient turned back: in halves (g c + f s, f c - g s), interleaved (g, f) c + (f, g) (s, -s)
+        auto back = [&](int h, uint64_t (&g)[2], uint64_t (&f)[2]) {
+            ga[h].get(g);
             if constexpr (PAIRS) {
-                if (item.turns) {
+                if (turns) {
 #pragma unroll
-                    for (int i = 0; i < C; i++) {
-                        const float y = g[2 * i], z = g[2 * i + 1];
-                        g[2 * i] = fmaf(y, c[i], z * s[i]);
-                        g[2 * i + 1] = fmaf(z, c[i], -(y * s[i]));
-                    }
+                    for (int i = 0; i < 2; i++) g[i] = fma2(swapped(g[i]), negated(s[i]), mul2(g[i], c[i]));
                 }
             } else {
-                rb.get(f);
+                gb[h].get(f);
 #pragma unroll
-                for (int i = 0; i < C; i++) {
-                    const float y = g[i], z = f[i];
-                    g[i] = fmaf(y, c[i], z * s[i]);
-                    f[i] = fmaf(z, c[i], -(y * s[i]));
+                for (int i = 0; i < 2; i++) {
+                    const uint64_t y = g[i], z = f[i];
+                    g[i] = fma2(z, s[i], mul2(y, c[i]));
+                    f[i] = fma2(y, negated(s[i]), mul2(z, c[i]));
                 }
             }
         };
-        float sq[2 * kHeadsBwd];          // squares; products with the gradient
+        float sq[2 * H];          // squares; products with the gradient
 #pragma unroll
-        for (int h = 0; h < kHeadsBwd; h++) {
-            float u[E], v[E], g[E], f[E];
-            back(ga[h], gb[h], g, f);
+        for (int h = 0; h < H; h++) {
+            uint64_t g[2], f[2], u[2];
+            back(h, g, f);
             xa[h].get(u);
-            float square = 0.f, dot = 0.f;
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                square = fmaf(u[i], u[i], square);
-                dot = fmaf(g[i] * weight[i], u[i], dot);
+            uint64_t square = fma2(u[1], u[1], mul2(u[0], u[0]));
+            uint64_t dot = fma2(mul2(g[1], w[1]), u[1], mul2(mul2(g[0], w[0]), u[0]));
+            if (second) {
+                xb[h].get(u);
+                square = fma2(u[1], u[1], fma2(u[0], u[0], square));
+                dot = fma2(mul2(f[1], v[1]), u[1], fma2(mul2(f[0], v[0]), u[0], dot));
             }
-            if constexpr (!PAIRS) {
-                xb[h].get(v);
-                if (second) {
-#pragma unroll
-                    for (int i = 0; i < E; i++) {
-                        square = fmaf(v[i], v[i], square);
-                        dot = fmaf(f[i] * weight2[i], v[i], dot);
-                    }
-                }
-            }
-            sq[2 * h] = square;
-            sq[2 * h + 1] = dot;
+            sq[2 * h] = sum_of(square);
+            sq[2 * h + 1] = sum_of(dot);
         }
         group_sums(sq, p, x.mask);
 #pragma unroll
-        for (int h = 0; h < kHeadsBwd; h++) {
-            if (h >= x.n || !there) break;
-            const float r = __frsqrt_rn(fmaf(sq[2 * h], p.inv_d, p.eps)), k = r * r * (sq[2 * h + 1] * p.inv_d);
-            float u[E], v[E], g[E], f[E];
-            back(ga[h], gb[h], g, f);
+        for (int h = 0; h < H; h++) {
+            const float r = inverse_root(fmaf(sq[2 * h], p.inv_d, p.eps)), k = -r * r * (sq[2 * h + 1] * p.inv_d);
+            if (h >= n) continue;
+            const uint64_t rr = f2(r, r), kk = f2(k, k);
+            uint64_t g[2], f[2], u[2];
+            back(h, g, f);
             xa[h].get(u);
 #pragma unroll
-            for (int i = 0; i < E; i++) {
-                dw[i] = fmaf(g[i], u[i] * r, dw[i]);
-                u[i] = r * fmaf(u[i], -k, g[i] * weight[i]);
+            for (int i = 0; i < 2; i++) {
+                dw[i] = fma2(g[i], mul2(u[i], rr), dw[i]);
+                u[i] = mul2(fma2(u[i], kk, mul2(g[i], w[i])), rr);
             }
             xa[h].set(u);
-            xa[h].store(to + t * from_stride + h * p.d);
+            xa[h].store(to + h * D);
             if (second) {
-                xb[h].get(v);
+                xb[h].get(u);
 #pragma unroll
-                for (int i = 0; i < E; i++) {
-                    dv[i] = fmaf(f[i], v[i] * r, dv[i]);
-                    v[i] = r * fmaf(v[i], -k, f[i] * weight2[i]);
+                for (int i = 0; i < 2; i++) {
+                    dv[i] = fma2(f[i], mul2(u[i], rr), dv[i]);
+                    u[i] = mul2(fma2(u[i], kk, mul2(f[i], v[i])), rr);
                 }
-                xb[h].set(v);
-                xb[h].store(to + t * from_stride + h * p.d + half);
+                xb[h].set(u);
+                xb[h].store(to + h * D + half);
             }
         }
     }
     if (!p.partial) return;
     if (there) {
-        float *mine = sums + threadIdx.x / p.lanes * p.d + item.off;
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-            mine[i] = dw[i];
-            if (second) mine[half + i] = dv[i];
+        float *mine = sums + threadIdx.x / p.lanes * D + item.off;
+        Four<float> out;
+        out.set(dw);
+        out.store(mine);
+        if (second) {
+            out.set(dv);
+            out.store(mine + half);
         }
     }
     __syncthreads();
-    write_partial(p, sums);
+    write_partial<H>(p, sums);
 }
 
 // Columns of the CTAs' parts, 32 to a CTA, summed in an order that the sizes alone decide.
@@ -747,7 +847,8 @@ Params norm_params(const attn_rope_shape *s, const attn_head_norm *n, const floa
 }
 
 // Divides a token's row into groups of `heads` heads of `vec` elements a lane;
-// CTAs that are resident, which stride over the tokens (.y: slices of a row).
+// CTAs of up to kThreads that are resident, which stride over the tokens
+// (.y: slices of a row).
 dim3 divide(Params &p, bool direct, int vec, int heads, int ctas) {
     p.turned = p.interleaved ? p.rot / vec : p.rot / 2 / vec;
     p.items = direct && !p.interleaved ? p.turned + (p.d - p.rot) / vec : p.d / vec;
@@ -757,29 +858,56 @@ dim3 divide(Params &p, bool direct, int vec, int heads, int ctas) {
     while (p.lanes < p.items) p.lanes *= 2;
     p.per_token = groups * p.lanes;
     p.tokens_per_block = std::max(1, kThreads / p.per_token);
-    const int slices = (p.per_token + kThreads - 1) / kThreads;
+    p.threads = std::min((p.per_token * p.tokens_per_block + 31) / 32 * 32, kThreads);
+    const int slices = (p.per_token + p.threads - 1) / p.threads;
     const int steps = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
-    return dim3(std::max(1, std::min(steps, std::max(1, sm_count_here() * ctas / slices))), slices);
+    return dim3(std::max(1, std::min(steps, std::max(1, sm_count_here() * (ctas * kThreads / p.threads) / slices))), slices);
 }
 
 bool even(const void *ptr) { return ((uintptr_t)ptr & 15) == 0; }
-// Both elements of every pair in one lane's vectors?
-bool direct_fits(const Params &p, bool wide, int vec) { return wide && even(p.table) && p.rot % (p.interleaved ? vec : 2 * vec) == 0; }
+// Addresses and strides that fours of T, and both elements of every pair in one lane, ask for?
+template <typename T, size_t N>
+bool direct_fits(const Params &p, const void *const (&tensors)[N], const long long (&strides)[5]) {
+    for (const void *x : tensors)
+        if ((uintptr_t)x % (4 * sizeof(T))) return false;
+    for (long long x : strides)
+        if (x % 4) return false;
+    return even(p.table) && p.rot % (p.interleaved ? 4 : 8) == 0;
+}
+
+template <typename T, int D, bool CODES>
+cudaError_t launch_direct(const Params &p, dim3 grid, cudaStream_t s) {
+    using namespace attn::nrope;
+    return launch_pdl(p.interleaved ? norm_rope_direct_kernel<T, D, true, CODES> : norm_rope_direct_kernel<T, D, false, CODES>, grid,
+                      dim3(p.threads), 0, s, p);
+}
+template <typename T, int D>
+cudaError_t launch_bwd_direct(const Params &p, dim3 grid, size_t smem, cudaStream_t s) {
+    using namespace attn::nrope;
+    return launch_pdl(p.interleaved ? norm_rope_bwd_direct_kernel<T, D, true> : norm_rope_bwd_direct_kernel<T, D, false>, grid,
+                      dim3(p.threads), smem, s, p);
+}
 
 template <typename T, bool CODES>
 int launch_forward(Params p, cudaStream_t s) {
     using namespace attn::nrope;
     constexpr int W = 16 / (int)sizeof(T);
-    const bool wide = even(p.q) && even(p.k) && even(p.v) && even(p.q_out) && even(p.k_out) && even(p.v_out) && p.q_stride % W == 0 &&
-                      p.k_stride % W == 0 && p.v_stride % W == 0 && p.qo_stride % W == 0 && p.ko_stride % W == 0;
-    const bool direct = direct_fits(p, wide, W);
-    const dim3 grid = divide(p, direct, W, kHeads, direct ? direct_ctas(p.interleaved) : kCtas);
-    if (direct)
-        return check_pdl(launch_pdl(p.interleaved ? norm_rope_direct_kernel<T, true, CODES> : norm_rope_direct_kernel<T, false, CODES>, grid,
-                                    dim3(kThreads), 0, s, p),
+    const void *const tensors[] = {p.q, p.k, p.v, p.q_out, p.k_out, p.v_out};
+    const long long strides[] = {p.q_stride, p.k_stride, p.v_stride, p.qo_stride, p.ko_stride};
+    if (direct_fits<T>(p, tensors, strides)) {
+        const dim3 grid = divide(p, true, 4, direct_heads(sizeof(T)), direct_ctas(CODES));
+        return check_pdl(p.d == 32   ? launch_direct<T, 32, CODES>(p, grid, s)
+                         : p.d == 64 ? launch_direct<T, 64, CODES>(p, grid, s)
+                         : p.d == 96 ? launch_direct<T, 96, CODES>(p, grid, s)
+                                     : launch_direct<T, 128, CODES>(p, grid, s),
                          "norm_rope_direct_kernel");
-    const size_t smem = (size_t)kThreads / p.lanes * p.d * 4;
-    return check_pdl(launch_pdl(wide ? norm_rope_kernel<T, true, CODES> : norm_rope_kernel<T, false, CODES>, grid, dim3(kThreads), smem, s, p),
+    }
+    bool wide = true;
+    for (const void *x : tensors) wide = wide && even(x);
+    for (long long x : strides) wide = wide && x % W == 0;
+    const dim3 grid = divide(p, false, W, kHeads, kCtas);
+    const size_t smem = (size_t)p.threads / p.lanes * p.d * 4;
+    return check_pdl(launch_pdl(wide ? norm_rope_kernel<T, true, CODES> : norm_rope_kernel<T, false, CODES>, grid, dim3(p.threads), smem, s, p),
                      "norm_rope_kernel");
 }
 
@@ -788,17 +916,22 @@ template <typename T>
 int launch_backward(Params p, int *parts, cudaStream_t s) {
     using namespace attn::nrope;
     constexpr int W = 16 / (int)sizeof(T);
-    const bool wide = even(p.q) && even(p.k) && even(p.dq_out) && even(p.dk_out) && even(p.dq) && even(p.dk) && p.q_stride % W == 0 &&
-                      p.k_stride % W == 0 && p.qo_stride % W == 0 && p.ko_stride % W == 0;
-    const bool direct = direct_fits(p, wide, W);
-    const dim3 grid = divide(p, direct, W, kHeadsBwd, kCtas);
+    const void *const tensors[] = {p.q, p.k, p.dq_out, p.dk_out, p.dq, p.dk};
+    const long long strides[] = {p.q_stride, p.k_stride, 0, p.qo_stride, p.ko_stride};
+    const bool direct = direct_fits<T>(p, tensors, strides);
+    const dim3 grid = divide(p, direct, direct ? 4 : W, direct ? direct_heads_bwd(sizeof(T)) : kHeadsBwd, kCtas);
     *parts = (int)(grid.x * grid.y);
-    const size_t smem = (size_t)kThreads / p.lanes * p.d * 4;
+    const size_t smem = (size_t)p.threads / p.lanes * p.d * 4;
     if (direct)
-        return check_pdl(launch_pdl(p.interleaved ? norm_rope_bwd_direct_kernel<T, true> : norm_rope_bwd_direct_kernel<T, false>, grid,
-                                    dim3(kThreads), smem, s, p),
+        return check_pdl(p.d == 32   ? launch_bwd_direct<T, 32>(p, grid, smem, s)
+                         : p.d == 64 ? launch_bwd_direct<T, 64>(p, grid, smem, s)
+                         : p.d == 96 ? launch_bwd_direct<T, 96>(p, grid, smem, s)
+                                     : launch_bwd_direct<T, 128>(p, grid, smem, s),
                          "norm_rope_bwd_direct_kernel");
-    return check_pdl(launch_pdl(wide ? norm_rope_bwd_kernel<T, true> : norm_rope_bwd_kernel<T, false>, grid, dim3(kThreads), smem, s, p),
+    bool wide = true;
+    for (const void *x : tensors) wide = wide && even(x);
+    for (long long x : strides) wide = wide && x % W == 0;
+    return check_pdl(launch_pdl(wide ? norm_rope_bwd_kernel<T, true> : norm_rope_bwd_kernel<T, false>, grid, dim3(p.threads), smem, s, p),
                      "norm_rope_bwd_kernel");
 }
 
@@ -830,8 +963,10 @@ size_t norm_rope_bwd_workspace(const attn_rope_shape *s) {
     size_t parts = 1;
     const attn_head_norm n = {};
     for (int i = 0; i < 8; i++) {
-        Params p = norm_params(s, &n, nullptr, nullptr, i & 4 ? s->kv_heads : 0, 0, nullptr);
-        const dim3 grid = divide(p, i & 2, i & 1 ? 8 : 4, attn::nrope::kHeadsBwd, attn::nrope::kCtas);
+        using namespace attn::nrope;
+        Params p = norm_params(s, &n, nullptr, nullptr, i & 1 ? s->kv_heads : 0, 0, nullptr);
+        const int bytes = i & 2 ? 2 : 4;
+        const dim3 grid = i < 4 ? divide(p, true, 4, direct_heads_bwd(bytes), kCtas) : divide(p, false, 16 / bytes, kHeadsBwd, kCtas);
         parts = std::max(parts, (size_t)grid.x * grid.y);
     }
     return (parts * 2 * s->head_dim * 4 + 255) / 256 * 256;
