@@ -43,6 +43,13 @@
 // in a fixed order: 217 us, its own instructions and waits take 1,730 cycles a pair;
 // four, one per product and warpgroup: no faster than two.)
 //
+// The instruction cache sets a limit of its own: the roles run different code
+// side by side, and what is unrolled only for convenience (a piece's end, the
+// lanes' copies, a copy of the products for each warpgroup where one piece
+// takes turns) cost 465 us, and 366 with one copy each, on 256 contexts of up to
+// 2000 rows with 16 drafts of four heads.  So did a warp that divided the pieces into a stream
+// for each warpgroup, with its own 300 instructions a step: slower by a fifth.
+//
 // Every wait is bounded; a timeout records a code in the device error word and
 // raises a CTA-wide flag, on which all roles fall through to the teardown.
 #include <algorithm>
@@ -288,7 +295,7 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 if (!ok) break;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-#pragma unroll 4
+#pragma unroll 1
                     for (int r0 = 0; r0 < 32; r0 += RPI) {
                         const int r = __shfl_sync(0xffffffffu, row[i], r0 + lr);
                         copy16(to + tile_at(32 * i + r0 + lr, ch), from + (long long)max(r, 0) * p.row_stride, r >= 0);
@@ -320,13 +327,11 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             for (int j = x.a; ok && j < x.b; j++, g++) {
                 const int slot = g % C::KS;
                 if (!(ok = wait(B_FULL + slot, g / C::KS, 0x812))) break;
-#pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    const int u = n >> 1, wg = n & 1, b = 2 * wg + u;
-                    if (!two && ((j - x.a) & 1) != wg) continue;
+                auto half = [&](int wg, int u) {
+                    const int b = 2 * wg + u;
                     // the product that reads this half's last P is done
-                    if (ok && t[wg] > 0) ok = wait(B_OD + b, t[wg] - 1, 0x813 + n);
-                    if (!ok) break;
+                    const int mine = wg ? t[1] : t[0];
+                    if (mine > 0 && !(ok = wait(B_OD + b, mine - 1, 0x813 + b))) return;
                     tc_fence_after();
                     if (leader) {
                         const uint64_t qd = sw128_desc(sQ + (two ? wg : place) * C::QTILE, 16, 1024);
@@ -340,7 +345,18 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                         mbar_arrive(BAR(B_SF + b));               // (hands on the copying warps' masks)
                     }
                     __syncwarp();
-                    if (u == 1) t[wg]++;
+                    if (u == 1) {
+                        if (wg) t[1]++;
+                        else t[0]++;
+                    }
+                };
+                if (two) {
+#pragma unroll
+                    for (int n = 0; n < 4; n++)
+                        if (ok) half(n & 1, n >> 1);
+                } else {                  // (one copy of the code: the SM's instruction cache is short of room)
+#pragma unroll 1
+                    for (int u = 0; ok && u < 2; u++) half((j - x.a) & 1, u);
                 }
                 if (!ok) break;
                 if (leader) {
@@ -364,14 +380,12 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             for (int j = x.a; ok && j < x.b; j++, g++) {
                 const int slot = C::KS + g % C::VS;
                 if (!(ok = wait(B_FULL + slot, g / C::VS, 0x821))) break;
-#pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    const int u = n >> 1, wg = n & 1, b = 2 * wg + u;
-                    if (!two && ((j - x.a) & 1) != wg) continue;
+                auto half = [&](int wg, int u) {
+                    const int b = 2 * wg + u;
                     const bool first = u == 0 && j - x.a < (two ? 1 : 2);   // of this warpgroup in this piece
-                    if (ok && first && done[wg] > 0) ok = wait(B_OF + wg, done[wg] - 1, 0x822 + wg);
-                    if (ok) ok = wait(B_PF + b, t[wg], 0x824 + n);
-                    if (!ok) break;
+                    const int mine = wg ? t[1] : t[0], pieces = wg ? done[1] : done[0];
+                    if (first && pieces > 0 && !(ok = wait(B_OF + wg, pieces - 1, 0x822 + wg))) return;
+                    if (!(ok = wait(B_PF + b, mine, 0x824 + b))) return;
                     tc_fence_after();
                     if (leader) {
                         const uint64_t vd = sw128_desc(sKV + slot * C::TILE + u * BH * 128, BM * 128, 1024);
@@ -381,7 +395,18 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                         mma_commit(BAR(B_OD + b));
                     }
                     __syncwarp();
-                    if (u == 1) t[wg]++;
+                    if (u == 1) {
+                        if (wg) t[1]++;
+                        else t[0]++;
+                    }
+                };
+                if (two) {
+#pragma unroll
+                    for (int n = 0; n < 4; n++)
+                        if (ok) half(n & 1, n >> 1);
+                } else {
+#pragma unroll 1
+                    for (int u = 0; ok && u < 2; u++) half((j - x.a) & 1, u);
                 }
                 if (!ok) break;
                 if (leader) mma_commit(BAR(B_FREE + slot));
@@ -404,7 +429,7 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             const int r = y.rows > BM ? wg * BM + row : row, at = y.row0 + min(r, y.rows - 1);
             const int s = y.first_req + at / p.ratio, h = y.hb * p.ratio + at % p.ratio;
             const long long from = s * p.q_stride + (long long)h * D;
-#pragma unroll
+#pragma unroll 4
             for (int r0 = 0; r0 < 32; r0 += RPI) {
                 const int n = r0 + lane / CPR, to = quad * 32 + n, ch = lane % CPR;
                 const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(p.q) + __shfl_sync(0xffffffffu, from, n) + 8 * ch;
@@ -501,7 +526,7 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                             if (!(ok = __all_sync(0xffffffffu, ok))) break;
                             tc_fence_after();
                             uint32_t o[32];
-#pragma unroll
+#pragma unroll 1
                             for (int c0 = 0; c0 < D; c0 += 32) {
                                 tmem_ld32(tO + c0, o);
                                 tmem_wait_ld();
@@ -547,7 +572,7 @@ prefix_tile_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             if (any) {
                 tc_fence_after();
                 if (!idle) {
-#pragma unroll
+#pragma unroll 1
                     for (int c0 = 0; c0 < D; c0 += 32) {
                         uint32_t o[32];
                         tmem_ld32(tO + c0, o);
