@@ -87,7 +87,11 @@ struct Part {
     int log_rows, rows;                   // query rows of a block (2^log_rows), of a slot
     int log_keys;                         // keys of a step (2^log_keys)
     int half;                             // see Pieces (0: one piece per slot)
-    long long after;                      // TREES: rows of the prefixes' pieces
+    // TREES: rows of the prefixes' pieces; for the join, each query token's request and group (-1: none), and each
+    // line's first query token, query rows and keys
+    long long after;
+    int2 *row_of;
+    int4 *line_info;
 };
 
 __device__ __forceinline__ int ceil_shift(int a, int log_b) { return (a + (1 << log_b) - 1) >> log_b; }
@@ -119,6 +123,15 @@ __host__ __device__ __forceinline__ long long segment_begin(const Part &w, const
     const int rb = row >> w.log_rows, hb = w.n_blocks == 1 ? 0 : hk / w.head_block;
     return line_begin + (long long)(rb * w.n_blocks + hb) * l.cost() + l.begin;
 }
+// Steps and costs of a line with its query tokens' rows and keys.
+template <int LINES>
+__device__ __forceinline__ void line_steps(const Part &w, Line &l) {
+    l.steps = ceil_shift(l.keys, w.log_keys);
+    if (LINES == TREES && w.half) {
+        l.weight = l.rows > w.half ? kFullStep : 1;
+        l.begin = kTileBegin;
+    }
+}
 template <int LINES>
 __device__ __forceinline__ Line line_of(const Params &p, const Part &w, int i) {
     Line l;
@@ -140,12 +153,19 @@ __device__ __forceinline__ Line line_of(const Params &p, const Part &w, int i) {
         l.base = i * w.blocks;
         l.keys = own_len(p, i);
     }
-    l.steps = ceil_shift(l.keys, w.log_keys);
-    if (LINES == TREES && w.half) {
-        l.weight = l.rows > w.half ? kFullStep : 1;
-        l.begin = kTileBegin;
-    }
+    line_steps<LINES>(w, l);
     return l;
+}
+// TREES: request s's query tokens are told the request and its group (ascending: by bisection).
+__device__ __forceinline__ void tell_rows(const Params &p, const Part &w, int s) {
+    int lo = 0, hi = p.n_groups;          // the last group that begins at or before s
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(p.group_begin + mid) <= s) lo = mid;
+        else hi = mid;
+    }
+    const bool in = p.n_groups && __ldg(p.group_begin + lo) <= s && s < __ldg(p.group_begin + lo + 1);
+    for (int r = row_first(p, s), end = row_first(p, s + 1); r < end; r++) w.row_of[r] = make_int2(s, in ? lo : -1);
 }
 
 // Running sums of the lines' costs, one per entry of w.per_entry lines, in
@@ -157,6 +177,9 @@ template <int LINES>
 __device__ __forceinline__ long long sum_lines(const Params &p, const Part &w, long long *sums, long long *warp_sums) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int entries = w.entries;
+    if constexpr (LINES == TREES) {
+        for (int s = (int)(blockIdx.x + gridDim.x * threadIdx.x); s < p.n_req; s += (int)(gridDim.x * blockDim.x)) tell_rows(p, w, s);
+    }
     long long carry = 0;
     for (int e0 = 0; e0 < entries; e0 += (int)blockDim.x) {
         const int e = e0 + threadIdx.x;
@@ -189,8 +212,10 @@ __device__ __forceinline__ long long sum_lines(const Params &p, const Part &w, l
         for (int e = threadIdx.x; e < entries; e += blockDim.x) {
             long long at = sums[e];
             for (int i = e * w.per_entry; i < min((e + 1) * w.per_entry, w.lines); i++) {
+                const Line l = line_of<LINES>(p, w, i);
                 w.line_first[i] = at;
-                at += line_of<LINES>(p, w, i).total(w);
+                if constexpr (LINES == TREES) w.line_info[i] = make_int4(l.first_req, l.rows, l.keys, 0);
+                at += l.total(w);
             }
         }
         if (threadIdx.x == 0) {

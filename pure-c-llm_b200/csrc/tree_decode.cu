@@ -18,62 +18,57 @@ namespace prefix {
 
 constexpr int kJoinWarps = 8;
 
-// The request of query token r (the last whose tokens begin at or before r),
-// or -1 where it has none.  By a warp, 32 probes at a time.
-__device__ __forceinline__ int request_of(const Params &p, int r) {
-    const int lane = threadIdx.x & 31;
-    int lo = 0, n = p.n_req;
-    while (true) {
-        const int step = (n + 31) / 32, i = lane * step;
-        const unsigned at = __ballot_sync(0xffffffffu, i < n && __ldg(p.row_begin + lo + i) <= r);
-        if (!at) return -1;
-        const int k = (__popc(at) - 1) * step;
-        lo += k;
-        n = min(step, n - k);
-        if (step == 1) break;
-    }
-    return r >= row_first(p, lo) && r < row_first(p, lo + 1) ? lo : -1;
+// Line i as the first kernel has told it.
+__device__ __forceinline__ Line told_line(const Params &p, const Part &w, int i, int4 info) {
+    Line l;
+    l.prefix = i < p.n_groups;
+    l.first_req = info.x;
+    l.rows = info.y;
+    l.keys = info.z;
+    l.blocks = ceil_shift(l.rows, w.log_rows);
+    l.base = (l.first_req * p.ratio >> w.log_rows) + (l.prefix ? i : i - p.n_groups);
+    line_steps<TREES>(w, l);
+    return l;
 }
 
-// The pieces of a query row in one line, from teams t0 .. t1; with `twice` each team left two.
+// The pieces of a query row in one line, from teams t0 .. t1, by their rows on
+// the workspace; where each team left two (Part::half), `apart` is not 0.
 struct Pieces {
-    const float *o;
-    const float2 *ml;
-    long long step;
-    int apart, n;
-    bool twice;
-    __device__ __forceinline__ long long at(int j) const { return twice ? (j >> 1) * step + (j & 1) * apart : j * step; }
+    long long first;
+    int step, apart, n;
+    __device__ __forceinline__ long long at(int j) const { return first + (apart ? (long long)(j >> 1) * step + (j & 1) * apart : (long long)j * step); }
 };
 template <int D>
 __device__ __forceinline__ Pieces pieces_of(const Params &p, const Part &w, const Line &l, int row, int hk, int t0, int t1) {
-    Pieces r = {};
-    if (l.steps == 0) return r;
     const int rb = row >> w.log_rows, hb = w.n_blocks == 1 ? 0 : hk / w.head_block, hw = hk - hb * w.head_block;
     const Place x = place_of<TREES>(p, w, l, rb, hb);
-    const long long at = x.first + t0 * x.step + (w.half ? 0 : (long long)hw * x.apart) + row - (rb << w.log_rows);
-    r.o = w.o + at * D;
-    r.ml = w.ml + at;
-    r.step = x.step;
-    r.apart = x.apart;
-    r.twice = w.half && l.rows - (rb << w.log_rows) <= w.half;
-    r.n = (t1 - t0 + 1) * (r.twice ? 2 : 1);
-    return r;
+    const bool twice = w.half && l.rows - (rb << w.log_rows) <= w.half;
+    return {x.first + t0 * x.step + (w.half ? 0 : (long long)hw * x.apart) + row - (rb << w.log_rows), (int)x.step, twice ? x.apart : 0,
+            (t1 - t0 + 1) * (twice ? 2 : 1)};
 }
 
 // Output type of a cache's calls.
 template <typename KV> struct Out { using Type = float; };
 template <> struct Out<__nv_bfloat16> { using Type = __nv_bfloat16; };
 
-// Four consecutive elements as floats, and back.
-__device__ __forceinline__ float4 four(const float *p) { return *reinterpret_cast<const float4 *>(p); }
-__device__ __forceinline__ float4 four(const __nv_bfloat16 *p) {
+using sm100::mul2;
+// Four consecutive elements as two packed pairs of floats.
+struct Quad { uint64_t a, b; };
+__device__ __forceinline__ Quad quad(float4 x) { return {f2(x.x, x.y), f2(x.z, x.w)}; }
+__device__ __forceinline__ Quad four(const float *p) { return quad(*reinterpret_cast<const float4 *>(p)); }
+__device__ __forceinline__ Quad four(const __nv_bfloat16 *p) {
     const uint2 w = *reinterpret_cast<const uint2 *>(p);
-    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                       __uint_as_float(w.y & 0xffff0000u));
+    return {f2(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u)), f2(__uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u))};
 }
-__device__ __forceinline__ float4 four(const int8_t *p) {
+__device__ __forceinline__ Quad four(const int8_t *p) {
     const char4 c = *reinterpret_cast<const char4 *>(p);
-    return make_float4(c.x, c.y, c.z, c.w);
+    return {f2(c.x, c.y), f2(c.z, c.w)};
+}
+__device__ __forceinline__ float4 floats(const Quad &q) {
+    float4 x;
+    f2_split(q.a, x.x, x.y);
+    f2_split(q.b, x.z, x.w);
+    return x;
 }
 
 // A warp takes one query token and four adjacent query heads, eight lanes a
@@ -82,55 +77,67 @@ __device__ __forceinline__ float4 four(const int8_t *p) {
 // so weights need none.  SHARED: the warps of a CTA share that, each taking some
 // of the drafted rows and pieces.
 template <typename KV, int D, bool SHARED>
-__global__ void __launch_bounds__(kJoinWarps * 32, 2)
+__global__ void __launch_bounds__(kJoinWarps * 32, 3)
 tree_join_kernel(const __grid_constant__ Params p, const __grid_constant__ Part w)
 {
     pdl_begin();                          // launched by launch_pdl
     using T = typename Out<KV>::Type;
-    constexpr int C = D / 32, KB = 4;     // elements of a lane, in fours; drafted rows, and pieces, at once
+    constexpr int C = D / 32, KB = 2;     // elements of a lane, in fours; drafted rows, and pieces, at once
     constexpr bool I8 = sizeof(KV) == 1;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int r = blockIdx.x;
     const int unit = (int)blockIdx.y * (SHARED ? 1 : kJoinWarps) + (SHARED ? 0 : warp);
-    if (r >= row_first(p, p.n_req) || 4 * unit >= p.heads) return;
-    const int req = request_of(p, r);
-    if (req < 0) return;
+    if (4 * unit >= p.heads) return;
+    // What counts here is the chain of dependent loads, so each link's go out together: the token's request, its mask and
+    // the number of tokens; then the lines; then the pieces' maxima and the page table; then the rows.
+    const int2 of = __ldcg(w.row_of + r);                     // (not written for rows of no request)
+    const int req = of.x, total = row_first(p, p.n_req);
+    unsigned bits = p.masks && p.max_nodes ? __ldg(p.masks + (long long)r * p.mask_words) : 0u;
+    if (r >= total || (unsigned)req >= (unsigned)p.n_req || r < row_first(p, req) || r >= row_first(p, req + 1)) return;
     const int h = min(4 * unit + lane / 8, p.heads - 1), mine = lane % 8 * 4;      // (idle lanes repeat the last head)
     const int hk = p.ratio == 1 ? h : h / p.ratio, hr = h - hk * p.ratio;
 
-    const Line ctx = line_of<TREES>(p, w, p.n_groups + req);
+    const int own = p.n_groups + req, group = (unsigned)of.y < (unsigned)p.n_groups ? of.y : -1;
+    const long long team = __ldcg(w.line_first + w.lines + 1), ctx_begin = __ldcg(w.line_first + own);
+    const long long pre_begin = group >= 0 ? __ldcg(w.line_first + group) : 0;
+    const int len = __ldg(p.lens + req);
+    const Line ctx = told_line(p, w, own, __ldcg(w.line_info + own));
     Line pre = {};
-    long long ctx_begin = 0, pre_begin = 0, team = 1;
-    if (w.lines) {
-        ctx_begin = __ldcg(w.line_first + p.n_groups + req);
-        team = __ldcg(w.line_first + w.lines + 1);
+    if (group >= 0) {
+        pre = told_line(p, w, group, __ldcg(w.line_info + group));
+        if ((r - pre.first_req) * p.ratio < 0 || (r - pre.first_req) * p.ratio >= pre.rows) pre.steps = 0;
     }
-    for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
-        const int g = g0 + lane;
-        const bool in = g < p.n_groups && r >= group_first<TREES>(p, g) && r < group_first<TREES>(p, g + 1);
-        const unsigned found = __ballot_sync(0xffffffffu, in);
-        if (found) {
-            const int at = g0 + __ffs(found) - 1;
-            if (w.lines) pre_begin = __ldcg(w.line_first + at);
-            pre = line_of<TREES>(p, w, at);
-            break;
-        }
-    }
-    const int drafts = checked_len(p, checked_len(p, __ldg(p.lens + req), p.max_len) - ctx.keys, p.max_nodes);
+    const int drafts = checked_len(p, checked_len(p, len, p.max_len) - ctx.keys, p.max_nodes);
+    // the pieces of the two lines, and the maxima and sums of the first ones
+    auto line_pieces = [&](const Line &line, long long begin) {
+        if (line.steps == 0) return Pieces{};
+        const int row = (r - line.first_req) * p.ratio + hr;
+        const long long first = segment_begin(w, line, row, hk, begin);
+        const int t0 = (int)quotient(max(first, 0LL), team), t1 = (int)quotient(max(first + (long long)(line.steps - 1) * line.weight, 0LL), team);
+        return pieces_of<D>(p, w, line, row, hk, t0, t1);
+    };
+    auto bring_ml = [&](const Pieces &a, int j0, float2 (&ml)[KB]) {
+#pragma unroll
+        for (int i = 0; i < KB; i++) ml[i] = j0 + i < a.n ? __ldcg(w.ml + a.at(j0 + i)) : make_float2(-INFINITY, 0.f);
+    };
+    const Pieces ctx_pieces = line_pieces(ctx, ctx_begin), pre_pieces = line_pieces(pre, pre_begin);
+    const int j_first = SHARED ? warp * KB : 0;
+    float2 ctx_ml[KB], pre_ml[KB];
+    bring_ml(ctx_pieces, j_first, ctx_ml);
+    bring_ml(pre_pieces, j_first, pre_ml);
 
-    float4 q[C], o[C];
+    Quad q[C], o[C];
     float m = -INFINITY, l = 0.f;
     const T *query = static_cast<const T *>(p.q) + r * p.q_stride + (long long)h * D + mine;
 #pragma unroll
     for (int c = 0; c < C; c++) {
         q[c] = four(query + 32 * c);
-        o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        o[c] = {0, 0};
     }
-    auto add = [&](int c, float f, float4 v) {
-        o[c].x = fmaf(f, v.x, o[c].x);
-        o[c].y = fmaf(f, v.y, o[c].y);
-        o[c].z = fmaf(f, v.z, o[c].z);
-        o[c].w = fmaf(f, v.w, o[c].w);
+    auto add = [&](float f, const Quad (&v)[C]) {
+        const uint64_t ff = f2(f, f);
+#pragma unroll
+        for (int c = 0; c < C; c++) o[c] = {fma2(ff, v[c].a, o[c].a), fma2(ff, v[c].b, o[c].b)};
     };
     // Takes in maxima x (-inf: none) with sums s; x becomes the weights.
     auto fold = [&](float (&x)[KB], const float (&s)[KB]) {
@@ -138,9 +145,12 @@ tree_join_kernel(const __grid_constant__ Params p, const __grid_constant__ Part 
 #pragma unroll
         for (int i = 0; i < KB; i++) mx = fmaxf(mx, x[i]);
         const float old = mx == m ? 1.f : exp2f(m - mx);
-        l *= old;
+        if (__any_sync(0xffffffffu, old != 1.f)) {
+            const uint64_t ff = f2(old, old);
+            l *= old;
 #pragma unroll
-        for (int c = 0; c < C; c++) o[c] = make_float4(o[c].x * old, o[c].y * old, o[c].z * old, o[c].w * old);
+            for (int c = 0; c < C; c++) o[c] = {mul2(o[c].a, ff), mul2(o[c].b, ff)};
+        }
         m = mx;
 #pragma unroll
         for (int i = 0; i < KB; i++) {
@@ -154,8 +164,8 @@ tree_join_kernel(const __grid_constant__ Params p, const __grid_constant__ Part 
     int seen = 0;
     for (int j0 = 0; j0 < drafts; j0 += 32) {
         const int last = r - ctx.first_req - j0;              // without masks a token sees itself and those before it
-        unsigned bits = p.masks ? __ldg(p.masks + (long long)r * p.mask_words + j0 / 32)
-                                : last >= 31 ? 0xffffffffu : last < 0 ? 0u : (2u << last) - 1;
+        if (!p.masks) bits = last >= 31 ? 0xffffffffu : last < 0 ? 0u : (2u << last) - 1;
+        else if (j0) bits = __ldg(p.masks + (long long)r * p.mask_words + j0 / 32);
         if (drafts - j0 < 32) bits &= (1u << (drafts - j0)) - 1;
         while (bits) {
             int row[KB];
@@ -173,20 +183,24 @@ tree_join_kernel(const __grid_constant__ Params p, const __grid_constant__ Part 
                 }
             }
             if (!any) continue;
-            float4 v[KB][C];
+            Quad v[KB][C];
             float x[KB], one[KB];
 #pragma unroll
             for (int i = 0; i < KB; i++) {
                 x[i] = 0.f;
                 one[i] = 1.f;
-                const long long at = max(row[i], 0) * p.row_stride + (long long)hk * D + mine;
+                if (row[i] < 0) continue;
+                const long long at = row[i] * p.row_stride + (long long)hk * D + mine;
+                uint64_t dot = 0;
 #pragma unroll
                 for (int c = 0; c < C; c++) {
-                    if (row[i] < 0) continue;
-                    const float4 k = four(static_cast<const KV *>(p.k) + at + 32 * c);
+                    const Quad k = four(static_cast<const KV *>(p.k) + at + 32 * c);
                     v[i][c] = four(static_cast<const KV *>(p.v) + at + 32 * c);
-                    x[i] = fmaf(q[c].x, k.x, fmaf(q[c].y, k.y, fmaf(q[c].z, k.z, fmaf(q[c].w, k.w, x[i]))));
+                    dot = fma2(q[c].b, k.b, fma2(q[c].a, k.a, dot));
                 }
+                float even, odd;
+                f2_split(dot, even, odd);
+                x[i] = even + odd;
             }
 #pragma unroll
             for (int k = 1; k < 8; k *= 2)
@@ -208,35 +222,27 @@ tree_join_kernel(const __grid_constant__ Params p, const __grid_constant__ Part 
             for (int i = 0; i < KB; i++) {
                 if (row[i] < 0) continue;
                 if constexpr (I8) x[i] *= vscale[i];
-#pragma unroll
-                for (int c = 0; c < C; c++) add(c, x[i], v[i][c]);
+                add(x[i], v[i]);
             }
         }
     }
 
-    // the pieces of the two lines
-    auto join = [&](const Line &line, long long begin) {
-        if (line.steps == 0) return;
-        const int row = (r - line.first_req) * p.ratio + hr;
-        const long long first = segment_begin(w, line, row, hk, begin);
-        const int t0 = (int)quotient(max(first, 0LL), team), t1 = (int)quotient(max(first + (long long)(line.steps - 1) * line.weight, 0LL), team);
-        const Pieces a = pieces_of<D>(p, w, line, row, hk, t0, t1);
+    auto join = [&](const Pieces &a, float2 (&ml)[KB]) {
         int most = a.n;                   // of the four heads
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 8));
         most = max(most, __shfl_xor_sync(0xffffffffu, most, 16));
-        for (int j0 = SHARED ? warp * KB : 0; j0 < most; j0 += KB * (SHARED ? kJoinWarps : 1)) {
+        for (int j0 = j_first; j0 < most; j0 += KB * (SHARED ? kJoinWarps : 1)) {
+            if (j0 != j_first) bring_ml(a, j0, ml);
             float x[KB], s[KB];
-            float4 v[KB][C];
+            Quad v[KB][C];
 #pragma unroll
             for (int i = 0; i < KB; i++) {
-                const int j = j0 + i;
-                const long long at = j < a.n ? a.at(j) : 0;
-                const float2 ml = j < a.n ? __ldcg(a.ml + at) : make_float2(-INFINITY, 0.f);
-                x[i] = ml.x;
-                s[i] = ml.y;
+                x[i] = ml[i].x;
+                s[i] = ml[i].y;
+                const long long at = j0 + i < a.n ? a.at(j0 + i) : 0;
 #pragma unroll
                 for (int c = 0; c < C; c++)
-                    v[i][c] = j < a.n ? __ldcg(reinterpret_cast<const float4 *>(a.o + at * D + mine + 32 * c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    v[i][c] = quad(j0 + i < a.n ? __ldcg(reinterpret_cast<const float4 *>(w.o + at * D + mine + 32 * c)) : make_float4(0.f, 0.f, 0.f, 0.f));
             }
             bool there[KB];
 #pragma unroll
@@ -246,21 +252,18 @@ tree_join_kernel(const __grid_constant__ Params p, const __grid_constant__ Part 
             // scores are low still hands on a value that is no number.
 #pragma unroll
             for (int i = 0; i < KB; i++)
-                if (there[i]) {
-#pragma unroll
-                    for (int c = 0; c < C; c++) add(c, x[i], v[i][c]);
-                }
+                if (there[i]) add(x[i], v[i]);
         }
     };
-    join(ctx, ctx_begin);
-    join(pre, pre_begin);
+    join(ctx_pieces, ctx_ml);
+    join(pre_pieces, pre_ml);
 
     if constexpr (SHARED) {
         __shared__ float2 s_ml[kJoinWarps][4];
         __shared__ float4 s_o[kJoinWarps][C][32];
         if (lane % 8 == 0) s_ml[warp][lane / 8] = make_float2(m, l);
 #pragma unroll
-        for (int c = 0; c < C; c++) s_o[warp][c][lane] = o[c];
+        for (int c = 0; c < C; c++) s_o[warp][c][lane] = floats(o[c]);
         __syncthreads();
         if (warp) return;
         for (int k0 = 1; k0 < kJoinWarps; k0 += KB) {
@@ -273,17 +276,23 @@ tree_join_kernel(const __grid_constant__ Params p, const __grid_constant__ Part 
             }
             fold(x, s);
 #pragma unroll
-            for (int i = 0; i < KB; i++)
+            for (int i = 0; i < KB; i++) {
+                if (k0 + i >= kJoinWarps) continue;
+                Quad v[C];
 #pragma unroll
-                for (int c = 0; c < C; c++)
-                    if (k0 + i < kJoinWarps) add(c, x[i], s_o[k0 + i][c][lane]);
+                for (int c = 0; c < C; c++) v[c] = quad(s_o[k0 + i][c][lane]);
+                add(x[i], v);
+            }
         }
     }
     if (4 * unit + lane / 8 >= p.heads) return;
     T *out = static_cast<T *>(p.out) + r * p.out_stride + (long long)h * D + mine;
     const float inv = l != l ? NAN : m == -INFINITY ? 0.f : 1.f / l;
 #pragma unroll
-    for (int c = 0; c < C; c++) store4(out + 32 * c, make_float4(o[c].x * inv, o[c].y * inv, o[c].z * inv, o[c].w * inv));
+    for (int c = 0; c < C; c++) {
+        const float4 x = floats(o[c]);
+        store4(out + 32 * c, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+    }
     if (p.lse && lane % 8 == 0) p.lse[(long long)r * p.heads + h] = l != l ? NAN : m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
@@ -304,7 +313,6 @@ using attn::prefix::Part;
 size_t lay_out(Part &w, const Params &p, int d, int seg_rows, int keys, int grid, bool tile, char *base) {
     using namespace attn::prefix;
     w = {};
-    if (!p.max_len && !(p.n_groups && p.max_prefix_len)) return 256;
     divide_part(w, p, p.n_groups + p.n_req, seg_rows, keys, grid, tile);
     const long long rows = (long long)p.n_seq * p.ratio, heads = (long long)w.n_blocks * w.head_block;
     w.rows = tile ? seg_rows : (int)std::min<long long>(rows, seg_rows);
@@ -317,6 +325,8 @@ size_t lay_out(Part &w, const Params &p, int d, int seg_rows, int keys, int grid
         return at;
     };
     w.line_first = reinterpret_cast<long long *>(take(((size_t)w.lines + 2) * 8));
+    w.row_of = reinterpret_cast<int2 *>(take((size_t)p.n_seq * 8));
+    w.line_info = reinterpret_cast<int4 *>(take((size_t)w.lines * 16));
     w.ml = reinterpret_cast<float2 *>(take(all * 8));
     w.o = reinterpret_cast<float *>(take(all * d * 4));
     return off;
@@ -339,7 +349,7 @@ int run(const Params &p, void *ws, size_t *need, cudaStream_t s) {
     Part w;
     const size_t bytes = lay_out(w, p, D, Path::ROWS, Path::KEYS, sm_count_here() * CTAS, false, static_cast<char *>(ws));
     if (need) { *need = bytes; return ATTN_OK; }
-    const int st = w.lines ? run_part<Path, TREES, D, CTAS>(p, w, 0, s) : ATTN_OK;
+    const int st = run_part<Path, TREES, D, CTAS>(p, w, 0, s);
     return st ? st : join<KV, D>(p, w, s);
 }
 template <int D>
@@ -347,7 +357,7 @@ int run_tile(const Params &p, void *ws, size_t *need, cudaStream_t s) {
     Part w;
     const size_t bytes = lay_out(w, p, D, 256, 128, sm_count_here(), true, static_cast<char *>(ws));
     if (need) { *need = bytes; return ATTN_OK; }
-    const int st = w.lines ? launch_tree_tile(p, w, D, s) : ATTN_OK;
+    const int st = launch_tree_tile(p, w, D, s);
     return st ? st : join<__nv_bfloat16, D>(p, w, s);
 }
 
