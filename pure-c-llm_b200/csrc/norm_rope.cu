@@ -234,7 +234,9 @@ __device__ __forceinline__ void angles(const Params &p, int pos, int e0, bool ba
         s[i] = second != back ? cs.y : -cs.y;
     }
 }
-// The E elements turned.  `row`: d floats of shared memory of the group's own.
+// The E elements turned.  `row`: d floats of shared memory of the group's own,
+// element e at (e % E) (d / E) + e / E, so that lanes side by side write, and read
+// their partners, at addresses side by side.
 template <int E>
 __device__ __forceinline__ void turn(const Params &p, int e0, bool there, unsigned mask, float *row, const float (&c)[E],
                                      const float (&s)[E], float (&x)[E]) {
@@ -248,21 +250,23 @@ __device__ __forceinline__ void turn(const Params &p, int e0, bool there, unsign
         }
         return;
     }
-    const int half = p.rot / 2;
+    const int half = p.rot / 2, items = p.d / E;
     __syncwarp(mask);                     // the row's last readers are done
     if (there) {
 #pragma unroll
-        for (int i = 0; i < E; i++) row[e0 + i] = x[i];
+        for (int i = 0; i < E; i++) row[i * items + e0 / E] = x[i];
     }
     __syncwarp(mask);
     if (there) {
 #pragma unroll
         for (int i = 0; i < E; i++) {
-            const int e = e0 + i;
-            if (e < p.rot) x[i] = fmaf(x[i], c[i], s[i] * row[e < half ? e + half : e - half]);
+            const int e = e0 + i, other = e < half ? e + half : e - half;
+            if (e < p.rot) x[i] = fmaf(x[i], c[i], s[i] * row[other % E * items + other / E]);
         }
     }
 }
+// Floats of shared memory from one group's row to the next: in other banks.
+__host__ __device__ __forceinline__ int row_pitch(const Params &p) { return p.d + p.lanes; }
 
 // CODES: k and v into an INT8 cache, quantised as quantize_int8_kernel does (kv.cu).
 template <typename T, bool WIDE, bool CODES>
@@ -272,12 +276,12 @@ norm_rope_kernel(const __grid_constant__ Params p)
     pdl_begin();                          // launched by launch_pdl
     using V = Vec<T, WIDE>;
     constexpr int E = V::E;
-    extern __shared__ float exchange[];   // d floats per group
+    extern __shared__ float exchange[];   // a row per group
     const Place x = place_of<kHeads>(p, (int)(blockIdx.y * blockDim.x + threadIdx.x));
     if (!x.there) return;
     const int e0 = x.item * E;
     const bool there = e0 < p.d;          // lanes past the head take part in the sums alone
-    float *row_buf = exchange + threadIdx.x / p.lanes * p.d;
+    float *row_buf = exchange + threadIdx.x / p.lanes * row_pitch(p);
     const float *weight = x.kind == 0 ? p.q_weight : p.k_weight;
     float w[E];
 #pragma unroll
@@ -357,11 +361,11 @@ norm_rope_bwd_kernel(const __grid_constant__ Params p)
     pdl_begin();                          // launched by launch_pdl
     using V = Vec<T, WIDE>;
     constexpr int E = V::E;
-    extern __shared__ float exchange[];   // d floats per group
+    extern __shared__ float exchange[];   // a row per group
     const Place x = place_of<kHeadsBwd>(p, (int)(blockIdx.y * blockDim.x + threadIdx.x));
     const int e0 = x.item * E;
     const bool there = x.there && e0 < p.d;
-    float *row_buf = exchange + threadIdx.x / p.lanes * p.d;
+    float *row_buf = exchange + threadIdx.x / p.lanes * row_pitch(p);
     const float *weight = x.kind == 0 ? p.q_weight : p.k_weight;
     float w[E], dw[E];
 #pragma unroll
@@ -420,7 +424,7 @@ norm_rope_bwd_kernel(const __grid_constant__ Params p)
     __syncthreads();
     if (there) {
 #pragma unroll
-        for (int i = 0; i < E; i++) row_buf[e0 + i] = dw[i];
+        for (int i = 0; i < E; i++) exchange[threadIdx.x / p.lanes * p.d + e0 + i] = dw[i];
     }
     __syncthreads();
     write_partial<kHeadsBwd>(p, exchange);
@@ -906,7 +910,7 @@ int launch_forward(Params p, cudaStream_t s) {
     for (const void *x : tensors) wide = wide && even(x);
     for (long long x : strides) wide = wide && x % W == 0;
     const dim3 grid = divide(p, false, W, kHeads, kCtas);
-    const size_t smem = (size_t)p.threads / p.lanes * p.d * 4;
+    const size_t smem = (size_t)p.threads / p.lanes * row_pitch(p) * 4;
     return check_pdl(launch_pdl(wide ? norm_rope_kernel<T, true, CODES> : norm_rope_kernel<T, false, CODES>, grid, dim3(p.threads), smem, s, p),
                      "norm_rope_kernel");
 }
@@ -921,7 +925,7 @@ int launch_backward(Params p, int *parts, cudaStream_t s) {
     const bool direct = direct_fits<T>(p, tensors, strides);
     const dim3 grid = divide(p, direct, direct ? 4 : W, direct ? direct_heads_bwd(sizeof(T)) : kHeadsBwd, kCtas);
     *parts = (int)(grid.x * grid.y);
-    const size_t smem = (size_t)p.threads / p.lanes * p.d * 4;
+    const size_t smem = (size_t)p.threads / p.lanes * row_pitch(p) * 4;
     if (direct)
         return check_pdl(p.d == 32   ? launch_bwd_direct<T, 32>(p, grid, smem, s)
                          : p.d == 64 ? launch_bwd_direct<T, 64>(p, grid, smem, s)

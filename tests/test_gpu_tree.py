@@ -524,3 +524,103 @@ def test_commit_leaves_and_pages_that_are_none(A):
     assert device_error(A) == 0x702
     for t, w in zip(c.caches[0], kept):
         np.testing.assert_array_equal(t.float().cpu().numpy(), w)
+
+
+# ---------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("cache", ["f32", "int8"])
+def test_drafts_example(A, cache):
+    """The example's loop: page plan, tree plan, projection, normed append, tree decode and commit, several steps; fp32
+    arithmetic, the repository's 1e-5."""
+    import os
+    import runpy
+    from conftest import ROOT
+    m = runpy.run_path(os.path.join(ROOT, "examples", "serve_drafts.py"))
+    assert m["main"](requests=5, prompt=130, steps=6, nodes=40 if cache == "f32" else 9, cache=cache) < 1e-5
+
+
+def test_a_captured_step(A):
+    """A whole step, from the page plan to the commit, captured and replayed on other lengths, drafts and leaves: what plain
+    calls give."""
+    import torch
+    r = np.random.RandomState(3)
+    n, nodes, page, heads, d, most = 7, 8, 4, 4, 64, 60
+    rows, cols = n * nodes, -(-(most + nodes) // page)
+    ids = r.permutation(n * cols).astype(np.int32)
+    free = np.full(n * cols, -1, np.int32)
+    q, k, v = (dev(synth.normal(50 + i, (rows, heads * d))) for i in range(3))
+    caches = [[dev(synth.normal(60 + 2 * i + j, (n * cols * page, heads * d))) for j in range(2)] for i in range(2)]
+    kv = [A.PageCache.of(*c) for c in caches]
+    weight = dev((1 + 0.1 * synth.normal(70, (d,))).astype(np.float32))
+    norm = A.HeadNorm.of(weight, weight, 1e-6)
+    table = dev(R.rope_table(d, most + 2 * nodes).astype(np.float32))
+    pages = A.PageShape(n, page, cols, rows, n * cols, 0)
+    out = A.page_outputs(pages)
+    z = dict(dtype=torch.int32, device="cuda")
+    state = dict(lens=torch.zeros(n, **z), new=torch.zeros(n, **z), free=dev(free), count=torch.zeros(1, **z), table=torch.zeros((n, cols), **z),
+                 parents=torch.zeros(rows, **z), leaf=torch.zeros(n, **z), masks=torch.zeros((rows, 1), **z), lens_out=torch.zeros(n, **z),
+                 counts=torch.zeros(4, **z), att=torch.zeros((rows, heads * d), device="cuda"), turned=torch.zeros((rows, heads * d), device="cuda"))
+    shape = A.RopeShape(rows, 0, heads, heads, d, d, 0, most + 2 * nodes, 0, 0, 0, 0, 0)
+    tree = A.TreeShape(n, rows, 0, heads, heads, d, A.F32, page, 0, cols, 0, cols * page, nodes, 1, 0, 0, 0.0)
+    work = torch.empty(A.tree_decode_workspace_bytes(tree, kv[0]), dtype=torch.uint8, device="cuda")
+    array = A.cache_array(kv)
+
+    def step():
+        s = state
+        A.page_plan_t(pages, s["lens"], s["new"], s["free"], s["count"], s["table"], out)
+        A.tree_plan_t(out["cu_new"], s["parents"], out["positions"], out["positions"], s["masks"])
+        for c in kv:
+            A.norm_rope_append_t(shape, norm, c, table, out["positions"], out["slot_map"], q, k, v, s["turned"])
+            A.tree_decode_t(tree, c, s["turned"], out["cu_new"], s["lens"], out["lens"], s["masks"], s["table"], s["att"], workspace=work)
+        A.tree_commit_t(pages, array, heads, d, out["cu_new"], s["lens"], out["lens"], s["leaf"], s["masks"], s["table"], s["free"], out["counts"][:1],
+                        s["lens_out"], s["counts"])
+
+    def load(seed):
+        x = np.random.RandomState(seed)
+        lens = x.randint(0, most - nodes, n).astype(np.int32)
+        new = x.randint(0, nodes + 1, n).astype(np.int32)
+        new[x.randint(0, n)] = -1
+        held = -(-lens // page)
+        tab, at = np.full((n, cols), -1, np.int32), 0
+        for s in range(n):
+            tab[s, :held[s]] = ids[at:at + held[s]]
+            at += held[s]
+        left = np.full(n * cols, -1, np.int32)
+        left[:n * cols - at] = ids[at:]
+        parents = np.zeros(rows, np.int32)
+        first = 0
+        for m in np.maximum(new, 0):
+            if m:
+                parents[first:first + m] = T.random_tree(x, int(m))
+            first += m
+        leaf = np.array([x.randint(-1, max(int(m), 1)) for m in new], np.int32)
+        for name, value in (("lens", lens), ("new", new), ("free", left), ("count", np.array([n * cols - at], np.int32)), ("table", tab), ("parents", parents),
+                            ("leaf", leaf)):
+            state[name].copy_(dev(value))
+        for i, c in enumerate(caches):
+            for j in range(2):
+                c[j].copy_(dev(synth.normal(60 + 2 * i + j, (n * cols * page, heads * d))))
+        for name in ("masks", "lens_out", "counts", "att"):
+            state[name].zero_()
+
+    def results():
+        torch.cuda.synchronize()
+        return [t.clone() for t in list(state.values()) + list(out.values()) + [c for pair in caches for c in pair]]
+
+    load(1)
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    device_error(A)
+    for seed in (2, 3, 4):
+        load(seed)
+        step()
+        want = results()
+        load(seed)
+        g.replay()
+        assert all(torch.equal(a, b) for a, b in zip(results(), want))
+        assert int(state["counts"][1]) > 0
+    assert device_error(A) == 0
