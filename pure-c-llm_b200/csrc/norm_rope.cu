@@ -478,10 +478,13 @@ __device__ __forceinline__ float sum_of(uint64_t x) {
     f2_split(x, a, b);
     return a + b;
 }
-// 1 / sqrt(x): the approximation and one step of Newton's, within 2^-23.  (The
-// rounded one is some 20 instructions.)  Of 0 and infinity as it is.
-__device__ __forceinline__ float inverse_root(float x) {
-    const float r = rsqrtf(x), better = r * fmaf(-0.5f * x * r, r, 1.5f);
+// 1 / sqrt(x).  For fp32 results the approximation (within 2^-22.9) and one step
+// of Newton's, within 2^-23 (the rounded one is some 20 instructions); what is
+// rounded to bf16 takes the approximation.  Of 0 and infinity as it is.
+template <typename T> __device__ __forceinline__ float inverse_root(float x) {
+    const float r = rsqrtf(x);
+    if constexpr (sizeof(T) == 2) return r;
+    const float better = r * fmaf(-0.5f * x * r, r, 1.5f);
     return x > 0.f && x < INFINITY ? better : r;
 }
 
@@ -611,7 +614,7 @@ norm_rope_direct_kernel(const __grid_constant__ Params p)
             }
             group_sums(r, p, x.mask);
 #pragma unroll
-            for (int h = 0; h < H; h++) r[h] = inverse_root(fmaf(r[h], p.inv_d, p.eps));
+            for (int h = 0; h < H; h++) r[h] = inverse_root<T>(fmaf(r[h], p.inv_d, p.eps));
         }
 #pragma unroll
         for (int h = 0; h < H; h++) {
@@ -758,7 +761,7 @@ norm_rope_bwd_direct_kernel(const __grid_constant__ Params p)
         group_sums(sq, p, x.mask);
 #pragma unroll
         for (int h = 0; h < H; h++) {
-            const float r = inverse_root(fmaf(sq[2 * h], p.inv_d, p.eps)), k = -r * r * (sq[2 * h + 1] * p.inv_d);
+            const float r = inverse_root<T>(fmaf(sq[2 * h], p.inv_d, p.eps)), k = -r * r * (sq[2 * h + 1] * p.inv_d);
             if (h >= n) continue;
             const uint64_t rr = f2(r, r), kk = f2(k, k);
             uint64_t g[2], f[2], u[2];
