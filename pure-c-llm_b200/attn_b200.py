@@ -250,14 +250,25 @@ def _dtype_code(t):
 
 def _device() -> int:
     """Number of torch's current device."""
-    import torch
-    return torch._C._cuda_getDevice()
+    return _torch()._C._cuda_getDevice()
 
 
 def _stream():
     """Handle of torch's current stream on the current device."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    cuda = _torch()._C
+    return cuda._cuda_getCurrentRawStream(cuda._cuda_getDevice())
+
+
+_TORCH = None
+
+
+def _torch():
+    """The torch module (imported with the first call; an import statement in each costs it 0.2 us)."""
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        _TORCH = torch
+    return _TORCH
 
 
 def forward_t(q, k, v, heads: int, batch: int, out=None, lse=None, want_lse=True):
@@ -507,15 +518,14 @@ class HeadNorm(HeadNormPtrs):
 
 def _norm_holds(device, norm, head_dim):
     """The weights of a HeadNorm have a head's elements (those of bare addresses cannot be looked at)."""
-    import torch
     if isinstance(norm, HeadNorm):
+        torch = _torch()
         _dense(device, ("q_weight", norm.tensors[0], torch.float32, head_dim), ("k_weight", norm.tensors[1], torch.float32, head_dim))
 
 
 def norm_rope_t(shape: RopeShape, norm: HeadNormPtrs, table, positions, q, k, q_out, k_out):
     """attn_norm_rope_ex on (tokens, heads * d) fp32 or bf16 tensors; positions int32 or None; k and k_out may be None."""
-    import torch
-    on, n, d, dtype = _device(), shape.tokens, shape.head_dim, q.dtype
+    torch, on, n, d, dtype = _torch(), _device(), shape.tokens, shape.head_dim, q.dtype
     _dense(on, ("table", table, torch.float32, shape.max_pos * shape.rot_dim), ("positions", positions, torch.int32, n))
     _norm_holds(on, norm, d)
     _rows(on, dtype, "q", q, n, shape.heads * d, shape.q_row_stride)
@@ -535,8 +545,7 @@ def norm_rope_bwd_t(shape: RopeShape, norm: HeadNormPtrs, table, positions, q, k
                     dk_weight=None, accumulate=False, workspace=None):
     """attn_norm_rope_bwd_ex: dq and dk lie as q and k, dq_out and dk_out as the forward's outputs.  With weight
     gradients and no workspace, one is allocated."""
-    import torch
-    on, n, d, dtype = _device(), shape.tokens, shape.head_dim, q.dtype
+    torch, on, n, d, dtype = _torch(), _device(), shape.tokens, shape.head_dim, q.dtype
     _dense(on, ("table", table, torch.float32, shape.max_pos * shape.rot_dim), ("positions", positions, torch.int32, n),
            ("dq_weight", dq_weight, torch.float32, d), ("dk_weight", dk_weight, torch.float32, d),
            ("workspace", workspace, workspace.dtype if workspace is not None else None, 0))
@@ -556,8 +565,7 @@ def norm_rope_bwd_t(shape: RopeShape, norm: HeadNormPtrs, table, positions, q, k
 
 def norm_rope_append_t(shape: RopeShape, norm: HeadNormPtrs, cache: PagedKV, table, positions, slot_map, q, k, v, q_out):
     """attn_norm_rope_append_ex: positions int32 or None, slot_map int64."""
-    import torch
-    on, n, d, heads, dtype = _device(), shape.tokens, shape.head_dim, shape.kv_heads, q.dtype
+    torch, on, n, d, heads, dtype = _torch(), _device(), shape.tokens, shape.head_dim, shape.kv_heads, q.dtype
     _dense(on, ("table", table, torch.float32, shape.max_pos * shape.rot_dim), ("positions", positions, torch.int32, n),
            ("slot_map", slot_map, torch.int64, n))
     _norm_holds(on, norm, d)
@@ -605,8 +613,7 @@ def prefix_decode_t(shape: PrefixShape, cache: PagedKV, q, group_begin, prefix_t
 def tree_plan_t(cu_rows, parents, positions, positions_out, masks):
     """attn_tree_plan_ex: int32 tensors; cu_rows (n_seq + 1), masks (rows, words), the others (rows).  positions_out may
     be positions."""
-    import torch
-    on, i32, rows = _device(), torch.int32, parents.numel()
+    on, i32, rows = _device(), _torch().int32, parents.numel()
     if masks.dim() != 2:
         raise ValueError(f"masks, {tuple(masks.shape)}, is not (rows, words)")
     _dense(on, ("cu_rows", cu_rows, i32, 1), ("parents", parents, i32, 0), ("positions", positions, i32, rows),
@@ -624,15 +631,16 @@ def tree_decode_t(shape: TreeShape, cache: PagedKV, q, cu_rows, ctx_lens, lens, 
                   prefix_table=None, prefix_lens=None, workspace=None):
     """attn_tree_decode_ex: q and out (n_rows, heads * d); masks (n_rows, mask_words) int32 or None; tables and lengths
     int32; the groups' tensors may be None when shape.n_groups is 0.  Without a workspace one is allocated."""
-    import torch
+    torch = _torch()
     on, n, rows, groups, heads, d, i32 = _device(), shape.n_seq, shape.n_rows, shape.n_groups, shape.heads, shape.head_dim, torch.int32
     dtype = torch.bfloat16 if shape.dtype == BF16 else torch.float32
     _dense(on, ("cu_rows", cu_rows, i32, n + 1), ("ctx_lens", ctx_lens, i32, n), ("lens", lens, i32, n),
-           ("masks", masks, i32, rows * shape.mask_words), ("lse", lse, torch.float32, rows * heads),
+           ("lse", lse, torch.float32, rows * heads),
            ("workspace", workspace, workspace.dtype if workspace is not None else None, 0))
     if groups > 0:
         _dense(on, ("group_begin", group_begin, i32, groups + 1), ("prefix_lens", prefix_lens, i32, groups))
         _rows(on, i32, "prefix_table", prefix_table, groups, shape.max_prefix_pages, 0)
+    _rows(on, i32, "masks", masks, rows, shape.mask_words, 0)
     _rows(on, i32, "block_table", block_table, n, shape.max_pages, 0)
     _rows(on, dtype, "q", q, rows, heads * d, shape.q_row_stride)
     _rows(on, dtype, "out", out, rows, heads * d, shape.out_row_stride)
@@ -660,8 +668,7 @@ def cache_array(caches):
 def tree_commit_t(shape: PageShape, caches, kv_heads: int, head_dim: int, cu_rows, ctx_lens, lens, leaf, masks, block_table, free_pages,
                   free_count, lens_out, counts):
     """attn_tree_commit_ex: caches by cache_array; int32 tensors; masks (rows, words) or None (chains, of up to 1024)."""
-    import torch
-    on, n, i32 = _device(), shape.n_seq, torch.int32
+    on, n, i32 = _device(), shape.n_seq, _torch().int32
     if masks is not None and masks.dim() != 2:
         raise ValueError(f"masks, {tuple(masks.shape)}, is not (rows, words)")
     words = masks.shape[1] if masks is not None else 32

@@ -114,6 +114,8 @@ def test_torch_forms(calls):  # noqa: F811
                         group_begin=kw["group_begin"], prefix_table=kw["prefix_table"], prefix_lens=kw["prefix_lens"], workspace=kw["workspace"])
     each_refused(decode, given, optional=("lse", "masks"))
     refused(decode, given, {"q": ints(9, 128, **f)}, TypeError)
+    for masks in (ints(18), ints(9, 3), ints(9, 1)):
+        refused(decode, given, {"masks": masks}, ValueError)
     with pytest.raises(ValueError, match="device 1"):
         decode(cache=A.PageCache.of(*(Given(torch.zeros((32, 64), **b), 1) for _ in range(2))), **given)
 
