@@ -1,6 +1,6 @@
 // abi_serve.cu -- the C ABI of serving over a paged cache
 // (include/attn_b200.h): argument checks and workspaces of the page plan, the
-// rotary embedding and the shared-prefix decode.
+// rotary embedding, plain and with normed heads, and the shared-prefix decode.
 #include <algorithm>
 
 #include "common.cuh"

@@ -10,11 +10,17 @@
 // r is formed again from x, which the backward pass reads anyway.
 //
 // Some 12 flops per element, 30 backward: memory bounds both.  A group of
-// lanes (the smallest power of two that covers a head with 16 bytes each)
-// takes kHeads heads of one token and keeps its place in the token's row over
-// the tokens that it strides over, so the weights stay in registers, and a
-// token's cosines and sines are read once for its heads.  Where the two
-// elements of a pair lie in different lanes, they meet in shared memory.
+// lanes takes a few heads of one token and keeps its place in the token's row
+// over the tokens that it strides over, so the weights stay where they are, and
+// a token's cosines and sines are read once for its heads.  Two kinds of kernels:
+//   direct, where the turned part is a multiple of 8 elements (4 in interleaved
+//   pairs) and rows are aligned to 4: a lane has both elements of its pairs, in
+//   fours, so a head needs no exchange but its sum;
+//   exchange, for the rest: a group is the smallest power of two of lanes that
+//   covers a head with 16 bytes each, takes kHeads heads, and where the two
+//   elements of a pair lie in different lanes, they meet in shared memory.
+// Through the exchange kernels the direct ones' cases took 2 to 4 times as long
+// (4096 tokens of 12/12 x 128 in fp32 53 us for 19.7, gradients 90 for 34.2; prompts 607 for 153).
 #include <algorithm>
 
 #include "common.cuh"
@@ -27,7 +33,7 @@ constexpr int kThreads = 256;
 constexpr int kHeads = 4, kHeadsBwd = 2;  // heads of a group
 constexpr int kCtas = 2;                  // of kThreads per SM, that the registers leave
 // The direct kernels' heads of a group and CTAs per SM.  Forward, 32749 tokens of 32/8 x 128 in bf16 with 4 heads and 3
-// CTAs 157 us, 4 and 4 (spilling) 177, 8 and 2 177, 4 and 2 220; 4096 of 12/12 x 128 in fp32 with 3 and 3 19.7 us,
+// CTAs 157 us (153 with inverse_root below), 4 and 4 (spilling) 177, 8 and 2 177, 4 and 2 220; 4096 of 12/12 x 128 in fp32 with 3 and 3 19.7 us,
 // 4 and 3 22.2, 2 and 3 20.3.  Backward with the next token's loads on their way while this one's are worked on, 2 CTAs:
 // fp32 with 2 heads 34.1 us (without 36.2; 3 heads 42.1, 3 CTAs 55), 8192 of 16/4 x 64 in bf16 with 4 heads 23 us (without 29.8).
 constexpr int direct_heads(size_t element) { return element == 2 ? 4 : 3; }

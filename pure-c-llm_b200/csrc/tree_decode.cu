@@ -335,8 +335,11 @@ size_t lay_out(Part &w, const Params &p, int d, int seg_rows, int keys, int grid
 template <typename KV, int D>
 int join(const Params &p, const Part &w, cudaStream_t s) {
     using namespace attn::prefix;
+    // SHARED while the tokens' units leave most warps without one (fp32, 16 heads of
+    // 32, contexts of up to 500: 32 tokens 15.8 us, 17.4 unshared, 128 tokens 17.6 to
+    // 18.5, 256 tokens 25.6 to 22.4, 512 41.2 to 34.2)
     const int units = (p.heads + 3) / 4;
-    const bool shared = (long long)p.n_seq * units < 8LL * sm_count_here();
+    const bool shared = (long long)p.n_seq * units < 4LL * sm_count_here();
     return check_pdl(launch_pdl(shared ? tree_join_kernel<KV, D, true> : tree_join_kernel<KV, D, false>,
                                 dim3(p.n_seq, shared ? units : (units + kJoinWarps - 1) / kJoinWarps), dim3(kJoinWarps * 32), 0, s, p, w),
                      "tree_join_kernel");
@@ -362,20 +365,35 @@ int run_tile(const Params &p, void *ws, size_t *need, cudaStream_t s) {
 }
 
 // Paths by the query rows that a line has on average (counted from the shape:
-// their numbers are on the device), as for prefixes (prefix_decode.cu).
+// their numbers are on the device), as for prefixes (prefix_decode.cu).  n rows
+// of capacity, lines of 1 to n rows (us, 64 requests, 500 to 4500 rows of context):
+//   bf16, tiles or warps with blocks of 16 (d 128) or 32 (d 64) rows.  d 128, 32/8
+//     heads: n 16 73 to 66, n 32 75 to 80, n 64 84 to 120; 8 groups sharing 8192
+//     rows, n 32 of a group 94 to 113, 64 93 to 151.  d 64, 32 heads (twice
+//     the segments for the same bytes): n 16 202 to 131, n 31 216 to 149, n 63 241 to
+//     224 (all of n rows: n 48 264 to 302, n 64 300 to 338); groups with n 32 261
+//     to 154, n 64 261 to 235, n 128 271 to 333.
+//   bf16, blocks of 8 rows or of 16 or 32: d 128, n 8 64 to 66, n 16 78 to 66.
+//   INT8, blocks of 4 rows or of 16 (d 64) or 8 (d 128): d 64, n 4 126 to 231, n 8
+//     180 to 235 (all of 8 rows 233 to 241), n 12 238 to 240; d 32, n 8 294 to 360;
+//     d 128, n 4 126 to 135, n 8 170 to 144; d 96, n 8 138 to 129.
+//   fp32, blocks of 4 rows or of 8: d 32, n 4 103 to 136, n 8 142 to 134; d 128, n 4
+//     407 to 392, n 8 598 to 390.
 template <int D>
 int run_d(const Params &p, int kv_dtype, void *ws, size_t *need, cudaStream_t s) {
     using namespace attn::prefix;
     const long long all = (long long)p.n_seq * p.ratio, rows = (all + p.n_req - 1) / p.n_req;
     if (kv_dtype == ATTN_BF16) {
         if constexpr (D == 64 || D == 128) {
-            if (rows >= 32 || (p.n_groups && p.max_prefix_len && all >= 32LL * p.n_groups)) return run_tile<D>(p, ws, need, s);
+            constexpr int OWN_ROWS = D == 64 ? 64 : 32, GROUP_ROWS = D == 64 ? 128 : 32;
+            if (rows >= OWN_ROWS || (p.n_groups && p.max_prefix_len && all >= (long long)GROUP_ROWS * p.n_groups))
+                return run_tile<D>(p, ws, need, s);
         }
         if (rows <= 8) return run<__nv_bfloat16, Bf16Path<D, 1>, D>(p, ws, need, s);
         return run<__nv_bfloat16, Bf16Path<D, D == 32 ? 8 : D == 64 ? 4 : 2>, D>(p, ws, need, s);
     }
     if (kv_dtype == ATTN_I8) {
-        if (rows <= 4) return run<int8_t, I8Path<D, 1>, D>(p, ws, need, s);
+        if (rows <= (D <= 64 ? 8 : 4)) return run<int8_t, I8Path<D, 1>, D>(p, ws, need, s);
         return run<int8_t, I8Path<D, D <= 64 ? 4 : 2>, D>(p, ws, need, s);
     }
     if (rows <= 4) return run<float, F32Path<D, 4>, D>(p, ws, need, s);

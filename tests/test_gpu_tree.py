@@ -240,6 +240,7 @@ def test_tree_query_rows(A, kind, drafts, ratio):
     (64, 16, 4, 16, [32] * 6, [129, 127, 400, 0, 3, 1000], (4, 2), (1000, 300)),
     (128, 4, 4, 4, [128, 60], [300, 257], (2,), (500,)),
     (64, 8, 1, 128, [100, 20, 16], [2000, 5, 50], (3,), (4097,)),
+    (64, 2, 2, 16, [5] * 40, [30] * 20 + [1] * 20, (40,), (300,)),
 ])
 def test_tree_tiles(A, d, heads, kv_heads, page, drafts, ctx, groups, prefix):
     """bf16 lines of many query rows: up to 128 of a block, more, pages below a box, prefixes beside contexts."""
