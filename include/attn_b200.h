@@ -490,7 +490,8 @@ ATTN_API int attn_norm_rope_ex(const attn_rope_shape *s, const attn_head_norm *n
  * dk_out of its outputs: dq, dk (SET; their rows lie as those of q and k, the
  * others as those of q_out and k_out) and, where wanted, the weights' gradients
  * dq_weight, dk_weight (head_dim floats, summed over tokens and heads; NULL:
- * not wanted; accumulate = 1 adds to them, 0 sets them).  dq may be dq_out or q
+ * not wanted; accumulate = 1 adds to them, 0 sets them; they must not overlap,
+ * where one weight serves both as well).  dq may be dq_out or q
  * where the row strides of the two are the same, dk likewise; k, dk_out and dk
  * may all be NULL (a dk_weight is then as over no tokens).  The same result on
  * every run.  `workspace` (256-byte aligned) is needed when a weight's gradient

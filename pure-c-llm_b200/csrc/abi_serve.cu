@@ -213,6 +213,9 @@ int attn_norm_rope_bwd_ex(const attn_rope_shape *s, const attn_head_norm *n, int
         if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
             return set_error(ATTN_ERR_WORKSPACE, "norm rope backward: weight gradients need a workspace of %zu bytes (256-byte aligned), got %zu",
                              need, workspace ? workspace_bytes : 0);
+        const size_t w = (size_t)s->head_dim * 4;
+        if (dq_weight && dk_weight && overlap(dq_weight, w, dk_weight, w))
+            return set_error(ATTN_ERR_INVALID, "norm rope backward: dq_weight and dk_weight overlap");
     }
     int *err = device_error_ptr();
     if (!err) return set_error(ATTN_ERR_CUDA, "norm rope backward: no device error word");

@@ -49,6 +49,8 @@ def test_backward_refusals():
     for bad in (dict(ws=None), dict(ws=P + 16), dict(ws_bytes=need - 1)):
         assert call(shape, **bad) == A.ERR_WORKSPACE, bad
     assert A.norm_rope_bwd_workspace_bytes(A.RopeShape(**{**OK, "head_dim": 80})) == 0
+    for dkw in (Q, Q + 4 * 63, Q - 4 * 63):                # one weight for q and k has two gradients
+        assert call(shape, dkw=dkw) == A.ERR_INVALID and "overlap" in A.last_error()
 
 
 def test_append_refusals():
