@@ -180,6 +180,12 @@ int attn_tree_commit_ex(const attn_page_shape *s, int n_layers, const attn_paged
     const size_t n = (size_t)s->n_seq * 4;
     if (overlap(lens_out, n, lens, n) || overlap(lens_out, n, ctx_lens, n) || overlap(lens_out, n, leaf, n) || overlap(counts, 16, free_count, 4))
         return set_error(ATTN_ERR_INVALID, "tree commit: lens_out and counts must not overlap lens, ctx_lens, leaf and free_count");
+    // (buffers that meet in part are left to the caller: layers may be interleaved in one)
+    for (int i = 0; i < n_layers; i++) {
+        bool twice = caches[i].k == caches[i].v;
+        for (int j = 0; j < i; j++) twice |= caches[i].k == caches[j].k || caches[i].v == caches[j].v;
+        if (twice) return set_error(ATTN_ERR_INVALID, "tree commit: the K or V of layer %d is there twice", i);
+    }
     int *err = device_error_ptr();
     if (!err) return set_error(ATTN_ERR_CUDA, "tree commit: no device error word");
     return launch_tree_commit(s, n_layers, caches, kv_heads, head_dim, cu_rows, ctx_lens, lens, leaf, masks, mask_words, block_table,

@@ -85,6 +85,9 @@ def test_commit_refusals():
                 dict(counts=None), dict(lens=P + 2), dict(masks=P + 1), dict(out=P + 4), dict(counts=P)):
         assert call(shape, **bad) == A.ERR_INVALID, bad
     assert "overlap" in A.last_error()
+    # a cache twice would have its rows moved twice at the same time
+    for caches in ((kv(), kv()), (kv(), kv(k=P + (1 << 20))), (kv(), kv(v=P + (1 << 20))), (kv(v=P), kv(k=P + (1 << 20), v=P + (2 << 20)))):
+        assert call(shape, caches=caches) == A.ERR_INVALID and "twice" in A.last_error()
 
 
 def test_torch_forms(calls):  # noqa: F811
