@@ -91,9 +91,9 @@ __device__ __forceinline__ void run_piece(const Params &p, uint32_t ring, const 
     path.finish(o, ml, rows);
 }
 
-// Slots of a warp's ring: as many (an odd number) as CTAS rings of kWarps fit an SM, up to 7.
-template <class Path, int CTAS> struct Ring {
-    static constexpr int FIT = ((CTAS == 1 ? 216 : 108) * 1024 / kWarps - Path::SCRATCH) / Path::SLOT;
+// Slots of a warp's ring: as many (an odd number) as CTAS rings of WARPS fit an SM, up to 7.
+template <class Path, int CTAS, int WARPS> struct Ring {
+    static constexpr int FIT = ((CTAS == 1 ? 216 : 108) * 1024 / WARPS - Path::SCRATCH) / Path::SLOT;
     static constexpr int SLOTS = FIT > 7 ? 7 : (FIT - 1) / 2 * 2 + 1;
     static constexpr int BYTES = SLOTS * Path::SLOT + Path::SCRATCH;
     static_assert(Path::SLOT % 128 == 0 && Path::SCRATCH % 128 == 0, "swizzled rows begin on 128 bytes");
@@ -102,11 +102,11 @@ template <class Path, int CTAS> struct Ring {
 // `second`: the launch before this one is the prefix part's, which has waited
 // for the work before it when this one may start; the two run side by side, and
 // this one ends after both.
-template <class Path, int LINES, int D, int CTAS>
-__global__ void __launch_bounds__(kWarps * 32, CTAS)
+template <class Path, int LINES, int D, int CTAS, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, CTAS)
 prefix_rows_kernel(const __grid_constant__ Params p, const __grid_constant__ Part w, int second)
 {
-    using R = Ring<Path, CTAS>;
+    using R = Ring<Path, CTAS, WARPS>;
     extern __shared__ __align__(128) uint8_t ring_bytes[];
     __shared__ long long sums[kEntries + 1];
     __shared__ long long warp_sums[32];
@@ -137,15 +137,16 @@ int sm_count_here();
 bool ensure_smem_attr(const void *func, size_t bytes);
 
 // Divides a part among the teams of `grid` CTAs: key heads per team, query rows of a block, keys of a step.
-inline void divide_part(attn::prefix::Part &w, const attn::prefix::Params &p, int lines, int seg_rows, int keys, int grid, bool tile) {
+inline void divide_part(attn::prefix::Part &w, const attn::prefix::Params &p, int lines, int seg_rows, int keys, int grid, bool tile,
+                        int warps = attn::prefix::kWarps) {
     using namespace attn::prefix;
     w.lines = lines;
     w.per_entry = (lines + kEntries - 1) / kEntries;
     w.entries = (lines + w.per_entry - 1) / w.per_entry;
     // Key heads per team: adjacent ones, in blocks that leave as few of a CTA's warps idle as may be.
     int best = 0;
-    for (int n = tile ? p.kv_heads : (p.kv_heads + kWarps - 1) / kWarps; n <= p.kv_heads; n++) {
-        const int block = (p.kv_heads + n - 1) / n, splits = tile ? 1 : kWarps / block;
+    for (int n = tile ? p.kv_heads : (p.kv_heads + warps - 1) / warps; n <= p.kv_heads; n++) {
+        const int block = (p.kv_heads + n - 1) / n, splits = tile ? 1 : warps / block;
         const int used = p.kv_heads * splits * 1000 / n;          // warps at work, in thousandths
         if (used <= best) continue;
         best = used;
@@ -159,13 +160,13 @@ inline void divide_part(attn::prefix::Part &w, const attn::prefix::Params &p, in
     w.half = tile ? 128 : 0;
 }
 
-template <class Path, int LINES, int D, int CTAS>
+template <class Path, int LINES, int D, int CTAS, int WARPS = attn::prefix::kWarps>
 int run_part(const attn::prefix::Params &p, const attn::prefix::Part &w, int second, cudaStream_t s) {
     using namespace attn::prefix;
-    using R = Ring<Path, CTAS>;
-    const auto kernel = prefix_rows_kernel<Path, LINES, D, CTAS>;
+    using R = Ring<Path, CTAS, WARPS>;
+    const auto kernel = prefix_rows_kernel<Path, LINES, D, CTAS, WARPS>;
     const int warps = w.splits * w.head_block;
-    if (!ensure_smem_attr((const void *)kernel, (size_t)R::BYTES * kWarps))
+    if (!ensure_smem_attr((const void *)kernel, (size_t)R::BYTES * WARPS))
         return set_error(ATTN_ERR_CUDA, "paged decode: cannot set shared-memory size");
     return check_pdl(launch_pdl(kernel, dim3(w.teams / w.splits), dim3(warps * 32), (size_t)R::BYTES * warps, s, p, w, second),
                      "prefix_rows_kernel");

@@ -310,10 +310,10 @@ using attn::prefix::Part;
 
 // The part on the workspace `base` (NULL to learn its size), in pieces of up to
 // seg_rows query rows.
-size_t lay_out(Part &w, const Params &p, int d, int seg_rows, int keys, int grid, bool tile, char *base) {
+size_t lay_out(Part &w, const Params &p, int d, int seg_rows, int keys, int grid, bool tile, int warps, char *base) {
     using namespace attn::prefix;
     w = {};
-    divide_part(w, p, p.n_groups + p.n_req, seg_rows, keys, grid, tile);
+    divide_part(w, p, p.n_groups + p.n_req, seg_rows, keys, grid, tile, warps);
     const long long rows = (long long)p.n_seq * p.ratio, heads = (long long)w.n_blocks * w.head_block;
     w.rows = tile ? seg_rows : (int)std::min<long long>(rows, seg_rows);
     w.after = p.n_groups ? (rows + (long long)w.half * p.n_groups) * heads : 0;
@@ -345,59 +345,100 @@ int join(const Params &p, const Part &w, cudaStream_t s) {
                      "tree_join_kernel");
 }
 
-template <typename KV, class Path, int D>
+template <typename KV, class Path, int D, int WARPS = attn::prefix::kWarps>
 int run(const Params &p, void *ws, size_t *need, cudaStream_t s) {
     using namespace attn::prefix;
     constexpr int CTAS = Path::LEAN ? 2 : 1;
     Part w;
-    const size_t bytes = lay_out(w, p, D, Path::ROWS, Path::KEYS, sm_count_here() * CTAS, false, static_cast<char *>(ws));
+    const size_t bytes = lay_out(w, p, D, Path::ROWS, Path::KEYS, sm_count_here() * CTAS, false, WARPS, static_cast<char *>(ws));
     if (need) { *need = bytes; return ATTN_OK; }
-    const int st = run_part<Path, TREES, D, CTAS>(p, w, 0, s);
+    const int st = run_part<Path, TREES, D, CTAS, WARPS>(p, w, 0, s);
     return st ? st : join<KV, D>(p, w, s);
 }
 template <int D>
 int run_tile(const Params &p, void *ws, size_t *need, cudaStream_t s) {
     Part w;
-    const size_t bytes = lay_out(w, p, D, 256, 128, sm_count_here(), true, static_cast<char *>(ws));
+    const size_t bytes = lay_out(w, p, D, 256, 128, sm_count_here(), true, 0, static_cast<char *>(ws));
     if (need) { *need = bytes; return ATTN_OK; }
     const int st = launch_tree_tile(p, w, D, s);
     return st ? st : join<__nv_bfloat16, D>(p, w, s);
 }
 
-// Paths by the query rows that a line has on average (counted from the shape:
-// their numbers are on the device), as for prefixes (prefix_decode.cu).  n rows
-// of capacity, lines of 1 to n rows (us, 64 requests, 500 to 4500 rows of context):
-//   bf16, tiles or warps with blocks of 16 (d 128) or 32 (d 64) rows.  d 128, 32/8
-//     heads: n 16 73 to 66, n 32 75 to 80, n 64 84 to 120; 8 groups sharing 8192
-//     rows, n 32 of a group 94 to 113, 64 93 to 151.  d 64, 32 heads (twice
-//     the segments for the same bytes): n 16 202 to 131, n 31 216 to 149, n 63 241 to
-//     224 (all of n rows: n 48 264 to 302, n 64 300 to 338); groups with n 32 261
-//     to 154, n 64 261 to 235, n 128 271 to 333.
-//   bf16, blocks of 8 rows or of 16 or 32: d 128, n 8 64 to 66, n 16 78 to 66.
-//   INT8, blocks of 4 rows or of 16 (d 64) or 8 (d 128): d 64, n 4 126 to 231, n 8
-//     180 to 235 (all of 8 rows 233 to 241), n 12 238 to 240; d 32, n 8 294 to 360;
-//     d 128, n 4 126 to 135, n 8 170 to 144; d 96, n 8 138 to 129.
-//   fp32, blocks of 4 rows or of 8: d 32, n 4 103 to 136, n 8 142 to 134; d 128, n 4
-//     407 to 392, n 8 598 to 390.
+// The path with the least time, by bounds: rows of keys (the shape's bounds of
+// the lengths, as the lengths are on the device) times the blocks of query rows
+// that pass over them (the rows that a line has on average) times what such a
+// pass costs.  Costs are us of full blocks, one to each of 64 contexts of 500 to
+// 4500 rows (bf16, 500 to 8200 for INT8, 250 to 4000 for fp32; 0.25 to 0.6 GB), and
+// both sides of each choice follow from them and hold as measured:
+//   bf16, d 64, 32 heads, tiles, blocks of 32, 16, 8: 16 rows 202, 143, 114, 180, 32 rows
+//     235, 171, 204, 341, 64 rows 300, 338, -, 686; 8 groups sharing 8192 rows, 32 rows
+//     of a group 261, 154, -, 264, 128 rows 271, 333, -, 616.
+//   bf16, d 128, 8 key heads, tiles, blocks of 16, 8: 16 rows 73, 68, 92, 32 rows 83, 105, 157.
+//   bf16, d 32, blocks of 64, 16, 8: 8 rows 157, 72, 63, 32 rows 191, 148, 184, 64 rows 246, 298, 367.
+//   INT8, d 64, blocks of 16, 8, 4: 4 rows 229, 156, 127, 8 rows 240, 165, 234, 16 rows 252, 306, -.
+//   fp32, d 32, blocks of 8, 4: 4 rows 132, 104, 8 rows 139, 177; d 128 210, 231 and 215, 404.
+// Lines of fewer rows than the shape leaves room for would want smaller blocks:
+// INT8 with room for 16 rows and 8 on average takes 245 in blocks of 16, 234 in 8.
+template <int N>
+int least(const Params &p, const int (&blocks)[N], const int (&costs)[N]) {
+    const long long all = (long long)p.n_seq * p.ratio, own = (all + p.n_req - 1) / p.n_req, group = p.n_groups ? (all + p.n_groups - 1) / p.n_groups : 0;
+    int best = 0;
+    double time = 0.;
+    for (int i = 0; i < N; i++) {
+        const double passes = (double)p.n_req * p.max_len * (double)((own + blocks[i] - 1) / blocks[i]) +
+                              (double)p.n_groups * p.max_prefix_len * (double)((group + blocks[i] - 1) / blocks[i]);
+        if (i && passes * costs[i] >= time) continue;
+        best = i;
+        time = passes * costs[i];
+    }
+    return best;
+}
+// Blocks of 8 INT8 or 16 bf16 rows at d 32 and 64 leave the registers for 12
+// warps an SM (INT8, d 64: 160 us, 183 with 8 warps; bf16 104 and 109).
+constexpr int kMoreWarps = 12;
+
 template <int D>
 int run_d(const Params &p, int kv_dtype, void *ws, size_t *need, cudaStream_t s) {
     using namespace attn::prefix;
-    const long long all = (long long)p.n_seq * p.ratio, rows = (all + p.n_req - 1) / p.n_req;
+    using B = __nv_bfloat16;
     if (kv_dtype == ATTN_BF16) {
-        if constexpr (D == 64 || D == 128) {
-            constexpr int OWN_ROWS = D == 64 ? 64 : 32, GROUP_ROWS = D == 64 ? 128 : 32;
-            if (rows >= OWN_ROWS || (p.n_groups && p.max_prefix_len && all >= (long long)GROUP_ROWS * p.n_groups))
-                return run_tile<D>(p, ws, need, s);
+        if constexpr (D == 32) {
+            switch (least<3>(p, {8, 16, 64}, {63, 82, 220})) {
+                case 0: return run<B, Bf16Path<D, 1>, D>(p, ws, need, s);
+                case 1: return run<B, Bf16Path<D, 2>, D, kMoreWarps>(p, ws, need, s);
+                default: return run<B, Bf16Path<D, 8>, D>(p, ws, need, s);
+            }
+        } else if constexpr (D == 64) {
+            switch (least<4>(p, {8, 16, 32, 128}, {103, 114, 171, 250})) {
+                case 0: return run<B, Bf16Path<D, 1>, D>(p, ws, need, s);
+                case 1: return run<B, Bf16Path<D, 2>, D, kMoreWarps>(p, ws, need, s);
+                case 2: return run<B, Bf16Path<D, 4>, D>(p, ws, need, s);
+                default: return run_tile<D>(p, ws, need, s);
+            }
+        } else if constexpr (D == 96) {
+            return least<2>(p, {8, 16}, {50, 55}) ? run<B, Bf16Path<D, 2>, D>(p, ws, need, s) : run<B, Bf16Path<D, 1>, D>(p, ws, need, s);
+        } else {
+            switch (least<3>(p, {8, 16, 128}, {64, 68, 90})) {
+                case 0: return run<B, Bf16Path<D, 1>, D>(p, ws, need, s);
+                case 1: return run<B, Bf16Path<D, 2>, D>(p, ws, need, s);
+                default: return run_tile<D>(p, ws, need, s);
+            }
         }
-        if (rows <= 8) return run<__nv_bfloat16, Bf16Path<D, 1>, D>(p, ws, need, s);
-        return run<__nv_bfloat16, Bf16Path<D, D == 32 ? 8 : D == 64 ? 4 : 2>, D>(p, ws, need, s);
     }
     if (kv_dtype == ATTN_I8) {
-        if (rows <= (D <= 64 ? 8 : 4)) return run<int8_t, I8Path<D, 1>, D>(p, ws, need, s);
-        return run<int8_t, I8Path<D, D <= 64 ? 4 : 2>, D>(p, ws, need, s);
+        if constexpr (D <= 64) {
+            switch (D == 32 ? least<3>(p, {4, 8, 16}, {200, 253, 365}) : least<3>(p, {4, 8, 16}, {127, 163, 245})) {
+                case 0: return run<int8_t, I8Path<D, 1>, D>(p, ws, need, s);
+                case 1: return run<int8_t, I8Path<D, 2>, D, kMoreWarps>(p, ws, need, s);
+                default: return run<int8_t, I8Path<D, 4>, D>(p, ws, need, s);
+            }
+        } else {
+            return (D == 96 ? least<2>(p, {4, 8}, {103, 133}) : least<2>(p, {4, 8}, {130, 146})) ? run<int8_t, I8Path<D, 2>, D>(p, ws, need, s)
+                                                                                               : run<int8_t, I8Path<D, 1>, D>(p, ws, need, s);
+        }
     }
-    if (rows <= 4) return run<float, F32Path<D, 4>, D>(p, ws, need, s);
-    return run<float, F32Path<D, 8>, D>(p, ws, need, s);
+    const bool eight = D == 32 ? least<2>(p, {4, 8}, {104, 137}) : D == 64 ? least<2>(p, {4, 8}, {193, 226}) : least<2>(p, {4, 8}, {231, 213});
+    return eight ? run<float, F32Path<D, 8>, D>(p, ws, need, s) : run<float, F32Path<D, 4>, D>(p, ws, need, s);
 }
 
 }  // namespace

@@ -235,6 +235,17 @@ def test_tree_query_rows(A, kind, drafts, ratio):
         c.check(*c.run())
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("kv_heads", [1, 5, 13])
+def test_tree_blocks(A, kind, d, kv_heads):
+    """Blocks of each size at each head size, full and in part, with key heads that divide a CTA's warps and that do not."""
+    for drafts, groups in (([3, 4, 2, 4], ()), ([7, 5, 8, 8], ()), ([7, 5, 8, 8], (2, 1)), ([16, 9, 13, 16], ()), ([16, 30, 32, 25], (1, 2)),
+                           ([64, 50, 33, 60], ())):
+        c = TreeCase(A, d + len(groups), kind, d, kv_heads, kv_heads, 16, drafts, [300, 5, 31, 129], groups, (200, 65)[:len(groups)], spare=0)
+        c.check(*c.run())
+
+
 @pytest.mark.parametrize("d,heads,kv_heads,page,drafts,ctx,groups,prefix", [
     (128, 8, 2, 64, [40, 33, 1, 64], [700, 256, 128, 1], (), ()),
     (64, 16, 4, 16, [32] * 6, [129, 127, 400, 0, 3, 1000], (4, 2), (1000, 300)),
