@@ -634,8 +634,9 @@ ATTN_API int attn_tree_decode_ex(const attn_tree_shape *s, const attn_paged_kv *
 /* Keeps, of every request's drafts, the path that ends at draft leaf[s] (-1:
  * none): the drafts in the leaf's mask (masks NULL: drafts 0 .. leaf[s]) go, in
  * their order, to rows ctx_lens[s], ctx_lens[s] + 1, ... in each of the n_layers
- * caches (a HOST array, at most ATTN_MAX_LAYERS, all of one type and different
- * from one another, as layers that share a cache pass it once; K, V and scales), whose rows follow block_table.  Of the page shape, max_tokens is the
+ * caches (a HOST array, at most ATTN_MAX_LAYERS, all of one type; K, V and
+ * scales, none of them there twice in any part, as layers that share a cache
+ * pass it once), whose rows follow block_table.  Of the page shape, max_tokens is the
  * rows of masks.  Written besides:
  *   lens_out[n_seq]: ctx_lens + the drafts kept (lens where there were none);
  *   free_pages past *free_count: the pages behind the kept rows, in request and

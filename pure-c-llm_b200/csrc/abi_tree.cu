@@ -1,6 +1,8 @@
 // abi_tree.cu -- the C ABI of drafted token trees over a paged cache
 // (include/attn_b200.h): argument checks of the tree plan, the tree decode and
 // the commit.
+#include <algorithm>
+
 #include "common.cuh"
 #include "prefix.cuh"
 #include "serve_checks.cuh"
@@ -180,11 +182,19 @@ int attn_tree_commit_ex(const attn_page_shape *s, int n_layers, const attn_paged
     const size_t n = (size_t)s->n_seq * 4;
     if (overlap(lens_out, n, lens, n) || overlap(lens_out, n, ctx_lens, n) || overlap(lens_out, n, leaf, n) || overlap(counts, 16, free_count, 4))
         return set_error(ATTN_ERR_INVALID, "tree commit: lens_out and counts must not overlap lens, ctx_lens, leaf and free_count");
-    // (buffers that meet in part are left to the caller: layers may be interleaved in one)
+    // Rows and scales are moved by a CTA for each layer, K and V side by side, so none may be there twice, in whatever
+    // part.  (Buffers that meet otherwise are left to the caller: layers may be interleaved in one.)
+    const int arrays = n_layers && caches[0].kv_dtype == ATTN_I8 ? 4 : 2;
+    const void *held[4 * ATTN_MAX_LAYERS];
     for (int i = 0; i < n_layers; i++) {
-        bool twice = caches[i].k == caches[i].v;
-        for (int j = 0; j < i; j++) twice |= caches[i].k == caches[j].k || caches[i].v == caches[j].v;
-        if (twice) return set_error(ATTN_ERR_INVALID, "tree commit: the K or V of layer %d is there twice", i);
+        const void *const mine[4] = {caches[i].k, caches[i].v, caches[i].kscale, caches[i].vscale};
+        for (int a = 0; a < arrays; a++) {
+            const void **end = held + arrays * i + a;
+            if (std::find((const void **)held, end, mine[a]) != end)
+                return set_error(ATTN_ERR_INVALID, "tree commit: the %s of layer %d is there twice",
+                                 a < 2 ? "K or V" : "scale of K or V", i);
+            *end = mine[a];
+        }
     }
     int *err = device_error_ptr();
     if (!err) return set_error(ATTN_ERR_CUDA, "tree commit: no device error word");

@@ -90,6 +90,25 @@ def test_commit_refusals():
         assert call(shape, caches=caches) == A.ERR_INVALID and "twice" in A.last_error()
 
 
+def test_commit_refuses_an_array_in_another_part():
+    """K of one layer that is V of another, and scales that two layers, or K and V, share: rows and scales would be moved twice
+    at the same time."""
+    shape = A.PageShape(n_seq=4, page_size=16, max_pages=8, max_tokens=32, n_pages=64, table_stride=0)
+
+    def call(*caches):
+        caches = (A.PagedKV * len(caches))(*caches)
+        return A.lib.attn_tree_commit_ex(shape, len(caches), caches, 2, 64, P, P, P, P, P, 1, P, P, P, Q, Q + 64, None)
+
+    def layer(i, **kw):
+        at = {name: P + (4 * i + j + 1 << 20) for j, name in enumerate(("k", "v", "kscale", "vscale"))}
+        return kv(**{**at, **kw})
+    one, i8 = layer(0), dict(kv_dtype=A.I8)
+    for caches in ((one, layer(1, k=one.v)), (one, layer(1, v=one.k)), (one, layer(1), layer(2, v=one.k)),
+                   (layer(0, **i8), layer(1, kscale=one.kscale, **i8)), (layer(0, **i8), layer(1, vscale=one.vscale, **i8)),
+                   (layer(0, **i8), layer(1, vscale=one.kscale, **i8)), (layer(0, vscale=one.kscale, **i8),)):
+        assert call(*caches) == A.ERR_INVALID and "twice" in A.last_error(), A.last_error()
+
+
 def test_torch_forms(calls):  # noqa: F811
     import torch
     f, b = dict(dtype=torch.float32), dict(dtype=torch.bfloat16)
