@@ -636,8 +636,9 @@ ATTN_API int attn_tree_decode_ex(const attn_tree_shape *s, const attn_paged_kv *
  * their order, to rows ctx_lens[s], ctx_lens[s] + 1, ... in each of the n_layers
  * caches (a HOST array, at most ATTN_MAX_LAYERS, all of one type; K, V and
  * scales, none of them there twice in any part, as layers that share a cache
- * pass it once), whose rows follow block_table.  Of the page shape, max_tokens is the
- * rows of masks.  Written besides:
+ * pass it once), whose rows follow block_table.  Of the page shape, max_tokens is
+ * the rows of masks, to which cu_rows is clamped (without masks it is not looked
+ * at, nor is cu_rows clamped).  Written besides:
  *   lens_out[n_seq]: ctx_lens + the drafts kept (lens where there were none);
  *   free_pages past *free_count: the pages behind the kept rows, in request and
  *     page order (what passes n_pages entries is lost);

@@ -89,13 +89,15 @@ struct Accepted {
 __device__ __forceinline__ Accepted accepted(const CommitParams &p, int s, bool report) {
     Accepted a;
     const int cap = p.max_pages << p.log_page;
-    const int first = __ldg(p.cu_rows + s), end = __ldg(p.cu_rows + s + 1);
+    // (clamped to the rows of masks, as the plan and the decode clamp to theirs; chains have none)
+    const int most = p.masks ? p.n_rows : 0x7fffffff;
+    const int first = min(max(__ldg(p.cu_rows + s), 0), most), end = min(max(__ldg(p.cu_rows + s + 1), first), most);
     int leaf = __ldg(p.leaf + s);
     a.len = min(max(__ldg(p.lens + s), 0), cap);
     a.ctx = min(max(__ldg(p.ctx_lens + s), 0), a.len);
     a.drafts = min(a.len - a.ctx, 32 * p.words);
     // a leaf that is no draft accepts nothing; one of a request without drafted rows (refused ones) is not reported
-    if (leaf < -1 || leaf >= a.drafts || (leaf >= 0 && (first < 0 || end > p.n_rows || leaf >= end - first))) {
+    if (leaf < -1 || leaf >= a.drafts || leaf >= end - first) {
         if (report && a.drafts > 0) atomicExch(p.err, 0x706);
         leaf = -1;
     }

@@ -538,6 +538,48 @@ def test_commit_leaves_and_pages_that_are_none(A):
         np.testing.assert_array_equal(t.float().cpu().numpy(), w)
 
 
+def commit_of_rows(A, c, rows):
+    """The case's commit with `rows` rows of masks."""
+    import torch
+    shape = A.PageShape(c.n, c.page, c.table.shape[1], rows, len(c.free), 0)
+    free = dev(c.free)
+    lens_out, counts = (torch.full((n,), -9, dtype=torch.int32, device="cuda") for n in (c.n, 4))
+    A.tree_commit_t(shape, A.cache_array(c.kv), c.kv_heads, c.d, dev(c.cu), dev(c.ctx), dev(c.lens), dev(c.leaf),
+                    None if c.masks is None else dev(c.masks[:rows]), dev(c.table), free, dev(np.array([c.count], np.int32)), lens_out, counts)
+    return lens_out.cpu().numpy(), free.cpu().numpy(), counts.cpu().numpy()
+
+
+@pytest.mark.parametrize("kind", ["f32", "int8"])
+def test_commit_with_fewer_mask_rows_than_drafts(A, kind):
+    """cu_rows past the rows of masks: the drafts that have a row are drafts, as the plan and the decode have them, and the
+    others are none."""
+    for cut, leaves, want_leaf in ((2, [3, 4, 2], [3, 4, 2]), (2, [3, 4, 4], [3, 4, -1]), (5, [3, 5, 0], [3, 5, -1]), (8, [5, 2, 1], [5, 2, -1])):
+        c = CommitCase(A, 17 + cut, kind, 2, 2, 32, 4, [6, 6, 5], [5, 6, 7], leaves=leaves)
+        rows = int(c.cu[-1]) - cut
+        before = [t.float().cpu().numpy() for x in c.caches for t in x]
+        want = T.commit(c.cu, c.ctx, c.lens, np.array(want_leaf), c.masks, c.table, c.page, c.free, c.count, before)
+        device_error(A)
+        got = commit_of_rows(A, c, rows)
+        assert device_error(A) == (0x706 if want_leaf != leaves else 0)
+        for g, w in zip(got, want):
+            np.testing.assert_array_equal(g, w)
+        for t, w in zip((t for x in c.caches for t in x), before):
+            np.testing.assert_array_equal(t.float().cpu().numpy(), w)
+
+
+def test_commit_of_chains_needs_no_rows_of_masks(A):
+    c = CommitCase(A, 19, "f32", 1, 2, 32, 4, [6, 3, 40], [5, 6, 7], leaves=[4, -1, 39], chain=True)
+    device_error(A)
+    before = [t.float().cpu().numpy() for t in c.caches[0]]
+    want = T.commit(c.cu, c.ctx, c.lens, c.leaf, None, c.table, c.page, c.free, c.count, before)
+    got = commit_of_rows(A, c, 0)
+    assert device_error(A) == 0
+    for g, w in zip(got, want):
+        np.testing.assert_array_equal(g, w)
+    for t, w in zip(c.caches[0], before):
+        np.testing.assert_array_equal(t.float().cpu().numpy(), w)
+
+
 # ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------
