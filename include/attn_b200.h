@@ -647,7 +647,7 @@ ATTN_API int attn_tree_decode_ex(const attn_tree_shape *s, const attn_paged_kv *
  * A leaf that is no drafted row of its request keeps nothing and, unless the
  * request has no drafted rows, records 0x706 in the device error word; a page
  * outside a cache records 0x702 and its rows stay where they are.  lens_out and
- * counts must not overlap lens, ctx_lens, leaf and free_count. */
+ * counts must not overlap lens, ctx_lens, leaf, free_count and one another. */
 ATTN_API int attn_tree_commit_ex(const attn_page_shape *s, int n_layers, const attn_paged_kv *caches, int kv_heads, int head_dim,
                 const int *cu_rows, const int *ctx_lens, const int *lens, const int *leaf, const uint32_t *masks,
                 int mask_words, const int *block_table, int *free_pages, const int *free_count, int *lens_out,

@@ -180,8 +180,10 @@ int attn_tree_commit_ex(const attn_page_shape *s, int n_layers, const attn_paged
     for (const void *w : words)
         if (!aligned(w, 4)) return set_error(ATTN_ERR_INVALID, "tree commit: int arrays must be 4-byte aligned");
     const size_t n = (size_t)s->n_seq * 4;
-    if (overlap(lens_out, n, lens, n) || overlap(lens_out, n, ctx_lens, n) || overlap(lens_out, n, leaf, n) || overlap(counts, 16, free_count, 4))
-        return set_error(ATTN_ERR_INVALID, "tree commit: lens_out and counts must not overlap lens, ctx_lens, leaf and free_count");
+    const struct { const void *at; size_t bytes; } inputs[] = {{ctx_lens, n}, {lens, n}, {leaf, n}, {free_count, 4}};
+    for (const auto &in : inputs)
+        if (overlap(lens_out, n, in.at, in.bytes) || overlap(counts, 16, in.at, in.bytes))
+            return set_error(ATTN_ERR_INVALID, "tree commit: lens_out and counts must not overlap lens, ctx_lens, leaf and free_count");
     // Rows and scales are moved by a CTA for each layer, K and V side by side, so none may be there twice, in whatever
     // part.  (Buffers that meet otherwise are left to the caller: layers may be interleaved in one.)
     const int arrays = n_layers && caches[0].kv_dtype == ATTN_I8 ? 4 : 2;
@@ -196,6 +198,7 @@ int attn_tree_commit_ex(const attn_page_shape *s, int n_layers, const attn_paged
             *end = mine[a];
         }
     }
+    if (overlap(lens_out, n, counts, 16)) return set_error(ATTN_ERR_INVALID, "tree commit: lens_out and counts overlap");
     int *err = device_error_ptr();
     if (!err) return set_error(ATTN_ERR_CUDA, "tree commit: no device error word");
     return launch_tree_commit(s, n_layers, caches, kv_heads, head_dim, cu_rows, ctx_lens, lens, leaf, masks, mask_words, block_table,

@@ -109,6 +109,23 @@ def test_commit_refuses_an_array_in_another_part():
         assert call(*caches) == A.ERR_INVALID and "twice" in A.last_error(), A.last_error()
 
 
+def test_commit_refuses_outputs_over_inputs():
+    """Each of lens_out and counts over each of lens, ctx_lens, leaf, free_count and the other output, from either end."""
+    shape = A.PageShape(n_seq=8, page_size=16, max_pages=8, max_tokens=32, n_pages=64, table_stride=0)
+    at = dict(ctx=P + 256, lens=P + 512, leaf=P + 768, count=P + 1024, out=Q, counts=Q + 256)
+
+    def call(**kw):
+        x = {**at, **kw}
+        return A.lib.attn_tree_commit_ex(shape, 1, (A.PagedKV * 1)(kv(v=P + (1 << 20))), 2, 64, P, x["ctx"], x["lens"], x["leaf"], P, 1, P, P, x["count"],
+                                         x["out"], x["counts"], None)
+    for output in ("out", "counts"):
+        for other in ("ctx", "lens", "leaf", "count", "counts"):
+            if other == output:
+                continue
+            for by in (0, 4 if other != "count" else 0, -12):
+                assert call(**{output: at[other] + by}) == A.ERR_INVALID and "overlap" in A.last_error(), (output, other, by)
+
+
 def test_torch_forms(calls):  # noqa: F811
     import torch
     f, b = dict(dtype=torch.float32), dict(dtype=torch.bfloat16)
