@@ -335,3 +335,25 @@ def test_captured_with_two_streams(A):
     torch.cuda.synchronize()
     for w, x in zip(want, outs):
         assert all(torch.equal(p, q) for p, q in zip(w, x[1]))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("interleaved,rot", [(0, 32), (1, 32), (0, 2)])
+def test_weight_gradients_do_not_lose_bits_with_the_tokens(A, interleaved, rot, kind):
+    """2^17 tokens of eight heads, all one row, so that every rounding of a sum that is kept in fp32 falls on the same side:
+    a term is off by at most 13 u as above, chains of at most 8 terms in fp32 add 8 u, the parts' and the result's rounding
+    1 u each, however many tokens there are."""
+    import torch
+    tokens, heads, d = 2 ** 17, 8, 128
+    dt = torch.bfloat16 if kind == "bf16" else torch.float32
+    table = np.zeros((1, rot // 2, 2), np.float32)
+    table[..., 0] = 1.0
+    x = dev(1 + synth.uniform(71, d), dt)
+    g = dev(1 + synth.uniform(72, d), dt)
+    q, dq = x.repeat(tokens, heads), g.repeat(tokens, heads)
+    dw = torch.empty(d, device="cuda")
+    shape = A.RopeShape(tokens, tokens, heads, heads, d, rot, interleaved, tokens, 0, 0, 0, 0, 0)
+    A.norm_rope_bwd_t(shape, A.HeadNorm.of(eps=EPS), dev(np.repeat(table, tokens, 0)), None, q, None, dq, None, dq, None, dw)
+    x, g = host(x), host(g)
+    want = tokens * heads * g * x / np.sqrt((x * x).mean() + np.float64(np.float32(EPS)))
+    assert (np.abs(host(dw) - want) <= (13 + 8 + 2) * U * want).all(), np.abs(host(dw) / want - 1).max() / U
