@@ -34,11 +34,16 @@ constexpr int kHeads = 4, kHeadsBwd = 2;  // heads of a group
 constexpr int kCtas = 2;                  // of kThreads per SM, that the registers leave
 // The direct kernels' heads of a group and CTAs per SM.  Forward, 32749 tokens of 32/8 x 128 in bf16 with 4 heads and 3
 // CTAs 157 us (153 with inverse_root below), 4 and 4 (spilling) 177, 8 and 2 177, 4 and 2 220; 4096 of 12/12 x 128 in fp32 with 3 and 3 19.7 us,
-// 4 and 3 22.2, 2 and 3 20.3.  Backward with the next token's loads on their way while this one's are worked on, 2 CTAs:
-// fp32 with 2 heads 34.1 us (without 36.2; 3 heads 42.1, 3 CTAs 55), 8192 of 16/4 x 64 in bf16 with 4 heads 23 us (without 29.8).
+// 4 and 3 22.2, 2 and 3 20.3.  Backward with the next token's loads on their way while this one's are worked on, 2 CTAs
+// (us; without those loads fp32 36.2 and bf16 29.8 where they take 34.1 and 23, with 3 CTAs fp32 55):
+//   fp32, 4096 tokens of 12/12 x 128 with 1 head 41, 2 35, 3 42;
+//   bf16 in interleaved pairs, 8192 of 16/4 x 64 with 2 heads 30.3, 3 26.9, 4 23.7; 4096 of 32/8 x 128 55, 45.7, 52.3;
+//   bf16 in halves, 8192 of 16/4 x 64 24.4, 27.0, 36.7; 4096 of 32/8 x 128 48.6, 41.1, 62; 12/12 x 96 27.1, 25.2, 43.
+// (In halves 4 heads spill 136 bytes and 3 24; interleaved none.  The 16 and 20 groups of 32/8 heads with 2 or 4 of them
+// leave threads of a CTA without one.)
 constexpr int direct_heads(size_t element) { return element == 2 ? 4 : 3; }
 constexpr int direct_ctas(bool codes) { return codes ? 2 : 3; }
-constexpr int direct_heads_bwd(size_t element) { return element == 2 ? 4 : 2; }
+constexpr int direct_heads_bwd(size_t element, bool pairs) { return element == 4 ? 2 : pairs ? 4 : 3; }
 
 struct Params {
     const void *q, *k, *v;                // inputs of the forward pass
@@ -710,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 norm_rope_bwd_direct_kernel(const __grid_constant__ Params p)
 {
     pdl_begin();                          // launched by launch_pdl
-    constexpr int H = direct_heads_bwd(sizeof(T));
+    constexpr int H = direct_heads_bwd(sizeof(T), PAIRS);
     extern __shared__ __align__(16) double sums[];            // of each group
     __shared__ __align__(16) float weights[2][128];
     bring_weights(p, weights);
@@ -976,7 +981,7 @@ int launch_backward(Params p, int *parts, cudaStream_t s) {
     const void *const tensors[] = {p.q, p.k, p.dq_out, p.dk_out, p.dq, p.dk};
     const long long strides[] = {p.q_stride, p.k_stride, 0, p.qo_stride, p.ko_stride};
     const bool direct = direct_fits<T>(p, tensors, strides);
-    const dim3 grid = divide(p, direct, direct ? 4 : W, direct ? direct_heads_bwd(sizeof(T)) : kHeadsBwd, kCtas);
+    const dim3 grid = divide(p, direct, direct ? 4 : W, direct ? direct_heads_bwd(sizeof(T), p.interleaved) : kHeadsBwd, kCtas);
     *parts = (int)(grid.x * grid.y);
     const size_t smem = (size_t)p.threads / p.lanes * (p.d * 8 + (direct ? 0 : row_pitch(p) * 4));
     if (direct)
@@ -1023,7 +1028,7 @@ size_t norm_rope_bwd_workspace(const attn_rope_shape *s) {
         using namespace attn::nrope;
         Params p = norm_params(s, &n, nullptr, nullptr, i & 1 ? s->kv_heads : 0, 0, nullptr);
         const int bytes = i & 2 ? 2 : 4;
-        const dim3 grid = i < 4 ? divide(p, true, 4, direct_heads_bwd(bytes), kCtas) : divide(p, false, 16 / bytes, kHeadsBwd, kCtas);
+        const dim3 grid = i < 4 ? divide(p, true, 4, direct_heads_bwd(bytes, p.interleaved), kCtas) : divide(p, false, 16 / bytes, kHeadsBwd, kCtas);
         parts = std::max(parts, (size_t)grid.x * grid.y);
     }
     return (parts * 2 * s->head_dim * 4 + 255) / 256 * 256;
