@@ -357,3 +357,26 @@ def test_weight_gradients_do_not_lose_bits_with_the_tokens(A, interleaved, rot, 
     x, g = host(x), host(g)
     want = tokens * heads * g * x / np.sqrt((x * x).mean() + np.float64(np.float32(EPS)))
     assert (np.abs(host(dw) - want) <= (13 + 8 + 2) * U * want).all(), np.abs(host(dw) / want - 1).max() / U
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("interleaved,rot", [(0, 64), (1, 64), (0, 26)])
+@pytest.mark.parametrize("seq_len", [13, 700, 4999, 9000])
+def test_positions_of_many_tokens(A, seq_len, interleaved, rot, kind):
+    """Positions by seq_len over several of a group's tokens: sequences shorter than the stride between them, longer, and
+    longer than the tokens there are."""
+    import torch
+    tokens = 5003
+    c = Case(A, seq_len + rot, tokens, 12, 4, 64, rot, interleaved, kind, max_pos=seq_len)
+    pos = np.arange(tokens) % seq_len
+    table = dev(c.table)
+    qo, ko = torch.empty_like(c.q), torch.empty_like(c.k)
+    device_error(A)
+    A.norm_rope_t(c.shape(seq_len), c.norm, table, None, c.q, c.k, qo, ko)
+    c.check_forward(qo, c.q, 12, c.qw, pos)
+    c.check_forward(ko, c.k, 4, c.kw, pos)
+    dqw, dkw = (torch.empty(64, device="cuda") for _ in range(2))
+    A.norm_rope_bwd_t(c.shape(seq_len), c.norm, table, None, c.q, c.k, c.gq, c.gk, qo, ko, dqw, dkw)
+    c.check_backward(qo, dqw, c.q, c.gq, 12, c.qw, pos)
+    c.check_backward(ko, dkw, c.k, c.gk, 4, c.kw, pos)
+    assert device_error(A) == 0
