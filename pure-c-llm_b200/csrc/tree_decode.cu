@@ -377,7 +377,7 @@ int run_tile(const Params &p, void *ws, size_t *need, cudaStream_t s) {
 //   bf16, d 32, blocks of 64, 16, 8: 8 rows 157, 72, 63, 32 rows 191, 148, 184, 64 rows 246, 298, 367.
 //   INT8, d 64, blocks of 16, 8, 4: 4 rows 229, 156, 127, 8 rows 240, 165, 234, 16 rows 252, 306, -.
 //   fp32, blocks of 8, 4: d 32, 4 rows 132, 104, 8 rows 139, 177; d 96, 12 heads, 2 rows 270, 206, 4 rows 277, 231;
-//     d 128, 4 rows 210, 231, 8 rows 215, 404, with 12 heads, 2 rows 304, 309, 4 rows 315, 325.
+//     d 128, 4 rows 210, 231, 8 rows 215, 404, with 12 heads, 2 rows 304, 309, 4 rows 315, 325: blocks of 8 alone.
 // Lines of fewer rows than the shape leaves room for would want smaller blocks:
 // INT8 with room for 16 rows and 8 on average takes 245 in blocks of 16, 234 in 8.
 template <int N>
@@ -438,11 +438,10 @@ int run_d(const Params &p, int kv_dtype, void *ws, size_t *need, cudaStream_t s)
                                                                                                : run<int8_t, I8Path<D, 1>, D>(p, ws, need, s);
         }
     }
-    {
+    if constexpr (D < 128) {
         const bool eight = D == 32   ? least<2>(p, {4, 8}, {104, 137})
                            : D == 64 ? least<2>(p, {4, 8}, {193, 226})
-                           : D == 96 ? least<2>(p, {4, 8}, {231, 277})
-                                     : least<2>(p, {4, 8}, {231, 213});
+                                     : least<2>(p, {4, 8}, {231, 277});
         if (!eight) return run<float, F32Path<D, 4>, D>(p, ws, need, s);
     }
     return run<float, F32Path<D, 8>, D>(p, ws, need, s);
