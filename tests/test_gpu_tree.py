@@ -259,6 +259,24 @@ def test_tree_tiles(A, d, heads, kv_heads, page, drafts, ctx, groups, prefix):
     c.check(*c.run())
 
 
+@pytest.mark.parametrize("d,heads,kv_heads,drafts,groups", [
+    (32, 4, 4, 6, ()), (32, 8, 2, 16, (2, 1)), (32, 8, 1, 30, ()), (64, 4, 4, 7, ()), (64, 4, 2, 8, (3,)), (64, 8, 2, 8, ()), (64, 8, 2, 32, ()),
+    (64, 16, 2, 40, (2, 1)), (96, 3, 3, 8, ()), (96, 6, 2, 16, (1, 2)), (128, 4, 4, 8, ()), (128, 4, 2, 8, ()), (128, 16, 2, 25, ()), (128, 8, 2, 40, (4,))])
+def test_tree_bf16_error_is_the_outputs_rounding(A, d, heads, kv_heads, drafts, groups):
+    """The same precision on every path: rounding the output (2^-8 of it), a probability's second part (what the first drops,
+    2^-8 of it, rounded in its turn: 2^-16 of sum p|v|), and the fp32 errors as above."""
+    c = TreeCase(A, d + drafts, "bf16", d, heads, kv_heads, 16, [drafts] * 4, [900, 33, 0, 400], groups, (700, 65)[:len(groups)])
+    out, _ = c.run()
+    out, q64 = out.float().cpu().numpy().astype(np.float64), c.q.float().cpu().numpy().astype(np.float64)
+    for s in range(c.n):
+        for i in range(0, drafts, 5):
+            x, rows = c.cu[s] + i, c.rows_of(s, i)
+            want, _, weight, reach = R.prefix_decode(q64[x], c.k64[rows], c.v64[rows], heads, kv_heads, 1.0 / np.sqrt(d))
+            own = (2.0 ** -16 + 4 * 2.0 ** -21 * (1 + np.repeat(reach, d))) * weight
+            tol = 2.0 ** -8 * (np.abs(want) + own) + own
+            assert (np.abs(out[x] - want) <= tol).all(), (s, i, (np.abs(out[x] - want) / tol).max())
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_tree_long(A, kind):
     """A long context beside short ones, drafts up to the limit of 1024 in a chain, and a tree of 1000."""
