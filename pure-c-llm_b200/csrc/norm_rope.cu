@@ -37,8 +37,8 @@ constexpr int kCtas = 2;                  // of kThreads per SM, that the regist
 // 4 and 3 22.2, 2 and 3 20.3.  Backward with the next token's loads on their way while this one's are worked on, 2 CTAs
 // (us; without those loads fp32 36.2 and bf16 29.8 where they take 34.1 and 23, with 3 CTAs fp32 55):
 //   fp32, 4096 tokens of 12/12 x 128 with 1 head 41, 2 35, 3 42;
-//   bf16 in interleaved pairs, 8192 of 16/4 x 64 with 2 heads 30.3, 3 26.9, 4 23.7; 4096 of 32/8 x 128 55, 45.7, 52.3;
-//   bf16 in halves, 8192 of 16/4 x 64 24.4, 27.0, 36.7; 4096 of 32/8 x 128 48.6, 41.1, 62; 12/12 x 96 27.1, 25.2, 43.
+//   bf16 in interleaved pairs, 8192 of 16/4 x 64 with 2 heads 30.3, 3 26.9, 4 23.8; 4096 of 32/8 x 128 55, 45.7, 52.4;
+//   bf16 in halves, 8192 of 16/4 x 64 24.4, 27.4, 36.7; 4096 of 32/8 x 128 48.6, 41.8, 62; 12/12 x 96 27.1, 25.9, 43.
 // (In halves 4 heads spill 136 bytes and 3 24; interleaved none.  The 16 and 20 groups of 32/8 heads with 2 or 4 of them
 // leave threads of a CTA without one.)
 constexpr int direct_heads(size_t element) { return element == 2 ? 4 : 3; }
@@ -50,7 +50,7 @@ struct Params {
     void *q_out, *k_out, *v_out;          // outputs; k_out, v_out: cache bases when slots != NULL
     const void *dq_out, *dk_out;          // backward: gradients of the outputs,
     void *dq, *dk;                        // of the inputs,
-    float *partial;                       // and of the weights: [CTA][2][d] (NULL: not wanted)
+    double *partial;                      // and of the weights: [CTA][2][d] (NULL: not wanted)
     const float *q_weight, *k_weight;     // NULL: ones
     const float *table;
     const int *positions;
@@ -351,13 +351,14 @@ norm_rope_kernel(const __grid_constant__ Params p)
 
 // The weights' gradients are sums over all tokens and heads.  A lane adds up to
 // kChain terms of a column in fp32 and then empties them into its group's sums,
-// in 64 bits and in shared memory, so the error does not grow with the tokens.
-// (All in fp32: of 12/12 x 128 in fp32, 4096 tokens 34.0 us and an error of
-// 1.3e-7 against 64 bits, 65536 tokens 404 us and 4.3e-7; so 35.0 and 413 us and
-// 9e-8 both, of which a term's own roundings are 6e-8.  Chains of 4 terms
-// 35.2 us, of 16 34.8 us and 1.0e-7.)
-constexpr int kChain = 8;
-template <int HEADS> constexpr int chain_tokens() { return kChain / HEADS; }
+// in 64 bits and in shared memory, and so do the CTAs' parts and their sum, so
+// the error does not grow with the tokens.  (All but the last sum in fp32: of
+// 12/12 x 128 in fp32, 4096 tokens 34.0 us and an error of 1.3e-7 against 64
+// bits, 65536 tokens 404 us and 4.3e-7; so 35.2 and 414 us and 7.4e-8 both, of
+// which a term's own roundings are some 6e-8.  Chains of 8 terms and parts in
+// fp32 34.9 us and 8.4e-8, chains of 2 terms 35.8 us.)
+constexpr int kChain = 4;
+template <int HEADS> constexpr int chain_tokens() { return kChain / HEADS > 1 ? kChain / HEADS : 1; }
 template <int N>
 __device__ __forceinline__ void empty_into(double *sums, float (&x)[N]) {
     double2 *at = reinterpret_cast<double2 *>(sums);
@@ -372,8 +373,7 @@ __device__ __forceinline__ void empty_into(double *sums, float (&x)[N]) {
 }
 
 // Each CTA's part of them: the groups' sums of a column, in the order of the
-// groups, rounded to fp32 (once a CTA, which adds no more than rounding the
-// result does).  sums: d of each group, at their columns.
+// groups.  sums: d of each group, at their columns.
 template <int HEADS>
 __device__ __forceinline__ void write_partial(const Params &p, const double *sums) {
     for (int col = threadIdx.x; col < 2 * p.d; col += p.threads) {
@@ -383,7 +383,7 @@ __device__ __forceinline__ void write_partial(const Params &p, const double *sum
             const Place y = place_of<HEADS>(p, (int)blockIdx.y * p.threads + u);
             if (y.there && y.kind == kind) sum += sums[u / p.lanes * p.d + e];
         }
-        p.partial[((long long)blockIdx.y * gridDim.x + blockIdx.x) * 2 * p.d + col] = (float)sum;
+        p.partial[((long long)blockIdx.y * gridDim.x + blockIdx.x) * 2 * p.d + col] = sum;
     }
 }
 
@@ -858,14 +858,14 @@ norm_rope_bwd_direct_kernel(const __grid_constant__ Params p)
 
 // Columns of the CTAs' parts, 32 to a CTA, summed in an order that the sizes alone decide.
 __global__ void __launch_bounds__(1024)
-norm_weight_kernel(const float *__restrict__ partial, int parts, int d, float *__restrict__ dq_weight,
+norm_weight_kernel(const double *__restrict__ partial, int parts, int d, float *__restrict__ dq_weight,
                    float *__restrict__ dk_weight, int accumulate)
 {
     pdl_begin();                          // launched by launch_pdl
     __shared__ double sums[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = (int)blockIdx.x * 32 + lane;
     double sum = 0.0;
-    for (int i = warp; i < parts; i += 32) sum += (double)__ldcg(partial + (long long)i * 2 * d + col);
+    for (int i = warp; i < parts; i += 32) sum += __ldcg(partial + (long long)i * 2 * d + col);
     sums[warp][lane] = sum;
     __syncthreads();
     if (warp) return;
@@ -1031,7 +1031,7 @@ size_t norm_rope_bwd_workspace(const attn_rope_shape *s) {
         const dim3 grid = i < 4 ? divide(p, true, 4, direct_heads_bwd(bytes, p.interleaved), kCtas) : divide(p, false, 16 / bytes, kHeadsBwd, kCtas);
         parts = std::max(parts, (size_t)grid.x * grid.y);
     }
-    return (parts * 2 * s->head_dim * 4 + 255) / 256 * 256;
+    return (parts * 2 * s->head_dim * 8 + 255) / 256 * 256;
 }
 
 int launch_norm_rope_bwd(const attn_rope_shape *s, const attn_head_norm *n, int dtype, const float *table, const int *positions, const void *q,
@@ -1040,14 +1040,14 @@ int launch_norm_rope_bwd(const attn_rope_shape *s, const attn_head_norm *n, int 
     Params p = norm_params(s, n, table, positions, k ? s->kv_heads : 0, 0, err);
     p.q = q; p.k = k; p.dq_out = dq_out; p.dk_out = dk_out; p.dq = dq; p.dk = dk;
     const bool weights = dq_weight || dk_weight;
-    p.partial = weights ? static_cast<float *>(ws) : nullptr;
+    p.partial = weights ? static_cast<double *>(ws) : nullptr;
     int parts = 0;
     if (p.tokens > 0) {
         const int st = dtype == ATTN_F32 ? launch_backward<float>(p, &parts, stream) : launch_backward<__nv_bfloat16>(p, &parts, stream);
         if (st) return st;
     }
     if (!weights) return ATTN_OK;
-    return check_pdl(launch_pdl(attn::nrope::norm_weight_kernel, dim3(2 * p.d / 32), dim3(1024), 0, stream, (const float *)p.partial, parts, p.d,
+    return check_pdl(launch_pdl(attn::nrope::norm_weight_kernel, dim3(2 * p.d / 32), dim3(1024), 0, stream, (const double *)p.partial, parts, p.d,
                                 dq_weight, dk_weight, accumulate),
                      "norm_weight_kernel");
 }
