@@ -20,7 +20,7 @@
 //   covers a head with 16 bytes each, takes kHeads heads, and where the two
 //   elements of a pair lie in different lanes, they meet in shared memory.
 // Through the exchange kernels the direct ones' cases took 2 to 4 times as long
-// (4096 tokens of 12/12 x 128 in fp32 53 us for 19.7, gradients 90 for 34.2; prompts 607 for 153).
+// (4096 tokens of 12/12 x 128 in fp32 53 us for 19.7, gradients 90 for 35; prompts 607 for 153).
 #include <algorithm>
 
 #include "common.cuh"
@@ -39,8 +39,8 @@ constexpr int kCtas = 2;                  // of kThreads per SM, that the regist
 //   fp32, 4096 tokens of 12/12 x 128 with 1 head 41, 2 35, 3 42;
 //   bf16 in interleaved pairs, 8192 of 16/4 x 64 with 2 heads 30.3, 3 26.9, 4 23.8; 4096 of 32/8 x 128 55, 45.7, 52.4;
 //   bf16 in halves, 8192 of 16/4 x 64 24.4, 27.4, 36.7; 4096 of 32/8 x 128 48.6, 41.8, 62; 12/12 x 96 27.1, 25.9, 43.
-// (In halves 4 heads spill 136 bytes and 3 24; interleaved none.  The 16 and 20 groups of 32/8 heads with 2 or 4 of them
-// leave threads of a CTA without one.)
+// (In halves 4 heads spill 136 bytes and 3 16; interleaved none.  32/8 x 128 are 320 threads with 2 heads in halves and
+// with 4 interleaved, two CTAs of 256, and 224 or 448 with 3.)
 constexpr int direct_heads(size_t element) { return element == 2 ? 4 : 3; }
 constexpr int direct_ctas(bool codes) { return codes ? 2 : 3; }
 constexpr int direct_heads_bwd(size_t element, bool pairs) { return element == 4 ? 2 : pairs ? 4 : 3; }

@@ -10,18 +10,23 @@
 // with probabilities in one part).  The times in brackets below were taken with
 // one part too, when the same call took 143 us.
 //
-// One CTA per SM walks its range of steps (prefix.cuh) of 128 keys.  A slot is
-// 256 query rows: with more than 128, warpgroup w takes rows [128 w, 128 w + 128)
+// One CTA per SM walks its range of steps (prefix.cuh) of 128 keys.  A piece has
+// up to 256 query rows: with more than 128, warpgroup w takes rows [128 w, 128 w + 128)
 // of every step; with fewer, both take the same rows and every other step, and
-// the merge finds two pieces in the slot.  12 warps:
-//   warp 0      K rows, warp 1 V rows.  A step whose 128 keys all have rows is a
-//               TMA box of 64 dims for each page (or 128 rows of one), a lane
-//               per box.  At a line's end, with pages of fewer than 8 rows or
-//               outside the cache, the lanes copy 16 bytes each into the same
-//               128-byte swizzled layout, with zeros for keys without a row, so
-//               that a probability of 0 never meets a NaN; they report such a
-//               half (K or V of a step) when their next one is on its way.
+// each leaves a state of its own.  12 warps:
+//   warp 0      K rows, warp 1 V rows.  With pages of 8 rows or more a step is a
+//               TMA box of 64 dims for each page that there is (or 128 rows of
+//               one), a lane per box; a page's rows behind the line's last key
+//               come with it.  In K's place keys without a row hold those, or what
+//               was there before: it is the scores that are masked, by the key
+//               masks that the K warp leaves, and they have to be.  In V's place
+//               the warp writes zeros over them before it reports the half (K or V
+//               of a step), so that a probability of 0 never meets a NaN.
+//               With smaller pages the lanes copy 16 bytes each into the same
+//               128-byte swizzled layout, zeros for keys without a row, and
+//               report a half when their next one is on its way.
 //               (All steps by lanes: 299 us, the copying instructions setting the pace.)
+//               The K warp walks and tells the others the pieces through a queue.
 //   warp 2      S_wu = Q_w K_u^T for the two halves u of a step's keys, M = 128,
 //               N = 64, both operands in shared memory
 //   warp 3      O_w += P_wu V_u (P in two bf16 parts from TMEM, V as it lies, MN-major)
